@@ -223,6 +223,73 @@ int npn_gqa_tail_verify_append(const uint16_t* query, const uint16_t* gate, cons
                                void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Paged 8-bit KV cache: block tables on the device, append, attention.
+ *   cache_k [n_blocks, Hkv, block_size, 256], cache_v [n_blocks, Hkv, 256, block_size]
+ *   (dims as rows) OCP e4m3fn bytes; k_scale, v_scale [n_blocks, Hkv] f32, powers of two
+ *   of at least 2^-100: value = e4m3 * scale. block_size is 16, 32, 64 or 128; slot =
+ *   block * block_size + row in the block. Caches are 16-byte aligned. (New ops: the
+ *   reference's decode graph has a dense cache, contrib/qwen3.6-27b/static_decode.py:880-931.)
+ * ------------------------------------------------------------------------- */
+
+/* torch.ops.paged.update_blocks_ -- moves every request to the blocks that its rows need:
+ * ceil((kv_len[b] + n_b) / block_size) of them, n_b = new_len[b] clamped to [0, T]
+ * (negative kv_len counts as 0).
+ *   block_table [B, max_blocks] int32, num_blocks [B] int32 (blocks held: entries
+ *   [0, num_blocks[b]) of row b), free_blocks [n_blocks] int32 (a stack of
+ *   free_count[0] block ids): updated in place.
+ * First, requests with more blocks give the rest back (their entries become -1); the last
+ * request's last block goes lowest on the stack, so that giving back what a call granted
+ * restores the stack. Then requests with fewer are granted theirs from the top of the
+ * stack in request order, as long as the needs up to and including a request's are no
+ * more than what is free; from the first that finds too few on, all that need any are
+ * refused. A request that cannot fit max_blocks is refused and not counted.
+ * Outputs: granted [B] int32 = n_b, or 0 where refused (the request's row and count then
+ * stay as they were); slots [B, T] int64 = the slots of positions kv_len[b] + t for
+ * t < granted[b], -1 behind. 1 <= B <= 65535, B * T and B * max_blocks <= 2^30. */
+int npn_paged_update_blocks(const int32_t* kv_len, const int32_t* new_len, int32_t* block_table,
+                            int32_t* num_blocks, int32_t* free_blocks, int32_t* free_count,
+                            int64_t* slots, int32_t* granted, int B, int max_blocks,
+                            int n_blocks, int block_size, int T, void* stream);
+
+/* torch.ops.gqa.kv_append_paged -- npn_gqa_kv_append's k-side math in fp32 (RMSNorm (1+w) and
+ * partial RoPE with the table rows kv_len[b] + t, clamped to [0, positions)), into e4m3 pages:
+ *   key, value [B, T, Hkv, 256] bf16; k_norm [256]; cos_table, sin_table [positions, 64];
+ *   slots [B, T] int64 as npn_paged_update_blocks makes them: a request's rows in order, -1
+ *   from its last one on. A row whose slot is out of [0, n_blocks * block_size) is skipped.
+ * Per (block, head) that gets rows: need = the least power of two with amax <= 448 need over
+ * the finite new values; the scale becomes need if row 0 of the block is among the new ones,
+ * else max(scale, need), and the block's older rows are moved to it (rounded to nearest even,
+ * exact but for e4m3 subnormals). New rows are e4m3(x / scale), nearest even; NaN and
+ * infinities are stored as NaN. Other rows keep their bytes. No two requests of a call may
+ * append to one block. */
+int npn_gqa_kv_append_paged(const uint16_t* key, const uint16_t* value, const float* k_norm,
+                            const float* cos_table, const float* sin_table, int positions,
+                            const int32_t* kv_len, const int64_t* slots, int8_t* cache_k,
+                            int8_t* cache_v, float* k_scale, float* v_scale, int B, int T,
+                            int kv_heads, int n_blocks, int block_size, void* stream);
+
+/* Workspace bytes for npn_gqa_tail_verify_paged with these sizes (0: unsupported sizes). */
+size_t npn_gqa_tail_verify_paged_workspace_size(int B, int T, int q_heads, int kv_heads,
+                                                int max_blocks, int block_size);
+
+/* torch.ops.gqa.tail_verify_paged -- npn_gqa_tail_verify's math over the paged cache: query
+ * row (b, t, h), t < q_len[b], attends the positions [0, kv_len[b] + t] that block_table
+ * [B, max_blocks] holds; rows t >= q_len[b] are 0. RoPE rows come from the tables, at row
+ * kv_len[b] + t clamped to them. Table entries out of [0, n_blocks) hide their positions; a row
+ * without any is 0. A row does not depend on the cache behind its last position, NaN included.
+ * T = 1 is plain decode; T may be long (a prompt's chunk).
+ * Limits: Hq/Hkv <= 48, Hq/Hkv * T <= 2^20, max_blocks * block_size <= 2^30,
+ * B * Hkv * ceil(Hq/Hkv * T / 48) <= 65535. */
+int npn_gqa_tail_verify_paged(const uint16_t* query, const uint16_t* gate, const float* q_norm,
+                              const float* cos_table, const float* sin_table, int positions,
+                              const int8_t* cache_k, const int8_t* cache_v,
+                              const float* k_scale, const float* v_scale,
+                              const int32_t* block_table, const int32_t* kv_len,
+                              const int32_t* q_len, uint16_t* out, int B, int T, int q_heads,
+                              int kv_heads, int n_blocks, int max_blocks, int block_size,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
  * FP8 W8A16 GEMM.
  * ------------------------------------------------------------------------- */
 

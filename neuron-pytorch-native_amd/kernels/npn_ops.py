@@ -2,7 +2,8 @@
 
   torch.ops.deltanet.{full, full_batched, full_fp8, verify_batched, verify_from_ckpt,
                       rollback, conv_rollback, chunked_prefill}
-  torch.ops.gqa.{tail, tail_verify, kv_append}
+  torch.ops.gqa.{tail, tail_verify, kv_append, tail_verify_paged, kv_append_paged}
+  torch.ops.paged.{update_blocks_}
   torch.ops.fp8.{matmul, matmul_partials, matmul_argmax, matmul_swiglu}
   torch.ops.spec.{accept_greedy, accept_rejection}
   torch.ops.normfuse.{rms_norm, residual_rms_norm}
@@ -22,3 +23,4 @@ import fp8_matmul_ops  # noqa: F401
 import spec_accept_ops  # noqa: F401
 import rms_norm_nki_ops  # noqa: F401
 import glue_ops  # noqa: F401
+import paged_kv_ops  # noqa: F401

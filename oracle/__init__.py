@@ -12,6 +12,7 @@ Modules
 - ``numerics``  bf16 <-> float32 bit conversions (round-to-nearest-even).
 - ``deltanet``  gated-DeltaNet token step, T-token verify, rollback.
 - ``gqa``       GQA attention tail (decode and T-token verify), KV append.
+- ``paged``     paged e4m3 KV cache: block tables, append, attention over the pages.
 - ``fp8``       OCP e4m3fn decode/encode, per-channel quantisation, W8A16 matmul.
 - ``accept``    greedy and rejection-sampling acceptance, with the integer
                 softmax contract shared bit-for-bit with the HIP kernels.

@@ -1,0 +1,383 @@
+"""GPU parity of the paged e4m3 KV cache ops against the oracle (oracle/paged.py): block tables
+bit for bit, appended pages byte for byte (V) or within one code where fp32 and 64 bits round a
+normed K value apart, attention within its roundings.
+
+Attention's tolerance: the kernel rounds q' and the softmax weights to bf16 and its output to bf16.
+A rounding to bf16 is off by at most 2^-8 relative, by 0.43 * 2^-8 = 0.0017 in the root mean square
+over a binade. Independent roundings of q' move a score by 0.0017 sqrt(sum (q k)^2) / 16, about
+0.0017 for normed q and unit k, and with it each weight by as much, like the weight's own rounding;
+both reach the output as independent errors of the keys' weights. Together sqrt(3) * 0.0017 = 0.0029
+in the norm: the bound is twice that. The largest element's error, over 10^5 elements of a standard
+deviation of at most 0.0024 |out|_rms beside the output's own rounding, stays under 6e-3 max|out|
+(max|out| is over 3 rms, so that is over 7 deviations).
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import gqa as og, paged as op
+from _util import BF16_U, assert_rel_close
+
+pytestmark = pytest.mark.gpu
+TOL = 6e-3
+BF = torch.bfloat16
+
+
+def cuda(x):
+    return torch.from_numpy(np.ascontiguousarray(x)).cuda()
+
+
+# ---- block tables -----------------------------------------------------------------------------------
+
+def _state(B, P, N, rng):
+    return dict(table=np.full((B, P), -1, np.int32), held=np.zeros(B, np.int32),
+                stack=rng.permutation(N).astype(np.int32), free=N)
+
+
+def _step(ops, s, d, kv, new, bs, T):
+    """One call on the device state d and on the oracle's state s; everything compared."""
+    got = ops.paged.update_blocks_(cuda(kv), cuda(new), d["table"], d["held"], d["stack"], d["free"], bs, T)
+    slots, granted, s["free"] = op.update_blocks(kv, new, s["table"], s["held"], s["stack"], s["free"], bs, T)
+    torch.cuda.synchronize()
+    assert np.array_equal(got[1].cpu().numpy(), granted)
+    assert np.array_equal(got[0].cpu().numpy(), slots)
+    for k in ("table", "held", "stack"):
+        assert np.array_equal(d[k].cpu().numpy(), s[k]), k
+    assert int(d["free"]) == s["free"]
+    return slots, granted
+
+
+def _device(s):
+    d = {k: cuda(v) for k, v in s.items() if k != "free"}
+    d["free"] = torch.tensor([s["free"]], dtype=torch.int32, device="cuda")
+    return d
+
+
+@pytest.mark.parametrize("B,P,N,bs,T", [
+    (1, 1, 1, 16, 1),          # the smallest pool
+    (7, 6, 20, 16, 40),        # refusals
+    (64, 40, 1200, 64, 8),     # a verify step's
+    (3, 300, 500, 16, 4097),   # odd T: the slots' own launch, unaligned rows
+    (1024, 4, 3000, 32, 5),    # one thread per request
+    (1025, 4, 2500, 128, 3),   # requests in two groups
+    (2500, 3, 5000, 16, 2),
+])
+def test_update_blocks(ops, B, P, N, bs, T):
+    """A run of calls: random growth past the pool, ends of requests, and calls in which some
+    requests give back while others are granted."""
+    rng = np.random.default_rng(B + T)
+    s = _state(B, P, N, rng)
+    d = _device(s)
+    kv = np.zeros(B, np.int32)
+    for _ in range(6):
+        new = rng.integers(0, T + 1, B).astype(np.int32)
+        _, granted = _step(ops, s, d, kv, new, bs, T)
+        kv = kv + (granted * rng.random(B)).astype(np.int32)
+        kv[rng.random(B) < 0.2] = 0
+    _step(ops, s, d, np.zeros(B, np.int32), np.zeros(B, np.int32), bs, T)
+    assert s["free"] == N
+
+
+def test_update_blocks_out_of_range_values(ops):
+    """Negative lengths and counts count as 0, new_len past T as T, counts past the row or the pool
+    as full; a request longer than its table row is refused without counting; the last free block
+    goes to the first that needs one."""
+    rng = np.random.default_rng(3)
+    s = _state(6, 3, 8, rng)
+    s["table"][:] = 7
+    s["held"][:] = [-5, 0, 9, 0, 0, 0]
+    s["free"] = 4
+    d = _device(s)
+    kv = np.array([-3, 100, 40, 0, 16, 2**31 - 1], np.int32)
+    new = np.array([-1, 5, 8, 99, 1, 8], np.int32)
+    _step(ops, s, d, kv, new, 16, 8)
+    s["free"], d["free"] = 99, torch.tensor([99], dtype=torch.int32, device="cuda")
+    _step(ops, s, d, kv, new, 16, 8)
+    s["free"], d["free"] = -4, torch.tensor([-4], dtype=torch.int32, device="cuda")
+    _step(ops, s, d, np.zeros(6, np.int32), new, 16, 8)
+
+
+# ---- append ---------------------------------------------------------------------------------------------
+
+def _empty_cache(N, H, bs, rng):
+    """Pages of random bytes (NaN among them) and scales: what an append does not write must stay."""
+    return [rng.integers(0, 256, (N, H, bs, 256)).astype(np.uint8),
+            rng.integers(0, 256, (N, H, 256, bs)).astype(np.uint8),
+            np.exp2(rng.integers(-9, -3, (N, H))).astype(np.float32),
+            np.exp2(rng.integers(-9, -3, (N, H))).astype(np.float32)]
+
+
+def _cuda_cache(c):
+    return [cuda(c[0].view(np.int8)), cuda(c[1].view(np.int8)), cuda(c[2]), cuda(c[3])]
+
+
+def _slots(kv, n, T, bs, N, rng):
+    """Slots of n[b] rows at positions kv[b] + t in distinct random pages, -1 behind; (slots, table)."""
+    B = len(kv)
+    P = max(1, max(-(-(int(kv[b]) + int(n[b])) // bs) for b in range(B)))
+    table = np.full((B, P), -1, np.int32)
+    ids, slots = rng.permutation(N), np.full((B, T), -1, np.int64)
+    used = 0
+    for b in range(B):
+        m = -(-(int(kv[b]) + int(n[b])) // bs)
+        table[b, :m] = ids[used:used + m]
+        used += m
+        pos = int(kv[b]) + np.arange(int(n[b]))
+        slots[b, :int(n[b])] = table[b, pos // bs].astype(np.int64) * bs + pos % bs
+    return slots, table
+
+
+def _same_cache(dev, ref):
+    for name, got, want in (("k_scale", dev[2], ref[2]), ("v_scale", dev[3], ref[3])):
+        assert np.array_equal(got.cpu().numpy(), want), name
+    k, v = dev[0].cpu().numpy().view(np.uint8), dev[1].cpu().numpy().view(np.uint8)
+    assert np.array_equal(v, ref[1]), f"{(v != ref[1]).sum()} V bytes differ"
+    off = np.abs((k & 0x7F).astype(int) - (ref[0] & 0x7F))
+    sign = (k ^ ref[0]) >> 7
+    assert off.max() <= 1 and not (sign & ((k & 0x7F) > 0)).any()
+    # fp32 norm and rotation are off by a few 2^-24 relative; a step is 2^-4 to 2^-3: codes differ
+    # where a value lies that near a border, in one of some 10^5
+    assert (off > 0).mean() <= 1e-3 + 2 / off.size
+
+
+def _append(ops, key, value, k_norm, cos, sin, kv, slots, cache):
+    ops.gqa.kv_append_paged(key, value, k_norm, cos, sin, kv, slots, *cache)
+
+
+@pytest.mark.parametrize("bs,T,H,kv,n", [
+    (16, 1, 4, [0, 1, 15, 16, 17], [1, 1, 1, 1, 1]),      # plain decode at every edge of a page
+    (64, 8, 4, [60, 0, 57, 64], [8, 8, 8, 8]),            # verify rows that cross a page end
+    (16, 8, 1, [5, 12, 16], [8, 0, 3]),                   # padded rows, an idle request
+    (32, 3, 2, [31, 30], [3, 2]),
+    (128, 300, 2, [5, 128], [300, 129]),                  # prompts over several pages
+    (16, 65, 1, [3], [65]),
+    (64, 129, 1, [0, 7], [129, 100]),
+    (128, 20, 1, [100], [20]),
+])
+def test_kv_append_paged(ops, bs, T, H, kv, n):
+    rng = np.random.default_rng(T + bs)
+    B = len(kv)
+    kv = np.array(kv, np.int32)
+    N = sum(-(-(int(a) + int(b)) // bs) for a, b in zip(kv, n)) + 3
+    slots, _ = _slots(kv, n, T, bs, N, rng)
+    cache = _empty_cache(N, H, bs, rng)
+    dev = _cuda_cache(cache)
+    g = torch.Generator().manual_seed(T)
+    key = (torch.randn(B, T, H, 256, generator=g) * 3).to(BF)
+    value = (torch.randn(B, T, H, 256, generator=g) * torch.rand(B, T, H, 1, generator=g) * 9).to(BF)
+    k_norm = torch.randn(256, generator=g) * 0.1
+    cos, sin = og.rope_cos_sin(np.arange(int(kv.max()) + T - 1))  # one short: the last row clamps
+    _append(ops, key.cuda(), value.cuda(), k_norm.cuda(), cuda(cos), cuda(sin), cuda(kv), cuda(slots), dev)
+    torch.cuda.synchronize()
+    op.kv_append(key.double().numpy(), value.double().numpy(), k_norm.double().numpy(), cos, sin, kv, slots,
+                 cache)
+    _same_cache(dev, cache)
+
+
+def test_kv_append_paged_scale_grows_and_shrinks(ops):
+    """Row after row into one page: tiny, zero, huge, then small values again (the scale stays),
+    and a new first row, which sets the scale anew whatever the stale rows held."""
+    rng = np.random.default_rng(5)
+    H, bs, N = 2, 16, 3
+    cache = _empty_cache(N, H, bs, rng)
+    dev = _cuda_cache(cache)
+    k_norm = np.zeros(256)
+    cos, sin = og.rope_cos_sin(np.arange(64))
+    seen = []
+    for pos, size in ((0, 1e-3), (1, 0.0), (2, 1e-30), (3, 7.0), (4, 3e4), (5, 1e38), (6, 1.0), (0, 1e-3), (1, 2.0)):
+        kv = np.array([pos], np.int32)
+        key = torch.randn(1, 1, H, 256).to(BF)
+        value = (torch.rand(1, 1, H, 256) * size).to(BF)
+        slots = np.array([[bs + pos]], np.int64)
+        _append(ops, key.cuda(), value.cuda(), cuda(k_norm.astype(np.float32)), cuda(cos), cuda(sin), cuda(kv),
+                cuda(slots), dev)
+        torch.cuda.synchronize()
+        op.kv_append(key.double().numpy(), value.double().numpy(), k_norm, cos, sin, kv, slots, cache)
+        _same_cache(dev, cache)
+        seen.append(float(cache[3][1, 0]))
+    assert seen[0] == seen[1] == seen[2] < seen[3] < seen[4] < seen[5] == seen[6] > seen[7] < seen[8]
+
+
+def test_kv_append_paged_non_finite_and_foreign_slots(ops):
+    """NaN and infinities become NaN bytes and leave the scale; slots past the pool or negative, and
+    rows behind a break in a request's slots, are skipped."""
+    rng = np.random.default_rng(6)
+    H, bs, N, T = 1, 16, 4, 4
+    cache = _empty_cache(N, H, bs, rng)
+    dev = _cuda_cache(cache)
+    key = torch.randn(4, T, H, 256).to(BF)
+    value = torch.randn(4, T, H, 256).to(BF)
+    value[0, 0, 0, 3], value[0, 1, 0, 4], value[0, 2, 0, 5] = float("nan"), float("inf"), -float("inf")
+    value[1] = float("nan")
+    key[0, 1, 0, 7] = float("nan")
+    kv = np.array([3, 14, 0, 0], np.int32)
+    slots = np.array([[3, 4, 5, 6], [30, 31, -1, -1], [N * bs, N * bs + 1, -1, -1], [-7, 50, 51, 52]], np.int64)
+    cos, sin = og.rope_cos_sin(np.arange(64))
+    z = torch.zeros(256)
+    _append(ops, key.cuda(), value.cuda(), z.cuda(), cuda(cos), cuda(sin), cuda(kv), cuda(slots), dev)
+    torch.cuda.synchronize()
+    slots[3] = -1  # a request without a first slot appends nothing
+    op.kv_append(key.double().numpy(), value.double().numpy(), z.double().numpy(), cos, sin, kv, slots, cache)
+    _same_cache(dev, cache)
+
+
+# ---- attention -----------------------------------------------------------------------------------------------
+
+def _attend_inputs(B, T, H, grp, bs, kv, n, seed, spare_pages=2):
+    rng = np.random.default_rng(seed)
+    kv = np.array(kv, np.int32)
+    N = sum(-(-(int(a) + int(b)) // bs) for a, b in zip(kv, n)) + spare_pages
+    _, table = _slots(kv, n, T, bs, N, rng)
+    # random finite e4m3 values up to 4 (code 0x48), in pages of different scales; and NaN wherever
+    # no row may look: whole spare pages, and the rows behind each request's last
+    code = lambda *s: (rng.integers(0, 0x49, s) | (rng.integers(0, 2, s) << 7)).astype(np.uint8)  # noqa: E731
+    cache = [code(N, H, bs, 256), code(N, H, 256, bs),
+             np.exp2(rng.integers(-2, 1, (N, H))).astype(np.float32),
+             np.exp2(rng.integers(-3, 2, (N, H))).astype(np.float32)]
+    used = set(table[table >= 0].tolist())
+    for i in set(range(N)) - used:
+        cache[0][i], cache[1][i], cache[2][i], cache[3][i] = 0x7F, 0xFF, np.nan, np.nan
+    for b in range(B):
+        end = int(kv[b]) + int(n[b])
+        if end % bs and end:
+            last = table[b, end // bs]
+            cache[0][last, :, end % bs:], cache[1][last, :, :, end % bs:] = 0xFF, 0x7F
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    cos, sin = og.rope_cos_sin(np.arange(max(int(kv.max()) + T, 1)))
+    return dict(query=r(B, T, H * grp, 256).to(BF), gate=r(B, T, H * grp, 256).to(BF), q_norm=r(256) * 0.1,
+                cos=cos, sin=sin, cache=cache, table=table, kv=kv, n=np.array(n, np.int32))
+
+
+def _attend(ops, d, dev=None):
+    dev = dev or _cuda_cache(d["cache"])
+    return ops.gqa.tail_verify_paged(d["query"].cuda(), d["gate"].cuda(), d["q_norm"].cuda(), cuda(d["cos"]),
+                                     cuda(d["sin"]), *dev, cuda(d["table"]), cuda(d["kv"]), cuda(d["n"]))
+
+
+def _oracle(d):
+    return op.tail_verify(d["query"].double().numpy(), d["gate"].double().numpy(), d["q_norm"].double().numpy(),
+                          d["cos"], d["sin"], d["cache"], d["table"], d["kv"], d["n"])
+
+
+def _check(ops, d):
+    out = _attend(ops, d)
+    torch.cuda.synchronize()
+    got, ref = out.float().cpu().double().numpy(), _oracle(d)
+    assert_rel_close(got, ref, tol=TOL, out_unit=BF16_U, name="tail_verify_paged")
+    for b, n in enumerate(d["n"]):
+        assert not got[b, max(int(n), 0):].any()
+
+
+@pytest.mark.parametrize("B,T,H,grp,bs,kv,n", [
+    (1, 1, 1, 1, 16, [0], [1]),                         # one key, one head
+    (1, 1, 1, 6, 64, [300], [1]),                       # one 16-row tile
+    (3, 1, 4, 6, 16, [0, 63, 64], [1, 1, 1]),           # step ends
+    (2, 8, 4, 6, 64, [37, 600], [8, 8]),                # three tiles
+    (3, 8, 4, 6, 32, [0, 1, 2000], [8, 8, 8]),
+    (4, 5, 2, 6, 128, [127, 128, 1500, 11], [5, 0, 3, 1]),  # two tiles, padded and idle requests
+    (2, 4, 2, 4, 16, [100, 33], [4, 4]),
+    (1, 7, 1, 48, 16, [50], [7]),                       # a token's heads fill a group: many groups
+    (2, 33, 2, 6, 16, [70, 0], [33, 20]),               # a prompt's chunk: groups without a live token
+    (1, 150, 1, 5, 64, [500], [150]),                   # tokens that straddle groups (48 rows, 5 heads)
+])
+def test_tail_verify_paged_matches_oracle(ops, B, T, H, grp, bs, kv, n):
+    _check(ops, _attend_inputs(B, T, H, grp, bs, kv, n, seed=B * 7 + T))
+
+
+def test_tail_verify_paged_ragged_batches(ops):
+    """More pairs than workgroups, some without a step; then one long request among short ones, so
+    that one pair has most workgroups."""
+    rng = np.random.default_rng(41)
+    kv, n = rng.integers(0, 301, 70), rng.integers(0, 4, 70)
+    _check(ops, _attend_inputs(70, 3, 4, 6, 16, kv, n, seed=41))
+    kv = rng.integers(0, 60, 40)
+    kv[7] = 9000
+    _check(ops, _attend_inputs(40, 5, 2, 6, 64, kv, [5] * 40, seed=43))
+
+
+def test_tail_verify_paged_long(ops):
+    """Chunks of pages beyond what a workgroup keeps in LDS at a time, alone and beside a neighbour."""
+    _check(ops, _attend_inputs(1, 1, 1, 6, 16, [33000], [1], seed=2))
+    _check(ops, _attend_inputs(2, 8, 4, 6, 128, [32768 - 8, 17000], [8, 8], seed=5))
+
+
+def test_tail_verify_paged_all_idle(ops):
+    d = _attend_inputs(3, 2, 2, 6, 16, [5, 0, 40], [0, 0, 0], seed=9)
+    assert not _attend(ops, d).any()
+
+
+def test_tail_verify_paged_missing_pages(ops):
+    """Table entries that are none or past the pool hide their positions; a row with none left is 0,
+    whatever its gate."""
+    d = _attend_inputs(3, 3, 2, 6, 16, [40, 5, 100], [3, 3, 3], seed=10)
+    d["table"][0, 1] = -1
+    d["table"][1, 0] = len(d["cache"][0])
+    d["table"][2, [0, 3, 6]] = [2**31 - 1, -2**31, -1]
+    d["gate"][1] = float("nan")
+    got, ref = _attend(ops, d).float().cpu().double().numpy(), None
+    d["gate"][1] = 0
+    ref = _oracle(d)
+    assert not got[1].any()
+    assert_rel_close(got, ref, tol=TOL, out_unit=BF16_U, name="missing pages")
+
+
+@pytest.mark.parametrize("where", ["k", "v"])
+def test_tail_verify_paged_nan_stays_with_its_rows(ops, where):
+    """A NaN among the new rows' keys or values reaches the rows that see it and no others."""
+    B, T, H, grp, bs = 2, 6, 2, 6, 16
+    d = _attend_inputs(B, T, H, grp, bs, [61, 30], [6, 6], seed=12)
+    clean = _attend(ops, d)
+    pos = 61 + 3
+    page, row = d["table"][0, pos // bs], pos % bs
+    if where == "k":
+        d["cache"][0][page, 1, row, 17] = 0x7F
+    else:
+        d["cache"][1][page, 1, 17, row] = 0xFF
+    got = _attend(ops, d)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    if where == "k":
+        hit[0, 3:, grp:] = True
+    else:
+        hit[0, 3:, grp:, 17] = True
+    assert torch.isnan(got[hit]).all()
+    assert torch.equal(got[~hit], clean[~hit])
+
+
+def test_tail_verify_paged_equals_dense_op_in_values(ops):
+    """The same positions through gqa::tail_verify's dense bf16 cache of the dequantised rows."""
+    B, T, H, grp, bs = 2, 8, 4, 6, 32
+    d = _attend_inputs(B, T, H, grp, bs, [100, 517], [8, 8], seed=14)
+    S = 544
+    k, v = torch.zeros(2, B, H, S, 256, dtype=BF)
+    for b in range(B):
+        for h in range(H):
+            n = int(d["kv"][b]) + T
+            kk, vv, _ = op.values(d["cache"], d["table"][b, :-(-n // bs)], h, n)
+            k[b, h, :n], v[b, h, :n] = torch.from_numpy(kk).to(BF), torch.from_numpy(vv).to(BF)
+    cos, sin = cuda(d["cos"]), cuda(d["sin"])
+    at = cuda(d["kv"]).long()[:, None] + torch.arange(T, device="cuda")
+    ref = ops.gqa.tail_verify(d["query"].cuda(), d["gate"].cuda(), d["q_norm"].cuda(), cos[at].contiguous(),
+                              sin[at].contiguous(), k.cuda(), v.cuda(), cuda(d["kv"]))
+    assert_rel_close(_attend(ops, d).float().cpu().numpy(), ref.float().cpu().numpy(), tol=TOL, out_unit=BF16_U)
+
+
+def test_refusals(ops):
+    d = _attend_inputs(1, 1, 1, 6, 16, [5], [1], seed=1)
+    args = [d["query"].cuda(), d["gate"].cuda(), d["q_norm"].cuda(), cuda(d["cos"]), cuda(d["sin"]),
+            *_cuda_cache(d["cache"]), cuda(d["table"]), cuda(d["kv"]), cuda(d["n"])]
+    for i, bad, err in ((0, args[0].float(), TypeError), (1, args[1][:, :, :3], RuntimeError),
+                        (5, args[5].float(), TypeError), (6, args[6].transpose(2, 3), RuntimeError),
+                        (7, args[7][:1], RuntimeError), (9, args[9].long(), TypeError),
+                        (10, args[10].cpu(), RuntimeError), (11, torch.cat([args[11]] * 2), RuntimeError)):
+        with pytest.raises(err):
+            ops.gqa.tail_verify_paged(*[bad if j == i else a for j, a in enumerate(args)])
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    plan = [i32(0), i32(1), i32(-1, -1).reshape(1, 2), i32(0), i32(0, 1), i32(2)]
+    for bs, T in ((8, 1), (16, 0)):
+        with pytest.raises(RuntimeError):
+            ops.paged.update_blocks_(*plan, bs, T)
+    with pytest.raises(TypeError):
+        ops.paged.update_blocks_(plan[0].long(), *plan[1:], 16, 1)
+    with pytest.raises(RuntimeError):
+        ops.paged.update_blocks_(i32(0, 1), *plan[1:], 16, 1)
