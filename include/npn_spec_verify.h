@@ -572,6 +572,27 @@ int npn_deltanet_rollback_commit(const uint16_t* const* mixed_qkv, uint16_t* con
                                  int32_t* kv_len, int32_t* committed, int B, int T, int k_heads,
                                  int v_heads, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Sampling.
+ * ------------------------------------------------------------------------- */
+
+/* torch.ops.spec.sample -- new op (plain decode's sampler; the reference's on-device path is an
+ * argmax, contrib/qwen3.6-27b/static_decode.py:1313): one token per row of logits [R, V] (f32, or
+ * bf16 with bf16 = 1) with the row's own settings, all [R].
+ * Tokens are ranked by logit, larger first, lower index first among equals, and weigh
+ * w = exp((l - max) / temperature). Kept are the first top_k ranks (<= 0 or >= V: all), of those
+ * as many as their weight takes to reach top_p of the top_k ranks' weight (at least one; >= 1 or
+ * NaN: all), of those the ones with w >= min_p (<= 0 or NaN: all; above 1 counts as 1).
+ * ids[r] (int64) is the first rank whose cumulative weight exceeds u of the kept ranks' weight; u
+ * is clamped to [0, 1 - 2^-24], NaN as 0. A temperature that is not above 0 takes the first
+ * rank. NaN logits count as -infinity, which is never kept; if the maximum is +infinity those at
+ * +infinity share all the weight. A row without a token above -infinity gives -1.
+ * Weights are integers round(w 2^42) and their sums exact: the same inputs give the same ids,
+ * and weights under 2^-43 of the largest count as 0. 1 <= V <= 2^20. */
+int npn_sample(const void* logits, int bf16, const float* temperature, const int32_t* top_k,
+               const float* top_p, const float* min_p, const float* u, int64_t* ids, int R, int V,
+               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

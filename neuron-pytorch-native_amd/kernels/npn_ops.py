@@ -5,7 +5,7 @@
   torch.ops.gqa.{tail, tail_verify, kv_append, tail_verify_paged, kv_append_paged}
   torch.ops.paged.{update_blocks_}
   torch.ops.fp8.{matmul, matmul_partials, matmul_argmax, matmul_swiglu}
-  torch.ops.spec.{accept_greedy, accept_rejection}
+  torch.ops.spec.{accept_greedy, accept_rejection, sample}
   torch.ops.normfuse.{rms_norm, residual_rms_norm}
   torch.ops.glue.{silu_mul, deltanet_split, gqa_split}
 
@@ -24,3 +24,4 @@ import spec_accept_ops  # noqa: F401
 import rms_norm_nki_ops  # noqa: F401
 import glue_ops  # noqa: F401
 import paged_kv_ops  # noqa: F401
+import spec_sample_ops  # noqa: F401

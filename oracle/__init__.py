@@ -14,6 +14,7 @@ Modules
 - ``gqa``       GQA attention tail (decode and T-token verify), KV append.
 - ``paged``     paged e4m3 KV cache: block tables, append, attention over the pages.
 - ``fp8``       OCP e4m3fn decode/encode, per-channel quantisation, W8A16 matmul.
+- ``sample``    per-row sampling with temperature, top-k, top-p and min-p.
 - ``accept``    greedy and rejection-sampling acceptance, with the integer
                 softmax contract shared bit-for-bit with the HIP kernels.
 - ``verify_step`` the 4-layer verify slice composed from the above.
