@@ -7,27 +7,34 @@
 //   K and V the e4m3 bytes times their (block, head) scale. Rows t >= q_len[b] are 0.
 //
 // The rows of a kv head (token-major, grp heads per token) are cut into groups of R = 16 NRT rows;
-// a (request, row group, kv head) is a "pair" of its rows and its keys. Two launches:
-//  1. attn: the pairs' 64-key steps are laid end to end and cut into W equal ranges, one per
-//     workgroup of four waves; every workgroup finds its range from the lengths itself (the host
-//     does not know them). Wave w takes every fourth step of a segment, on its own: no barrier and
-//     no LDS between the loads and the products.
-//       S^T[64 keys x 16 rows] = K Q'^T   A = K, 16 bytes per lane straight from the page: lane
-//         (i, G) of tile j holds key 16 (i / 4) + 4 j + i % 4, dims 64 c + 16 G + [0, 16) for load
-//         c; the product's k order follows (Q' lies in LDS in the same order), so the page row is
-//         read as it is;
+// a (request, row group) is a unit, a (unit, kv head) a pair of its rows and its keys, taken in steps
+// of 64 keys. Three launches:
+//  1. prep: q' of every pair as MFMA B operands, and, in its first block, the plan: the host does not
+//     know the lengths. A pair of n steps gets ceil(n / Q) workgroups, Q the least number of steps
+//     (a multiple of the waves') with which all pairs' workgroups are at most `most`. (Equal cuts
+//     through the pairs laid end to end balanced better and cost most workgroups a second segment,
+//     with its own start and end: 20 us of 80 for 64 sequences of one token.)
+//  2. attn: a workgroup takes an equal part of its pair's steps; its NW waves (eight for up to 16
+//     rows; four, with all of a SIMD's registers, for more) take those in turn, each on its own:
+//       S^T[64 keys x 16 rows] = K Q'^T   A = K, 16 bytes per lane as they lie in the page: lane (i, G)
+//         of tile j holds key 16 (i / 4) + 4 j + i % 4, dims 64 c + 16 G + [0, 16) for column c; the
+//         product's k order follows (Q' is laid out in the same order). In f16: every e4m3 value is
+//         an f16 number, q' over a power of two per row has 11 bits, and both scales go into the
+//         fp32 scores;
 //       online softmax per row in fp32, base 2; that key order puts keys 16 G + [0, 16) of a row
 //         into one lane, in order, so
 //       O^T[256 x 16 rows] += V^T P^T     takes P straight from the score registers as B, and A = V^T
-//         is 16 bytes of a page's dim row [dim][16 G + [0, 16)].
-//     The bytes go from the pages to a part of LDS that is the wave's own by DMA (a lane reads back
-//     the 16 bytes that it sent, so nothing but the wave's own vmcnt wait stands between), and
-//     become bf16 with the page's scale in v_cvt_scalef32_pk_bf16_fp8, exactly (an e4m3 value times
-//     a power of two is a bf16 number). The next step's K is sent for when this step's is used up,
-//     V likewise, so a wave has 16 to 32 KB in flight and no register holds them (held in
-//     registers, 128 a lane beside the accumulators, they spilled).
-//     The four waves' (m, l, O) meet in LDS at the segment's end.
-//  2. merge: the log-sum-exp merge of a pair's segments, times sigmoid(gate), to bf16.
+//         is 16 bytes of a page's dim row; its bytes become bf16 with the page's scale in
+//         v_cvt_scalef32_pk_bf16_fp8, exactly (an e4m3 value times a power of two is a bf16 number),
+//         and P is split into bf16 hi + lo parts (as gqa::tail_verify's: with hi alone the output's
+//         error was 0.0029 against its own rounding's 0.0017).
+//     The bytes go from the pages by DMA to a part of LDS that is the wave's own, in groups of 8 KB
+//     in the order of their use (two K tiles, or eight V tiles of 16 dims); a wave takes a group into
+//     registers, sends its place for a later one and works on it, with one (NW = 8) to three groups
+//     in flight. Nothing else may touch memory in that loop: a reload of a spilled register waits,
+//     in order, for every DMA before it.
+//     The waves' (m, l, O) meet in LDS; a pair with one workgroup is written out at once.
+//  3. merge: the log-sum-exp merge of the other pairs' workgroups, times sigmoid(gate), to bf16.
 #include "npn_common.h"
 
 namespace {
@@ -39,13 +46,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -1.0e30f;   // finite "no key yet" running max (avoids inf - inf)
 constexpr float kRescaleLog2 = 8.0f;  // the exponent base moves only when a row max grows > 2^8
 constexpr int KS = 64;                // keys per step
-constexpr int kWaves = 4;
-constexpr int kMaxWG = 256;           // one workgroup per CU: its rings fill the LDS
 constexpr int kChunk = 64;            // steps whose page ids and scales are in LDS at a time
 constexpr int kPages = kChunk * KS / 16 + 1;
 
 typedef __bf16 bf16x8 __attribute__((__vector_size__(8 * sizeof(__bf16))));
 typedef __bf16 bf16x2 __attribute__((__vector_size__(2 * sizeof(__bf16))));
+typedef _Float16 f16x8 __attribute__((__vector_size__(8 * sizeof(_Float16))));
+typedef _Float16 f16x2 __attribute__((__vector_size__(2 * sizeof(_Float16))));
 typedef float f32x4 __attribute__((__vector_size__(4 * sizeof(float))));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
@@ -63,10 +70,17 @@ struct PagedArgs {
   const int32_t* kv_len;
   const int32_t* q_len;
   uint16_t* out;
-  float* part_o;           // [kMaxWG + pairs][R][256]
-  float* part_ml;          // [kMaxWG + pairs][R][2]
-  int32_t* ustart;         // [U + 2]: first step of each unit, all steps, workgroups
-  int positions, B, T, Hq, Hkv, grp, R, RG, P, N, sh, min_steps;
+  u32x4* q;                // [pairs][8][NRT][64] q' as B operands
+  float* q_scale;          // [pairs][R]
+  float* part_o;           // [slots][R][256] O of the workgroups of split pairs
+  float* part_ml;          // [slots][R][2]
+  int32_t* wstart;         // [U + 1] first workgroup of each unit
+  int32_t* sstart;         // [U] first slot of each unit
+  int positions, B, T, Hq, Hkv, grp, R, RG, P, N, sh, nw;
+  uint64_t by_grp;         // 2^32 / grp + 1: rows are below 2^21
+
+  __device__ __forceinline__ int token_of(int row) const { return (int)((row * by_grp) >> 32); }
+  __device__ __forceinline__ int units() const { return B * RG; }
 };
 
 // Unit u = (request, row group): its keys [0, kend) and the tokens it covers.
@@ -78,23 +92,14 @@ __device__ __forceinline__ Unit unit_of(const PagedArgs& a, int u) {
   Unit r;
   r.b = u / a.RG;
   const int rg = u - r.b * a.RG;
-  r.t0 = rg * a.R / a.grp;  // the group's first token
-  const int t1 = min(((rg + 1) * a.R - 1) / a.grp, a.T - 1);
+  r.t0 = a.token_of(rg * a.R);  // the group's first token
+  const int t1 = min(a.token_of((rg + 1) * a.R - 1), a.T - 1);
   const int n = min(min(a.q_len[r.b], a.T), t1 + 1);  // tokens up to the group's last live one
   const int cap = a.P << a.sh;  // <= 2^30
   r.kv = min(max(a.kv_len[r.b], 0), cap);
   r.kend = n > r.t0 ? min(r.kv + n, cap) : 0;
   r.steps = (r.kend + KS - 1) / KS;
   return r;
-}
-
-// Workgroups that take part for S steps.
-__device__ __forceinline__ int paged_wgs(int S, int min_steps, int most) {
-  return max(1, min(most, S / min_steps));
-}
-
-__device__ __forceinline__ int wg_first_step(int w, int S, int W) {
-  return (int)((int64_t)w * S / W);
 }
 
 __device__ __forceinline__ float max_over_groups(float x) {
@@ -118,6 +123,16 @@ __device__ __forceinline__ bf16x8 dequant8(uint32_t w0, uint32_t w1, float scale
   const u32x4 v = {__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
                    __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)};
   return __builtin_bit_cast(bf16x8, v);
+}
+
+__device__ __forceinline__ f16x8 to_f16x8(uint32_t w0, uint32_t w1) {
+  const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, false);
+  const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, true);
+  const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, false);
+  const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true);
+  const u32x4 v = {__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
+                   __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)};
+  return __builtin_bit_cast(f16x8, v);
 }
 
 // A word's bytes of keys [0, n) kept, n <= 0: none, n >= 4: all.
@@ -145,6 +160,20 @@ __device__ __forceinline__ void dma16(const void* g, unsigned lds) {
       : "memory");
 }
 
+// The same with a wave-uniform address and a per-lane byte offset.
+__device__ __forceinline__ void dma16_soff(const void* base, unsigned voff, unsigned lds) {
+  unsigned saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %2\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(voff), "s"(base), "s"(lds)
+      : "memory");
+}
+
 // LDS by address, element k of 16 bytes (1 KB apart: one per lane) from a per-lane base. The bases are
 // hidden from the optimiser (opaque): left to itself it kept some hundred of base + offset sums,
 // past the 16-bit offset of an LDS instruction, in registers and spilled them.
@@ -155,484 +184,678 @@ __device__ __forceinline__ u32x4 lds_read(unsigned base, int k) {
 __device__ __forceinline__ void lds_write(unsigned base, int k, u32x4 v) {
   reinterpret_cast<lds_u32x4*>(base)[64 * k] = v;
 }
+// With a SIMD to itself a wave's accumulators stay in AGPRs: without a word at the places where VALU
+// work touches them, the compiler carried them in VGPRs and copied all of them twice a step.
+__device__ __forceinline__ void pin(f32x4& x) { asm volatile("" : "+a"(x)); }
 __device__ __forceinline__ unsigned opaque(unsigned x) {
   asm volatile("" : "+v"(x));
   return x;
 }
 
-template <int NRT>
+// Four dims of a row's output: o / l * sigmoid(gate); 0 for a row without keys (inv = 0), whatever its
+// gate, and for tokens past q_len.
+__device__ __forceinline__ void write_out(const PagedArgs& a, int b, int row, int h, int dim, f32x4 o, float inv) {
+  const int t = a.token_of(row), qh = h * a.grp + row - t * a.grp;
+  const size_t at = (((size_t)b * a.T + t) * a.Hq + qh) * DH + dim;
+  const uint2 g = *reinterpret_cast<const uint2*>(a.gate + at);
+  const uint32_t gw[2] = {g.x, g.y};
+  const bool live = inv != 0.f && t < a.q_len[b];
+  uint32_t y[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float v0 = o[2 * j] * inv * npn::sigmoid(npn::bf16lo(gw[j]));
+    const float v1 = o[2 * j + 1] * inv * npn::sigmoid(npn::bf16hi(gw[j]));
+    y[j] = live ? npn::f32_to_bf16(v0) | ((uint32_t)npn::f32_to_bf16(v1) << 16) : 0u;
+  }
+  *reinterpret_cast<uint2*>(a.out + at) = make_uint2(y[0], y[1]);
+}
+
+// ---- 1. prep ----------------------------------------------------------------------------------------
+constexpr int kPrepWaves = 8;
+constexpr int kPlanUnits = 4096;  // units whose steps the plan keeps in LDS
+
+// One workgroup per CU where the pairs with steps are few enough to be cut so; else one each and 512
+// more for the longest.
+__host__ __device__ constexpr int most_workgroups(int pairs) { return pairs <= 192 ? 256 : pairs + 512; }
+// Split pairs' workgroups: all of 256, or, as a pair of c >= 2 has c - 1 of the 512, twice those.
+constexpr int kSlots = 1024;
+
+// Workgroups of each unit's pairs: the least Q = nw k with sum ceil(n / Q) <= most lies between
+// k = S / (most nw) and S / ((most - pairs) nw); the eight waves test eight k of what is left at a time.
+__device__ void plan_block(const PagedArgs& a) {
+  __shared__ int s_n[kPlanUnits];
+  __shared__ int s_wave[kPrepWaves][2];
+  __shared__ int s_sum[kPrepWaves * 64][2];
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+  const int U = a.units();
+  auto steps_of = [&](int u) { return u < kPlanUnits ? s_n[u] : unit_of(a, u).steps; };
+  int sum = 0, some = 0;
+  for (int u = tid; u < U; u += kPrepWaves * 64) {
+    const int n = unit_of(a, u).steps;
+    if (u < kPlanUnits) s_n[u] = n;
+    sum += n;
+    some += n > 0;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    sum += __shfl_xor(sum, off, 64);
+    some += __shfl_xor(some, off, 64);
+  }
+  if (lane == 0) {
+    s_wave[w][0] = sum;
+    s_wave[w][1] = some;
+  }
+  __syncthreads();
+  sum = some = 0;
+  for (int k = 0; k < kPrepWaves; ++k) {
+    sum += s_wave[k][0];
+    some += s_wave[k][1];
+  }
+  const int S = sum * a.Hkv, pairs = some * a.Hkv;  // S < 2^30
+  const int most = most_workgroups(pairs);
+  auto up = [](int n, int d) { return (n + d - 1) / d; };
+  int lo = max(1, up(up(S, most), a.nw)), hi = max(lo, up(up(S, most - pairs), a.nw));
+  while (lo < hi) {
+    const int Q = (lo + (int)((int64_t)(hi - lo) * w / kPrepWaves)) * a.nw;
+    int g = 0;
+    for (int u = lane; u < U; u += 64) g += up(steps_of(u), Q);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) g += __shfl_xor(g, off, 64);
+    __syncthreads();  // s_wave has been read
+    if (lane == 0) s_wave[w][0] = g;
+    __syncthreads();
+    int nlo = lo, nhi = hi;
+    for (int k = kPrepWaves - 1; k >= 0; --k) {
+      const int t = lo + (int)((int64_t)(hi - lo) * k / kPrepWaves);
+      if ((int64_t)s_wave[k][0] * a.Hkv <= most) nhi = t;
+      else nlo = max(nlo, t + 1);
+    }
+    lo = min(nlo, nhi);
+    hi = nhi;
+  }
+  const int Q = hi * a.nw;
+  // First workgroup and first slot of each unit: scans over threads' slices of the units.
+  const int per = up(U, kPrepWaves * 64);
+  const int u0 = min(U, tid * per), u1 = min(U, u0 + per);
+  int wg = 0, slot = 0;
+  for (int u = u0; u < u1; ++u) {
+    const int c = up(steps_of(u), Q) * a.Hkv;
+    wg += c;
+    slot += c > a.Hkv ? c : 0;
+  }
+  const int wg_mine = wg, slot_mine = slot;
+  for (int off = 1; off < kPrepWaves * 64; off <<= 1) {
+    s_sum[tid][0] = wg;
+    s_sum[tid][1] = slot;
+    __syncthreads();
+    if (tid >= off) {
+      wg += s_sum[tid - off][0];
+      slot += s_sum[tid - off][1];
+    }
+    __syncthreads();
+  }
+  if (tid == kPrepWaves * 64 - 1) a.wstart[U] = wg;
+  wg -= wg_mine;
+  slot -= slot_mine;
+  for (int u = u0; u < u1; ++u) {
+    const int c = up(steps_of(u), Q) * a.Hkv;
+    a.wstart[u] = wg;
+    a.sstart[u] = slot;
+    wg += c;
+    slot += c > a.Hkv ? c : 0;
+  }
+}
+
+// q' of one padded row per wave (rows that are none repeat the pair's last), f16 over the least power
+// of two above the row's largest element; dim d = 64 c + 16 g + 8 h + e is element e of lane group g
+// in k step 2 c + h.
+__global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagedArgs a) {
+  if (blockIdx.x == 0) {
+    plan_block(a);
+    return;
+  }
+  const int64_t wave = (int64_t)(blockIdx.x - 1) * kPrepWaves + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int pair = (int)(wave / a.R), r = (int)(wave - (int64_t)pair * a.R);
+  if (pair >= a.units() * a.Hkv) return;
+  const int u = pair / a.Hkv, h = pair - u * a.Hkv;
+  const int b = u / a.RG;
+  const int row = min((u - b * a.RG) * a.R + r, a.T * a.grp - 1);
+  const int t = a.token_of(row), qh = h * a.grp + row - t * a.grp;
+  const uint2 q = *reinterpret_cast<const uint2*>(a.query + (((size_t)b * a.T + t) * a.Hq + qh) * DH + 4 * lane);
+  const int kv = min(max(a.kv_len[b], 0), a.P << a.sh);
+  const size_t pos = (size_t)min(kv + t, a.positions - 1) * ROPE + 4 * (lane & 15);
+  const float4 c = *reinterpret_cast<const float4*>(a.cos + pos);
+  const float4 s = *reinterpret_cast<const float4*>(a.sin + pos);
+  const float4 nw = *reinterpret_cast<const float4*>(a.q_norm + 4 * lane);
+  float v[4] = {npn::bf16lo(q.x), npn::bf16hi(q.x), npn::bf16lo(q.y), npn::bf16hi(q.y)};
+  const float ss = npn::wave_sum(v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3]);
+  const float rn = rsqrtf(ss * (1.0f / DH) + kEps);
+  v[0] = (1.0f + nw.x) * (v[0] * rn);
+  v[1] = (1.0f + nw.y) * (v[1] * rn);
+  v[2] = (1.0f + nw.z) * (v[2] * rn);
+  v[3] = (1.0f + nw.w) * (v[3] * rn);
+  float y[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = __shfl_xor(v[j], 8, 64);  // dim d ^ 32
+  if (lane < ROPE / 4) {
+    const float sg = lane < ROPE / 8 ? -1.0f : 1.0f;
+    v[0] = v[0] * c.x + sg * y[0] * s.x;
+    v[1] = v[1] * c.y + sg * y[1] * s.y;
+    v[2] = v[2] * c.z + sg * y[2] * s.z;
+    v[3] = v[3] * c.w + sg * y[3] * s.w;
+  }
+  const float big = npn::wave_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+  const uint32_t e = min(max(__float_as_uint(big) >> 23, 64u), 190u);  // 2^-63 to 2^63
+  const float inv = __uint_as_float((253u - e) << 23);                // 2^-(e - 126)
+  if (lane == 0) a.q_scale[(size_t)pair * a.R + r] = __uint_as_float((e + 1) << 23) * (kLog2e / 16.0f);
+  uint32_t two[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const f16x2 x = {(_Float16)(v[2 * j] * inv), (_Float16)(v[2 * j + 1] * inv)};
+    two[j] = __builtin_bit_cast(uint32_t, x);
+  }
+  const int d = 4 * lane;
+  const int step = 2 * (d >> 6) + ((d >> 3) & 1), g = (d >> 4) & 3;
+  u32x4* dst = a.q + (((size_t)pair * 8 + step) * (a.R / 16) + (r >> 4)) * 64 + 16 * g + (r & 15);
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint32_t*>(dst) + ((d & 4) >> 1)) = make_uint2(two[0], two[1]);
+}
+
+// ---- 2. attn ----------------------------------------------------------------------------------------
+template <int NRT, int NW>
 struct PagedSmem {
+  static constexpr int DR = NRT == 3 ? 8 : 16;  // 16-dim tiles of O that all waves have in LDS at once
   union {
-    struct {
-      u32x4 k[4][4][64];                  // a step's K as sent: [key tile][64-dim column][lane]
-      u32x4 v[16][64];                    // and V: [dim tile][lane]
-    } ring[kWaves];
-    f32x4 o[2][NRT][16][64];              // two waves' O on their way to the other two
+    uint8_t ring[NW][16 / NW][8192];            // each wave's groups
+    f32x4 o[NW][NRT][DR][64];
   };
-  u32x4 q[8][NRT][64];                    // q' as B operands: [k step][row tile][lane]
-  float m[kWaves][NRT * 16], l[kWaves][NRT * 16];
-  int page[kPages];                       // -1: none
+  u32x4 q[8][NW == 4 ? NRT : 1][64];            // q' as B operands: [k step][row tile][lane]
+  float m[NW][NRT * 16], l[NW][NRT * 16], inv[NRT * 16];
+  int page[kPages];                             // -1: none
   float ks[kPages], vs[kPages];
-  int scan[256];
 };
 
-template <int NRT>
-__global__ __launch_bounds__(256, 1) void paged_attn_kernel(PagedArgs a) {
+template <int NRT, int NW>
+__global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a) {
   constexpr int R = NRT * 16;
-  __shared__ __attribute__((aligned(16))) PagedSmem<NRT> sm;
+  constexpr int NR = 16 / NW;  // groups in a wave's ring
+  constexpr int kThreads = NW * 64;
+  using Smem = PagedSmem<NRT, NW>;
+  __shared__ __attribute__((aligned(1024))) Smem sm;
   const int tid = threadIdx.x;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int i = lane & 15, G = lane >> 4;
   const int bs = 1 << a.sh;
-  const int U = a.B * a.RG;
-  const unsigned ring_lds = __builtin_amdgcn_readfirstlane(npn::lds_addr(&sm.ring[w]));
-  const unsigned k_at = opaque(npn::lds_addr(&sm.ring[w].k[0][0][lane]));
-  const unsigned v_at = opaque(npn::lds_addr(&sm.ring[w].v[0][lane]));
-  const unsigned q_at = opaque(npn::lds_addr(&sm.q[0][0][lane]));
-  const unsigned o_at = opaque(npn::lds_addr(&sm.o[0][0][0][lane]));
+  const int U = a.units();
 
-  // The steps of all units: thread t sums its slice of them, and a scan over the slices.
-  const int per = (U + 255) / 256;
-  const int u0 = min(U, tid * per), u1 = min(U, u0 + per);
-  int mine = 0;
-  for (int u = u0; u < u1; ++u) mine += unit_of(a, u).steps;
-  sm.scan[tid] = mine * a.Hkv;
-  __syncthreads();
-  for (int off = 1; off < 256; off <<= 1) {
-    const int v = tid >= off ? sm.scan[tid - off] : 0;
+  // This workgroup's unit (64-way search in the starts), kv head and steps [s_lo, s_lo + steps).
+  if ((int)blockIdx.x >= a.wstart[U]) return;
+  int u = 0;
+  for (int n = U; n > 1;) {
+    const int stride = (n + 63) / 64, at = u + lane * stride;
+    const bool le = at < u + n && a.wstart[at] <= (int)blockIdx.x;
+    const int last = __popcll(__builtin_amdgcn_ballot_w64(le)) - 1;
+    n = min(stride, n - last * stride);
+    u = __builtin_amdgcn_readfirstlane(u + last * stride);
+  }
+  const Unit un = unit_of(a, u);
+  const int w0 = a.wstart[u], parts = (a.wstart[u + 1] - w0) / a.Hkv;
+  const int h = ((int)blockIdx.x - w0) / parts, part = (int)blockIdx.x - w0 - h * parts;
+  const int s_lo = (int)((int64_t)part * un.steps / parts);
+  const int steps = (int)((int64_t)(part + 1) * un.steps / parts) - s_lo;
+  const int pair = u * a.Hkv + h;
+  const int row0 = (u - un.b * a.RG) * R;  // the group's first row
+  const int rows = min(R, a.T * a.grp - row0);
+
+  // The last key of each of this lane's rows (one per tile); -1 for rows that are none.
+  int lim[NRT];
+  float q_scale[NRT], m_run[NRT], l_run[NRT];
+#pragma unroll
+  for (int nt = 0; nt < NRT; ++nt) {
+    const int r = 16 * nt + i, t = a.token_of(row0 + r);
+    lim[nt] = r < rows && t < a.q_len[un.b] ? min(un.kv + t, un.kend - 1) : -1;
+    q_scale[nt] = a.q_scale[(size_t)pair * R + r];
+    m_run[nt] = kNegBig;
+    l_run[nt] = 0.f;
+  }
+  const int lim0 = un.kv + un.t0;  // no row of the group sees less
+  const unsigned ring_lds = __builtin_amdgcn_readfirstlane(npn::lds_addr(&sm.ring[w][0][0]));
+  const u32x4* qsrc = a.q + (size_t)pair * 8 * NRT * 64 + lane;
+  u32x4 qreg[NW == 8 ? 8 : 1];
+  if constexpr (NW == 8) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) qreg[k] = qsrc[64 * k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < 2 * NRT; ++k)
+      dma16(qsrc + 64 * (w * 2 * NRT + k),
+            __builtin_amdgcn_readfirstlane(npn::lds_addr(&sm.q[0][0][0])) + (w * 2 * NRT + k) * 1024u);
+  }
+
+  // K goes four whole rows (1 KB) to a DMA, column c of row r (of the step's 64) to place c ^ f(r) of
+  // the row's 256 bytes, f(r) = 4 (r / 16) + r % 4: lane (i, G)'s row of a tile has f = i, so the 16
+  // rows that a tile reads at one column lie in 16 different places. A group holds rows 16 k + 8 n
+  // .. + 7 for k = 0..3 as its rows 8 k .. + 7. Sources and places of the k (or c) differ in bits 6
+  // and 7 alone.
+  const unsigned ksrc = (unsigned)(G * DH + ((i ^ G) << 4));
+  const unsigned k_at = ring_lds + (unsigned)((8 * (i >> 2) + (i & 3)) * DH + ((i ^ G) << 4));
+  const unsigned v_at = ring_lds + lane * 16u;
+  const unsigned q_at = npn::lds_addr(&sm.q[0][0][lane]);
+
+  // Steps are taken kChunk at a time, [c0, c0 + cn) of this workgroup's, with their pages in LDS.
+  int cn, key0, page0;
+  auto k_page = [&](int s, int k) {  // of keys 16 k .. + 15 of a step (wave-uniform)
+    const int key = key0 + s * KS + 16 * k;
+    const int id = __builtin_amdgcn_readfirstlane(max(sm.page[(key >> a.sh) - page0], 0));
+    return a.cache_k + ((((size_t)id * a.Hkv + h) << a.sh) + (key & (bs - 1))) * DH;
+  };
+  auto load_k = [&](const uint8_t* const (&pg)[4], int n, int at) {  // tiles 2 n, 2 n + 1
+    const unsigned src = opaque(ksrc);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        dma16_soff(pg[k] + (2 * n + j) * 4 * DH, src ^ (k << 6),
+                   ring_lds + (unsigned)(at * 8192 + (k * 2 + j) * 1024));
+  };
+  auto v_page = [&](int s) {  // the lane's place, dim i, in the page of its 16 keys of a step
+    const int key = key0 + s * KS + 16 * G;
+    const int id = max(sm.page[(key >> a.sh) - page0], 0);
+    return a.cache_v + ((((size_t)id * a.Hkv + h) * DH + i) << a.sh) + (key & (bs - 1));
+  };
+  auto load_v = [&](const uint8_t* pg, int n, int at) {  // dims 128 n .. + 127
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+      dma16(pg + ((size_t)(8 * n + d) << (a.sh + 4)), ring_lds + (unsigned)(at * 8192 + d * 1024));
+  };
+  auto begin_chunk = [&](int c0) {
+    cn = min(kChunk, steps - c0);
+    key0 = (s_lo + c0) * KS;
+    page0 = key0 >> a.sh;
+    const int pages = ((min(key0 + cn * KS, un.kend) - 1) >> a.sh) - page0 + 1;
+    __syncthreads();  // the last chunk's pages have been used
+    for (int p = tid; p < kPages; p += kThreads) {
+      int id = -1;
+      if (p < pages) id = a.table[(size_t)un.b * a.P + page0 + p];
+      const bool ok = id >= 0 && id < a.N;
+      sm.page[p] = ok ? id : -1;
+      sm.ks[p] = ok ? a.k_scale[(size_t)id * a.Hkv + h] : 1.0f;
+      sm.vs[p] = ok ? a.v_scale[(size_t)id * a.Hkv + h] : 1.0f;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // and q' is in LDS
     __syncthreads();
-    sm.scan[tid] += v;
-    __syncthreads();
-  }
-  const int S = sm.scan[255];
-  const int W = paged_wgs(S, a.min_steps, (int)gridDim.x);
-  if (blockIdx.x == 0) {  // the merge finds the segments by these
-    int run = sm.scan[tid] - mine * a.Hkv;
-    for (int u = u0; u < u1; ++u) {
-      a.ustart[u] = run;
-      run += unit_of(a, u).steps * a.Hkv;
-    }
-    if (tid == 0) {
-      a.ustart[U] = S;
-      a.ustart[U + 1] = W;
-    }
-  }
-  if ((int)blockIdx.x >= W) return;
-  int x = wg_first_step(blockIdx.x, S, W);
-  const int x_end = wg_first_step(blockIdx.x + 1, S, W);
-  if (x >= x_end) return;
-
-  // The unit of step x: the slice with it, then the unit inside the slice.
-  int slice = 0;
-  for (int n = 256; n > 1;) {
-    const int half = n >> 1;
-    if (sm.scan[slice + half - 1] <= x) {
-      slice += half;
-      n -= half;
-    } else {
-      n = half;
-    }
-  }
-  int u = __builtin_amdgcn_readfirstlane(slice * per);
-  int ubeg = __builtin_amdgcn_readfirstlane(slice > 0 ? sm.scan[slice - 1] : 0);
-  Unit un = unit_of(a, u);
-  while (ubeg + un.steps * a.Hkv <= x) {
-    ubeg += un.steps * a.Hkv;
-    un = unit_of(a, ++u);
-  }
-
-  while (x < x_end) {
-    const int h = (x - ubeg) / un.steps;
-    const int s_lo = (x - ubeg) - h * un.steps;
-    const int steps = min(x_end - x, un.steps - s_lo);
-    const int pair = u * a.Hkv + h;
-    const int row0 = (u - un.b * a.RG) * R;  // the group's first row
-    const int rows = min(R, a.T * a.grp - row0);
-
-    // q' of the group's rows, as B operands in LDS: wave w prepares rows w, w + 4, ...
-    __syncthreads();  // the previous segment is done with LDS
-    {
-      const float4 nw = *reinterpret_cast<const float4*>(a.q_norm + 4 * lane);
-      for (int r = w; r < R; r += kWaves) {
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (r < rows) {
-          const int t = (row0 + r) / a.grp, qh = h * a.grp + (row0 + r) - t * a.grp;
-          const uint2 p = *reinterpret_cast<const uint2*>(
-              a.query + (((size_t)un.b * a.T + t) * a.Hq + qh) * DH + 4 * lane);
-          v[0] = npn::bf16lo(p.x);
-          v[1] = npn::bf16hi(p.x);
-          v[2] = npn::bf16lo(p.y);
-          v[3] = npn::bf16hi(p.y);
-          const float ss = npn::wave_sum(v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3]);
-          const float rn = rsqrtf(ss * (1.0f / DH) + kEps);
-          v[0] = (1.0f + nw.x) * (v[0] * rn);
-          v[1] = (1.0f + nw.y) * (v[1] * rn);
-          v[2] = (1.0f + nw.z) * (v[2] * rn);
-          v[3] = (1.0f + nw.w) * (v[3] * rn);
-          float y[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = __shfl_xor(v[j], 8, 64);  // dim d ^ 32
-          if (lane < ROPE / 4) {
-            const int64_t pos = min((int64_t)un.kv + t, (int64_t)a.positions - 1);
-            const float4 c = *reinterpret_cast<const float4*>(a.cos + pos * ROPE + 4 * lane);
-            const float4 s = *reinterpret_cast<const float4*>(a.sin + pos * ROPE + 4 * lane);
-            const float sg = lane < ROPE / 8 ? -1.0f : 1.0f;
-            v[0] = v[0] * c.x + sg * y[0] * s.x;
-            v[1] = v[1] * c.y + sg * y[1] * s.y;
-            v[2] = v[2] * c.z + sg * y[2] * s.z;
-            v[3] = v[3] * c.w + sg * y[3] * s.w;
-          }
-        }
-        uint32_t b[2];
-        constexpr float scale = kLog2e / 16.0f;  // softmax scale 1/sqrt(256), in base 2
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          b[j] = npn::f32_to_bf16(v[2 * j] * scale) |
-                 ((uint32_t)npn::f32_to_bf16(v[2 * j + 1] * scale) << 16);
-        // dim d = 64 c + 16 g + 8 h + e sits in k step 2 c + h, lane group g, element e
-        const int d = 4 * lane;
-        const int step = 2 * (d >> 6) + ((d >> 3) & 1), g = (d >> 4) & 3;
-        uint32_t* dst = reinterpret_cast<uint32_t*>(&sm.q[step][r >> 4][16 * g + (r & 15)]) +
-                        ((d & 4) >> 1);
-        dst[0] = b[0];
-        dst[1] = b[1];
+  };
+  auto first_sends = [&]() {
+    if (w < cn) {
+      const uint8_t* const kp[4] = {k_page(w, 0), k_page(w, 1), k_page(w, 2), k_page(w, 3)};
+      load_k(kp, 0, 0);
+      load_k(kp, 1, 1);
+      if constexpr (NR == 4) {
+        const uint8_t* const vp = v_page(w);
+        load_v(vp, 0, 2);
+        load_v(vp, 1, 3);
       }
     }
-
-    // The last key of each of this lane's rows (one per tile); -1 for rows that are none.
-    int lim[NRT];
+  };
+  begin_chunk(0);
+  // What was loaded so far is waited for here: a wait behind the first DMAs would drain them.
 #pragma unroll
-    for (int nt = 0; nt < NRT; ++nt) {
-      const int r = 16 * nt + i, t = (row0 + r) / a.grp;
-      lim[nt] = r < rows && t < a.q_len[un.b] ? min(un.kv + t, un.kend - 1) : -1;
+  for (int nt = 0; nt < NRT; ++nt) asm volatile("" : "+v"(lim[nt]), "+v"(q_scale[nt]));
+#pragma unroll
+  for (int k = 0; k < (NW == 8 ? 8 : 1); ++k) asm volatile("" : "+v"(qreg[k]));
+  first_sends();
+
+  f32x4 acc[NRT][16];
+#pragma unroll
+  for (int nt = 0; nt < NRT; ++nt)
+#pragma unroll
+    for (int d = 0; d < 16; ++d) acc[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (int c0 = 0; c0 < steps; c0 += kChunk) {
+    if (c0 > 0) {
+      begin_chunk(c0);
+      first_sends();
     }
-    const int lim0 = un.kv + un.t0;  // no row of the group sees less
-
-    float m_run[NRT], l_run[NRT];
-    f32x4 acc[NRT][16];
-#pragma unroll
-    for (int nt = 0; nt < NRT; ++nt) {
-      m_run[nt] = kNegBig;
-      l_run[nt] = 0.f;
-#pragma unroll
-      for (int dt = 0; dt < 16; ++dt) acc[nt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-
-    for (int c0 = 0; c0 < steps; c0 += kChunk) {
-      const int cn = min(kChunk, steps - c0);
-      const int key0 = (s_lo + c0) * KS;
-      const int page0 = key0 >> a.sh;
-      const int pages = ((min(key0 + cn * KS, un.kend) - 1) >> a.sh) - page0 + 1;
-      __syncthreads();  // the last chunk's pages have been used; q' is in LDS
-      for (int p = tid; p < kPages; p += 256) {
-        int id = -1;
-        if (p < pages) id = a.table[(size_t)un.b * a.P + page0 + p];
-        const bool ok = id >= 0 && id < a.N;
-        sm.page[p] = ok ? id : -1;
-        sm.ks[p] = ok ? a.k_scale[(size_t)id * a.Hkv + h] : 1.0f;
-        sm.vs[p] = ok ? a.v_scale[(size_t)id * a.Hkv + h] : 1.0f;
-      }
-      __syncthreads();
-
-      auto load_k = [&](int s) {
-        const int key = key0 + s * KS + 16 * (i >> 2);
-        const int id = max(sm.page[(key >> a.sh) - page0], 0);
-        const uint8_t* p = a.cache_k +
-            ((((size_t)id * a.Hkv + h) << a.sh) + (key & (bs - 1)) + (i & 3)) * DH + 16 * G;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) dma16(p + j * 4 * DH + c * 64, ring_lds + (j * 4 + c) * 1024);
-      };
-      auto load_v = [&](int s) {
-        const int key = key0 + s * KS + 16 * G;
-        const int id = max(sm.page[(key >> a.sh) - page0], 0);
-        const uint8_t* p = a.cache_v + ((((size_t)id * a.Hkv + h) * DH + i) << a.sh) + (key & (bs - 1));
-#pragma unroll
-        for (int dt = 0; dt < 16; ++dt)
-          dma16(p + ((size_t)dt << (a.sh + 4)), ring_lds + 16384 + dt * 1024);
-      };
-      if (w < cn) {
-        load_k(w);
-        load_v(w);
-      }
-      for (int s = w; s < cn; s += kWaves) {
-        const int k0 = key0 + s * KS;
-        const float ks = sm.ks[((k0 + 16 * (i >> 2)) >> a.sh) - page0];
-        const int vpage = ((k0 + 16 * G) >> a.sh) - page0;
-        const float vs = sm.vs[vpage];
-        const bool held = sm.page[vpage] >= 0;  // this lane's 16 keys exist
-        const bool next = s + kWaves < cn;
-
-        // The 16 DMAs of this step's K are older than the 16 of its V.
-        asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-        f32x4 st[NRT][4];
+    for (int s = w; s < cn; s += NW) {
+      if constexpr (NW == 4) {
 #pragma unroll
         for (int nt = 0; nt < NRT; ++nt)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) st[nt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int d = 0; d < 16; ++d) pin(acc[nt][d]);
+      }
+      const int k0 = key0 + s * KS;
+      const int page = ((k0 + 16 * G) >> a.sh) - page0;  // of this lane's 16 keys
+      const float ks = sm.ks[page], vs = sm.vs[page];
+      const bool held = sm.page[page] >= 0;  // they exist
+      const bool next = s + NW < cn;
+      const int sn = next ? s + NW : s;
+      const uint8_t* const vp = v_page(NR == 4 ? sn : s);
+      const uint8_t* const kp[4] = {k_page(sn, 0), k_page(sn, 1), k_page(sn, 2), k_page(sn, 3)};
+
+      f32x4 st[NRT][4];
+#pragma unroll
+      for (int nt = 0; nt < NRT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) st[nt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      // Groups K 0, K 1, V 0, V 1 (0 to 3) in places 0 .. NR - 1 in turn. A group has landed when at
+      // most the DMAs of the NR - 1 after it are in flight (fewer at the end); once it is in
+      // registers its place is sent for the group NR further on.
+      auto landed = [&](int g) {
+        if (next || 3 - g >= NR - 1)
+          asm volatile("s_waitcnt vmcnt(%0)" ::"n"(8 * (NR - 1)) : "memory");
+        else if (g == 1)
+          asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+        else if (g == 2)
+          asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        else
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      };
+      auto send = [&](int g) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if constexpr (NR == 4) {
+          if (next) {
+            if (g < 2) load_k(kp, g, g);
+            else load_v(vp, g - 2, g);
+          }
+        } else {
+          if (g < 2) load_v(vp, g, g);
+          else if (next) load_k(kp, g - 2, g - 2);
+        }
+      };
+      const unsigned kat = opaque(k_at), vat = opaque(v_at);
+      if constexpr (NW == 8) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          landed(n);
+          u32x4 kw[2][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) kw[j][c] = lds_read(kat ^ (c << 6), 8 * n + j);
+          send(n);
+#pragma unroll
+          for (int step = 0; step < 8; ++step)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const u32x4 k4 = kw[j][step >> 1];
+              const f16x8 kf = (step & 1) ? to_f16x8(k4[2], k4[3]) : to_f16x8(k4[0], k4[1]);
+              st[0][2 * n + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  kf, __builtin_bit_cast(f16x8, qreg[step]), st[0][2 * n + j], 0, 0, 0);
+            }
+        }
+      } else {  // both K groups together, so that q' is read from LDS once
+        asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+        const unsigned qat = opaque(q_at);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           u32x4 kw[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) kw[j] = lds_read(k_at, 4 * j + c);
+          for (int j = 0; j < 4; ++j) kw[j] = lds_read(kat ^ (c << 6), 8 * (j >> 1) + (j & 1));
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            bf16x8 q[NRT];
+            f16x8 q[NRT];
 #pragma unroll
             for (int nt = 0; nt < NRT; ++nt)
-              q[nt] = __builtin_bit_cast(bf16x8, lds_read(q_at, (2 * c + half) * NRT + nt));
+              q[nt] = __builtin_bit_cast(f16x8, lds_read(qat, (2 * c + half) * NRT + nt));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const bf16x8 kf = dequant8(kw[j][2 * half], kw[j][2 * half + 1], ks);
+              const f16x8 kf = to_f16x8(kw[j][2 * half], kw[j][2 * half + 1]);
 #pragma unroll
               for (int nt = 0; nt < NRT; ++nt)
-                st[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[nt], st[nt][j], 0, 0, 0);
+                st[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, q[nt], st[nt][j], 0, 0, 0);
             }
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (next) {  // this step's K has been read into registers
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          load_k(s + kWaves);
-        }
+        send(0);
+        send(1);
+      }
 
-        // A step with keys past the group's first limit, or past a page that is none, is masked.
-        const bool tail = k0 + KS - 1 > lim0 || __builtin_amdgcn_ballot_w64(!held) != 0;
-        if (tail) {
-          const int kb = k0 + 16 * G;
+      // A step with keys past the group's first limit, or past a page that is none, is masked.
+      const bool tail = k0 + KS - 1 > lim0 || __builtin_amdgcn_ballot_w64(!held) != 0;
 #pragma unroll
-          for (int nt = 0; nt < NRT; ++nt)
+      for (int nt = 0; nt < NRT; ++nt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j) st[nt][j] *= ks * q_scale[nt];
+      if (tail) {
+        const int kb = k0 + 16 * G;
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (!held || kb + 4 * j + r > lim[nt]) st[nt][j][r] = -INFINITY;
-        }
-
-        bf16x8 p[NRT][2];
-#pragma unroll
-        for (int nt = 0; nt < NRT; ++nt) {
-          float mx = st[nt][0][0];
+        for (int nt = 0; nt < NRT; ++nt)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[nt][j][r]);
-          mx = max_over_groups(mx);
-          const bool grow = mx > m_run[nt] + kRescaleLog2;
-          if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-            const float mnew = grow ? mx : m_run[nt];
-            const float corr = exp2f(m_run[nt] - mnew);
-            m_run[nt] = mnew;
-            l_run[nt] *= corr;
+            for (int r = 0; r < 4; ++r)
+              if (!held || kb + 4 * j + r > lim[nt]) st[nt][j][r] = -INFINITY;
+      }
+
+      bf16x8 ph[NRT][2], pl[NRT][2];
 #pragma unroll
-            for (int dt = 0; dt < 16; ++dt) acc[nt][dt] *= corr;
+      for (int nt = 0; nt < NRT; ++nt) {
+        float mx = st[nt][0][0];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[nt][j][r]);
+        mx = max_over_groups(mx);
+        const bool grow = mx > m_run[nt] + kRescaleLog2;
+        if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+          const float mnew = grow ? mx : m_run[nt];
+          const float corr = exp2f(m_run[nt] - mnew);
+          m_run[nt] = mnew;
+          l_run[nt] *= corr;
+#pragma unroll
+          for (int d = 0; d < 16; ++d) {
+            acc[nt][d] *= corr;
+            if constexpr (NW == 4) pin(acc[nt][d]);
           }
-          float sum = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float pv = __builtin_amdgcn_exp2f(st[nt][j][r] - m_run[nt]);
-              sum += pv;
-              p[nt][j >> 1][(j & 1) * 4 + r] = (__bf16)pv;
-            }
-          l_run[nt] += sum;
         }
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float pv = __builtin_amdgcn_exp2f(st[nt][j][r] - m_run[nt]);
+            sum += pv;
+            const __bf16 hi = (__bf16)pv;
+            ph[nt][j >> 1][(j & 1) * 4 + r] = hi;
+            pl[nt][j >> 1][(j & 1) * 4 + r] = (__bf16)(pv - (float)hi);
+          }
+        l_run[nt] += sum;
+      }
 
-        if (next)
-          asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-        else
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        landed(2 + n);
+        u32x4 v[8];
+#pragma unroll
+        for (int d = 0; d < 8; ++d) v[d] = lds_read(vat, 8 * ((2 + n) % NR) + d);
+        send(2 + n);
         if (tail) {
           // V bytes of keys that no row sees are cleared (0 times NaN is NaN). A NaN at a key that
-          // some rows see reaches those and no others: the rows' products with "is NaN" say which
-          // outputs become NaN, and the byte is then cleared too.
+          // some rows see reaches those and no others: it is cleared too, and the product of "is
+          // NaN" and "sees it", 2^100 each, makes the outputs that it belongs in infinite, which
+          // the segment's end makes NaN (as it would a sum past the largest float).
           const int live = held ? un.kend - (k0 + 16 * G) : 0;
           uint32_t nan_seen = 0;
-#pragma unroll 1
-          for (int dt = 0; dt < 16; ++dt) {
-            u32x4 v = lds_read(v_at, dt);
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              v[k] &= keep_bytes(live - 4 * k);
-              nan_seen |= nan_bytes(v[k]);
+              v[d][k] &= keep_bytes(live - 4 * k);
+              nan_seen |= nan_bytes(v[d][k]);
             }
-            lds_write(v_at, dt, v);
-          }
           if (__builtin_amdgcn_ballot_w64(nan_seen != 0) != 0) {
             bf16x8 see[NRT][2];
 #pragma unroll
             for (int nt = 0; nt < NRT; ++nt)
 #pragma unroll
               for (int e = 0; e < 16; ++e)
-                see[nt][e >> 3][e & 7] = (__bf16)(k0 + 16 * G + e <= lim[nt] ? 1.0f : 0.0f);
+                see[nt][e >> 3][e & 7] = (__bf16)(k0 + 16 * G + e <= lim[nt] ? 0x1p100f : 0.0f);
 #pragma unroll
-            for (int dt = 0; dt < 16; ++dt) {
-              u32x4 v = lds_read(v_at, dt), is;
+            for (int d = 0; d < 8; ++d) {
+              u32x4 is;
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                is[k] = nan_bytes(v[k]) & 0x38383838u;  // e4m3 1.0
-                v[k] &= ~nan_bytes(v[k]);
+                is[k] = nan_bytes(v[d][k]) & 0x38383838u;  // e4m3 1.0
+                v[d][k] &= ~nan_bytes(v[d][k]);
               }
-              lds_write(v_at, dt, v);
 #pragma unroll
-              for (int nt = 0; nt < NRT; ++nt) {
-                f32x4 hit = {0.f, 0.f, 0.f, 0.f};
+              for (int nt = 0; nt < NRT; ++nt)
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
-                  hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                      dequant8(is[2 * k], is[2 * k + 1], 1.0f), see[nt][k], hit, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  if (hit[r] > 0.f) acc[nt][dt][r] = NAN;
-              }
+                  acc[nt][8 * n + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                      dequant8(is[2 * k], is[2 * k + 1], 0x1p100f), see[nt][k], acc[nt][8 * n + d], 0, 0, 0);
             }
           }
         }
 #pragma unroll
-        for (int dt = 0; dt < 16; ++dt) {
-          const u32x4 v = lds_read(v_at, dt);
+        for (int d = 0; d < 8; ++d) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const bf16x8 vf = dequant8(v[2 * k], v[2 * k + 1], vs);
+            const bf16x8 vf = dequant8(v[d][2 * k], v[d][2 * k + 1], vs);
 #pragma unroll
             for (int nt = 0; nt < NRT; ++nt)
-              acc[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, p[nt][k], acc[nt][dt], 0, 0, 0);
+              acc[nt][8 * n + d] =
+                  __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ph[nt][k], acc[nt][8 * n + d], 0, 0, 0);
+#pragma unroll
+            for (int nt = 0; nt < NRT; ++nt)
+              acc[nt][8 * n + d] =
+                  __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[nt][k], acc[nt][8 * n + d], 0, 0, 0);
           }
-          if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-        }
-        if (next) {
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          load_v(s + kWaves);
+          if (d % 2) __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
+  }
 
-    // The four waves' rows meet: all scaled to the common maximum, then waves 2 and 3 hand theirs
-    // to 0 and 1, and 1 to 0.
+  // The waves' rows meet: all scaled to the common maximum, DR dim tiles of every wave's O into LDS,
+  // where each wave sums its share over the waves and writes it: the partial of a split pair, else
+  // the output.
 #pragma unroll
-    for (int nt = 0; nt < NRT; ++nt) {
-      l_run[nt] = sum_over_groups(l_run[nt]);
-      if (G == 0) {
-        sm.m[w][16 * nt + i] = m_run[nt];
-        sm.l[w][16 * nt + i] = l_run[nt];
+  for (int nt = 0; nt < NRT; ++nt) {
+    l_run[nt] = sum_over_groups(l_run[nt]);
+    if (G == 0) {
+      sm.m[w][16 * nt + i] = m_run[nt];
+      sm.l[w][16 * nt + i] = l_run[nt];
+    }
+  }
+  __syncthreads();  // every wave is done with its ring, which O takes over
+  const size_t slot = (size_t)a.sstart[u] + h * parts + part;
+#pragma unroll
+  for (int nt = 0; nt < NRT; ++nt) {
+    float m = kNegBig, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) m = fmaxf(m, sm.m[k][16 * nt + i]);
+#pragma unroll
+    for (int k = 0; k < NW; ++k) l += exp2f(sm.m[k][16 * nt + i] - m) * sm.l[k][16 * nt + i];
+    const float f = exp2f(m_run[nt] - m);
+#pragma unroll
+    for (int d = 0; d < 16; ++d) acc[nt][d] *= f;
+    if (w == 0 && G == 0) {
+      const int r = 16 * nt + i;
+      sm.inv[r] = l != 0.f ? 1.0f / l : 0.f;
+      if (parts > 1) {
+        a.part_ml[(slot * R + r) * 2] = m;
+        a.part_ml[(slot * R + r) * 2 + 1] = l;
       }
     }
+  }
+  const unsigned o_at = npn::lds_addr(&sm.o[w][0][0][lane]), o_all = npn::lds_addr(&sm.o[0][0][0][lane]);
+#pragma unroll
+  for (int d0 = 0; d0 < 16; d0 += Smem::DR) {
+    if (d0 > 0) __syncthreads();  // the tiles before have been summed
+#pragma unroll
+    for (int nt = 0; nt < NRT; ++nt)
+#pragma unroll
+      for (int d = 0; d < Smem::DR; ++d)
+        lds_write(o_at, nt * Smem::DR + d, __builtin_bit_cast(u32x4, acc[nt][d0 + d]));
     __syncthreads();
-    float m_all[NRT], l_all[NRT];
+    for (int k = w; k < NRT * Smem::DR; k += NW) {
+      const int nt = k / Smem::DR, d = d0 + k % Smem::DR;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int nt = 0; nt < NRT; ++nt) {
-      float m = kNegBig, l = 0.f;
-#pragma unroll
-      for (int k = 0; k < kWaves; ++k) m = fmaxf(m, sm.m[k][16 * nt + i]);
-#pragma unroll
-      for (int k = 0; k < kWaves; ++k) l += exp2f(sm.m[k][16 * nt + i] - m) * sm.l[k][16 * nt + i];
-      m_all[nt] = m;
-      l_all[nt] = l;
-      const float f = exp2f(m_run[nt] - m);
-#pragma unroll
-      for (int dt = 0; dt < 16; ++dt) acc[nt][dt] *= f;
-    }
-    __syncthreads();  // every wave is done with its ring, which O takes over
-    auto put = [&](int k) {
-      const unsigned at = o_at + (unsigned)(k * sizeof(sm.o[0]));
-#pragma unroll
-      for (int nt = 0; nt < NRT; ++nt)
-#pragma unroll
-        for (int dt = 0; dt < 16; ++dt)
-          lds_write(at, nt * 16 + dt, __builtin_bit_cast(u32x4, acc[nt][dt]));
-    };
-    auto add = [&](int k) {
-      const unsigned at = o_at + (unsigned)(k * sizeof(sm.o[0]));
-#pragma unroll
-      for (int nt = 0; nt < NRT; ++nt)
-#pragma unroll
-        for (int dt = 0; dt < 16; ++dt) {
-          acc[nt][dt] += __builtin_bit_cast(f32x4, lds_read(at, nt * 16 + dt));
-          if (dt % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    if (w >= 2) put(w - 2);
-    __syncthreads();
-    if (w < 2) add(w);
-    if (w == 1) put(1);  // its own buffer, read by itself alone
-    __syncthreads();
-    if (w == 0) {
-      add(1);
-      const size_t slot = (size_t)blockIdx.x + pair;  // unique: a workgroup's pairs are consecutive
-#pragma unroll
-      for (int nt = 0; nt < NRT; ++nt) {
-        const int r = 16 * nt + i;
-        float* po = a.part_o + (slot * R + r) * DH;
-#pragma unroll
-        for (int dt = 0; dt < 16; ++dt) *reinterpret_cast<f32x4*>(po + 16 * dt + 4 * G) = acc[nt][dt];
-        if (G == 0) {
-          a.part_ml[(slot * R + r) * 2] = m_all[nt];
-          a.part_ml[(slot * R + r) * 2 + 1] = l_all[nt];
-        }
-      }
-    }
-
-    x += steps;
-    if (x - ubeg >= un.steps * a.Hkv && x < x_end) {
-      do {
-        ubeg += un.steps * a.Hkv;
-        un = unit_of(a, ++u);
-      } while (un.steps == 0);  // ends: a step of a later unit is in this range
+      for (int v = 0; v < NW; ++v)
+        o += __builtin_bit_cast(f32x4, lds_read(o_all + k * 1024, v * NRT * Smem::DR));
+      o += o * 0.0f;  // infinite: NaN
+      const int r = 16 * nt + i;
+      if (parts > 1)
+        *reinterpret_cast<f32x4*>(a.part_o + (slot * R + r) * DH + 16 * d + 4 * G) = o;
+      else if (r < rows)
+        write_out(a, un.b, row0 + r, h, 16 * d + 4 * G, o, sm.inv[r]);
     }
   }
 }
 
-// One wave per (row of a pair): the segments' (m, l, O) merged in segment order.
+// ---- 3. merge ---------------------------------------------------------------------------------------
+// The workgroups' (m, l, O) of a row of a pair, WPR waves to a row: wave q takes parts q, q + WPR, ...,
+// four loads of each at a time, and the first wave merges the waves'. One wave a row where pairs
+// have few parts, four where one pair has most of the chip (25 us for one sequence of 32768 keys
+// with one wave walking its 64 parts a load at a time).
+template <int WPR>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
-  const int q = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int r = blockIdx.x * 4 + q;
+  const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int q = wv % WPR;
+  const int r = blockIdx.x * (4 / WPR) + wv / WPR;
   const int pair = blockIdx.y;
   const int u = pair / a.Hkv, h = pair - u * a.Hkv;
+  const int parts = (a.wstart[u + 1] - a.wstart[u]) / a.Hkv;
+  if (parts == 1) return;  // written by its workgroup
   const int b = u / a.RG;
   const int row = (u - b * a.RG) * a.R + r;
-  if (r >= a.R || row >= a.T * a.grp) return;
-  const int t = row / a.grp, qh = h * a.grp + row - t * a.grp;
-  const size_t oi = (((size_t)b * a.T + t) * a.Hq + qh) * DH + 4 * lane;
-  const int U = a.B * a.RG;
-  const int S = a.ustart[U], W = a.ustart[U + 1];
-  const int ub = a.ustart[u], steps = (a.ustart[u + 1] - ub) / a.Hkv;
+  if (row >= a.T * a.grp) return;  // the whole workgroup where WPR = 4; no barrier where WPR = 1
+  const size_t slot = (size_t)a.sstart[u] + h * parts;
   float m = kNegBig, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  if (steps > 0 && t < a.q_len[b]) {
-    const int x0 = ub + h * steps, x1 = x0 + steps - 1;
-    const int w0 = (int)(((int64_t)(x0 + 1) * W - 1) / S);
-    const int w1 = (int)(((int64_t)(x1 + 1) * W - 1) / S);
-    for (int w = w0; w <= w1; ++w) {
-      const size_t at = ((size_t)w + pair) * a.R + r;
-      const float mv = a.part_ml[2 * at], lv = a.part_ml[2 * at + 1];
-      const f32x4 ov = *reinterpret_cast<const f32x4*>(a.part_o + at * DH + 4 * lane);
-      const float mn = fmaxf(m, mv);
-      const float f0 = exp2f(m - mn), f1 = exp2f(mv - mn);
-      m = mn;
-      l = l * f0 + lv * f1;
-      o = o * f0 + ov * f1;
+  for (int k = q; k < parts; k += 4 * WPR) {
+    float mv[4], lv[4];
+    f32x4 ov[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool ok = k + j * WPR < parts;
+      const size_t at = (slot + k + j * WPR) * a.R + r;
+      mv[j] = ok ? a.part_ml[2 * at] : kNegBig;
+      lv[j] = ok ? a.part_ml[2 * at + 1] : 0.f;
+      ov[j] = ok ? *reinterpret_cast<const f32x4*>(a.part_o + at * DH + 4 * lane)
+                 : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const float mn = fmaxf(fmaxf(fmaxf(m, mv[0]), fmaxf(mv[1], mv[2])), mv[3]);
+    const float f = exp2f(m - mn);
+    l *= f;
+    o *= f;
+    m = mn;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float fj = exp2f(mv[j] - mn);
+      l += lv[j] * fj;
+      o += ov[j] * fj;
     }
   }
-  const float inv = l != 0.f ? 1.0f / l : 0.f;  // a row without keys (pages that are none) is 0
-  const uint2 g = *reinterpret_cast<const uint2*>(a.gate + oi);
-  const uint32_t gw[2] = {g.x, g.y};
-  uint32_t y[2];
+  if constexpr (WPR > 1) {
+    __shared__ float s_m[WPR], s_l[WPR];
+    __shared__ f32x4 s_o[WPR][64];
+    if (lane == 0) {
+      s_m[q] = m;
+      s_l[q] = l;
+    }
+    s_o[q][lane] = o;
+    __syncthreads();
+    if (q != 0) return;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    float v0 = o[2 * j] * inv * npn::sigmoid(npn::bf16lo(gw[j]));
-    float v1 = o[2 * j + 1] * inv * npn::sigmoid(npn::bf16hi(gw[j]));
-    if (l == 0.f) v0 = v1 = 0.f;  // whatever the gate
-    y[j] = npn::f32_to_bf16(v0) | ((uint32_t)npn::f32_to_bf16(v1) << 16);
+    for (int k = 1; k < WPR; ++k) {
+      const float mn = fmaxf(m, s_m[k]);
+      const float f0 = exp2f(m - mn), f1 = exp2f(s_m[k] - mn);
+      m = mn;
+      l = l * f0 + s_l[k] * f1;
+      o = o * f0 + s_o[k][lane] * f1;
+    }
   }
-  *reinterpret_cast<uint2*>(a.out + oi) = make_uint2(y[0], y[1]);
+  write_out(a, b, row, h, 4 * lane, o, l != 0.f ? 1.0f / l : 0.f);
 }
 
 struct PagedPlan {
   bool ok;
-  int grp, R, RG, pairs;
-  size_t o_ml, o_us, bytes;  // part_o first
+  int grp, R, RG, pairs, grid, nw;
+  size_t o_qs, o_po, o_ml, o_ws, o_ss, bytes;  // q first
 };
 
 PagedPlan paged_plan(int B, int T, int q_heads, int kv_heads, int max_blocks, int block_size) {
@@ -646,13 +869,19 @@ PagedPlan paged_plan(int B, int T, int q_heads, int kv_heads, int max_blocks, in
   p.RG = (int)((rows + p.R - 1) / p.R);
   const int64_t pairs = (int64_t)B * p.RG * kv_heads;
   const int64_t keys = (int64_t)max_blocks * block_size;
-  if (pairs > 65535 || pairs * ((keys + KS - 1) / KS) >= (int64_t)1 << 31) return p;
+  if (pairs > 65535 || pairs * ((keys + KS - 1) / KS) >= (int64_t)1 << 30) return p;
   p.pairs = (int)pairs;
-  const size_t slots = (size_t)kMaxWG + p.pairs;
+  p.nw = p.R == 16 ? 8 : 4;
+  p.grid = most_workgroups(p.pairs);
+  const size_t slots = pairs <= 192 ? 256 : kSlots;
+  const size_t units = (size_t)B * p.RG;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  p.o_ml = up(slots * p.R * DH * sizeof(float));
-  p.o_us = p.o_ml + up(slots * p.R * 2 * sizeof(float));
-  p.bytes = p.o_us + up(((size_t)B * p.RG + 2) * sizeof(int32_t));
+  p.o_qs = up((size_t)pairs * p.R * DH * 2);
+  p.o_po = p.o_qs + up((size_t)pairs * p.R * sizeof(float));
+  p.o_ml = p.o_po + up(slots * p.R * DH * sizeof(float));
+  p.o_ws = p.o_ml + up(slots * p.R * 2 * sizeof(float));
+  p.o_ss = p.o_ws + up((units + 1) * sizeof(int32_t));
+  p.bytes = p.o_ss + up(units * sizeof(int32_t));
   p.ok = true;
   return p;
 }
@@ -684,17 +913,24 @@ extern "C" int npn_gqa_tail_verify_paged(
   const PagedArgs a{query, gate, q_norm, cos_table, sin_table,
                     reinterpret_cast<const uint8_t*>(cache_k),
                     reinterpret_cast<const uint8_t*>(cache_v), k_scale, v_scale, block_table,
-                    kv_len, q_len, out, reinterpret_cast<float*>(ws),
-                    reinterpret_cast<float*>(ws + p.o_ml), reinterpret_cast<int32_t*>(ws + p.o_us),
-                    positions, B, T, q_heads, kv_heads, p.grp, p.R, p.RG, max_blocks, n_blocks, sh, 4};
+                    kv_len, q_len, out, reinterpret_cast<u32x4*>(ws),
+                    reinterpret_cast<float*>(ws + p.o_qs), reinterpret_cast<float*>(ws + p.o_po),
+                    reinterpret_cast<float*>(ws + p.o_ml), reinterpret_cast<int32_t*>(ws + p.o_ws),
+                    reinterpret_cast<int32_t*>(ws + p.o_ss), positions, B, T, q_heads, kv_heads, p.grp,
+                    p.R, p.RG, max_blocks, n_blocks, sh, p.nw, (1ull << 32) / p.grp + 1};
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int nrt = p.R / 16;
+  hipLaunchKernelGGL(paged_prep_kernel, dim3(1 + (p.pairs * nrt * 16 + kPrepWaves - 1) / kPrepWaves),
+                     dim3(kPrepWaves * 64), 0, s, a);
   if (nrt == 1)
-    hipLaunchKernelGGL(paged_attn_kernel<1>, dim3(kMaxWG), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_attn_kernel<1, 8>), dim3(p.grid), dim3(512), 0, s, a);
   else if (nrt == 2)
-    hipLaunchKernelGGL(paged_attn_kernel<2>, dim3(kMaxWG), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_attn_kernel<2, 4>), dim3(p.grid), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL(paged_attn_kernel<3>, dim3(kMaxWG), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(paged_merge_kernel, dim3(p.R / 4, p.pairs), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((paged_attn_kernel<3, 4>), dim3(p.grid), dim3(256), 0, s, a);
+  if (p.pairs < 32)
+    hipLaunchKernelGGL(paged_merge_kernel<4>, dim3(p.R, p.pairs), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(paged_merge_kernel<1>, dim3(p.R / 4, p.pairs), dim3(256), 0, s, a);
   return npn_launch_status();
 }
