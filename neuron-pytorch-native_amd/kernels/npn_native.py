@@ -116,6 +116,46 @@ def call(name, *args):
         raise RuntimeError(f"{name} failed with status {status}: {text}")
 
 
+def register(qualname, schema, fake):
+    """Decorator: registers the function as torch.ops.<qualname> for HIP tensors with `schema` and
+    the shape propagation `fake`. Like torch.library.custom_op, minus its autograd wrapper, which
+    costs 8 us a call: more than these ops' kernels take at their smallest sizes."""
+    def wrap(fn):
+        torch.library.define(qualname, schema)
+        torch.library.impl(qualname, "cuda", fn)
+        torch.library.register_fake(qualname, fake)
+        return fn
+    return wrap
+
+
+def check_all(dev, *specs):
+    """specs: (tensor, name, dtype, shape, or a number of elements in any shape). `require` for all
+    of them, and that they are on `dev`."""
+    for t, name, dtype, shape in specs:
+        if isinstance(shape, int):
+            ok = t.numel() == shape
+        else:
+            ok = t.shape == shape
+        if not (ok and t.dtype == dtype and t.device == dev and t.is_contiguous()):
+            require(t, name, dtype, **({"numel": shape} if isinstance(shape, int) else {"shape": shape}))
+            raise RuntimeError(f"{name} must be on {dev}, got {t.device}")
+
+
+def launch(dev, name, *args):
+    """`call` of an entry point that ends with a stream, on dev's current stream and with dev as the
+    current device; the tensors' devices have been checked."""
+    raw = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    fn = getattr(lib(), name)
+    if dev.index == torch.cuda.current_device():
+        status = fn(*raw, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*raw, torch._C._cuda_getCurrentRawStream(dev.index))
+    if status != 0:
+        text = lib().npn_status_string(status).decode()
+        raise RuntimeError(f"{name} failed with status {status}: {text}")
+
+
 def query(name, *args):
     """Call a size-query entry point and return its value."""
     return int(getattr(lib(), name)(*args))

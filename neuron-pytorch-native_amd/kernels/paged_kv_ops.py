@@ -26,142 +26,111 @@ include/npn_spec_verify.h has the details and limits.
 """
 import torch
 
-from npn_native import call, query as size_query, require, stream_of
+from npn_native import check_all, launch, query as size_query, register
 
 HEAD_DIM = 256
 ROPE_DIM = 64
 BLOCK_SIZES = (16, 32, 64, 128)
+I32, I64, I8, F32, BF16 = torch.int32, torch.int64, torch.int8, torch.float32, torch.bfloat16
 
 
-def _require_cache(cache_k, cache_v, k_scale, v_scale):
-    """Checks the four cache tensors; returns (N, Hkv, block size)."""
+def _cache_sizes(cache_k):
+    """(N, Hkv, block size) of a cache's keys."""
     if cache_k.dim() != 4:
         raise RuntimeError(f"cache_k must be [N, Hkv, bs, {HEAD_DIM}], got {tuple(cache_k.shape)}")
     n, hkv, bs, _ = cache_k.shape
     if bs not in BLOCK_SIZES:
         raise RuntimeError(f"block size must be one of {BLOCK_SIZES}, got {bs}")
-    require(cache_k, "cache_k", torch.int8, shape=(n, hkv, bs, HEAD_DIM))
-    require(cache_v, "cache_v", torch.int8, shape=(n, hkv, HEAD_DIM, bs))
-    require(k_scale, "k_scale", torch.float32, shape=(n, hkv))
-    require(v_scale, "v_scale", torch.float32, shape=(n, hkv))
     return n, hkv, bs
 
 
-@torch.library.custom_op("paged::update_blocks_", device_types="cuda",
-                         mutates_args=("block_table", "num_blocks", "free_blocks", "free_count"))
-def update_blocks_(
-    kv_len: torch.Tensor,       # [B] int32
-    new_len: torch.Tensor,      # [B] int32
-    block_table: torch.Tensor,  # [B, P] int32 (in place)
-    num_blocks: torch.Tensor,   # [B] int32 (in place)
-    free_blocks: torch.Tensor,  # [N] int32 (in place)
-    free_count: torch.Tensor,   # [1] int32 (in place)
-    block_size: int,
-    T: int,
-) -> tuple[torch.Tensor, torch.Tensor]:
+def _dims(t, name, n):
+    if t.dim() != n:
+        raise RuntimeError(f"{name} must have {n} dimensions, got {tuple(t.shape)}")
+    return t.shape
+
+
+def _update_blocks_fake(kv_len, new_len, block_table, num_blocks, free_blocks, free_count,
+                        block_size, T):
+    B = block_table.shape[0]
+    return kv_len.new_empty((B, T), dtype=I64), kv_len.new_empty((B,))
+
+
+@register("paged::update_blocks_",
+          "(Tensor kv_len, Tensor new_len, Tensor(a!) block_table, Tensor(b!) num_blocks, "
+          "Tensor(c!) free_blocks, Tensor(d!) free_count, int block_size, int T) "
+          "-> (Tensor, Tensor)", _update_blocks_fake)
+def update_blocks_(kv_len, new_len, block_table, num_blocks, free_blocks, free_count, block_size, T):
     if block_size not in BLOCK_SIZES:
         raise RuntimeError(f"block size must be one of {BLOCK_SIZES}, got {block_size}")
     if T < 1:
         raise RuntimeError(f"T must be at least 1, got {T}")
-    B, P = block_table.shape
+    B, P = _dims(block_table, "block_table", 2)
     n = free_blocks.numel()
-    require(kv_len, "kv_len", torch.int32, numel=B)
-    require(new_len, "new_len", torch.int32, numel=B)
-    require(block_table, "block_table", torch.int32)
-    require(num_blocks, "num_blocks", torch.int32, numel=B)
-    require(free_blocks, "free_blocks", torch.int32)
-    require(free_count, "free_count", torch.int32, numel=1)
-    slots = torch.empty((B, T), dtype=torch.int64, device=kv_len.device)
-    granted = torch.empty(B, dtype=torch.int32, device=kv_len.device)
-    with torch.cuda.device(kv_len.device):
-        call("npn_paged_update_blocks", kv_len, new_len, block_table, num_blocks, free_blocks,
-             free_count, slots, granted, B, P, n, block_size, T, stream_of(kv_len))
+    dev = kv_len.device
+    check_all(dev, (kv_len, "kv_len", I32, B), (new_len, "new_len", I32, B),
+              (block_table, "block_table", I32, (B, P)), (num_blocks, "num_blocks", I32, B),
+              (free_blocks, "free_blocks", I32, n), (free_count, "free_count", I32, 1))
+    slots = torch.empty((B, T), dtype=I64, device=dev)
+    granted = torch.empty(B, dtype=I32, device=dev)
+    launch(dev, "npn_paged_update_blocks", kv_len, new_len, block_table, num_blocks, free_blocks,
+           free_count, slots, granted, B, P, n, block_size, T)
     return slots, granted
 
 
-@update_blocks_.register_fake
-def _(kv_len, new_len, block_table, num_blocks, free_blocks, free_count, block_size, T):
-    B = block_table.shape[0]
-    return (kv_len.new_empty((B, T), dtype=torch.int64), kv_len.new_empty((B,)))
-
-
-@torch.library.custom_op("gqa::kv_append_paged", device_types="cuda",
-                         mutates_args=("cache_k", "cache_v", "k_scale", "v_scale"))
-def kv_append_paged(
-    key: torch.Tensor,        # [B, T, Hkv, 256] bf16 (k projection, pre-norm)
-    value: torch.Tensor,      # [B, T, Hkv, 256] bf16
-    k_norm: torch.Tensor,     # [256] f32
-    cos_table: torch.Tensor,  # [positions, 64] f32
-    sin_table: torch.Tensor,  # [positions, 64] f32
-    kv_len: torch.Tensor,     # [B] int32
-    slots: torch.Tensor,      # [B, T] int64
-    cache_k: torch.Tensor,    # [N, Hkv, bs, 256] int8 (in place)
-    cache_v: torch.Tensor,    # [N, Hkv, 256, bs] int8 (in place)
-    k_scale: torch.Tensor,    # [N, Hkv] f32 (in place)
-    v_scale: torch.Tensor,    # [N, Hkv] f32 (in place)
-) -> None:
-    n, hkv, bs = _require_cache(cache_k, cache_v, k_scale, v_scale)
-    B, T = slots.shape
-    positions = cos_table.shape[0]
-    require(key, "key", torch.bfloat16, shape=(B, T, hkv, HEAD_DIM))
-    require(value, "value", torch.bfloat16, shape=(B, T, hkv, HEAD_DIM))
-    require(k_norm, "k_norm", torch.float32, numel=HEAD_DIM)
-    require(cos_table, "cos_table", torch.float32, shape=(positions, ROPE_DIM))
-    require(sin_table, "sin_table", torch.float32, shape=(positions, ROPE_DIM))
-    require(kv_len, "kv_len", torch.int32, numel=B)
-    require(slots, "slots", torch.int64)
-    with torch.cuda.device(key.device):
-        call("npn_gqa_kv_append_paged", key, value, k_norm, cos_table, sin_table, positions,
-             kv_len, slots, cache_k, cache_v, k_scale, v_scale, B, T, hkv, n, bs, stream_of(key))
-
-
-@kv_append_paged.register_fake
-def _(key, value, k_norm, cos_table, sin_table, kv_len, slots, cache_k, cache_v, k_scale, v_scale):
+def _kv_append_fake(key, value, k_norm, cos_table, sin_table, kv_len, slots, cache_k, cache_v,
+                    k_scale, v_scale):
     return None
 
 
-@torch.library.custom_op("gqa::tail_verify_paged", mutates_args=(), device_types="cuda")
-def tail_verify_paged(
-    query: torch.Tensor,        # [B, T, Hq, 256] bf16
-    gate: torch.Tensor,         # [B, T, Hq, 256] bf16
-    q_norm: torch.Tensor,       # [256] f32
-    cos_table: torch.Tensor,    # [positions, 64] f32
-    sin_table: torch.Tensor,    # [positions, 64] f32
-    cache_k: torch.Tensor,      # [N, Hkv, bs, 256] int8
-    cache_v: torch.Tensor,      # [N, Hkv, 256, bs] int8
-    k_scale: torch.Tensor,      # [N, Hkv] f32
-    v_scale: torch.Tensor,      # [N, Hkv] f32
-    block_table: torch.Tensor,  # [B, P] int32
-    kv_len: torch.Tensor,       # [B] int32
-    q_len: torch.Tensor,        # [B] int32
-) -> torch.Tensor:
-    n, hkv, bs = _require_cache(cache_k, cache_v, k_scale, v_scale)
-    B, T, hq, dh = query.shape
-    if dh != HEAD_DIM:
-        raise RuntimeError(f"head dim must be {HEAD_DIM}")
-    P, positions = block_table.shape[-1], cos_table.shape[0]
-    require(query, "query", torch.bfloat16)
-    require(gate, "gate", torch.bfloat16, shape=query.shape)
-    require(q_norm, "q_norm", torch.float32, numel=HEAD_DIM)
-    require(cos_table, "cos_table", torch.float32, shape=(positions, ROPE_DIM))
-    require(sin_table, "sin_table", torch.float32, shape=(positions, ROPE_DIM))
-    require(block_table, "block_table", torch.int32, shape=(B, P))
-    require(kv_len, "kv_len", torch.int32, numel=B)
-    require(q_len, "q_len", torch.int32, numel=B)
+@register("gqa::kv_append_paged",
+          "(Tensor key, Tensor value, Tensor k_norm, Tensor cos_table, Tensor sin_table, "
+          "Tensor kv_len, Tensor slots, Tensor(a!) cache_k, Tensor(b!) cache_v, "
+          "Tensor(c!) k_scale, Tensor(d!) v_scale) -> ()", _kv_append_fake)
+def kv_append_paged(key, value, k_norm, cos_table, sin_table, kv_len, slots, cache_k, cache_v,
+                    k_scale, v_scale):
+    n, hkv, bs = _cache_sizes(cache_k)
+    B, T = _dims(slots, "slots", 2)
+    positions = cos_table.shape[0]
+    dev, row, table = key.device, (B, T, hkv, HEAD_DIM), (positions, ROPE_DIM)
+    check_all(dev, (key, "key", BF16, row), (value, "value", BF16, row),
+              (k_norm, "k_norm", F32, HEAD_DIM), (cos_table, "cos_table", F32, table),
+              (sin_table, "sin_table", F32, table), (kv_len, "kv_len", I32, B),
+              (slots, "slots", I64, (B, T)), (cache_k, "cache_k", I8, (n, hkv, bs, HEAD_DIM)),
+              (cache_v, "cache_v", I8, (n, hkv, HEAD_DIM, bs)), (k_scale, "k_scale", F32, (n, hkv)),
+              (v_scale, "v_scale", F32, (n, hkv)))
+    launch(dev, "npn_gqa_kv_append_paged", key, value, k_norm, cos_table, sin_table, positions,
+           kv_len, slots, cache_k, cache_v, k_scale, v_scale, B, T, hkv, n, bs)
+
+
+def _tail_verify_fake(query, gate, q_norm, cos_table, sin_table, cache_k, cache_v, k_scale, v_scale,
+                      block_table, kv_len, q_len):
+    return torch.empty_like(query)
+
+
+@register("gqa::tail_verify_paged",
+          "(Tensor query, Tensor gate, Tensor q_norm, Tensor cos_table, Tensor sin_table, "
+          "Tensor cache_k, Tensor cache_v, Tensor k_scale, Tensor v_scale, Tensor block_table, "
+          "Tensor kv_len, Tensor q_len) -> Tensor", _tail_verify_fake)
+def tail_verify_paged(query, gate, q_norm, cos_table, sin_table, cache_k, cache_v, k_scale, v_scale,
+                      block_table, kv_len, q_len):
+    n, hkv, bs = _cache_sizes(cache_k)
+    B, T, hq, _ = _dims(query, "query", 4)
+    P, positions = _dims(block_table, "block_table", 2)[1], cos_table.shape[0]
+    dev, row, table = query.device, (B, T, hq, HEAD_DIM), (positions, ROPE_DIM)
+    check_all(dev, (query, "query", BF16, row), (gate, "gate", BF16, row),
+              (q_norm, "q_norm", F32, HEAD_DIM), (cos_table, "cos_table", F32, table),
+              (sin_table, "sin_table", F32, table), (cache_k, "cache_k", I8, (n, hkv, bs, HEAD_DIM)),
+              (cache_v, "cache_v", I8, (n, hkv, HEAD_DIM, bs)), (k_scale, "k_scale", F32, (n, hkv)),
+              (v_scale, "v_scale", F32, (n, hkv)), (block_table, "block_table", I32, (B, P)),
+              (kv_len, "kv_len", I32, B), (q_len, "q_len", I32, B))
     n_ws = size_query("npn_gqa_tail_verify_paged_workspace_size", B, T, hq, hkv, P, bs)
     if n_ws == 0:
         raise RuntimeError(f"unsupported tail_verify_paged sizes B={B} T={T} Hq={hq} Hkv={hkv} "
                            f"P={P} bs={bs}")
-    ws = torch.empty(n_ws, dtype=torch.uint8, device=query.device)
+    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
     out = torch.empty_like(query)
-    with torch.cuda.device(query.device):
-        call("npn_gqa_tail_verify_paged", query, gate, q_norm, cos_table, sin_table, positions,
-             cache_k, cache_v, k_scale, v_scale, block_table, kv_len, q_len, out, B, T, hq, hkv, n,
-             P, bs, ws, n_ws, stream_of(query))
+    launch(dev, "npn_gqa_tail_verify_paged", query, gate, q_norm, cos_table, sin_table, positions,
+           cache_k, cache_v, k_scale, v_scale, block_table, kv_len, q_len, out, B, T, hq, hkv, n, P,
+           bs, ws, n_ws)
     return out
-
-
-@tail_verify_paged.register_fake
-def _(query, gate, q_norm, cos_table, sin_table, cache_k, cache_v, k_scale, v_scale, block_table,
-      kv_len, q_len):
-    return torch.empty_like(query)

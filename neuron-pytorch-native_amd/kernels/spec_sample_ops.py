@@ -14,33 +14,27 @@ ids in every run and whatever else shares the batch.
 """
 import torch
 
-from npn_native import call, require, stream_of
+from npn_native import check_all, launch, register
+
+I32, F32 = torch.int32, torch.float32
 
 
-@torch.library.custom_op("spec::sample", mutates_args=(), device_types="cuda")
-def sample(
-    logits: torch.Tensor,       # [R, V] f32 or bf16
-    temperature: torch.Tensor,  # [R] f32
-    top_k: torch.Tensor,        # [R] int32
-    top_p: torch.Tensor,        # [R] f32
-    min_p: torch.Tensor,        # [R] f32
-    u: torch.Tensor,            # [R] f32
-) -> torch.Tensor:
+def _sample_fake(logits, temperature, top_k, top_p, min_p, u):
+    return logits.new_empty((logits.shape[0],), dtype=torch.int64)
+
+
+@register("spec::sample",
+          "(Tensor logits, Tensor temperature, Tensor top_k, Tensor top_p, Tensor min_p, Tensor u) "
+          "-> Tensor", _sample_fake)
+def sample(logits, temperature, top_k, top_p, min_p, u):
+    if logits.dim() != 2:
+        raise RuntimeError(f"logits must be [R, V], got {tuple(logits.shape)}")
     R, V = logits.shape
     bf16 = logits.dtype == torch.bfloat16
-    require(logits, "logits", torch.bfloat16 if bf16 else torch.float32)
-    require(temperature, "temperature", torch.float32, numel=R)
-    require(top_k, "top_k", torch.int32, numel=R)
-    require(top_p, "top_p", torch.float32, numel=R)
-    require(min_p, "min_p", torch.float32, numel=R)
-    require(u, "u", torch.float32, numel=R)
-    ids = torch.empty(R, dtype=torch.int64, device=logits.device)
-    with torch.cuda.device(logits.device):
-        call("npn_sample", logits, int(bf16), temperature, top_k, top_p, min_p, u, ids, R, V,
-             stream_of(logits))
+    dev = logits.device
+    check_all(dev, (logits, "logits", torch.bfloat16 if bf16 else F32, (R, V)),
+              (temperature, "temperature", F32, R), (top_k, "top_k", I32, R),
+              (top_p, "top_p", F32, R), (min_p, "min_p", F32, R), (u, "u", F32, R))
+    ids = torch.empty(R, dtype=torch.int64, device=dev)
+    launch(dev, "npn_sample", logits, int(bf16), temperature, top_k, top_p, min_p, u, ids, R, V)
     return ids
-
-
-@sample.register_fake
-def _(logits, temperature, top_k, top_p, min_p, u):
-    return logits.new_empty((logits.shape[0],), dtype=torch.int64)
