@@ -588,10 +588,12 @@ int npn_deltanet_rollback_commit(const uint16_t* const* mixed_qkv, uint16_t* con
  * rank. NaN logits count as -infinity, which is never kept; if the maximum is +infinity those at
  * +infinity share all the weight. A row without a token above -infinity gives -1.
  * Weights are integers round(w 2^42) and their sums exact: the same inputs give the same ids,
- * and weights under 2^-43 of the largest count as 0. 1 <= V <= 2^20. */
+ * and weights under 2^-43 of the largest count as 0. 1 <= R <= 65535, 1 <= V <= 2^20; the
+ * workspace has npn_sample_workspace_size(R, V) bytes (0: unsupported sizes). */
+size_t npn_sample_workspace_size(int R, int V);
 int npn_sample(const void* logits, int bf16, const float* temperature, const int32_t* top_k,
                const float* top_p, const float* min_p, const float* u, int64_t* ids, int R, int V,
-               void* stream);
+               void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -15,6 +15,17 @@
 // most 2^62), so sums are exact whatever their order and every run gives the same token; tokens that
 // round to 0 (w < 2^-43) have no part in it. 32-bit exponentials would not do: the ranks' borders in
 // a flat row of 150000 tokens lie 10^-5 of the sum apart or less.
+//
+// Four launches, C workgroups to a row in the first three:
+//  1. max: the row's maximum (and its first index, for greedy rows) and least finite logit.
+//  2. histogram over 2048 bins of equal width in (m - l) / T: counts where a top-k of at most kCap
+//     applies (no exponentials are needed then), else weights, whose running sums say to within a bin
+//     where the top-p prefix ends, where min-p cuts and between which bins the sample must lie.
+//  3. collect: the tokens of the bins in question (all down to the k-th's bin, or the few bins of the
+//     borders) go into a list of at most kCap.
+//  4. finish: one workgroup sorts the list by rank, and with the bins' sums before each the three
+//     ranks are exact. A row whose list is too long (thousands of equal logits), or a longer top-k, is
+//     searched by the digits of its keys instead, which reads it some ten times.
 #include "npn_common.h"
 
 namespace {
@@ -22,8 +33,10 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 constexpr double kOne = 4398046511104.0;  // 2^42
-constexpr int kDigit = 11;                // bits of a key per level of the search
+constexpr int kDigit = 11;                // bits of a key per level of the search by digits
 constexpr int kBins = 1 << kDigit;
+constexpr int kCap = 4096;                // list entries per row
+constexpr float kMaxExp = 43.0f;          // weights below 2^-43 of the largest round to 0
 
 struct SampleArgs {
   const uint8_t* logits;  // [R][V] f32 or bf16
@@ -33,7 +46,13 @@ struct SampleArgs {
   const float* min_p;
   const float* u;
   int64_t* ids;
-  int R, V;
+  int R, V, C;
+  float* cmax;      // [R][C] each chunk's maximum, its first index and its least finite logit
+  int32_t* cidx;
+  float* cmin;
+  uint64_t* hist;   // [R][kBins] counts or weights
+  int32_t* listed;  // [R] tokens that go on the list
+  uint64_t* list;   // [R][kCap] inverted key above index: ascending is rank order
 };
 
 // A row's logits in 16-byte groups at 16-byte aligned addresses (rows of odd length start anywhere):
@@ -82,17 +101,58 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float(key ^ ((uint32_t)(~(int)key >> 31) | 0x80000000u));
 }
 
-// exp((x - m) / T), 0 for -inf; in a row with m = +inf those at +inf share it all.
+// 2^y for y in [-44, 0], to 2^-49 relative: 2^(j/16) from the table by y's nearest sixteenth, times
+// the series of e^r, |r| <= ln(2)/32, to r^7/5040 (the next term is under 2^-59).
+__device__ __forceinline__ double exp2_neg(double y, const double* table) {
+  const double t = rint(y * 16.0);
+  const int n = (int)t;
+  const double r = (y - t * 0.0625) * 0.69314718055994530942;
+  double p = fma(r, 1.0 / 5040, 1.0 / 720);
+  p = fma(r, p, 1.0 / 120);
+  p = fma(r, p, 1.0 / 24);
+  p = fma(r, p, 1.0 / 6);
+  p = fma(r, p, 0.5);
+  p = fma(r, p, 1.0);
+  p = fma(r, p, 1.0);
+  return ldexp(p * table[n & 15], n >> 4);
+}
+
+// 2^((x - m) log2(e) / T), 0 for -inf; in a row with m = +inf those at +inf share it all. y(x), in
+// base 2 and never above 0, also gives the bin: equal logits share one, larger ones never lie in a
+// later one.
 struct Weigh {
   float m;
-  double inv;
-  __device__ __forceinline__ double real(float x) const {
-    if (x == m) return 1.0;
-    if (x == -INFINITY || m == INFINITY) return 0.0;
-    return exp(((double)x - (double)m) * inv);
+  double c;             // log2(e) / T
+  double scale;         // bins per unit of -y
+  const double* table;  // 2^(j/16)
+  __device__ __forceinline__ bool in(float x) const {
+    return x == m || (x != -INFINITY && m != INFINITY);
   }
-  __device__ __forceinline__ uint64_t fixed(float x) const { return (uint64_t)rint(real(x) * kOne); }
+  __device__ __forceinline__ double y(float x) const {
+    return x == m ? 0.0 : ((double)x - (double)m) * c;
+  }
+  __device__ __forceinline__ double real(float x) const {
+    if (!in(x)) return 0.0;
+    const double e = y(x);
+    return e < -44.0 ? 0.0 : exp2_neg(e, table);
+  }
+  // round(w 2^42): the sum with 2^52 has the integer in its low bits.
+  __device__ __forceinline__ uint64_t fixed(float x) const {
+    return (uint64_t)__double_as_longlong(real(x) * kOne + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+  }
+  __device__ __forceinline__ int bin(float x) const { return min(kBins - 1, (int)(-y(x) * scale)); }
 };
+
+__device__ __forceinline__ void fill_table(double* table) {
+  if (threadIdx.x < 16) table[threadIdx.x] = exp2(threadIdx.x * 0.0625);
+}
+
+// Whether the row's top-k goes by counts.
+__device__ __forceinline__ bool counts_row(const SampleArgs& a, int k) {
+  return k > 0 && k < a.V && k <= kCap;
+}
+// A longer one needs counts and weights both: such a row is searched by digits from the start.
+__device__ __forceinline__ bool digits_row(const SampleArgs& a, int k) { return k > kCap && k < a.V; }
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
   return ((uint64_t)(uint32_t)__shfl_up((int)(v >> 32), d, 64) << 32) |
@@ -246,19 +306,72 @@ struct RowSearch {
     __syncthreads();
     return (int)sm.found[3];
   }
+
+  // The row's token: top-k, top-p, min-p (as given) and a cleaned u.
+  __device__ int sample(int k, float p, float min_p, float u) const {
+    histogram(0, 0);
+    uint64_t count, mass;
+    scan64((uint64_t)sm.count[2 * threadIdx.x] + sm.count[2 * threadIdx.x + 1], sm.wave, count);
+    scan64(sm.mass[2 * threadIdx.x] + sm.mass[2 * threadIdx.x + 1], sm.wave, mass);
+    bool level0 = true;
+    if (k > 0 && (uint64_t)k < count) {
+      const auto f = find(true, (uint64_t)k, level0);
+      mass = f.mass + ((uint64_t)k - f.count) * weigh.fixed(logit_of(f.key));
+      level0 = false;
+    }
+    uint64_t kept = mass;
+    if (p < 1.0f) {
+      const uint64_t target = p > 0.0f ? max(ceil_mul(p, mass), (uint64_t)1) : 1;
+      const auto f = find(false, target, level0);
+      const uint64_t w = weigh.fixed(logit_of(f.key));
+      kept = min(kept, f.mass + (target - f.mass + w - 1) / w * w);
+      level0 = false;
+    }
+    if (min_p > 0.0f) {
+      const float mp = fminf(min_p, 1.0f);
+      uint64_t sum = 0;
+      for (int g = threadIdx.x; g < row.groups; g += kThreads) {
+        float x[Row<BF>::VE];
+        row.load(g, x);
+#pragma unroll
+        for (int j = 0; j < Row<BF>::VE; ++j)
+          if (weigh.real(x[j]) >= (double)mp) sum += weigh.fixed(x[j]);
+      }
+      uint64_t total;
+      scan64(sum, sm.wave, total);
+      kept = min(kept, total);
+    }
+    const uint64_t target = floor_mul(u, kept) + 1;
+    const auto f = find(false, target, level0);
+    const uint64_t w = weigh.fixed(logit_of(f.key));
+    return nth(f.key, (target - f.mass + w - 1) / w);
+  }
 };
 
+// ---- 1. max -----------------------------------------------------------------------------------------
+// The groups of chunk c of C.
 template <bool BF>
-__global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a) {
-  __shared__ RowSmem sm;
-  const int r = blockIdx.x;
+__device__ __forceinline__ void chunk_of(const Row<BF>& row, int c, int C, int& g0, int& g1) {
+  g0 = (int)((int64_t)row.groups * c / C);
+  g1 = (int)((int64_t)row.groups * (c + 1) / C);
+}
+
+template <bool BF>
+__global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a) {
+  __shared__ uint32_t s_key[kWaves];
+  __shared__ int s_idx[kWaves];
+  __shared__ float s_min[kWaves];
+  const int c = blockIdx.x, r = blockIdx.y;
   const Row<BF> row(a, r);
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-
-  // the maximum and its first index
+  int g0, g1;
+  chunk_of(row, c, a.C, g0, g1);
+  for (int b = c * kThreads + threadIdx.x; b < kBins; b += a.C * kThreads) a.hist[(size_t)r * kBins + b] = 0;
+  if (c == 0 && threadIdx.x == 0) a.listed[r] = 0;
   uint32_t key = 0;
   int idx = 0x7FFFFFFF;
-  for (int g = threadIdx.x; g < row.groups; g += kThreads) {
+  float low = INFINITY;
+  for (int g = g0 + threadIdx.x; g < g1; g += kThreads) {
     float x[Row<BF>::VE];
     row.load(g, x);
 #pragma unroll
@@ -268,6 +381,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a) {
         key = k;
         idx = row.first(g) + j;
       }
+      low = fminf(low, x[j] == -INFINITY ? INFINITY : x[j]);
     }
   }
 #pragma unroll
@@ -278,78 +392,392 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(SampleArgs a) {
       key = ok;
       idx = oi;
     }
+    low = fminf(low, __shfl_xor(low, off, 64));
   }
   if (lane == 0) {
-    sm.red_key[wv] = key;
-    sm.red_idx[wv] = idx;
+    s_key[wv] = key;
+    s_idx[wv] = idx;
+    s_min[wv] = low;
   }
   __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kWaves; ++k)
-    if (sm.red_key[k] > key || (sm.red_key[k] == key && sm.red_idx[k] < idx)) {
-      key = sm.red_key[k];
-      idx = sm.red_idx[k];
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < kWaves; ++k) {
+      if (s_key[k] > key || (s_key[k] == key && s_idx[k] < idx)) {
+        key = s_key[k];
+        idx = s_idx[k];
+      }
+      low = fminf(low, s_min[k]);
     }
-  const float m = logit_of(key), T = a.temperature[r];
-  if (m == -INFINITY || !(T > 0.0f)) {  // nothing to sample, or greedy
-    if (threadIdx.x == 0) a.ids[r] = m == -INFINITY ? -1 : idx;
+    a.cmax[(size_t)r * a.C + c] = key == 0 ? -INFINITY : logit_of(key);
+    a.cidx[(size_t)r * a.C + c] = idx;
+    a.cmin[(size_t)r * a.C + c] = low;
+  }
+}
+
+// What the later launches know of a row; false: its token is known (a.ids is written by thread 0 of
+// the workgroup with `write`).
+struct RowInfo {
+  float m, T;
+  int k;
+  Weigh weigh;
+};
+__device__ __forceinline__ bool row_info(const SampleArgs& a, int r, const double* table, RowInfo& o, bool write) {
+  float m = -INFINITY, low = INFINITY;
+  int idx = 0x7FFFFFFF;
+  for (int c = 0; c < a.C; ++c) {  // ascending, so the first of equal maxima stays
+    const float v = a.cmax[(size_t)r * a.C + c];
+    if (v > m) {
+      m = v;
+      idx = a.cidx[(size_t)r * a.C + c];
+    }
+    low = fminf(low, a.cmin[(size_t)r * a.C + c]);
+  }
+  const float T = a.temperature[r];
+  if (m == -INFINITY || !(T > 0.0f)) {
+    if (write && threadIdx.x == 0) a.ids[r] = m == -INFINITY ? -1 : idx;
+    return false;
+  }
+  o.m = m;
+  o.T = T;
+  o.k = a.top_k[r];
+  const double c = 1.4426950408889634074 / (double)T;
+  // bins over what weighs something at all, or over the row's range where that is less
+  const double range = fmin((double)kMaxExp + 1.0, ((double)m - (double)low) * c);
+  o.weigh = Weigh{m, c, range > 0.0 && m != INFINITY ? kBins / range : 0.0, table};
+  return true;
+}
+
+// ---- 2. histogram -------------------------------------------------------------------------------------
+template <bool BF>
+__global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleArgs a) {
+  __shared__ double s_table[16];
+  __shared__ uint64_t s_hist[kBins];
+  const int c = blockIdx.x, r = blockIdx.y;
+  fill_table(s_table);
+  RowInfo info;
+  if (!row_info(a, r, s_table, info, c == 0) || digits_row(a, info.k)) return;
+  const Weigh& weigh = info.weigh;
+  const bool counts = counts_row(a, info.k);
+  for (int b = threadIdx.x; b < kBins; b += kThreads) s_hist[b] = 0;
+  __syncthreads();
+  const Row<BF> row(a, r);
+  int g0, g1;
+  chunk_of(row, c, a.C, g0, g1);
+  for (int g = g0 + threadIdx.x; g < g1; g += kThreads) {
+    float x[Row<BF>::VE];
+    row.load(g, x);
+#pragma unroll
+    for (int j = 0; j < Row<BF>::VE; ++j) {
+      if (!weigh.in(x[j])) continue;
+      const double y = weigh.y(x[j]);
+      if (y < -(double)kMaxExp - 1.0) continue;
+      if (counts) {
+        atomicAdd(reinterpret_cast<uint32_t*>(&s_hist[weigh.bin(x[j])]), 1u);
+      } else {
+        const uint64_t w = weigh.fixed(x[j]);
+        if (w != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&s_hist[weigh.bin(x[j])]), (unsigned long long)w);
+      }
+    }
+  }
+  __syncthreads();
+  uint64_t* hist = a.hist + (size_t)r * kBins;
+  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+    if (a.C == 1) hist[b] = s_hist[b];
+    else if (s_hist[b] != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&hist[b]), (unsigned long long)s_hist[b]);
+  }
+}
+
+// ---- 3. collect ---------------------------------------------------------------------------------------
+// The bins whose tokens decide: up to four ranges [lo, hi].
+struct Ranges {
+  int lo[3], hi[3];
+  __device__ __forceinline__ bool has(int b) const {
+    return (b >= lo[0] && b <= hi[0]) || (b >= lo[1] && b <= hi[1]) || (b >= lo[2] && b <= hi[2]);
+  }
+};
+
+struct BinSmem {
+  uint64_t before[kBins];  // sums of the bins before each
+  uint64_t wave[kWaves];
+  uint64_t total;
+  int at[8];
+};
+
+// First bin whose running sum (with it) reaches each of n targets (at least 1, at most the total),
+// into sm.at[0, n).
+__device__ __forceinline__ void reach(BinSmem& sm, const uint64_t (&h)[2], uint64_t first, const uint64_t* target, int n) {
+  const int b = 2 * threadIdx.x;
+  for (int k = 0; k < n; ++k) {
+    if (first < target[k] && first + h[0] >= target[k]) sm.at[k] = b;
+    else if (first + h[0] < target[k] && first + h[0] + h[1] >= target[k]) sm.at[k] = b + 1;
+  }
+}
+
+// Sums before every bin, and the deciding bins.
+__device__ void deciding_bins(const SampleArgs& a, int r, const RowInfo& info, BinSmem& sm, Ranges& out) {
+  const uint64_t* hist = a.hist + (size_t)r * kBins;
+  const int b = 2 * threadIdx.x;
+  const uint64_t h[2] = {hist[b], hist[b + 1]};
+  uint64_t total;
+  const uint64_t first = scan64(h[0] + h[1], sm.wave, total) - h[0] - h[1];
+  sm.before[b] = first;
+  sm.before[b + 1] = first + h[0];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    out.lo[k] = 1;
+    out.hi[k] = 0;
+  }
+  if (counts_row(a, info.k)) {  // everything down to the k-th token's bin (or all)
+    if (threadIdx.x == 0) sm.at[0] = kBins - 1;
+    __syncthreads();
+    const uint64_t target = (uint64_t)info.k;
+    if (target <= total) reach(sm, h, first, &target, 1);
+    __syncthreads();
+    out.lo[0] = 0;
+    out.hi[0] = sm.at[0];
     return;
   }
-  const Weigh weigh{m, 1.0 / (double)T};
-  const RowSearch<BF> search{row, weigh, sm};
+  // the prefix's weight, and its bounds where a border's bin is all that is known
+  uint64_t lo = total, hi = total;
+  __syncthreads();
+  const float p = a.top_p[r];
+  const uint64_t goal = p > 0.0f ? max(ceil_mul(p, total), (uint64_t)1) : 1;  // used where p < 1
+  if (p < 1.0f) {
+    reach(sm, h, first, &goal, 1);
+    __syncthreads();
+    const int at = sm.at[0];
+    out.lo[0] = out.hi[0] = at;
+    lo = sm.before[at];
+    hi = at + 1 < kBins ? sm.before[at + 1] : total;
+  }
+  if (a.min_p[r] > 0.0f) {  // w = min_p at y = log2(min_p), give or take the roundings of y and w
+    const double y = -log2((double)fminf(a.min_p[r], 1.0f)), scale = info.weigh.scale;
+    const int m0 = (int)fmin(fmax((y - 1e-14) * scale * (1.0 - 1e-12) - 1e-6, 0.0), (double)(kBins - 1));
+    const int m1 = (int)fmin((y + 1e-14) * scale * (1.0 + 1e-12) + 1e-6, (double)(kBins - 1));
+    out.lo[1] = m0;
+    out.hi[1] = m1;
+    lo = min(lo, sm.before[m0]);
+    hi = min(hi, m1 + 1 < kBins ? sm.before[m1 + 1] : total);
+  }
+  const float u = clean_u(a.u[r]);
+  const uint64_t target[2] = {floor_mul(u, lo) + 1, min(floor_mul(u, hi) + 1, total)};
+  __syncthreads();
+  reach(sm, h, first, target, 2);
+  __syncthreads();
+  out.lo[2] = sm.at[0];
+  out.hi[2] = sm.at[1];
+}
 
-  search.histogram(0, 0);
-  uint64_t count, mass;
-  scan64((uint64_t)sm.count[2 * threadIdx.x] + sm.count[2 * threadIdx.x + 1], sm.wave, count);
-  scan64(sm.mass[2 * threadIdx.x] + sm.mass[2 * threadIdx.x + 1], sm.wave, mass);
-  bool level0 = true;
-  const int k = a.top_k[r];
-  if (k > 0 && (uint64_t)k < count) {
-    const auto f = search.find(true, (uint64_t)k, level0);
-    mass = f.mass + ((uint64_t)k - f.count) * weigh.fixed(logit_of(f.key));
-    level0 = false;
+template <bool BF>
+__global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a) {
+  __shared__ double s_table[16];
+  __shared__ BinSmem sm;
+  const int c = blockIdx.x, r = blockIdx.y;
+  fill_table(s_table);
+  RowInfo info;
+  if (!row_info(a, r, s_table, info, false) || digits_row(a, info.k)) return;
+  __syncthreads();
+  Ranges ranges;
+  deciding_bins(a, r, info, sm, ranges);
+  const Row<BF> row(a, r);
+  int g0, g1;
+  chunk_of(row, c, a.C, g0, g1);
+  const Weigh& weigh = info.weigh;
+  const int lane = threadIdx.x & 63;
+  for (int g = g0 + threadIdx.x; g < g1; g += kThreads) {
+    float x[Row<BF>::VE];
+    row.load(g, x);
+#pragma unroll
+    for (int j = 0; j < Row<BF>::VE; ++j) {
+      const bool on = weigh.in(x[j]) && weigh.y(x[j]) >= -(double)kMaxExp - 1.0 && ranges.has(weigh.bin(x[j]));
+      const uint64_t all = __builtin_amdgcn_ballot_w64(on);
+      if (all == 0) continue;
+      // one addition per wave; their order does not matter: they are sorted
+      const int first = __ffsll((unsigned long long)all) - 1;
+      int at = 0;
+      if (lane == first) at = atomicAdd(&a.listed[r], __popcll(all));
+      at = __shfl(at, first, 64) + __popcll(all & ((1ull << lane) - 1));
+      if (on && at < kCap)
+        a.list[(size_t)r * kCap + at] = ((uint64_t)~key_of(x[j]) << 32) | (uint32_t)(row.first(g) + j);
+    }
+  }
+}
+
+// ---- 4. finish ----------------------------------------------------------------------------------------
+struct FinishSmem {
+  BinSmem bins;
+  union {
+    struct {
+      uint64_t item[kCap];     // sorted: inverted key, index
+      uint64_t upto[kCap];     // weights up to and including each
+      uint64_t skipped[kBins]; // listed weights before a bin's first listed token
+    } s;
+    RowSmem row;
+  };
+  uint64_t value[4];
+};
+
+template <bool BF>
+__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
+  __shared__ double s_table[16];
+  __shared__ FinishSmem sm;
+  const int r = blockIdx.x, tid = threadIdx.x;
+  fill_table(s_table);
+  RowInfo info;
+  if (!row_info(a, r, s_table, info, false)) return;
+  __syncthreads();
+  const Weigh& weigh = info.weigh;
+  const float p = a.top_p[r], mp = a.min_p[r], u = clean_u(a.u[r]);
+  const int n = a.listed[r];
+  if (n > kCap || digits_row(a, info.k)) {
+    const Row<BF> row(a, r);
+    const RowSearch<BF> search{row, weigh, sm.row};
+    const int id = search.sample(info.k, p, mp, u);
+    if (tid == 0) a.ids[r] = id;
+    return;
+  }
+  Ranges ranges;
+  deciding_bins(a, r, info, sm.bins, ranges);
+  int size = 64;
+  while (size < n) size *= 2;
+  for (int k = tid; k < size; k += kThreads) sm.s.item[k] = k < n ? a.list[(size_t)r * kCap + k] : ~0ull;
+  __syncthreads();
+  for (int len = 2; len <= size; len *= 2)  // bitonic
+    for (int step = len / 2; step > 0; step /= 2) {
+      for (int k = tid; k < size / 2; k += kThreads) {
+        const int lo = 2 * k - (k & (step - 1)), hi = lo + step;
+        const uint64_t x = sm.s.item[lo], y = sm.s.item[hi];
+        if ((x > y) == ((lo & len) == 0)) {
+          sm.s.item[lo] = y;
+          sm.s.item[hi] = x;
+        }
+      }
+      __syncthreads();
+    }
+  auto logit = [&](int k) { return logit_of(~(uint32_t)(sm.s.item[k] >> 32)); };
+  // Running weights of the list, kCap / kThreads tokens a thread.
+  constexpr int PER = kCap / kThreads;
+  uint64_t w[PER], sum = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int k = tid * PER + j;
+    w[j] = k < n ? weigh.fixed(logit(k)) : 0;
+    sum += w[j];
+  }
+  uint64_t total;
+  uint64_t run = scan64(sum, sm.bins.wave, total) - sum;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int k = tid * PER + j;
+    if (k < n) {
+      const int b = weigh.bin(logit(k));
+      if (k == 0 || weigh.bin(logit(k - 1)) != b) sm.s.skipped[b] = run;
+      sm.s.upto[k] = run + w[j];
+    }
+    run += w[j];
+  }
+  const bool counts = counts_row(a, info.k);
+  __syncthreads();
+  // ... and of the row: the weights of all bins before, and of the token's own bin up to it.
+  if (!counts) {
+    for (int k = tid; k < n; k += kThreads) {
+      const int b = weigh.bin(logit(k));
+      sm.s.upto[k] += sm.bins.before[b] - sm.s.skipped[b];
+    }
+    __syncthreads();
+  }
+  // First listed token whose running weight reaches x.
+  auto rank_of = [&](uint64_t x) {
+    if (tid == 0) sm.bins.at[7] = n - 1;
+    __syncthreads();
+    for (int k = tid; k < n; k += kThreads)
+      if (sm.s.upto[k] >= x && (k == 0 || sm.s.upto[k - 1] < x)) sm.bins.at[7] = k;
+    __syncthreads();
+    const int k = sm.bins.at[7];
+    __syncthreads();
+    return k;
+  };
+  uint64_t mass;  // of the top-k prefix
+  if (counts) {
+    mass = sm.s.upto[min(info.k, n) - 1];
+  } else {
+    const uint64_t last = a.hist[(size_t)r * kBins + kBins - 1];
+    mass = sm.bins.before[kBins - 1] + last;
   }
   uint64_t kept = mass;
-  const float p = a.top_p[r];
-  if (p < 1.0f) {
-    const uint64_t target = p > 0.0f ? max(ceil_mul(p, mass), (uint64_t)1) : 1;
-    const auto f = search.find(false, target, level0);
-    const uint64_t w = weigh.fixed(logit_of(f.key));
-    kept = min(kept, f.mass + (target - f.mass + w - 1) / w * w);
-    level0 = false;
+  if (p < 1.0f) kept = min(kept, sm.s.upto[rank_of(p > 0.0f ? max(ceil_mul(p, mass), (uint64_t)1) : 1)]);
+  if (mp > 0.0f) {
+    // listed tokens are a run of ranks around the border: the last with w >= min_p ends the prefix, or
+    // the bins before the border's first do
+    const double least = (double)fminf(mp, 1.0f);
+    if (tid == 0) sm.value[0] = counts ? 0 : sm.bins.before[ranges.lo[1]];
+    __syncthreads();
+    for (int k = tid; k < n; k += kThreads)
+      if (weigh.real(logit(k)) >= least && (k + 1 == n || weigh.real(logit(k + 1)) < least))
+        atomicMax(reinterpret_cast<unsigned long long*>(&sm.value[0]), (unsigned long long)sm.s.upto[k]);
+    __syncthreads();
+    kept = min(kept, sm.value[0]);
   }
-  if (a.min_p[r] > 0.0f) {
-    const float mp = fminf(a.min_p[r], 1.0f);
-    uint64_t sum = 0;
-    for (int g = threadIdx.x; g < row.groups; g += kThreads) {
-      float x[Row<BF>::VE];
-      row.load(g, x);
-#pragma unroll
-      for (int j = 0; j < Row<BF>::VE; ++j)
-        if (weigh.real(x[j]) >= (double)mp) sum += weigh.fixed(x[j]);
-    }
-    uint64_t total;
-    scan64(sum, sm.wave, total);
-    kept = min(kept, total);
-  }
-  const uint64_t target = floor_mul(clean_u(a.u[r]), kept) + 1;
-  const auto f = search.find(false, target, level0);
-  const uint64_t w = weigh.fixed(logit_of(f.key));
-  const int id = search.nth(f.key, (target - f.mass + w - 1) / w);
-  if (threadIdx.x == 0) a.ids[r] = id;
+  const int at = rank_of(floor_mul(u, kept) + 1);
+  if (tid == 0) a.ids[r] = (int64_t)(uint32_t)sm.s.item[at];
+}
+
+struct SamplePlan {
+  int C;
+  size_t o_idx, o_min, o_hist, o_listed, o_list, bytes;
+};
+
+constexpr int kRows = 2048;  // rows at a time: a row has 48 KB of workspace
+
+SamplePlan sample_plan(int R, int V) {
+  SamplePlan p{};
+  if (R < 1 || V < 1 || V > 1 << 20 || R > 65535) return p;
+  R = R < kRows ? R : kRows;
+  // Workgroups per row: two per CU in all, chunks of 4096 tokens at least.
+  p.C = max(1, min(512 / R, (V + 4095) / 4096));
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  const size_t chunks = up((size_t)R * p.C * 4);
+  p.o_idx = chunks;
+  p.o_min = 2 * chunks;
+  p.o_hist = 3 * chunks;
+  p.o_listed = p.o_hist + (size_t)R * kBins * 8;
+  p.o_list = p.o_listed + up((size_t)R * 4);
+  p.bytes = p.o_list + (size_t)R * kCap * 8;
+  return p;
+}
+
+template <bool BF>
+void sample_launch(const SampleArgs& a, hipStream_t s) {
+  const dim3 grid(a.C, a.R), block(kThreads);
+  hipLaunchKernelGGL(sample_max_kernel<BF>, grid, block, 0, s, a);
+  hipLaunchKernelGGL(sample_hist_kernel<BF>, grid, block, 0, s, a);
+  hipLaunchKernelGGL(sample_collect_kernel<BF>, grid, block, 0, s, a);
+  hipLaunchKernelGGL(sample_finish_kernel<BF>, dim3(a.R), block, 0, s, a);
 }
 
 }  // namespace
 
+extern "C" size_t npn_sample_workspace_size(int R, int V) { return sample_plan(R, V).bytes; }
+
 extern "C" int npn_sample(const void* logits, int bf16, const float* temperature,
                           const int32_t* top_k, const float* top_p, const float* min_p,
-                          const float* u, int64_t* ids, int R, int V, void* stream) {
+                          const float* u, int64_t* ids, int R, int V, void* workspace,
+                          size_t workspace_bytes, void* stream) {
   NPN_REQUIRE(logits && temperature && top_k && top_p && min_p && u && ids, NPN_ERR_NULL);
-  NPN_REQUIRE(R >= 1 && V >= 1 && V <= 1 << 20 && (bf16 == 0 || bf16 == 1), NPN_ERR_SHAPE);
-  NPN_REQUIRE(NPN_ALIGNED16(logits), NPN_ERR_ALIGN);
-  const SampleArgs a{static_cast<const uint8_t*>(logits), temperature, top_k, top_p, min_p, u, ids, R, V};
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  if (bf16) hipLaunchKernelGGL(sample_rows_kernel<true>, dim3(R), dim3(kThreads), 0, s, a);
-  else hipLaunchKernelGGL(sample_rows_kernel<false>, dim3(R), dim3(kThreads), 0, s, a);
+  const SamplePlan p = sample_plan(R, V);
+  NPN_REQUIRE(p.bytes != 0 && (bf16 == 0 || bf16 == 1), NPN_ERR_SHAPE);
+  NPN_REQUIRE(NPN_ALIGNED16(logits) && NPN_ALIGNED16(workspace), NPN_ERR_ALIGN);
+  NPN_REQUIRE(workspace != nullptr && workspace_bytes >= p.bytes, NPN_ERR_WORKSPACE);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  for (int r0 = 0; r0 < R; r0 += kRows) {
+    const int n = R - r0 < kRows ? R - r0 : kRows;
+    const SampleArgs a{static_cast<const uint8_t*>(logits) + (size_t)r0 * V * (bf16 ? 2 : 4), temperature + r0,
+                       top_k + r0, top_p + r0, min_p + r0, u + r0, ids + r0, n, V, p.C,
+                       reinterpret_cast<float*>(ws), reinterpret_cast<int32_t*>(ws + p.o_idx),
+                       reinterpret_cast<float*>(ws + p.o_min), reinterpret_cast<uint64_t*>(ws + p.o_hist),
+                       reinterpret_cast<int32_t*>(ws + p.o_listed), reinterpret_cast<uint64_t*>(ws + p.o_list)};
+    if (bf16) sample_launch<true>(a, static_cast<hipStream_t>(stream));
+    else sample_launch<false>(a, static_cast<hipStream_t>(stream));
+  }
   return npn_launch_status();
 }

@@ -67,7 +67,8 @@ SIGNATURES = {
     "npn_gqa_kv_append_paged": (_I, [_P] * 5 + [_I] + [_P] * 6 + [_I] * 5 + [_P]),
     "npn_gqa_tail_verify_paged_workspace_size": (_Z, [_I] * 6),
     "npn_gqa_tail_verify_paged": (_I, [_P] * 5 + [_I] + [_P] * 8 + [_I] * 7 + [_P, _Z, _P]),
-    "npn_sample": (_I, [_P, _I] + [_P] * 6 + [_I] * 2 + [_P]),
+    "npn_sample_workspace_size": (_Z, [_I] * 2),
+    "npn_sample": (_I, [_P, _I] + [_P] * 6 + [_I] * 2 + [_P, _Z, _P]),
     "npn_deltanet_full_fp8_workspace_size": (_Z, [_I] * 3),
     "npn_deltanet_full_fp8": (_I, [_P] * 19 + [_I] * 3 + [_P, _Z, _P]),
 }

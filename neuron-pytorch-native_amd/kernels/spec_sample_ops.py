@@ -14,7 +14,7 @@ ids in every run and whatever else shares the batch.
 """
 import torch
 
-from npn_native import check_all, launch, register
+from npn_native import check_all, launch, query as size_query, register
 
 I32, F32 = torch.int32, torch.float32
 
@@ -36,5 +36,10 @@ def sample(logits, temperature, top_k, top_p, min_p, u):
               (temperature, "temperature", F32, R), (top_k, "top_k", I32, R),
               (top_p, "top_p", F32, R), (min_p, "min_p", F32, R), (u, "u", F32, R))
     ids = torch.empty(R, dtype=torch.int64, device=dev)
-    launch(dev, "npn_sample", logits, int(bf16), temperature, top_k, top_p, min_p, u, ids, R, V)
+    n_ws = size_query("npn_sample_workspace_size", R, V)
+    if n_ws == 0:
+        raise RuntimeError(f"unsupported sample sizes R={R} V={V}")
+    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
+    launch(dev, "npn_sample", logits, int(bf16), temperature, top_k, top_p, min_p, u, ids, R, V, ws,
+           n_ws)
     return ids

@@ -17,7 +17,7 @@ NAN, INF = float("nan"), float("inf")
 
 def _settings(R, rng):
     return dict(temperature=rng.choice([0.0, 0.1, 0.6, 1.0, 1.0, 2.0, 30.0], R).astype(np.float32),
-                top_k=rng.choice([0, 0, 1, 2, 20, 1000, 10**6], R).astype(np.int32),
+                top_k=rng.choice([0, 0, 1, 2, 20, 1000, 4096, 4097, 10**6], R).astype(np.int32),
                 top_p=rng.choice([1.0, 1.0, 0.0, 0.3, 0.9, 0.999], R).astype(np.float32),
                 min_p=rng.choice([0.0, 0.0, 1e-4, 0.1, 1.0], R).astype(np.float32),
                 u=rng.random(R).astype(np.float32))
@@ -41,11 +41,12 @@ def _check(ops, logits, s):
 @pytest.mark.parametrize("R,V,kind", [
     (5, 1, "flat"), (9, 2, "flat"), (40, 17, "peaked"), (33, 1000, "flat"), (64, 4099, "peaked"),
     (50, 32001, "flat"), (24, 151936, "flat"), (24, 151937, "peaked"), (7, 248320, "wide"),
-    (300, 5003, "wide"), (2, 1 << 20, "flat"), (12, 20001, "equal"), (12, 50000, "two"), (12, 30011, "narrow"),
+    (300, 5003, "wide"), (2, 1 << 20, "flat"), (2100, 300, "flat"), (12, 20001, "equal"), (12, 50000, "two"), (12, 30011, "narrow"),
 ])
 def test_sample_matches_oracle(ops, R, V, kind, dtype):
     """Rows from one token to the longest, odd lengths (rows at every alignment), flat, peaked and
-    wide; all tokens equal, two values only, and values that differ in their last bits."""
+    wide; all tokens equal, two values only, and values that differ in their last bits; more rows than
+    one pass takes."""
     rng = np.random.default_rng(R + V)
     x = rng.standard_normal((R, V)).astype(np.float32)
     if kind == "peaked":

@@ -51,13 +51,16 @@ def test_refusals_on_the_host():
     import npn_native
     A = 1 << 20
 
-    def st(ptrs=[A] * 7, bf16=0, R=2, V=10):
-        return npn_native.lib().npn_sample(ptrs[0], bf16, *ptrs[1:], R, V, None)
+    def st(ptrs=[A] * 7, bf16=0, R=2, V=10, ws=A, n=1 << 40):
+        return npn_native.lib().npn_sample(ptrs[0], bf16, *ptrs[1:], R, V, ws, n, None)
     for i in range(7):
         assert st([0 if j == i else A for j in range(7)]) == 1
     for bad in (dict(R=0), dict(V=0), dict(V=(1 << 20) + 1), dict(bf16=2), dict(bf16=-1)):
         assert st(**bad) == 2, bad
-    assert st([A + 4] + [A] * 6) == 3
+    assert st([A + 4] + [A] * 6) == 3 and st(ws=A + 8) == 3
+    n = npn_native.query("npn_sample_workspace_size", 2, 10)
+    assert n > 0 and st(n=n - 1) == 4 and st(ws=None) == 4
+    assert npn_native.query("npn_sample_workspace_size", 65536, 10) == 0
 
 
 def test_op_refuses_cpu_tensors_and_propagates_shapes():
