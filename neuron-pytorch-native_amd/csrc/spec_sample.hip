@@ -38,6 +38,7 @@ constexpr int kBins = 1 << kDigit;
 constexpr int kCap = 4096;                // list entries per row
 constexpr float kMaxExp = 43.0f;          // weights below 2^-43 of the largest round to 0
 
+struct RowState;
 struct SampleArgs {
   const uint8_t* logits;  // [R][V] f32 or bf16
   const float* temperature;
@@ -51,6 +52,8 @@ struct SampleArgs {
   int32_t* cidx;
   float* cmin;
   uint64_t* hist;   // [R][kBins] counts or weights
+  RowState* state;    // [R] settings
+  RowState* decided;  // [R] and the deciding bins
   int32_t* listed;  // [R] tokens that go on the list
   uint64_t* list;   // [R][kCap] inverted key above index: ascending is rank order
 };
@@ -101,58 +104,48 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float(key ^ ((uint32_t)(~(int)key >> 31) | 0x80000000u));
 }
 
-// 2^y for y in [-44, 0], to 2^-49 relative: 2^(j/16) from the table by y's nearest sixteenth, times
-// the series of e^r, |r| <= ln(2)/32, to r^7/5040 (the next term is under 2^-59).
-__device__ __forceinline__ double exp2_neg(double y, const double* table) {
-  const double t = rint(y * 16.0);
-  const int n = (int)t;
-  const double r = (y - t * 0.0625) * 0.69314718055994530942;
-  double p = fma(r, 1.0 / 5040, 1.0 / 720);
-  p = fma(r, p, 1.0 / 120);
-  p = fma(r, p, 1.0 / 24);
-  p = fma(r, p, 1.0 / 6);
-  p = fma(r, p, 0.5);
+// 2^(t/64) for t in [-60 * 64, 0], to 2^-51 relative: 2^(j/64) from the table by t's nearest whole
+// number, times the series of e^r, |r| <= ln(2)/128, to r^5/120 (the next term is under 2^-54); the
+// power's whole part goes into the exponent's bits.
+__device__ __forceinline__ double exp2_64ths(double t, const double* table) {
+  constexpr double L = 0.69314718055994530942 / 64;
+  const double whole = rint(t), r = t - whole;
+  const int n = (int)whole;
+  double p = fma(r, L * L * L * L * L / 120, L * L * L * L / 24);
+  p = fma(r, p, L * L * L / 6);
+  p = fma(r, p, L * L / 2);
+  p = fma(r, p, L);
   p = fma(r, p, 1.0);
-  p = fma(r, p, 1.0);
-  return ldexp(p * table[n & 15], n >> 4);
+  return __longlong_as_double(__double_as_longlong(p * table[n & 63]) + ((int64_t)(n >> 6) << 52));
 }
 
-// 2^((x - m) log2(e) / T), 0 for -inf; in a row with m = +inf those at +inf share it all. y(x), in
-// base 2 and never above 0, also gives the bin: equal logits share one, larger ones never lie in a
-// later one.
+// 2^((x - m) log2(e) / T), no less than 2^-60 (which weighs nothing). In a row with m = +inf those at
+// +inf share it all: what lies below is infinitely far off.
 struct Weigh {
   float m;
-  double c;             // log2(e) / T
-  double scale;         // bins per unit of -y
-  const double* table;  // 2^(j/16)
-  __device__ __forceinline__ bool in(float x) const {
-    return x == m || (x != -INFINITY && m != INFINITY);
-  }
-  __device__ __forceinline__ double y(float x) const {
-    return x == m ? 0.0 : ((double)x - (double)m) * c;
-  }
+  double c64;           // 64 log2(e) / T
+  const double* table;  // 2^(j/64)
   __device__ __forceinline__ double real(float x) const {
-    if (!in(x)) return 0.0;
-    const double e = y(x);
-    return e < -44.0 ? 0.0 : exp2_neg(e, table);
+    const double d = x == m ? 0.0 : (double)x - (double)m;
+    return exp2_64ths(fmax(d * c64, -60.0 * 64), table);
   }
   // round(w 2^42): the sum with 2^52 has the integer in its low bits.
   __device__ __forceinline__ uint64_t fixed(float x) const {
-    return (uint64_t)__double_as_longlong(real(x) * kOne + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    return (uint64_t)__double_as_longlong(fma(real(x), kOne, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
   }
-  __device__ __forceinline__ int bin(float x) const { return min(kBins - 1, (int)(-y(x) * scale)); }
 };
 
-__device__ __forceinline__ void fill_table(double* table) {
-  if (threadIdx.x < 16) table[threadIdx.x] = exp2(threadIdx.x * 0.0625);
+// The bin of a token x >= cut, `scale` bins per unit of m - x. Equal logits share a bin and larger ones
+// never lie in a later one: that is all the bins have to be, so 32 bits do. The last bin has the rest,
+// among it all that weighs nothing.
+__device__ __forceinline__ int bin_of(float x, float m, float scale) {
+  const float t = x == m ? 0.0f : fminf(m - x, 3.4e38f) * scale;
+  return (int)fminf(t, (float)(kBins - 1));
 }
 
-// Whether the row's top-k goes by counts.
-__device__ __forceinline__ bool counts_row(const SampleArgs& a, int k) {
-  return k > 0 && k < a.V && k <= kCap;
+__device__ __forceinline__ void fill_table(double* table) {
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2(threadIdx.x * 0.015625);
 }
-// A longer one needs counts and weights both: such a row is searched by digits from the start.
-__device__ __forceinline__ bool digits_row(const SampleArgs& a, int k) { return k > kCap && k < a.V; }
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
   return ((uint64_t)(uint32_t)__shfl_up((int)(v >> 32), d, 64) << 32) |
@@ -414,248 +407,323 @@ __global__ __launch_bounds__(kThreads) void sample_max_kernel(SampleArgs a) {
   }
 }
 
-// What the later launches know of a row; false: its token is known (a.ids is written by thread 0 of
-// the workgroup with `write`).
-struct RowInfo {
-  float m, T;
+// A row's settings, and the bins whose tokens decide, in up to three ranges, ascending and disjoint.
+struct RowState {
+  enum { kDone, kCounts, kWeights, kDigits };
+  float m, cut, scale;
+  int mode, ranges;
+  int lo[3], hi[3];
   int k;
-  Weigh weigh;
+  float p, min_p, u;
+  double c;
+  uint64_t base[3];  // sum of the bins before each range
+  uint64_t total;    // and of all
+  uint64_t above;    // of those whose tokens are all past min_p
 };
-__device__ __forceinline__ bool row_info(const SampleArgs& a, int r, const double* table, RowInfo& o, bool write) {
+
+// The row's settings, from its chunks (every wave for itself, a lane per chunk); a row whose token is
+// known by its maximum gets it.
+__device__ __forceinline__ void row_settings(const SampleArgs& a, int r, RowState& o, int& id) {
+  const float T = a.temperature[r];
+  o.k = a.top_k[r];
+  o.p = a.top_p[r];
+  o.min_p = a.min_p[r];
+  o.u = clean_u(a.u[r]);
   float m = -INFINITY, low = INFINITY;
   int idx = 0x7FFFFFFF;
-  for (int c = 0; c < a.C; ++c) {  // ascending, so the first of equal maxima stays
-    const float v = a.cmax[(size_t)r * a.C + c];
-    if (v > m) {
+  for (int c = threadIdx.x & 63; c < a.C; c += 64) {
+    const size_t at = (size_t)r * a.C + c;
+    const float v = a.cmax[at], w = a.cmin[at];
+    const int i = a.cidx[at];
+    if (v > m) {  // chunks ascend, so the first of equal maxima stays
       m = v;
-      idx = a.cidx[(size_t)r * a.C + c];
+      idx = i;
     }
-    low = fminf(low, a.cmin[(size_t)r * a.C + c]);
+    low = fminf(low, w);
   }
-  const float T = a.temperature[r];
-  if (m == -INFINITY || !(T > 0.0f)) {
-    if (write && threadIdx.x == 0) a.ids[r] = m == -INFINITY ? -1 : idx;
-    return false;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) {
+    const float om = __shfl_xor(m, off, 64);
+    const int oi = __shfl_xor(idx, off, 64);
+    if (om > m || (om == m && oi < idx)) {
+      m = om;
+      idx = oi;
+    }
+    low = fminf(low, __shfl_xor(low, off, 64));
   }
+  id = m == -INFINITY ? -1 : idx;
   o.m = m;
-  o.T = T;
-  o.k = a.top_k[r];
-  const double c = 1.4426950408889634074 / (double)T;
+  o.cut = m == INFINITY ? INFINITY : -3.402823466e38f;
+  o.ranges = 0;
+  o.c = 1.4426950408889634074 / (double)T;
   // bins over what weighs something at all, or over the row's range where that is less
-  const double range = fmin((double)kMaxExp + 1.0, ((double)m - (double)low) * c);
-  o.weigh = Weigh{m, c, range > 0.0 && m != INFINITY ? kBins / range : 0.0, table};
-  return true;
+  const double range = fmin(((double)kMaxExp + 1.0) / o.c, (double)m - (double)low);
+  o.scale = !(range > 0.0) || m == INFINITY ? 0.0f : (float)fmin(kBins / range, 3.4e38);
+  const bool cut_k = o.k > 0 && o.k < a.V;
+  o.mode = m == -INFINITY || !(T > 0.0f) ? RowState::kDone
+           : !cut_k ? RowState::kWeights : o.k <= kCap ? RowState::kCounts : RowState::kDigits;
 }
 
 // ---- 2. histogram -------------------------------------------------------------------------------------
+struct BinSmem {
+  uint64_t before[kBins];  // sums of the bins before each
+  uint64_t wave[kWaves];
+  int at[4];
+};
+
+// First bin whose running sum (with it) reaches the target (at least 1, at most the total), by the
+// thread that has it, into *out.
+__device__ __forceinline__ void reach(const uint64_t (&h)[2], uint64_t first, uint64_t target, int* out) {
+  if (first < target && first + h[0] >= target) *out = 2 * threadIdx.x;
+  else if (first + h[0] < target && first + h[0] + h[1] >= target) *out = 2 * threadIdx.x + 1;
+}
+
+// The deciding bins into o (in LDS), from this thread's bins 2 tid and 2 tid + 1.
+__device__ void decide(const uint64_t (&h)[2], RowState& o, BinSmem& sm) {
+  const int tid = threadIdx.x;
+  uint64_t total;
+  const uint64_t first = scan64(h[0] + h[1], sm.wave, total) - h[0] - h[1];
+  sm.before[2 * tid] = first;
+  sm.before[2 * tid + 1] = first + h[0];
+  if (tid < 4) sm.at[tid] = kBins - 1;
+  __syncthreads();
+  if (o.mode == RowState::kCounts) {  // everything down to the k-th token's bin (or all)
+    if ((uint64_t)o.k <= total) reach(h, first, (uint64_t)o.k, &sm.at[0]);
+    __syncthreads();
+    if (tid == 0) {
+      o.total = total;
+      o.above = 0;
+      o.ranges = 1;
+      o.lo[0] = 0;
+      o.hi[0] = sm.at[0];
+      o.base[0] = 0;
+    }
+    __syncthreads();
+    return;
+  }
+  // The kept prefix's weight, between its bounds where a border's bin is all that is known, and with
+  // it the bins that the sample may lie in.
+  auto sum_to = [&](int bin) { return bin + 1 < kBins ? sm.before[bin + 1] : total; };
+  uint64_t least = total, most = total;
+  const bool by_p = o.p < 1.0f, by_min = o.min_p > 0.0f;
+  if (by_p) {
+    reach(h, first, o.p > 0.0f ? max(ceil_mul(o.p, total), (uint64_t)1) : 1, &sm.at[0]);
+    __syncthreads();
+    least = sm.before[sm.at[0]];
+    most = sum_to(sm.at[0]);
+  }
+  int m0 = 0, m1 = 0;
+  if (by_min) {  // w = min_p at -y = log2(1 / min_p), give or take the roundings of y, w and bins
+    const double per = (double)o.scale / o.c;  // bins per unit of y
+    const double y = -log2((double)fminf(o.min_p, 1.0f));
+    m0 = (int)fmin(fmax((y - 1e-14) * per * (1.0 - 1e-6) - 1e-6, 0.0), (double)(kBins - 1));
+    m1 = (int)fmin((y + 1e-14) * per * (1.0 + 1e-6) + 1e-6, (double)(kBins - 1));
+    least = min(least, sm.before[m0]);
+    most = min(most, sum_to(m1));
+  }
+  reach(h, first, floor_mul(o.u, least) + 1, &sm.at[1]);
+  reach(h, first, min(floor_mul(o.u, most) + 1, total), &sm.at[2]);
+  __syncthreads();
+  if (tid == 0) {
+    int n = 0;
+    auto add = [&](int lo, int hi) {  // ascending by lo, touching ranges as one
+      int k = n;
+      for (; k > 0 && lo < o.lo[k - 1]; --k) {
+        o.lo[k] = o.lo[k - 1];
+        o.hi[k] = o.hi[k - 1];
+      }
+      o.lo[k] = lo;
+      o.hi[k] = hi;
+      ++n;
+    };
+    add(sm.at[1], sm.at[2]);
+    if (by_p) add(sm.at[0], sm.at[0]);
+    if (by_min) add(m0, m1);
+    int k = 0;
+    for (int i = 1; i < n; ++i) {
+      if (o.lo[i] <= o.hi[k] + 1) {
+        o.hi[k] = max(o.hi[k], o.hi[i]);
+      } else {
+        ++k;
+        o.lo[k] = o.lo[i];
+        o.hi[k] = o.hi[i];
+      }
+    }
+    o.ranges = k + 1;
+    for (int i = 0; i <= k; ++i) o.base[i] = sm.before[o.lo[i]];
+    o.total = total;
+    o.above = sm.before[m0];
+  }
+  __syncthreads();
+}
+
 template <bool BF>
 __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleArgs a) {
-  __shared__ double s_table[16];
+  __shared__ double s_table[64];
   __shared__ uint64_t s_hist[kBins];
-  const int c = blockIdx.x, r = blockIdx.y;
+  const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
   fill_table(s_table);
-  RowInfo info;
-  if (!row_info(a, r, s_table, info, c == 0) || digits_row(a, info.k)) return;
-  const Weigh& weigh = info.weigh;
-  const bool counts = counts_row(a, info.k);
-  for (int b = threadIdx.x; b < kBins; b += kThreads) s_hist[b] = 0;
+  RowState st;
+  int id;
+  row_settings(a, r, st, id);
+  if (c == 0 && tid == 0) {
+    a.state[r] = st;
+    if (st.mode == RowState::kDone) a.ids[r] = id;
+  }
+  if (st.mode == RowState::kDone || st.mode == RowState::kDigits) return;
+  const bool counts = st.mode == RowState::kCounts;
+  for (int b = tid; b < kBins; b += kThreads) s_hist[b] = 0;
   __syncthreads();
   const Row<BF> row(a, r);
+  const Weigh weigh{st.m, 64.0 * st.c, s_table};
   int g0, g1;
   chunk_of(row, c, a.C, g0, g1);
-  for (int g = g0 + threadIdx.x; g < g1; g += kThreads) {
+  for (int g = g0 + tid; g < g1; g += kThreads) {
     float x[Row<BF>::VE];
     row.load(g, x);
+    if (counts) {
 #pragma unroll
-    for (int j = 0; j < Row<BF>::VE; ++j) {
-      if (!weigh.in(x[j])) continue;
-      const double y = weigh.y(x[j]);
-      if (y < -(double)kMaxExp - 1.0) continue;
-      if (counts) {
-        atomicAdd(reinterpret_cast<uint32_t*>(&s_hist[weigh.bin(x[j])]), 1u);
-      } else {
+      for (int j = 0; j < Row<BF>::VE; ++j)
+        if (x[j] >= st.cut)
+          atomicAdd(reinterpret_cast<uint32_t*>(&s_hist[bin_of(x[j], st.m, st.scale)]), 1u);
+    } else {
+#pragma unroll
+      for (int j = 0; j < Row<BF>::VE; ++j) {
         const uint64_t w = weigh.fixed(x[j]);
-        if (w != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&s_hist[weigh.bin(x[j])]), (unsigned long long)w);
+        if (w != 0)
+          atomicAdd(reinterpret_cast<unsigned long long*>(&s_hist[bin_of(x[j], st.m, st.scale)]),
+                    (unsigned long long)w);
       }
     }
   }
   __syncthreads();
-  uint64_t* hist = a.hist + (size_t)r * kBins;
-  for (int b = threadIdx.x; b < kBins; b += kThreads) {
+  unsigned long long* hist = reinterpret_cast<unsigned long long*>(a.hist + (size_t)r * kBins);
+  for (int b = tid; b < kBins; b += kThreads) {
     if (a.C == 1) hist[b] = s_hist[b];
-    else if (s_hist[b] != 0) atomicAdd(reinterpret_cast<unsigned long long*>(&hist[b]), (unsigned long long)s_hist[b]);
+    else if (s_hist[b] != 0) atomicAdd(&hist[b], (unsigned long long)s_hist[b]);
   }
 }
 
 // ---- 3. collect ---------------------------------------------------------------------------------------
-// The bins whose tokens decide: up to four ranges [lo, hi].
-struct Ranges {
-  int lo[3], hi[3];
-  __device__ __forceinline__ bool has(int b) const {
-    return (b >= lo[0] && b <= hi[0]) || (b >= lo[1] && b <= hi[1]) || (b >= lo[2] && b <= hi[2]);
-  }
-};
-
-struct BinSmem {
-  uint64_t before[kBins];  // sums of the bins before each
-  uint64_t wave[kWaves];
-  uint64_t total;
-  int at[8];
-};
-
-// First bin whose running sum (with it) reaches each of n targets (at least 1, at most the total),
-// into sm.at[0, n).
-__device__ __forceinline__ void reach(BinSmem& sm, const uint64_t (&h)[2], uint64_t first, const uint64_t* target, int n) {
-  const int b = 2 * threadIdx.x;
-  for (int k = 0; k < n; ++k) {
-    if (first < target[k] && first + h[0] >= target[k]) sm.at[k] = b;
-    else if (first + h[0] < target[k] && first + h[0] + h[1] >= target[k]) sm.at[k] = b + 1;
-  }
-}
-
-// Sums before every bin, and the deciding bins.
-__device__ void deciding_bins(const SampleArgs& a, int r, const RowInfo& info, BinSmem& sm, Ranges& out) {
-  const uint64_t* hist = a.hist + (size_t)r * kBins;
-  const int b = 2 * threadIdx.x;
-  const uint64_t h[2] = {hist[b], hist[b + 1]};
-  uint64_t total;
-  const uint64_t first = scan64(h[0] + h[1], sm.wave, total) - h[0] - h[1];
-  sm.before[b] = first;
-  sm.before[b + 1] = first + h[0];
-#pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    out.lo[k] = 1;
-    out.hi[k] = 0;
-  }
-  if (counts_row(a, info.k)) {  // everything down to the k-th token's bin (or all)
-    if (threadIdx.x == 0) sm.at[0] = kBins - 1;
-    __syncthreads();
-    const uint64_t target = (uint64_t)info.k;
-    if (target <= total) reach(sm, h, first, &target, 1);
-    __syncthreads();
-    out.lo[0] = 0;
-    out.hi[0] = sm.at[0];
-    return;
-  }
-  // the prefix's weight, and its bounds where a border's bin is all that is known
-  uint64_t lo = total, hi = total;
-  __syncthreads();
-  const float p = a.top_p[r];
-  const uint64_t goal = p > 0.0f ? max(ceil_mul(p, total), (uint64_t)1) : 1;  // used where p < 1
-  if (p < 1.0f) {
-    reach(sm, h, first, &goal, 1);
-    __syncthreads();
-    const int at = sm.at[0];
-    out.lo[0] = out.hi[0] = at;
-    lo = sm.before[at];
-    hi = at + 1 < kBins ? sm.before[at + 1] : total;
-  }
-  if (a.min_p[r] > 0.0f) {  // w = min_p at y = log2(min_p), give or take the roundings of y and w
-    const double y = -log2((double)fminf(a.min_p[r], 1.0f)), scale = info.weigh.scale;
-    const int m0 = (int)fmin(fmax((y - 1e-14) * scale * (1.0 - 1e-12) - 1e-6, 0.0), (double)(kBins - 1));
-    const int m1 = (int)fmin((y + 1e-14) * scale * (1.0 + 1e-12) + 1e-6, (double)(kBins - 1));
-    out.lo[1] = m0;
-    out.hi[1] = m1;
-    lo = min(lo, sm.before[m0]);
-    hi = min(hi, m1 + 1 < kBins ? sm.before[m1 + 1] : total);
-  }
-  const float u = clean_u(a.u[r]);
-  const uint64_t target[2] = {floor_mul(u, lo) + 1, min(floor_mul(u, hi) + 1, total)};
-  __syncthreads();
-  reach(sm, h, first, target, 2);
-  __syncthreads();
-  out.lo[2] = sm.at[0];
-  out.hi[2] = sm.at[1];
-}
-
 template <bool BF>
 __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a) {
-  __shared__ double s_table[16];
-  __shared__ BinSmem sm;
+  // The workgroup's finds meet in LDS and go out together: their order does not matter, they are
+  // sorted. More than kCap of them make the row's list too long whatever the others find.
+  __shared__ uint64_t s_list[kCap];
+  __shared__ int s_count, s_at;
   const int c = blockIdx.x, r = blockIdx.y;
-  fill_table(s_table);
-  RowInfo info;
-  if (!row_info(a, r, s_table, info, false) || digits_row(a, info.k)) return;
+  __shared__ BinSmem bins;
+  const uint64_t* hist = a.hist + (size_t)r * kBins + 2 * threadIdx.x;
+  const uint64_t h[2] = {hist[0], hist[1]};
+  const int mode = a.state[r].mode;
+  if (mode != RowState::kCounts && mode != RowState::kWeights) return;
+  __shared__ RowState st;
+  if (threadIdx.x == 0) st = a.state[r];
+  decide(h, st, bins);
+  if (c == 0 && threadIdx.x == 0) a.decided[r] = st;
+  const float m = st.m, cut = st.cut, scale = st.scale;
+  uint32_t lo[3], width[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    lo[k] = k < st.ranges ? st.lo[k] : kBins;  // none: no bin is there
+    width[k] = k < st.ranges ? st.hi[k] - st.lo[k] : 0;
+  }
+  if (threadIdx.x == 0) s_count = 0;
   __syncthreads();
-  Ranges ranges;
-  deciding_bins(a, r, info, sm, ranges);
   const Row<BF> row(a, r);
   int g0, g1;
   chunk_of(row, c, a.C, g0, g1);
-  const Weigh& weigh = info.weigh;
-  const int lane = threadIdx.x & 63;
   for (int g = g0 + threadIdx.x; g < g1; g += kThreads) {
     float x[Row<BF>::VE];
     row.load(g, x);
+    uint32_t hits = 0;
 #pragma unroll
     for (int j = 0; j < Row<BF>::VE; ++j) {
-      const bool on = weigh.in(x[j]) && weigh.y(x[j]) >= -(double)kMaxExp - 1.0 && ranges.has(weigh.bin(x[j]));
-      const uint64_t all = __builtin_amdgcn_ballot_w64(on);
-      if (all == 0) continue;
-      // one addition per wave; their order does not matter: they are sorted
-      const int first = __ffsll((unsigned long long)all) - 1;
-      int at = 0;
-      if (lane == first) at = atomicAdd(&a.listed[r], __popcll(all));
-      at = __shfl(at, first, 64) + __popcll(all & ((1ull << lane) - 1));
-      if (on && at < kCap)
-        a.list[(size_t)r * kCap + at] = ((uint64_t)~key_of(x[j]) << 32) | (uint32_t)(row.first(g) + j);
+      const uint32_t b = (uint32_t)bin_of(x[j], m, scale);
+      const bool on = x[j] >= cut && ((b - lo[0] <= width[0]) | (b - lo[1] <= width[1]) | (b - lo[2] <= width[2]));
+      hits |= (on ? 1u : 0u) << j;
+    }
+    if (hits == 0) continue;
+#pragma unroll
+    for (int j = 0; j < Row<BF>::VE; ++j) {
+      if (!(hits >> j & 1)) continue;
+      const int at = atomicAdd(&s_count, 1);
+      if (at < kCap) s_list[at] = ((uint64_t)~key_of(x[j]) << 32) | (uint32_t)(row.first(g) + j);
     }
   }
+  __syncthreads();
+  const int n = s_count;
+  if (n == 0) return;
+  if (threadIdx.x == 0) s_at = atomicAdd(&a.listed[r], n);
+  __syncthreads();
+  const int at = s_at;
+  if (at + n > kCap) return;
+  for (int k = threadIdx.x; k < n; k += kThreads) a.list[(size_t)r * kCap + at + k] = s_list[k];
 }
 
 // ---- 4. finish ----------------------------------------------------------------------------------------
 struct FinishSmem {
-  BinSmem bins;
   union {
     struct {
-      uint64_t item[kCap];     // sorted: inverted key, index
-      uint64_t upto[kCap];     // weights up to and including each
-      uint64_t skipped[kBins]; // listed weights before a bin's first listed token
+      uint64_t item[kCap];  // sorted: inverted key, index
+      uint64_t upto[kCap];  // weights up to and including each
     } s;
     RowSmem row;
   };
-  uint64_t value[4];
+  uint64_t wave[kWaves];
+  uint64_t skipped[3], end;
+  int at;
 };
 
 template <bool BF>
 __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
-  __shared__ double s_table[16];
+  __shared__ double s_table[64];
   __shared__ FinishSmem sm;
   const int r = blockIdx.x, tid = threadIdx.x;
+  __shared__ RowState st;
+  const int n = a.listed[r], mode = a.state[r].mode;
+  if (mode == RowState::kDone) return;
+  if (tid == 0) st = mode == RowState::kDigits ? a.state[r] : a.decided[r];
   fill_table(s_table);
-  RowInfo info;
-  if (!row_info(a, r, s_table, info, false)) return;
   __syncthreads();
-  const Weigh& weigh = info.weigh;
-  const float p = a.top_p[r], mp = a.min_p[r], u = clean_u(a.u[r]);
-  const int n = a.listed[r];
-  if (n > kCap || digits_row(a, info.k)) {
+  const Weigh weigh{st.m, 64.0 * st.c, s_table};
+  if (n > kCap || mode == RowState::kDigits) {
     const Row<BF> row(a, r);
     const RowSearch<BF> search{row, weigh, sm.row};
-    const int id = search.sample(info.k, p, mp, u);
+    const int id = search.sample(st.k, st.p, st.min_p, st.u);
     if (tid == 0) a.ids[r] = id;
     return;
   }
-  Ranges ranges;
-  deciding_bins(a, r, info, sm.bins, ranges);
   int size = 64;
   while (size < n) size *= 2;
   for (int k = tid; k < size; k += kThreads) sm.s.item[k] = k < n ? a.list[(size_t)r * kCap + k] : ~0ull;
   __syncthreads();
-  for (int len = 2; len <= size; len *= 2)  // bitonic
+  // Bitonic; each wave keeps to its own share of the items wherever the step lies inside it, so only
+  // the wide steps meet at a barrier.
+  const int share = max(size / kWaves, 64), wv = tid >> 6, lane = tid & 63;
+  for (int len = 2; len <= size; len *= 2)
     for (int step = len / 2; step > 0; step /= 2) {
-      for (int k = tid; k < size / 2; k += kThreads) {
-        const int lo = 2 * k - (k & (step - 1)), hi = lo + step;
-        const uint64_t x = sm.s.item[lo], y = sm.s.item[hi];
-        if ((x > y) == ((lo & len) == 0)) {
-          sm.s.item[lo] = y;
-          sm.s.item[hi] = x;
+      if (step >= share) __syncthreads();
+      if (wv * share < size)
+        for (int k = (wv * share >> 1) + lane; k < ((wv + 1) * share >> 1); k += 64) {
+          const int lo = 2 * k - (k & (step - 1)), hi = lo + step;
+          const uint64_t x = sm.s.item[lo], y = sm.s.item[hi];
+          if ((x > y) == ((lo & len) == 0)) {
+            sm.s.item[lo] = y;
+            sm.s.item[hi] = x;
+          }
         }
-      }
-      __syncthreads();
+      if (step >= share) __syncthreads();
+      else __builtin_amdgcn_wave_barrier();
     }
+  __syncthreads();
   auto logit = [&](int k) { return logit_of(~(uint32_t)(sm.s.item[k] >> 32)); };
-  // Running weights of the list, kCap / kThreads tokens a thread.
+  // Running weights of the row: those of the list (kCap / kThreads tokens a thread), with what lies
+  // before a token's range in place of the list's before it.
+  auto range_of = [&](int k) {
+    const int b = bin_of(logit(k), st.m, st.scale);
+    return (st.ranges > 1 && b >= st.lo[1] ? 1 : 0) + (st.ranges > 2 && b >= st.lo[2] ? 1 : 0);
+  };
   constexpr int PER = kCap / kThreads;
   uint64_t w[PER], sum = 0;
 #pragma unroll
@@ -665,66 +733,54 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
     sum += w[j];
   }
   uint64_t total;
-  uint64_t run = scan64(sum, sm.bins.wave, total) - sum;
+  uint64_t run = scan64(sum, sm.wave, total) - sum;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int k = tid * PER + j;
     if (k < n) {
-      const int b = weigh.bin(logit(k));
-      if (k == 0 || weigh.bin(logit(k - 1)) != b) sm.s.skipped[b] = run;
+      const int g = range_of(k);
+      if (k == 0 || range_of(k - 1) != g) sm.skipped[g] = run;
       sm.s.upto[k] = run + w[j];
     }
     run += w[j];
   }
-  const bool counts = counts_row(a, info.k);
+  if (tid == 0) sm.end = st.above;
   __syncthreads();
-  // ... and of the row: the weights of all bins before, and of the token's own bin up to it.
-  if (!counts) {
-    for (int k = tid; k < n; k += kThreads) {
-      const int b = weigh.bin(logit(k));
-      sm.s.upto[k] += sm.bins.before[b] - sm.s.skipped[b];
-    }
-    __syncthreads();
+  for (int k = tid; k < n; k += kThreads) {
+    const int g = range_of(k);
+    sm.s.upto[k] += st.base[g] - sm.skipped[g];
   }
+  __syncthreads();
   // First listed token whose running weight reaches x.
   auto rank_of = [&](uint64_t x) {
-    if (tid == 0) sm.bins.at[7] = n - 1;
+    if (tid == 0) sm.at = n - 1;
     __syncthreads();
     for (int k = tid; k < n; k += kThreads)
-      if (sm.s.upto[k] >= x && (k == 0 || sm.s.upto[k - 1] < x)) sm.bins.at[7] = k;
+      if (sm.s.upto[k] >= x && (k == 0 || sm.s.upto[k - 1] < x)) sm.at = k;
     __syncthreads();
-    const int k = sm.bins.at[7];
+    const int k = sm.at;
     __syncthreads();
     return k;
   };
-  uint64_t mass;  // of the top-k prefix
-  if (counts) {
-    mass = sm.s.upto[min(info.k, n) - 1];
-  } else {
-    const uint64_t last = a.hist[(size_t)r * kBins + kBins - 1];
-    mass = sm.bins.before[kBins - 1] + last;
-  }
+  const uint64_t mass = mode == RowState::kCounts ? sm.s.upto[min(st.k, n) - 1] : st.total;
   uint64_t kept = mass;
-  if (p < 1.0f) kept = min(kept, sm.s.upto[rank_of(p > 0.0f ? max(ceil_mul(p, mass), (uint64_t)1) : 1)]);
-  if (mp > 0.0f) {
-    // listed tokens are a run of ranks around the border: the last with w >= min_p ends the prefix, or
-    // the bins before the border's first do
-    const double least = (double)fminf(mp, 1.0f);
-    if (tid == 0) sm.value[0] = counts ? 0 : sm.bins.before[ranges.lo[1]];
-    __syncthreads();
+  if (st.p < 1.0f)
+    kept = min(kept, sm.s.upto[rank_of(st.p > 0.0f ? max(ceil_mul(st.p, mass), (uint64_t)1) : 1)]);
+  if (st.min_p > 0.0f) {  // the last listed token past min_p ends that prefix, or the bins before all that may
+    const double least = (double)fminf(st.min_p, 1.0f);
     for (int k = tid; k < n; k += kThreads)
       if (weigh.real(logit(k)) >= least && (k + 1 == n || weigh.real(logit(k + 1)) < least))
-        atomicMax(reinterpret_cast<unsigned long long*>(&sm.value[0]), (unsigned long long)sm.s.upto[k]);
+        atomicMax(reinterpret_cast<unsigned long long*>(&sm.end), (unsigned long long)sm.s.upto[k]);
     __syncthreads();
-    kept = min(kept, sm.value[0]);
+    kept = min(kept, sm.end);
   }
-  const int at = rank_of(floor_mul(u, kept) + 1);
+  const int at = rank_of(floor_mul(st.u, kept) + 1);
   if (tid == 0) a.ids[r] = (int64_t)(uint32_t)sm.s.item[at];
 }
 
 struct SamplePlan {
   int C;
-  size_t o_idx, o_min, o_hist, o_listed, o_list, bytes;
+  size_t o_idx, o_min, o_hist, o_state, o_decided, o_listed, o_list, bytes;
 };
 
 constexpr int kRows = 2048;  // rows at a time: a row has 48 KB of workspace
@@ -733,14 +789,16 @@ SamplePlan sample_plan(int R, int V) {
   SamplePlan p{};
   if (R < 1 || V < 1 || V > 1 << 20 || R > 65535) return p;
   R = R < kRows ? R : kRows;
-  // Workgroups per row: two per CU in all, chunks of 4096 tokens at least.
-  p.C = max(1, min(512 / R, (V + 4095) / 4096));
+  // Workgroups per row: two per CU in all, and more of at most 32768 tokens each (rows differ in cost), chunks of 4096 tokens at least.
+  p.C = max(1, max(min(512 / R, (V + 4095) / 4096), V / 32768));
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   const size_t chunks = up((size_t)R * p.C * 4);
   p.o_idx = chunks;
   p.o_min = 2 * chunks;
   p.o_hist = 3 * chunks;
-  p.o_listed = p.o_hist + (size_t)R * kBins * 8;
+  p.o_state = p.o_hist + (size_t)R * kBins * 8;
+  p.o_decided = p.o_state + up((size_t)R * sizeof(RowState));
+  p.o_listed = p.o_decided + up((size_t)R * sizeof(RowState));
   p.o_list = p.o_listed + up((size_t)R * 4);
   p.bytes = p.o_list + (size_t)R * kCap * 8;
   return p;
@@ -775,6 +833,7 @@ extern "C" int npn_sample(const void* logits, int bf16, const float* temperature
                        top_k + r0, top_p + r0, min_p + r0, u + r0, ids + r0, n, V, p.C,
                        reinterpret_cast<float*>(ws), reinterpret_cast<int32_t*>(ws + p.o_idx),
                        reinterpret_cast<float*>(ws + p.o_min), reinterpret_cast<uint64_t*>(ws + p.o_hist),
+                       reinterpret_cast<RowState*>(ws + p.o_state), reinterpret_cast<RowState*>(ws + p.o_decided),
                        reinterpret_cast<int32_t*>(ws + p.o_listed), reinterpret_cast<uint64_t*>(ws + p.o_list)};
     if (bf16) sample_launch<true>(a, static_cast<hipStream_t>(stream));
     else sample_launch<false>(a, static_cast<hipStream_t>(stream));
