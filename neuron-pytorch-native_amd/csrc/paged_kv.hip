@@ -82,20 +82,34 @@ __device__ __forceinline__ Req load_req(const PlanArgs& a, int b) {
   return r;
 }
 
-// The request (index in this group of kPlanThreads) whose moves hold item i: the first with
-// upto > i, upto the inclusive prefix sums.
-__device__ __forceinline__ int find_req(const int* upto, int i) {
-  int lo = 0, n = kPlanThreads;
-  while (n > 1) {
-    const int half = n >> 1;
-    if (upto[lo + half - 1] <= i) {
-      lo += half;
-      n -= half;
-    } else {
-      n = half;
+// Moves i = 0 .. n - 1 of a group of requests, one a thread and four at a time in flight: a move's
+// request is the first whose inclusive prefix sum `upto` passes i, its table entry counts from there.
+// from(i, entry) is where the block's id lies, to(i, entry, id) takes it. (One at a time, 16384 blocks'
+// searches and round trips to memory took 18 us.)
+template <class From, class To>
+__device__ __forceinline__ void move_blocks(const PlanArgs& a, const int* upto, const int* at, int b0, int n,
+                                            From from, To to) {
+  for (int i0 = threadIdx.x; i0 < n; i0 += 4 * kPlanThreads) {
+    int i[4], q[4] = {0, 0, 0, 0};
+    int32_t* entry[4];
+    int32_t id[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) i[k] = min(i0 + k * kPlanThreads, n - 1);
+#pragma unroll
+    for (int half = kPlanThreads / 2; half > 0; half /= 2)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) q[k] += upto[q[k] + half - 1] <= i[k] ? half : 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int before = q[k] > 0 ? upto[q[k] - 1] : 0;
+      entry[k] = a.table + (size_t)(b0 + q[k]) * a.P + at[q[k]] + (i[k] - before);
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) id[k] = *from(i[k], entry[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (i0 + k * kPlanThreads < n) to(i[k], entry[k], id[k]);
   }
-  return lo;
 }
 
 __device__ __forceinline__ int64_t slot_of(const PlanArgs& a, int b, int t, int kv, int granted) {
@@ -129,14 +143,12 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
       s_upto[tid] = upto;
       s_at[tid] = r.want;
       __syncthreads();
-      for (int i = tid; i < total; i += kPlanThreads) {
-        const int q = find_req(s_upto, i);
-        const int first = q > 0 ? s_upto[q - 1] : 0;
-        int32_t* e = a.table + (size_t)(b0 + q) * a.P + s_at[q] + (i - first);
-        const int64_t at = (int64_t)count0 + (given - 1 - (run + i));
-        if (at < a.N) a.stack[at] = *e;
-        *e = -1;
-      }
+      move_blocks(a, s_upto, s_at, b0, total, [&](int, int32_t* entry) { return entry; },
+                  [&](int i, int32_t* entry, int32_t id) {
+                    const int64_t at = (int64_t)count0 + (given - 1 - (run + i));
+                    if (at < a.N) a.stack[at] = id;
+                    *entry = -1;
+                  });
       run += total;
       __syncthreads();
     }
@@ -159,11 +171,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
     s_upto[tid] = moved;
     s_at[tid] = r.held;
     __syncthreads();
-    for (int i = tid; i < took; i += kPlanThreads) {
-      const int q = find_req(s_upto, i);
-      const int first = q > 0 ? s_upto[q - 1] : 0;
-      a.table[(size_t)(b0 + q) * a.P + s_at[q] + (i - first)] = a.stack[count - 1 - (taken + i)];
-    }
+    move_blocks(a, s_upto, s_at, b0, took, [&](int i, int32_t*) { return a.stack + (count - 1 - (taken + i)); },
+                [&](int, int32_t* entry, int32_t id) { *entry = id; });
     taken += took;
     asked += total;
     if (b < a.B) {
@@ -212,7 +221,7 @@ __global__ __launch_bounds__(256) void paged_slots_kernel(PlanArgs a) {
 // the block's first row is new, else max(old, need), and older rows move to it; new rows are
 // round-to-nearest-even e4m3(x / scale). NaN and infinities are stored as NaN and leave the scale.
 //
-// One workgroup of four waves per (request, block touched, head, K or V): it owns the page, so the
+// One workgroup per (request, block touched, head, K or V): it owns the page, so the
 // scale and the older rows need no atomics. Lane l of a wave holds dims 4l..4l+3 of its rows in
 // registers from the first load to the rounding (RPW rows per wave), so each input is read once.
 struct PagedAppendArgs {
@@ -261,8 +270,22 @@ __device__ __forceinline__ uint32_t rescale_e4m3(uint32_t w, float by) {
   return to_e4m3(x, by);
 }
 
-template <int RPW>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
+// Sum over the wave: inside 16-lane rows by DPP, then across them by gfx950's row swaps.
+__device__ __forceinline__ float wave_sum_valu(float v) {
+  v += __uint_as_float(npn::dpp32<npn::kDppStep[0]>(__float_as_uint(v)));
+  v += __uint_as_float(npn::dpp32<npn::kDppStep[1]>(__float_as_uint(v)));
+  v += __uint_as_float(npn::dpp32<npn::kDppStep[2]>(__float_as_uint(v)));
+  v += __uint_as_float(npn::dpp32<npn::kDppStep[3]>(__float_as_uint(v)));
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// NW waves, RPW rows each: below 4 rows w, w + NW, ..; from 4 on blocks of four rows w, w + NW, .., whose 4 x 4
+// bytes a lane turns from rows into dims in registers.
+template <int RPW, int NW>
+__global__ __launch_bounds__(NW * 64, RPW == 16 ? 2 : 4) void paged_append_kernel(PagedAppendArgs a) {
   const int b = blockIdx.z, h = blockIdx.y >> 1;
   const bool is_v = blockIdx.y & 1;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -275,71 +298,83 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
   const int off0 = (int)(first & (bs - 1));
   const int t0 = blockIdx.x == 0 ? 0 : bs - off0 + ((int)blockIdx.x - 1) * bs;
   if (t0 >= a.T) return;
+  const int room = min(blockIdx.x == 0 ? bs - off0 : bs, a.T - t0);
+  auto row_of = [&](int i) { return RPW < 4 ? w + NW * i : 4 * (w + NW * (i >> 2)) + (i & 3); };
+
+  // This wave's rows, from the input once (those past the last one repeat it and go nowhere).
+  uint2 in[RPW];
+  const uint16_t* src = (is_v ? a.value : a.key) + (((size_t)b * a.T + t0) * a.Hkv + h) * DH + 4 * lane;
+#pragma unroll
+  for (int i = 0; i < RPW; ++i)
+    in[i] = *reinterpret_cast<const uint2*>(src + (size_t)min(row_of(i), room - 1) * a.Hkv * DH);
   const int64_t slot = slots[t0];
   if (slot < 0 || slot >= (int64_t)a.N << a.sh) return;
   const int64_t block = slot >> a.sh;
   const int off = (int)(slot & (bs - 1));
+  const int most = min(bs - off, room);
+  float x[RPW][4];
+#pragma unroll
+  for (int i = 0; i < RPW; ++i) {
+    x[i][0] = npn::bf16lo(in[i].x);
+    x[i][1] = npn::bf16hi(in[i].x);
+    x[i][2] = npn::bf16lo(in[i].y);
+    x[i][3] = npn::bf16hi(in[i].y);
+  }
+  // Padding, or another block, may begin before the block ends.
   __shared__ int s_rows;
-  if (threadIdx.x == 0) s_rows = min(bs - off, a.T - t0);
+  __shared__ float s_amax[NW];
+  if (threadIdx.x == 0) s_rows = most;
   __syncthreads();
-  if ((int)threadIdx.x < min(bs - off, a.T - t0) && slots[t0 + threadIdx.x] != slot + threadIdx.x)
-    atomicMin(&s_rows, (int)threadIdx.x);  // padding (or another block) begins here
+  if ((int)threadIdx.x < most && slots[t0 + threadIdx.x] != slot + threadIdx.x)
+    atomicMin(&s_rows, (int)threadIdx.x);
   __syncthreads();
   const int rows = s_rows;
 
-  // This wave's rows w, w + 4, ... of them.
-  float x[RPW][4];
-  const uint16_t* src = (is_v ? a.value : a.key) + (((size_t)b * a.T + t0) * a.Hkv + h) * DH + 4 * lane;
-#pragma unroll
-  for (int i = 0; i < RPW; ++i) {
-    const int r = w + 4 * i;
-    uint2 u = make_uint2(0u, 0u);
-    if (r < rows) u = *reinterpret_cast<const uint2*>(src + (size_t)r * a.Hkv * DH);
-    x[i][0] = npn::bf16lo(u.x);
-    x[i][1] = npn::bf16hi(u.x);
-    x[i][2] = npn::bf16lo(u.y);
-    x[i][3] = npn::bf16hi(u.y);
-  }
-  float amax = 0.f;
   if (!is_v) {
     const float4 nw = *reinterpret_cast<const float4*>(a.k_norm + 4 * lane);
     const float wt[4] = {1.0f + nw.x, 1.0f + nw.y, 1.0f + nw.z, 1.0f + nw.w};
     const int64_t pos0 = (int64_t)a.kv_len[b] + t0;
+    constexpr int BATCH = RPW < 4 ? RPW : 4;  // rows whose RoPE rows are loaded at a time, without branches
 #pragma unroll
-    for (int i = 0; i < RPW; ++i) {
-      const int r = w + 4 * i;
-      if (r >= rows) break;  // wave-uniform
-      const float ss = npn::wave_sum(x[i][0] * x[i][0] + x[i][1] * x[i][1] + x[i][2] * x[i][2] +
-                                     x[i][3] * x[i][3]);
-      const float rn = rsqrtf(ss * (1.0f / DH) + kEps);
-      float y[4];
+    for (int i0 = 0; i0 < RPW; i0 += BATCH) {
+      float4 c[BATCH], s[BATCH];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[i][j] = wt[j] * (x[i][j] * rn);
-        y[j] = __shfl_xor(x[i][j], 8, 64);  // dim d ^ 32
-      }
-      if (lane < ROPE / 4) {
-        int64_t pos = pos0 + r;
+      for (int k = 0; k < BATCH; ++k) {
+        int64_t pos = pos0 + min(row_of(i0 + k), most - 1);
         pos = pos < 0 ? 0 : (pos >= a.positions ? a.positions - 1 : pos);
-        const float4 c = *reinterpret_cast<const float4*>(a.cos + pos * ROPE + 4 * lane);
-        const float4 s = *reinterpret_cast<const float4*>(a.sin + pos * ROPE + 4 * lane);
+        c[k] = *reinterpret_cast<const float4*>(a.cos + pos * ROPE + 4 * (lane & 15));
+        s[k] = *reinterpret_cast<const float4*>(a.sin + pos * ROPE + 4 * (lane & 15));
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        float* v = x[i0 + k];
+        const float ss = wave_sum_valu(v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3]);
+        const float rn = rsqrtf(ss * (1.0f / DH) + kEps);
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[j] = wt[j] * (v[j] * rn);
+          y[j] = __shfl_xor(v[j], 8, 64);  // dim d ^ 32
+        }
         const float sg = lane < ROPE / 8 ? -1.0f : 1.0f;
-        x[i][0] = x[i][0] * c.x + sg * y[0] * s.x;
-        x[i][1] = x[i][1] * c.y + sg * y[1] * s.y;
-        x[i][2] = x[i][2] * c.z + sg * y[2] * s.z;
-        x[i][3] = x[i][3] * c.w + sg * y[3] * s.w;
+        const float t[4] = {v[0] * c[k].x + sg * y[0] * s[k].x, v[1] * c[k].y + sg * y[1] * s[k].y,
+                            v[2] * c[k].z + sg * y[2] * s[k].z, v[3] * c[k].w + sg * y[3] * s[k].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = lane < ROPE / 4 ? t[j] : v[j];
       }
     }
   }
+  float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < RPW; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) amax = fmaxf(amax, finite(x[i][j]) ? fabsf(x[i][j]) : 0.f);
-  __shared__ float s_amax[4];
+    for (int j = 0; j < 4; ++j)
+      amax = fmaxf(amax, row_of(i) < rows && finite(x[i][j]) ? fabsf(x[i][j]) : 0.f);
   amax = npn::wave_max(amax);
   if (lane == 0) s_amax[w] = amax;
   __syncthreads();
-  amax = fmaxf(fmaxf(s_amax[0], s_amax[1]), fmaxf(s_amax[2], s_amax[3]));
+#pragma unroll
+  for (int k = 0; k < NW; ++k) amax = fmaxf(amax, s_amax[k]);
   float* scale = (is_v ? a.v_scale : a.k_scale) + block * a.Hkv + h;
   const float need = scale_of(amax);
   const float old = off > 0 ? *scale : need;
@@ -352,55 +387,78 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
   if (!is_v) {
     uint8_t* page = a.cache_k + ((size_t)block * a.Hkv + h) * ((size_t)DH << a.sh) + 4 * lane;
     if (grew)
-      for (int r = w; r < off; r += 4) {
+      for (int r = w; r < off; r += NW) {
         uint32_t* p = reinterpret_cast<uint32_t*>(page + (size_t)r * DH);
         *p = rescale_e4m3(*p, by);
       }
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
-      const int r = w + 4 * i;
-      if (r >= rows) break;
-      *reinterpret_cast<uint32_t*>(page + (size_t)(off + r) * DH) = to_e4m3(x[i], inv);
+      const int r = row_of(i);
+      if (r < rows) *reinterpret_cast<uint32_t*>(page + (size_t)(off + r) * DH) = to_e4m3(x[i], inv);
     }
     return;
   }
-  // V: the rows become columns. Bytes go through LDS as [dim][row] (16 bytes of padding per dim
-  // keep the four-dim writes of a row off one bank), then thread d reads, changes and writes the
-  // 16-row groups of dim d that hold new rows (or older ones, if the scale grew); the page is this
-  // workgroup's alone, and bytes of rows that it does not touch go back as they were.
-  constexpr int kStride = RPW * 4 + 16;
-  __shared__ __attribute__((aligned(16))) uint8_t s_v[DH * kStride];
+  // V: the rows become columns, through LDS as [dim][row]. Dim d lies in line 64 (d % 4) + d / 4, of an
+  // odd number of words, so that a wave's writes of four rows (or one) of a dim a lane meet no bank
+  // twice (or four times).
+  constexpr int kLine = RPW < 4 ? (RPW * NW + 3) / 4 | 1 : RPW * NW / 4 + 1;  // words
+  __shared__ uint32_t s_v[DH * kLine];
+  uint8_t* bytes = reinterpret_cast<uint8_t*>(s_v);
+  if constexpr (RPW < 4) {
 #pragma unroll
-  for (int i = 0; i < RPW; ++i) {
-    const int r = w + 4 * i;
-    if (r >= rows) break;
-    const uint32_t q = to_e4m3(x[i], inv);
+    for (int i = 0; i < RPW; ++i) {
+      const uint32_t q = to_e4m3(x[i], inv);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s_v[(4 * lane + j) * kStride + r] = (uint8_t)(q >> (8 * j));
+      for (int j = 0; j < 4; ++j) bytes[(64 * j + lane) * kLine * 4 + w + NW * i] = (uint8_t)(q >> (8 * j));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < RPW; i += 4) {
+      const uint32_t q0 = to_e4m3(x[i], inv), q1 = to_e4m3(x[i + 1], inv);
+      const uint32_t q2 = to_e4m3(x[i + 2], inv), q3 = to_e4m3(x[i + 3], inv);
+      const uint32_t a0 = __builtin_amdgcn_perm(q1, q0, 0x05010400u);  // rows 0, 1 of dims 0, 1
+      const uint32_t a1 = __builtin_amdgcn_perm(q1, q0, 0x07030602u);  // and of dims 2, 3
+      const uint32_t b0 = __builtin_amdgcn_perm(q3, q2, 0x05010400u);
+      const uint32_t b1 = __builtin_amdgcn_perm(q3, q2, 0x07030602u);
+      const uint32_t d[4] = {__builtin_amdgcn_perm(b0, a0, 0x05040100u), __builtin_amdgcn_perm(b0, a0, 0x07060302u),
+                             __builtin_amdgcn_perm(b1, a1, 0x05040100u), __builtin_amdgcn_perm(b1, a1, 0x07060302u)};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s_v[(64 * j + lane) * kLine + w + NW * (i >> 2)] = d[j];
+    }
   }
   __syncthreads();
-  const int d = threadIdx.x;
-  uint8_t* page = a.cache_v + ((size_t)block * a.Hkv + h) * ((size_t)DH << a.sh) + ((size_t)d << a.sh);
-  const uint8_t* sv = s_v + d * kStride;
-  const int end = off + rows;
-  for (int g = grew ? 0 : off & ~15; g < end; g += 16) {
-    uint4 v = *reinterpret_cast<const uint4*>(page + g);
+  // 16 rows of a dim at a time, all that hold new rows (or older ones, if the scale grew); neighbours
+  // write neighbouring 16 bytes. The page is this workgroup's alone, and bytes of rows that it does
+  // not touch go back as they were.
+  uint8_t* page = a.cache_v + ((size_t)block * a.Hkv + h) * ((size_t)DH << a.sh);
+  const int end = off + rows, g0 = grew ? 0 : off >> 4, groups = ((end + 15) >> 4) - g0;
+  for (int k = threadIdx.x; k < DH * groups; k += NW * 64) {
+    const int d = k / groups, g = (g0 + k - d * groups) * 16;
+    const uint32_t* line = s_v + (64 * (d & 3) + (d >> 2)) * kLine;
+    uint4* dst = reinterpret_cast<uint4*>(page + ((size_t)d << a.sh) + g);
+    if (RPW >= 4 && g >= off && g + 16 <= end && (off & 3) == 0) {
+      const uint32_t* v = line + ((g - off) >> 2);
+      *dst = make_uint4(v[0], v[1], v[2], v[3]);
+      continue;
+    }
+    const uint4 v = *dst;
     uint32_t word[4] = {v.x, v.y, v.z, v.w};
+    const uint8_t* sv = reinterpret_cast<const uint8_t*>(line);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int r0 = g + 4 * k;
-      const uint32_t moved = grew && r0 < off ? rescale_e4m3(word[k], by) : word[k];
+    for (int q = 0; q < 4; ++q) {
+      const int r0 = g + 4 * q;
+      const uint32_t moved = grew && r0 < off ? rescale_e4m3(word[q], by) : word[q];
       uint32_t out = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = r0 + j;
-        uint32_t byte = ((r < off ? moved : word[k]) >> (8 * j)) & 0xFFu;
+        uint32_t byte = ((r < off ? moved : word[q]) >> (8 * j)) & 0xFFu;
         if (r >= off && r < end) byte = sv[r - off];
         out |= byte << (8 * j);
       }
-      word[k] = out;
+      word[q] = out;
     }
-    *reinterpret_cast<uint4*>(page + g) = make_uint4(word[0], word[1], word[2], word[3]);
+    *dst = make_uint4(word[0], word[1], word[2], word[3]);
   }
 }
 
@@ -460,13 +518,13 @@ extern "C" int npn_gqa_kv_append_paged(const uint16_t* key, const uint16_t* valu
   // A request's rows touch at most 1 + ceil((T - 1) / bs) blocks.
   const dim3 grid(1 + (T - 1 + block_size - 1) / block_size, 2 * kv_heads, B);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int rpw = ((T < block_size ? T : block_size) + 3) / 4;
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
-  if (rpw <= 1) launch(paged_append_kernel<1>);
-  else if (rpw <= 2) launch(paged_append_kernel<2>);
-  else if (rpw <= 4) launch(paged_append_kernel<4>);
-  else if (rpw <= 8) launch(paged_append_kernel<8>);
-  else if (rpw <= 16) launch(paged_append_kernel<16>);
-  else launch(paged_append_kernel<32>);
+  const int rows = T < block_size ? T : block_size;
+  auto launch = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, s, a); };
+  if (rows <= 4) launch(paged_append_kernel<1, 4>, 4);
+  else if (rows <= 8) launch(paged_append_kernel<2, 4>, 4);
+  else if (rows <= 16) launch(paged_append_kernel<4, 4>, 4);
+  else if (rows <= 32) launch(paged_append_kernel<4, 8>, 8);
+  else if (rows <= 64) launch(paged_append_kernel<8, 8>, 8);
+  else launch(paged_append_kernel<16, 8>, 8);
   return npn_launch_status();
 }
