@@ -9,6 +9,8 @@ per sequence instead of one:
       DeltaNet layer: fp8 in-proj [qkv | z | a | b] -> deltanet::verify_from_ckpt -> fp8 out-proj
       GQA layer:      fp8 [q+gate | k | v] -> gqa::tail_verify_append (k norm + RoPE + KV
                       append in the attention's query-prep launch) -> fp8 o-proj
+                      (with a paged e4m3 cache: paged::update_blocks_ once a step, then
+                      gqa::kv_append_paged -> gqa::tail_verify_paged per layer)
     -> residual -> post RMSNorm(1+w) -> fp8 gate/up -> SiLU * up -> fp8 down -> residual
   logits -> spec::accept_rejection (or accept_greedy)
   rollback: DeltaNet state = checkpoint[accepted] (read in place by the next step),
@@ -112,8 +114,11 @@ class VerifySlice:
     with the decode state of B sequences."""
 
     def __init__(self, B, K, kv_lens, s_max, pattern="DDDG", seed=0, device="cuda",
-                 fuse_splitk=True, fuse_swiglu=True, fuse_launches=True):
+                 fuse_splitk=True, fuse_swiglu=True, fuse_launches=True, paged_block=None):
+        """paged_block: None for dense bf16 KV caches, or the block size of a paged e4m3 cache
+        with one block table for all GQA layers, planned on the device at every step."""
         self.B, self.K, self.T = B, K, K + 1
+        self.paged_block = paged_block
         self.fuse_splitk = fuse_splitk
         self.fuse_swiglu = fuse_swiglu
         self.fuse_launches = fuse_launches
@@ -147,11 +152,27 @@ class VerifySlice:
                 L["o_proj"] = random_fp8_linear(HIDDEN, GQA_HQ * GQA_DH, g, device)
                 L["q_norm"] = torch.randn(GQA_DH, generator=g, device=device) * 0.1
                 L["k_norm"] = torch.randn(GQA_DH, generator=g, device=device) * 0.1
-                shape = (B, GQA_HKV, s_max, GQA_DH)
-                L["cache_k"] = torch.randn(shape, generator=g, device=device).to(torch.bfloat16)
-                L["cache_v"] = torch.randn(shape, generator=g, device=device).to(torch.bfloat16)
+                if paged_block is None:
+                    shape = (B, GQA_HKV, s_max, GQA_DH)
+                    L["cache_k"] = torch.randn(shape, generator=g, device=device).to(torch.bfloat16)
+                    L["cache_v"] = torch.randn(shape, generator=g, device=device).to(torch.bfloat16)
+                else:  # N(0, 1) rows over a scale of 2^-6, which takes them to 7 without clipping
+                    n = B * -(-s_max // paged_block)
+                    for name, shape in (("k", (n, GQA_HKV, paged_block, GQA_DH)),
+                                        ("v", (n, GQA_HKV, GQA_DH, paged_block))):
+                        x = torch.randn(shape, generator=g, device=device) * 64
+                        L[f"cache_{name}"] = x.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.int8)
+                        L[f"{name}_scale"] = torch.full(shape[:2], 2.0 ** -6, device=device)
             self.layers.append(L)
         self.kv_len = torch.as_tensor(kv_lens, dtype=torch.int32, device=device).clone()
+        if paged_block is not None:
+            i32 = dict(dtype=torch.int32, device=device)
+            P = -(-s_max // paged_block)
+            self.pages = {"table": torch.full((B, P), -1, **i32), "held": torch.zeros(B, **i32),
+                          "free": torch.randperm(B * P, generator=g, device=device).int(),
+                          "count": torch.full((1,), B * P, **i32)}
+            self.new_len = torch.full((B,), self.T, **i32)
+            self._plan_pages(torch.zeros(B, **i32))  # the blocks of the rows that are there
         # RoPE table of every cache position, built once (the reference's _init_rope); each
         # step gathers the rows of its T positions.
         self.rope_cos, self.rope_sin = rope_tables(torch.arange(s_max, device=device))
@@ -160,6 +181,12 @@ class VerifySlice:
         self.persistent = False
         self.parity = 0
         self.graphs = None
+
+    def _plan_pages(self, new_len):
+        """Blocks for new_len more rows of every sequence (and those past them given back)."""
+        p = self.pages
+        return torch.ops.paged.update_blocks_(self.kv_len, new_len, p["table"], p["held"], p["free"],
+                                              p["count"], self.paged_block, self.T)
 
     # ---- layers: each takes the normed input and returns the residual delta -------------
     def _deltanet(self, L, h):
@@ -207,7 +234,15 @@ class VerifySlice:
         gate = gate.reshape(B, T, GQA_HQ, GQA_DH)
         key = key.reshape(B, T, GQA_HKV, GQA_DH)
         value = value.reshape(B, T, GQA_HKV, GQA_DH)
-        if cos is None:  # append, RoPE rows from the tables and attention in one op
+        if self.paged_block is not None:
+            slots, granted = self.plan
+            pages = (L["cache_k"], L["cache_v"], L["k_scale"], L["v_scale"])
+            self.timer("gqa.kv_append_paged", torch.ops.gqa.kv_append_paged, key, value, L["k_norm"],
+                       self.rope_cos, self.rope_sin, self.kv_len, slots, *pages)
+            attn = self.timer("gqa.tail_verify_paged", torch.ops.gqa.tail_verify_paged, query, gate,
+                              L["q_norm"], self.rope_cos, self.rope_sin, *pages, self.pages["table"],
+                              self.kv_len, granted)
+        elif cos is None:  # append, RoPE rows from the tables and attention in one op
             attn = self.timer("gqa.tail_verify_append", torch.ops.gqa.tail_verify_append,
                               query, gate, key, value, L["q_norm"], L["k_norm"], self.rope_cos,
                               self.rope_sin, L["cache_k"], L["cache_v"], self.kv_len)
@@ -249,7 +284,11 @@ class VerifySlice:
         whose results the fused op equals bit for bit. If `trace` is a list,
         the residual stream entering each sublayer (mixer, then MLP, per layer) and the final
         hidden are appended to it."""
-        if cos is None and not self.fuse_launches and "G" in self.pattern:
+        if self.paged_block is not None and "G" in self.pattern:
+            if cos is not None:
+                raise ValueError("the paged cache takes its RoPE rows from the tables")
+            self.plan = self.timer("paged.update_blocks", self._plan_pages, self.new_len)
+        elif cos is None and not self.fuse_launches and "G" in self.pattern:
             cos, sin = self.timer("gqa.rope_rows", torch.ops.gqa.rope_rows, self.rope_cos,
                                   self.rope_sin, self.kv_len, self.T)
         layers = self.layers
