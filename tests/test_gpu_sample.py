@@ -105,3 +105,28 @@ def test_sample_refusals(ops):
                         (5, torch.ones(3).cuda(), RuntimeError)):
         with pytest.raises(err):
             ops.spec.sample(*[bad if j == i else a for j, a in enumerate(args)])
+
+
+@pytest.mark.parametrize("R,V,kind", [
+    (16, 100003, "ascending"), (16, 100003, "descending"), (300, 9001, "descending"), (16, 100003, "block"),
+    (16, 100003, "few"), (16, 100003, "infinite"), (3, 3, "infinite"), (8, 1 << 20, "flat"), (513, 40000, "flat"),
+])
+def test_sample_top_k_wherever_the_largest_lie(ops, R, V, kind):
+    """Every size of top-k, with the row's largest logits spread, sorted, side by side, or fewer than k."""
+    rng = np.random.default_rng(R * V + len(kind))
+    x = rng.standard_normal((R, V)).astype(np.float32)
+    if kind == "ascending":
+        x.sort(axis=1)
+    elif kind == "descending":
+        x = -np.sort(-x, axis=1)
+    elif kind == "block":
+        x[:, 5001:10101] += 20
+    elif kind == "few":
+        x[rng.random((R, V)) > 40 / V] = -INF
+        x[:, 77] = 1
+    elif kind == "infinite":
+        x[rng.random((R, V)) < max(0.01, 1 / V)] = INF
+    s = _settings(R, rng)
+    s["temperature"][:] = rng.choice([0.3, 1.0, 5.0], R)
+    s["top_k"] = np.resize(np.array([1, 7, 64, 700, 1200, 1201, 2047, 2048, 2049, 3100, 4095, 4096, 4097], np.int32), R)
+    _check(ops, torch.from_numpy(x), s)
