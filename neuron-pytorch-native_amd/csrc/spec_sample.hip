@@ -32,13 +32,13 @@
 //     (thousands of equal logits), or a longer top-k, is searched by the digits of its keys instead,
 //     which reads it some ten times.
 //
-// Measured on 256 rows of 151936 bf16 logits (78 MB, in the caches after the first pass), settings mixed:
-// 25 + 43 + 44 + 12 us for the four launches where one reading from HBM takes 13; 32 rows in float 7 + 10
-// + 13 + 11, one row of 151936 4.5 + 5.5 + 7 + 4.4. All passes are bound by instructions to an element,
-// not by the loads: three loads in flight instead of one made each slower (max 25 -> 36, hist 66 -> 110
-// us), and taking the cleaning of NaN and -0 out of the loads, maxima by groups of 16 bytes and t for
-// weight and bin at once made them 1.3 times faster. The weights' pass is the longest, 66 us when no row
-// has a top-k, some 26 vector instructions a token, most of them in 64 bits.
+// Measured on 256 rows of 248320 bf16 logits (127 MB), settings mixed: 25 + 43 + 38 + 12 us for the four
+// launches, where one reading takes 21 from HBM at 6.15 TB/s; on 32 rows of 151936 in float 7 + 11 + 12 +
+// 11 us, on one 4.4 + 5.4 + 7 + 4.4. The first pass runs at 5.1 TB/s. The others are bound by instructions:
+// three loads in flight instead of one made them slower (all rows without top-k: histogram 66 -> 110 us),
+// while loads without the cleaning of NaN and -0, maxima by groups of 16 bytes, and one t for both weight
+// and bin made them 1.3 times faster. Weights are the longest, 66 us when no row has a top-k, next the
+// start of collect, some 6 us for each of the rounds that its workgroups run in.
 #include "npn_common.h"
 
 namespace {
@@ -527,7 +527,7 @@ __device__ __forceinline__ void range_logits(RowState& o) {
   }
 }
 
-// Every workgroup of a row does this for itself, some 4 us: once a row, by the last of the histogram's
+// In collect every workgroup of a row does this for itself: once a row, by the last of the histogram's
 // workgroups to arrive, the fence that its sums need cost 20 times the histogram.
 // The deciding bins into o (in LDS), from this thread's bins 2 tid and 2 tid + 1.
 __device__ __forceinline__ void decide(const uint64_t (&h)[2], RowState& o, BinSmem& sm) {
@@ -643,7 +643,7 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleArgs a) {
   for (int b = tid; b < kBins; b += kThreads) s_hist[b] = 0;
   fill_table(s_table);
   __syncthreads();
-  const RowState& st = s_state;
+  RowState& st = s_state;
   if (st.mode == RowState::kDone || st.mode == RowState::kDigits) return;
   const bool tops = st.mode == RowState::kTops, counts = st.mode == RowState::kCounts;
   if (tops && c != 0) return;
@@ -685,9 +685,16 @@ __global__ __launch_bounds__(kThreads) void sample_hist_kernel(SampleArgs a) {
     }
   }
   __syncthreads();
+  if (tops) {  // all of the row's counts are here
+    __shared__ BinSmem s_bins;
+    const uint64_t h[2] = {s_hist[2 * tid], s_hist[2 * tid + 1]};
+    decide(h, st, s_bins);
+    if (tid == 0) a.decided[r] = st;
+    return;
+  }
   unsigned long long* hist = reinterpret_cast<unsigned long long*>(a.hist + (size_t)r * kBins);
   for (int b = tid; b < kBins; b += kThreads) {
-    if (a.C == 1 || tops) hist[b] = s_hist[b];
+    if (a.C == 1) hist[b] = s_hist[b];
     else if (s_hist[b] != 0) atomicAdd(&hist[b], (unsigned long long)s_hist[b]);
   }
 }
@@ -702,17 +709,22 @@ __global__ __launch_bounds__(kThreads, 8) void sample_collect_kernel(SampleArgs 
   const int c = blockIdx.x, r = blockIdx.y;
   __shared__ BinSmem bins;
   __shared__ RowState st;
-  const uint64_t* hist = a.hist + (size_t)r * kBins + 2 * threadIdx.x;
-  const uint64_t h[2] = {hist[0], hist[1]};
   const int mode = a.state[r].mode;
   if (mode == RowState::kDone || mode == RowState::kDigits) return;
-  if (threadIdx.x == 0) {
-    st = a.state[r];
-    s_count = 0;
-  }
+  const bool tops = mode == RowState::kTops;
+  const uint64_t* hist = a.hist + (size_t)r * kBins + 2 * threadIdx.x;
+  const uint64_t h[2] = {tops ? 0 : hist[0], tops ? 0 : hist[1]};
+  constexpr int kWords = sizeof(RowState) / 4;
+  if (threadIdx.x < kWords)
+    reinterpret_cast<uint32_t*>(&st)[threadIdx.x] =
+        reinterpret_cast<const uint32_t*>(tops ? &a.decided[r] : &a.state[r])[threadIdx.x];
+  if (threadIdx.x == 0) s_count = 0;
   __syncthreads();
-  decide(h, st, bins);
-  if (c == 0 && threadIdx.x == 0) a.decided[r] = st;
+  if (!tops) {
+    decide(h, st, bins);
+    if (c == 0 && threadIdx.x < kWords)
+      reinterpret_cast<uint32_t*>(&a.decided[r])[threadIdx.x] = reinterpret_cast<const uint32_t*>(&st)[threadIdx.x];
+  }
   float least[3], most[3];
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
@@ -727,6 +739,9 @@ __global__ __launch_bounds__(kThreads, 8) void sample_collect_kernel(SampleArgs 
     const int at = atomicAdd(&s_count, 1);
     if (at < kCap) s_list[at] = ((uint64_t)~key_of(x + 0.0f) << 32) | (uint32_t)e;
   };
+  // Lanes whose group's maximum is too small have nothing to list.
+  if (tops && !(a.tops[(size_t)r * a.G + ((c * kThreads + threadIdx.x) >> a.gl)] >= least[0]))
+    g1 = g0;
   for (int g = g0 + threadIdx.x; g < g1; g += kThreads) {
     float x[Row<BF>::VE];
     row.load(g, x);
@@ -820,8 +835,7 @@ __device__ __forceinline__ void sort_items(FinishSmem& sm, const RowState& st, i
     if (k < n) {
       mine[j] = item[k];
       place[j] = atomicAdd(&sm.s.start[bin(mine[j])], 1u);
-      // A bin too full to be searched item by item: 96 of 4096, which takes the 10 us or so of the
-      // 78 steps below.
+      // A bin too full to be searched item by item (96 of 4096): as many compares as the steps below.
       if (place[j] * n > 400000) sm.at = 1;
     }
   }
@@ -882,7 +896,10 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a) {
   int n = a.listed[r];
   const int mode = a.state[r].mode;
   if (mode == RowState::kDone) return;
-  if (tid == 0) st = mode == RowState::kDigits ? a.state[r] : a.decided[r];
+  constexpr int kWords = sizeof(RowState) / 4;
+  if (tid < kWords)
+    reinterpret_cast<uint32_t*>(&st)[tid] =
+        reinterpret_cast<const uint32_t*>(mode == RowState::kDigits ? &a.state[r] : &a.decided[r])[tid];
   fill_table(s_table);
   for (int k = tid; k < n && n <= kCap; k += kThreads) sm.s.item[k] = a.list[(size_t)r * kCap + k];
   __syncthreads();
@@ -1001,9 +1018,9 @@ SamplePlan sample_plan(int R, int V) {
   SamplePlan p{};
   if (R < 1 || V < 1 || V > 1 << 20 || R > 65535) return p;
   R = R < kRows ? R : kRows;
-  // Workgroups per row: two per CU in all (what their registers and LDS let run at once), with chunks of
-  // 4096 tokens at least, below which a workgroup has nothing to do but its sums; and of many rows chunks
-  // of 32768 at most, since greedy rows are done at once and others take three passes.
+  // Workgroups per row: two per CU in all (what their registers let run at once), chunks of 4096 tokens at
+  // least, a load or two a thread; and of many long rows chunks of 32768 at most, since greedy rows are
+  // done at once: 256 rows of 248320 took 119 us so, 160 with 65536, 173 with 131072.
   p.C = max(1, max(min(512 / R, (V + 4095) / 4096), V / 32768));
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   const size_t chunks = up((size_t)R * p.C * 4);

@@ -109,7 +109,7 @@ def test_sample_refusals(ops):
 
 @pytest.mark.parametrize("R,V,kind", [
     (16, 100003, "ascending"), (16, 100003, "descending"), (300, 9001, "descending"), (16, 100003, "block"),
-    (16, 100003, "few"), (16, 100003, "infinite"), (3, 3, "infinite"), (8, 1 << 20, "flat"), (513, 40000, "flat"),
+    (16, 100003, "few"), (16, 100003, "infinite"), (16, 30001, "crowded"), (3, 3, "infinite"), (8, 1 << 20, "flat"), (513, 40000, "flat"),
 ])
 def test_sample_top_k_wherever_the_largest_lie(ops, R, V, kind):
     """Every size of top-k, with the row's largest logits spread, sorted, side by side, or fewer than k."""
@@ -124,6 +124,11 @@ def test_sample_top_k_wherever_the_largest_lie(ops, R, V, kind):
     elif kind == "few":
         x[rng.random((R, V)) > 40 / V] = -INF
         x[:, 77] = 1
+    elif kind == "crowded":  # thousands of different values in one bin, some rows within the list's length
+        x = 1e-3 * x - 8
+        x[:, 9000::7] = -60
+        x[:13, 3000:] = -60
+        x[:, 4] = 9
     elif kind == "infinite":
         x[rng.random((R, V)) < max(0.01, 1 / V)] = INF
     s = _settings(R, rng)
