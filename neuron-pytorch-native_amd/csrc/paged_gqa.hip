@@ -24,10 +24,13 @@
 //       online softmax per row in fp32, base 2; that key order puts keys 16 G + [0, 16) of a row
 //         into one lane, in order, so
 //       O^T[256 x 16 rows] += V^T P^T     takes P straight from the score registers as B, and A = V^T
-//         is 16 bytes of a page's dim row; its bytes become bf16 with the page's scale in
-//         v_cvt_scalef32_pk_bf16_fp8, exactly (an e4m3 value times a power of two is a bf16 number),
-//         and P is split into bf16 hi + lo parts (as gqa::tail_verify's: with hi alone the output's
-//         error was 0.0029 against its own rounding's 0.0017).
+//         is 16 bytes of a page's dim row. In f16 again: V's bytes as they are, and P times its page's
+//         scale, over a running power of two per row that keeps the largest of these products between
+//         2^11 and 2^15 (a second running maximum, of log2 of P times the scale): 11 bits of those down
+//         to 2^-25 of it, and steps of 2^-35 below, where the cache's own are 2^-10 of a page's scale.
+//         (P in bf16 with the scale in V: the output's error was 0.0029 against its own rounding's
+//         0.0017. P in two bf16 parts: as exact as f16, with twice these products; 16 x 8 rows over up to
+//         32768 keys took 142 us instead of 135, 2 x 256 over up to 8192 178 instead of 158.)
 //     The bytes go from the pages by DMA to a part of LDS that is the wave's own, in groups of 8 KB
 //     in the order of their use (two K tiles, or eight V tiles of 16 dims); a wave takes a group into
 //     registers, sends its place for a later one and works on it, with one (NW = 8) to three groups
@@ -44,7 +47,8 @@ constexpr int ROPE = 64;
 constexpr float kEps = 1e-6f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -1.0e30f;   // finite "no key yet" running max (avoids inf - inf)
-constexpr float kRescaleLog2 = 8.0f;  // the exponent base moves only when a row max grows > 2^8
+constexpr float kRescaleLog2 = 4.0f;  // a row's exponents' bases move only when its maxima grow by > 2^4
+constexpr float kPLog2 = 11.0f;       // P in f16 is at most 2^(4 + 11), under its 65504
 constexpr int KS = 64;                // keys per step
 constexpr int kChunk = 64;            // steps whose page ids and scales are in LDS at a time
 constexpr int kPages = kChunk * KS / 16 + 1;
@@ -372,7 +376,7 @@ struct PagedSmem {
   u32x4 q[8][NW == 4 ? NRT : 1][64];            // q' as B operands: [k step][row tile][lane]
   float m[NW][NRT * 16], l[NW][NRT * 16], inv[NRT * 16];
   int page[kPages];                             // -1: none
-  float ks[kPages], vs[kPages];
+  float ks[kPages], vs[kPages];                 // the keys' scales, the logarithms of the values'
 };
 
 template <int NRT, int NW>
@@ -409,13 +413,14 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
 
   // The last key of each of this lane's rows (one per tile); -1 for rows that are none.
   int lim[NRT];
-  float q_scale[NRT], m_run[NRT], l_run[NRT];
+  float q_scale[NRT], m_run[NRT], l_run[NRT], w_run[NRT];
 #pragma unroll
   for (int nt = 0; nt < NRT; ++nt) {
     const int r = 16 * nt + i, t = a.token_of(row0 + r);
     lim[nt] = r < rows && t < a.q_len[un.b] ? min(un.kv + t, un.kend - 1) : -1;
     q_scale[nt] = a.q_scale[(size_t)pair * R + r];
     m_run[nt] = kNegBig;
+    w_run[nt] = kNegBig;
     l_run[nt] = 0.f;
   }
   const int lim0 = un.kv + un.t0;  // no row of the group sees less
@@ -480,7 +485,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
       const bool ok = id >= 0 && id < a.N;
       sm.page[p] = ok ? id : -1;
       sm.ks[p] = ok ? a.k_scale[(size_t)id * a.Hkv + h] : 1.0f;
-      sm.vs[p] = ok ? a.v_scale[(size_t)id * a.Hkv + h] : 1.0f;
+      sm.vs[p] = ok ? log2f(a.v_scale[(size_t)id * a.Hkv + h]) : 0.0f;
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // and q' is in LDS
     __syncthreads();
@@ -613,10 +618,6 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
 
       // A step with keys past the group's first limit, or past a page that is none, is masked.
       const bool tail = k0 + KS - 1 > lim0 || __builtin_amdgcn_ballot_w64(!held) != 0;
-#pragma unroll
-      for (int nt = 0; nt < NRT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) st[nt][j] *= ks * q_scale[nt];
       if (tail) {
         const int kb = k0 + 16 * G;
 #pragma unroll
@@ -628,37 +629,40 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
               if (!held || kb + 4 * j + r > lim[nt]) st[nt][j][r] = -INFINITY;
       }
 
-      bf16x8 ph[NRT][2], pl[NRT][2];
+      f16x8 pw[NRT][2];
 #pragma unroll
       for (int nt = 0; nt < NRT; ++nt) {
+        const float c = fmaxf(ks * q_scale[nt], 0x1p-126f);  // not 0: -inf stays
         float mx = st[nt][0][0];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[nt][j][r]);
+        mx *= c;
+        const float wx = max_over_groups(mx + vs);
         mx = max_over_groups(mx);
-        const bool grow = mx > m_run[nt] + kRescaleLog2;
-        if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-          const float mnew = grow ? mx : m_run[nt];
-          const float corr = exp2f(m_run[nt] - mnew);
+        const bool grow = mx > m_run[nt] + kRescaleLog2, wgrow = wx > w_run[nt] + kRescaleLog2;
+        if (__builtin_amdgcn_ballot_w64(grow || wgrow) != 0) {
+          const float mnew = grow ? mx : m_run[nt], wnew = wgrow ? wx : w_run[nt];
+          const float corr = exp2f(w_run[nt] - wnew);
+          l_run[nt] *= exp2f(m_run[nt] - mnew);
           m_run[nt] = mnew;
-          l_run[nt] *= corr;
+          w_run[nt] = wnew;
 #pragma unroll
           for (int d = 0; d < 16; ++d) {
             acc[nt][d] *= corr;
             if constexpr (NW == 4) pin(acc[nt][d]);
           }
         }
+        const float f = __builtin_amdgcn_exp2f(fminf(m_run[nt] + vs - w_run[nt] + kPLog2, 120.0f));
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float pv = __builtin_amdgcn_exp2f(st[nt][j][r] - m_run[nt]);
+            const float pv = __builtin_amdgcn_exp2f(fmaf(st[nt][j][r], c, -m_run[nt]));
             sum += pv;
-            const __bf16 hi = (__bf16)pv;
-            ph[nt][j >> 1][(j & 1) * 4 + r] = hi;
-            pl[nt][j >> 1][(j & 1) * 4 + r] = (__bf16)(pv - (float)hi);
+            pw[nt][j >> 1][(j & 1) * 4 + r] = (_Float16)(pv * f);
           }
         l_run[nt] += sum;
       }
@@ -712,15 +716,11 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
         for (int d = 0; d < 8; ++d) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const bf16x8 vf = dequant8(v[d][2 * k], v[d][2 * k + 1], vs);
+            const f16x8 vf = to_f16x8(v[d][2 * k], v[d][2 * k + 1]);
 #pragma unroll
             for (int nt = 0; nt < NRT; ++nt)
               acc[nt][8 * n + d] =
-                  __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ph[nt][k], acc[nt][8 * n + d], 0, 0, 0);
-#pragma unroll
-            for (int nt = 0; nt < NRT; ++nt)
-              acc[nt][8 * n + d] =
-                  __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[nt][k], acc[nt][8 * n + d], 0, 0, 0);
+                  __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pw[nt][k], acc[nt][8 * n + d], 0, 0, 0);
           }
           if (d % 2) __builtin_amdgcn_sched_barrier(0);
         }
@@ -748,7 +748,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
     for (int k = 0; k < NW; ++k) m = fmaxf(m, sm.m[k][16 * nt + i]);
 #pragma unroll
     for (int k = 0; k < NW; ++k) l += exp2f(sm.m[k][16 * nt + i] - m) * sm.l[k][16 * nt + i];
-    const float f = exp2f(m_run[nt] - m);
+    const float f = exp2f(w_run[nt] - m - kPLog2);
 #pragma unroll
     for (int d = 0; d < 16; ++d) acc[nt][d] *= f;
     if (w == 0 && G == 0) {

@@ -3,8 +3,8 @@ bit for bit, appended pages byte for byte (V) or within one code where fp32 and 
 normed K value apart, attention within its roundings.
 
 Attention's tolerance: the kernel rounds q' to f16 relative to the row's largest element (at most
-2^-11, 0.0002 in the root mean square), the softmax weights to two bf16 numbers (2^-16) and its
-output to bf16, at most 2^-8 relative and 0.43 * 2^-8 = 0.0017 in the root mean square over a binade:
+2^-11, 0.0002 in the root mean square), the softmax weights to f16 (2^-11 as well) and its output to
+bf16, at most 2^-8 relative and 0.43 * 2^-8 = 0.0017 in the root mean square over a binade:
 2e-3 in the norm, and for an element its own rounding (BF16_U) beside 2e-3 of the largest.
 """
 import numpy as np
@@ -316,6 +316,25 @@ def test_tail_verify_paged_missing_pages(ops):
     ref = _oracle(d)
     assert not got[1].any()
     assert_rel_close(got, ref, tol=TOL, out_unit=BF16_U, name="missing pages")
+
+
+@pytest.mark.parametrize("B,T,n", [(2, 1, [1, 1]), (2, 8, [8, 5]), (1, 40, [40])])
+def test_tail_verify_paged_scales_far_apart(ops, B, T, n):
+    """Value scales from 2^-100 to 2^20 among a request's pages, row by row against the oracle's row: a
+    row's largest product of weight and scale may lie in any page. Scores have a deviation of about 5.6,
+    so q's rounding (2^-11, 0.0003 in the root mean square) moves a weight by 0.0017 in the root mean
+    square, which a row of few large weights shows in full beside its output's 0.0017: 0.0024 together,
+    and three times that is no row's by chance."""
+    kv = [700, 131][:B]
+    d = _attend_inputs(B, T, 2, 6, 16, kv, n, seed=77 + T)
+    rng = np.random.default_rng(T)
+    live = d["cache"][3][np.isfinite(d["cache"][3])]
+    d["cache"][2][:] *= 8
+    d["cache"][3][np.isfinite(d["cache"][3])] = np.exp2(rng.choice([-100, -60, -12, -3, 0, 5, 20], live.shape))
+    got, ref = _attend(ops, d).float().cpu().double().numpy(), _oracle(d)
+    err, size = np.linalg.norm(got - ref, axis=-1), np.linalg.norm(ref, axis=-1)
+    for b in range(B):
+        assert (size[b, :n[b]] > 0).all() and (err[b, :n[b]] <= 0.0072 * size[b, :n[b]]).all()
 
 
 @pytest.mark.parametrize("where", ["k", "v"])
