@@ -278,8 +278,9 @@ size_t npn_gqa_tail_verify_paged_workspace_size(int B, int T, int q_heads, int k
  * kv_len[b] + t clamped to them. Table entries out of [0, n_blocks) hide their positions; a row
  * without any is 0. A row does not depend on the cache behind its last position, NaN included.
  * T = 1 is plain decode; T may be long (a prompt's chunk).
- * Limits: Hq/Hkv <= 48, Hq/Hkv * T <= 2^20, max_blocks * block_size <= 2^30,
- * B * Hkv * ceil(Hq/Hkv * T / 48) <= 65535. */
+ * Limits: Hq/Hkv <= 48, Hq/Hkv * T <= 2^20, max_blocks * block_size <= 2^30, and with the
+ * Hq/Hkv * T rows of a kv head in groups of 128 (one group up to 48), B * Hkv * groups <= 65535
+ * and that times max_blocks * block_size / 64 < 2^30. */
 int npn_gqa_tail_verify_paged(const uint16_t* query, const uint16_t* gate, const float* q_norm,
                               const float* cos_table, const float* sin_table, int positions,
                               const int8_t* cache_k, const int8_t* cache_v,

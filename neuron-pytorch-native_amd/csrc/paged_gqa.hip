@@ -6,16 +6,16 @@
 //   64); s_j = q'.K_j / 16 over the keys j <= kv_len[b] + t; out = (softmax(s) V) * sigmoid(gate),
 //   K and V the e4m3 bytes times their (block, head) scale. Rows t >= q_len[b] are 0.
 //
-// The rows of a kv head (token-major, grp heads per token) are cut into groups of R = 16 NRT rows;
-// a (request, row group) is a unit, a (unit, kv head) a pair of its rows and its keys, taken in steps
-// of 64 keys. Three launches:
+// The rows of a kv head (token-major, grp heads per token) are cut into groups of R = 16, 32 or 48 rows,
+// as they need, or of 128 where they are more; a (request, row group) is a unit, a (unit, kv head) a
+// pair of its rows and its keys, taken in steps of 64 keys (128 with R = 128). Three launches:
 //  1. prep: q' of every pair as MFMA B operands, and, in its first block, the plan: the host does not
 //     know the lengths. A pair of n steps gets ceil(n / Q) workgroups, Q the least number of steps
-//     (a multiple of the waves') with which all pairs' workgroups are at most `most`. (Equal cuts
-//     through the pairs laid end to end balanced better and cost most workgroups a second segment,
-//     with its own start and end: 20 us of 80 for 64 sequences of one token.)
-//  2. attn: a workgroup takes an equal part of its pair's steps; its NW waves (eight for up to 16
-//     rows; four, with all of a SIMD's registers, for more) take those in turn, each on its own:
+//     (a multiple of what the waves take at a time) with which all pairs' workgroups are at most `most`.
+//     (Equal cuts through the pairs laid end to end balanced better and cost most workgroups a second
+//     segment, with its own start and end: 20 us of 80 for 64 sequences of one token.)
+//  2. attn, up to 48 rows: a workgroup takes an equal part of its pair's steps; its NW waves (eight for
+//     up to 16 rows; four, with all of a SIMD's registers, for more) take those in turn, each alone:
 //       S^T[64 keys x 16 rows] = K Q'^T   A = K, 16 bytes per lane as they lie in the page: lane (i, G)
 //         of tile j holds key 16 (i / 4) + 4 j + i % 4, dims 64 c + 16 G + [0, 16) for column c; the
 //         product's k order follows (Q' is laid out in the same order). In f16: every e4m3 value is
@@ -29,15 +29,28 @@
 //         2^11 and 2^15 (a second running maximum, of log2 of P times the scale): 11 bits of those down
 //         to 2^-25 of it, and steps of 2^-35 below, where the cache's own are 2^-10 of a page's scale.
 //         (P in bf16 with the scale in V: the output's error was 0.0029 against its own rounding's
-//         0.0017. P in two bf16 parts: as exact as f16, with twice these products; 16 x 8 rows over up to
-//         32768 keys took 142 us instead of 135, 2 x 256 over up to 8192 178 instead of 158.)
+//         0.0017. P in two bf16 parts: as exact as f16, with twice these products; 16 requests of 8 x 6
+//         rows over up to 32768 keys took 142 us instead of 134.)
 //     The bytes go from the pages by DMA to a part of LDS that is the wave's own, in groups of 8 KB
 //     in the order of their use (two K tiles, or eight V tiles of 16 dims); a wave takes a group into
 //     registers, sends its place for a later one and works on it, with one (NW = 8) to three groups
 //     in flight. Nothing else may touch memory in that loop: a reload of a spilled register waits,
 //     in order, for every DMA before it.
-//     The waves' (m, l, O) meet in LDS; a pair with one workgroup is written out at once.
+//     The waves' (m, l, O) meet in LDS; a pair with one workgroup is written out at once. Bound by
+//     the cache's bytes: one row group over 32768 keys of 4 heads (67 MB) 18 us, 3.7 TB/s with the start
+//     and end in it; 64 sequences of up to 16384 (271 MB) 57 us, 4.7 TB/s; the 16 requests above (607 MB)
+//     134 us, 4.5 TB/s; a large read reaches 6.15.
+//  2b. rows, R = 128: eight waves of 16 rows share the steps, which pass once through LDS, two steps in
+//     all there. Half of the instructions above made f16 of K's and V's bytes, for 16 to 48 rows at
+//     a time, and the matrix units were busy for a quarter of the time. Here the bytes go into
+//     the 16x16x128 products as they are, and q' and P as three e4m3 parts of four bits each, 2^-4
+//     and 2^-8 in the product's scale operand: 12 bits, for 1.5 times the f16 products' time. 2 chunks of
+//     256 x 6 rows over up to 8192 keys: 128 us (157 with groups of 48 rows; 142 with 128 rows in f16),
+//     616 TFLOP/s by the formula's operations. Matrix units 51 %, vector units 55 % busy, and they do
+//     not overlap: priorities for one wave of each SIMD, or its V products half a step behind the
+//     other's, changed nothing.
 //  3. merge: the log-sum-exp merge of the other pairs' workgroups, times sigmoid(gate), to bf16.
+// prep takes 4 to 9 us and merge 5 to 10 for these.
 #include "npn_common.h"
 
 namespace {
@@ -52,6 +65,7 @@ constexpr float kPLog2 = 11.0f;       // P in f16 is at most 2^(4 + 11), under i
 constexpr int KS = 64;                // keys per step
 constexpr int kChunk = 64;            // steps whose page ids and scales are in LDS at a time
 constexpr int kPages = kChunk * KS / 16 + 1;
+constexpr int kRows = 128;            // rows of a group of many
 
 typedef __bf16 bf16x8 __attribute__((__vector_size__(8 * sizeof(__bf16))));
 typedef __bf16 bf16x2 __attribute__((__vector_size__(2 * sizeof(__bf16))));
@@ -59,6 +73,7 @@ typedef _Float16 f16x8 __attribute__((__vector_size__(8 * sizeof(_Float16))));
 typedef _Float16 f16x2 __attribute__((__vector_size__(2 * sizeof(_Float16))));
 typedef float f32x4 __attribute__((__vector_size__(4 * sizeof(float))));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 struct PagedArgs {
   const uint16_t* query;  // [B][T][Hq][256]
@@ -74,13 +89,13 @@ struct PagedArgs {
   const int32_t* kv_len;
   const int32_t* q_len;
   uint16_t* out;
-  u32x4* q;                // [pairs][8][NRT][64] q' as B operands
+  u32x4* q;                // q' as B operands: [pairs][8][NRT][64], or [pairs][8][2][3 parts][2][64] for R = 128
   float* q_scale;          // [pairs][R]
   float* part_o;           // [slots][R][256] O of the workgroups of split pairs
   float* part_ml;          // [slots][R][2]
   int32_t* wstart;         // [U + 1] first workgroup of each unit
   int32_t* sstart;         // [U] first slot of each unit
-  int positions, B, T, Hq, Hkv, grp, R, RG, P, N, sh, nw;
+  int positions, B, T, Hq, Hkv, grp, R, RG, P, N, sh, nw, ks;  // ks: keys of a step
   uint64_t by_grp;         // 2^32 / grp + 1: rows are below 2^21
 
   __device__ __forceinline__ int token_of(int row) const { return (int)((row * by_grp) >> 32); }
@@ -102,8 +117,22 @@ __device__ __forceinline__ Unit unit_of(const PagedArgs& a, int u) {
   const int cap = a.P << a.sh;  // <= 2^30
   r.kv = min(max(a.kv_len[r.b], 0), cap);
   r.kend = n > r.t0 ? min(r.kv + n, cap) : 0;
-  r.steps = (r.kend + KS - 1) / KS;
+  r.steps = (r.kend + a.ks - 1) / a.ks;
   return r;
+}
+
+// The last of n ascending starts that is at most x (wave-uniform; the first is), 64 at a time.
+__device__ __forceinline__ int last_start(const int32_t* start, int n, int x) {
+  const int lane = threadIdx.x & 63;
+  int u = 0;
+  while (n > 1) {
+    const int stride = (n + 63) / 64, at = lane * stride;
+    const bool le = at < n && start[u + at] <= x;
+    const int last = __popcll(__builtin_amdgcn_ballot_w64(le)) - 1;
+    n = min(stride, n - last * stride);
+    u = __builtin_amdgcn_readfirstlane(u + last * stride);
+  }
+  return u;
 }
 
 __device__ __forceinline__ float max_over_groups(float x) {
@@ -178,6 +207,14 @@ __device__ __forceinline__ void dma16_soff(const void* base, unsigned voff, unsi
       : "memory");
 }
 
+__device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b) {
+  return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+}
+// D = A B 16^-part + C over 128 e4m3 of k (lane (i, G): 32 of row or column i).
+__device__ __forceinline__ f32x4 mfma_e4m3(i32x8 a, i32x8 b, f32x4 c, int part) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 127, 0, 127 - 4 * part);
+}
+
 // LDS by address, element k of 16 bytes (1 KB apart: one per lane) from a per-lane base. The bases are
 // hidden from the optimiser (opaque): left to itself it kept some hundred of base + offset sums,
 // past the 16-bit offset of an LDS instruction, in registers and spilled them.
@@ -214,14 +251,37 @@ __device__ __forceinline__ void write_out(const PagedArgs& a, int b, int row, in
   *reinterpret_cast<uint2*>(a.out + at) = make_uint2(y[0], y[1]);
 }
 
+// Four numbers of at most 448 as a word each of three e4m3 parts, x = p0 + p1 / 16 + p2 / 256: each part
+// takes 4 bits of what the ones before leave, 12 in all, down to steps of 2^-17.
+__device__ __forceinline__ void split3(float x0, float x1, float x2, float x3, uint32_t (&part)[3]) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, w, true);
+    part[k] = (uint32_t)w;
+    if (k == 2) break;
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    x0 = (x0 - lo[0]) * 16.0f;
+    x1 = (x1 - lo[1]) * 16.0f;
+    x2 = (x2 - hi[0]) * 16.0f;
+    x3 = (x3 - hi[1]) * 16.0f;
+  }
+}
+
 // ---- 1. prep ----------------------------------------------------------------------------------------
 constexpr int kPrepWaves = 8;
 constexpr int kPlanUnits = 4096;  // units whose steps the plan keeps in LDS
 
 // One workgroup per CU where the pairs with steps are few enough to be cut so; else one each and 512
-// more for the longest.
-__host__ __device__ constexpr int most_workgroups(int pairs) { return pairs <= 192 ? 256 : pairs + 512; }
-// Split pairs' workgroups: all of 256, or, as a pair of c >= 2 has c - 1 of the 512, twice those.
+// more for the longest. Groups of 128 rows are few and long, so that a second round of workgroups may
+// pay where the first leaves many CUs idle (96 pairs make 192): the plan takes the cheaper by the steps
+// of 128 keys that the rounds last, with 1.5 for a workgroup's start and end and 2.5 for writing and
+// merging the parts of 256.
+__host__ __device__ constexpr int most_workgroups(int R, int pairs, int rounds) {
+  return R == kRows && rounds == 2 && pairs > 64 && pairs <= 448 ? 512 : pairs <= 192 ? 256 : pairs + 512;
+}
+// Split pairs' workgroups: all of 256 or 512, or, as a pair of c >= 2 has c - 1 of the 512 more, twice
+// those.
 constexpr int kSlots = 1024;
 
 // Workgroups of each unit's pairs: the least Q = nw k with sum ceil(n / Q) <= most lies between
@@ -256,28 +316,43 @@ __device__ void plan_block(const PagedArgs& a) {
     some += s_wave[k][1];
   }
   const int S = sum * a.Hkv, pairs = some * a.Hkv;  // S < 2^30
-  const int most = most_workgroups(pairs);
   auto up = [](int n, int d) { return (n + d - 1) / d; };
-  int lo = max(1, up(up(S, most), a.nw)), hi = max(lo, up(up(S, most - pairs), a.nw));
-  while (lo < hi) {
-    const int Q = (lo + (int)((int64_t)(hi - lo) * w / kPrepWaves)) * a.nw;
-    int g = 0;
-    for (int u = lane; u < U; u += 64) g += up(steps_of(u), Q);
+  // The least Q that `most` workgroups allow, and the workgroups that it makes.
+  auto least = [&](int most, int& made) {
+    int lo = max(1, up(up(S, most), a.nw)), hi = max(lo, up(up(S, max(most - pairs, 1)), a.nw));
+    made = most;
+    while (lo < hi) {
+      const int Q = (lo + (int)((int64_t)(hi - lo) * w / kPrepWaves)) * a.nw;
+      int g = 0;
+      for (int u = lane; u < U; u += 64) g += up(steps_of(u), Q);
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) g += __shfl_xor(g, off, 64);
-    __syncthreads();  // s_wave has been read
-    if (lane == 0) s_wave[w][0] = g;
-    __syncthreads();
-    int nlo = lo, nhi = hi;
-    for (int k = kPrepWaves - 1; k >= 0; --k) {
-      const int t = lo + (int)((int64_t)(hi - lo) * k / kPrepWaves);
-      if ((int64_t)s_wave[k][0] * a.Hkv <= most) nhi = t;
-      else nlo = max(nlo, t + 1);
+      for (int off = 32; off > 0; off >>= 1) g += __shfl_xor(g, off, 64);
+      __syncthreads();  // s_wave has been read
+      if (lane == 0) s_wave[w][0] = g;
+      __syncthreads();
+      int nlo = lo, nhi = hi;
+      for (int k = kPrepWaves - 1; k >= 0; --k) {
+        const int t = lo + (int)((int64_t)(hi - lo) * k / kPrepWaves);
+        if ((int64_t)s_wave[k][0] * a.Hkv <= most) {
+          nhi = t;
+          made = s_wave[k][0] * a.Hkv;
+        } else {
+          nlo = max(nlo, t + 1);
+        }
+      }
+      lo = min(nlo, nhi);
+      hi = nhi;
     }
-    lo = min(nlo, nhi);
-    hi = nhi;
+    return hi * a.nw;
+  };
+  int made;
+  int Q = least(most_workgroups(a.R, pairs, 1), made);
+  if (a.R == kRows && most_workgroups(a.R, pairs, 2) > most_workgroups(a.R, pairs, 1)) {
+    auto cost = [&](int q, int g) { return up(g, 256) * (q + 1.5f) + g * 0.01f; };
+    const float one = cost(Q, made);
+    const int Q2 = least(most_workgroups(a.R, pairs, 2), made);
+    if (cost(Q2, made) < one) Q = Q2;
   }
-  const int Q = hi * a.nw;
   // First workgroup and first slot of each unit: scans over threads' slices of the units.
   const int per = up(U, kPrepWaves * 64);
   const int u0 = min(U, tid * per), u1 = min(U, u0 + per);
@@ -310,9 +385,9 @@ __device__ void plan_block(const PagedArgs& a) {
   }
 }
 
-// q' of one padded row per wave (rows that are none repeat the pair's last), f16 over the least power
-// of two above the row's largest element; dim d = 64 c + 16 g + 8 h + e is element e of lane group g
-// in k step 2 c + h.
+// q' of one padded row per wave (rows that are none repeat the pair's last), over the least power of
+// two above the row's largest element. In f16 dim d = 64 c + 16 g + 8 h + e is element e of lane group
+// g in k step 2 c + h; in e4m3 parts d = 128 m + 64 x + 16 g + e is byte 16 x + e of group g in step m.
 __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagedArgs a) {
   if (blockIdx.x == 0) {
     plan_block(a);
@@ -351,15 +426,28 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagedArgs a
   }
   const float big = npn::wave_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
   const uint32_t e = min(max(__float_as_uint(big) >> 23, 64u), 190u);  // 2^-63 to 2^63
-  const float inv = __uint_as_float((253u - e) << 23);                // 2^-(e - 126)
-  if (lane == 0) a.q_scale[(size_t)pair * a.R + r] = __uint_as_float((e + 1) << 23) * (kLog2e / 16.0f);
+  float inv = __uint_as_float((253u - e) << 23);                      // 2^-(e - 126)
+  float q_scale = __uint_as_float((e + 1) << 23) * (kLog2e / 16.0f);
+  const int d = 4 * lane;
+  if (a.R == kRows) {  // three e4m3 parts of 256 times as much
+    inv *= 256.0f;
+    q_scale *= 1.0f / 256;
+    if (lane == 0) a.q_scale[(size_t)pair * a.R + r] = q_scale;
+    uint32_t part[3];
+    split3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv, part);
+    const size_t at = ((((size_t)pair * 8 + (r >> 4)) * 2 + (d >> 7)) * 3 * 2 + ((d >> 6) & 1)) * 64;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.q + at + 16 * ((d >> 4) & 3) + (r & 15));
+#pragma unroll
+    for (int k = 0; k < 3; ++k) dst[k * 512 + ((d >> 2) & 3)] = part[k];
+    return;
+  }
+  if (lane == 0) a.q_scale[(size_t)pair * a.R + r] = q_scale;
   uint32_t two[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const f16x2 x = {(_Float16)(v[2 * j] * inv), (_Float16)(v[2 * j + 1] * inv)};
     two[j] = __builtin_bit_cast(uint32_t, x);
   }
-  const int d = 4 * lane;
   const int step = 2 * (d >> 6) + ((d >> 3) & 1), g = (d >> 4) & 3;
   u32x4* dst = a.q + (((size_t)pair * 8 + step) * (a.R / 16) + (r >> 4)) * 64 + 16 * g + (r & 15);
   *reinterpret_cast<uint2*>(reinterpret_cast<uint32_t*>(dst) + ((d & 4) >> 1)) = make_uint2(two[0], two[1]);
@@ -392,16 +480,9 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
   const int bs = 1 << a.sh;
   const int U = a.units();
 
-  // This workgroup's unit (64-way search in the starts), kv head and steps [s_lo, s_lo + steps).
+  // This workgroup's unit, kv head and steps [s_lo, s_lo + steps).
   if ((int)blockIdx.x >= a.wstart[U]) return;
-  int u = 0;
-  for (int n = U; n > 1;) {
-    const int stride = (n + 63) / 64, at = u + lane * stride;
-    const bool le = at < u + n && a.wstart[at] <= (int)blockIdx.x;
-    const int last = __popcll(__builtin_amdgcn_ballot_w64(le)) - 1;
-    n = min(stride, n - last * stride);
-    u = __builtin_amdgcn_readfirstlane(u + last * stride);
-  }
+  const int u = last_start(a.wstart, U, (int)blockIdx.x);
   const Unit un = unit_of(a, u);
   const int w0 = a.wstart[u], parts = (a.wstart[u + 1] - w0) / a.Hkv;
   const int h = ((int)blockIdx.x - w0) / parts, part = (int)blockIdx.x - w0 - h * parts;
@@ -786,6 +867,295 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
   }
 }
 
+// ---- 2b. attn of many rows ----------------------------------------------------------------------------
+struct RowsSmem {
+  union {
+    uint8_t ring[2][65536];  // two steps of 128 keys: for each half two groups of K and two of V, as above
+    f32x4 o[8][16][64];      // 16 rows of 256 to a wave
+  };
+  float inv[kRows];
+  int lim[kRows];
+  int nan_key[DH];         // the first key past lim0 whose value at a dim is NaN
+  int page[kPages];
+  float ks[kPages], vs[kPages];
+};
+
+__global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
+  constexpr int R = kRows, KR = 128, kSteps = kChunk * KS / KR;
+  constexpr float kP = 4.0f;  // P is at most 2^(4 + 4), under e4m3's 448
+  __shared__ __attribute__((aligned(1024))) RowsSmem sm;
+  const int tid = threadIdx.x;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int i = lane & 15, G = lane >> 4;
+  const int bs = 1 << a.sh;
+  const int U = a.units();
+
+  if ((int)blockIdx.x >= a.wstart[U]) return;
+  const int u = last_start(a.wstart, U, (int)blockIdx.x);
+  const Unit un = unit_of(a, u);
+  const int w0 = a.wstart[u], parts = (a.wstart[u + 1] - w0) / a.Hkv;
+  const int h = ((int)blockIdx.x - w0) / parts, part = (int)blockIdx.x - w0 - h * parts;
+  const int s_lo = (int)((int64_t)part * un.steps / parts);
+  const int steps = (int)((int64_t)(part + 1) * un.steps / parts) - s_lo;
+  const int pair = u * a.Hkv + h;
+  const int row0 = (u - un.b * a.RG) * R;
+  const int rows = min(R, a.T * a.grp - row0);
+
+  const int r = 16 * w + i, t = a.token_of(row0 + r);  // this lane's row and its last key, or -1
+  int lim = r < rows && t < a.q_len[un.b] ? min(un.kv + t, un.kend - 1) : -1;
+  float q_scale = a.q_scale[(size_t)pair * R + r];
+  float m_run = kNegBig, w_run = kNegBig, l_run = 0.f;
+  const int lim0 = un.kv + un.t0;
+  i32x8 q[2][3];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const u32x4* src = a.q + ((((size_t)pair * 8 + w) * 2 + m) * 3 + k) * 128 + lane;
+      q[m][k] = join(src[0], src[64]);
+    }
+
+  const unsigned ring_lds = __builtin_amdgcn_readfirstlane(npn::lds_addr(&sm.ring[0][0]));
+  const unsigned ksrc = (unsigned)(G * DH + ((i ^ G) << 4)) ^ ((w >> 1) << 6);
+  const unsigned k_at = ring_lds + (unsigned)((8 * (i >> 2) + (i & 3)) * DH + ((i ^ G) << 4));
+  const unsigned v_at = ring_lds + lane * 16u;
+
+  int cn, key0, page0;
+  // A wave's eight of a step's 64 DMAs: one to each group.
+  auto load_step = [&](int s) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const unsigned at = ring_lds + (unsigned)((s & 1) * 65536 + half * 32768 + w * 1024);
+      const int k0 = key0 + s * KR + half * KS;
+      const int kk = k0 + 16 * (w >> 1), kv = k0 + 16 * G;
+      const int kid = __builtin_amdgcn_readfirstlane(max(sm.page[(kk >> a.sh) - page0], 0));
+      const uint8_t* const kp =
+          a.cache_k + ((((size_t)kid * a.Hkv + h) << a.sh) + (kk & (bs - 1))) * DH + (w & 1) * 4 * DH;
+      dma16_soff(kp, ksrc, at);
+      dma16_soff(kp + 8 * DH, ksrc, at + 8192);
+      const int vid = max(sm.page[(kv >> a.sh) - page0], 0);
+      const uint8_t* const vp =
+          a.cache_v + ((((size_t)vid * a.Hkv + h) * DH + 16 * w + i) << a.sh) + (kv & (bs - 1));
+      dma16(vp, at + 2 * 8192);
+      dma16(vp + ((size_t)128 << a.sh), at + 3 * 8192);
+    }
+  };
+  // V bytes of keys that no row sees are cleared (0 times NaN is NaN), each wave those that it sent for. So
+  // is a NaN at a key that some rows see, and the first such key of its dim noted: the rows that see it
+  // get the NaN at the end.
+  auto clean = [&](int k0, unsigned place) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int k1 = k0 + KS * half + 16 * G;
+      const int live = sm.page[(k1 >> a.sh) - page0] >= 0 ? un.kend - k1 : 0;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const unsigned at = opaque(v_at + place + half * 32768u + (2 + n) * 8192u + w * 1024u);
+        u32x4 v = lds_read(at, 0);
+#pragma unroll
+        for (int k = 3; k >= 0; --k) {
+          v[k] &= keep_bytes(live - 4 * k);
+          const uint32_t nan = nan_bytes(v[k]);
+          if (nan != 0) {
+            atomicMin(&sm.nan_key[16 * (w + 8 * n) + i], k1 + 4 * k + (__ffs(nan) - 1) / 8);
+            v[k] &= ~nan;
+          }
+        }
+        lds_write(at, 0, v);
+      }
+    }
+  };
+  auto missing = [&](int k0) {  // a page of the step is none
+    return __builtin_amdgcn_ballot_w64(sm.page[((k0 + 16 * G) >> a.sh) - page0] < 0 ||
+                                       sm.page[((k0 + KS + 16 * G) >> a.sh) - page0] < 0) != 0;
+  };
+  auto begin_chunk = [&](int c0) {
+    cn = min(kSteps, steps - c0);
+    key0 = (s_lo + c0) * KR;
+    page0 = key0 >> a.sh;
+    const int pages = ((min(key0 + cn * KR, un.kend) - 1) >> a.sh) - page0 + 1;
+    __syncthreads();  // the last chunk's pages and steps have been used
+    for (int p = tid; p < kPages; p += 512) {
+      int id = -1;
+      if (p < pages) id = a.table[(size_t)un.b * a.P + page0 + p];
+      const bool ok = id >= 0 && id < a.N;
+      sm.page[p] = ok ? id : -1;
+      sm.ks[p] = ok ? a.k_scale[(size_t)id * a.Hkv + h] : 1.0f;
+      sm.vs[p] = ok ? log2f(a.v_scale[(size_t)id * a.Hkv + h]) : 0.0f;
+    }
+    __syncthreads();
+  };
+  if (tid < DH) sm.nan_key[tid] = 0x7FFFFFFF;
+  begin_chunk(0);
+  // What was loaded so far is waited for before the first DMAs.
+  asm volatile("" : "+v"(lim), "+v"(q_scale));
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) asm volatile("" : "+v"(q[m][k]));
+  load_step(0);
+
+  f32x4 acc[16];
+#pragma unroll
+  for (int d = 0; d < 16; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (int c0 = 0; c0 < steps; c0 += kSteps) {
+    if (c0 > 0) {
+      begin_chunk(c0);
+      load_step(0);
+    }
+    for (int s = 0; s < cn; ++s) {
+      // The step has landed for every wave past the barrier, and all are done with the step before,
+      // whose place the next takes.
+      const int k0 = key0 + s * KR;
+      const bool tail = k0 + KR - 1 > lim0 || missing(k0);
+      if (tail) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        clean(k0, (unsigned)(s & 1) * 65536u);
+      }
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (s + 1 < cn) load_step(s + 1);
+      if (__builtin_amdgcn_ballot_w64(lim >= k0) == 0) continue;  // none of the wave's rows sees it
+      const unsigned place = (unsigned)(s & 1) * 65536u;
+      float ks[2], vs[2];
+      bool held[2];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int page = ((k0 + KS * half + 16 * G) >> a.sh) - page0;
+        ks[half] = sm.ks[page];
+        vs[half] = sm.vs[page];
+        held[half] = sm.page[page] >= 0;
+      }
+
+      f32x4 st[2][4];
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const unsigned kat = opaque(k_at + place + half * 32768u);
+          u32x4 kw[2][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) kw[j][c] = lds_read(kat ^ (c << 6), 8 * n + j);
+          f32x4 x[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) x[j] = mfma_e4m3(join(kw[j][2 * m], kw[j][2 * m + 1]), q[m][k], x[j], k);
+          st[half][2 * n] = x[0];
+          st[half][2 * n + 1] = x[1];
+          asm volatile("" : "+v"(st[half][2 * n]), "+v"(st[half][2 * n + 1])::"memory");
+          __builtin_amdgcn_sched_barrier(0);
+        }
+
+      if (tail) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!held[half] || k0 + KS * half + 16 * G + 4 * j + e > lim) st[half][j][e] = -INFINITY;
+      }
+
+      float c[2], mx = -INFINITY, wx = -INFINITY;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        c[half] = fmaxf(ks[half] * q_scale, 0x1p-126f);  // not 0: -inf stays
+        float x = st[half][0][0];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x = fmaxf(x, st[half][j][e]);
+        mx = fmaxf(mx, x * c[half]);
+        wx = fmaxf(wx, x * c[half] + vs[half]);
+      }
+      wx = max_over_groups(wx);
+      mx = max_over_groups(mx);
+      const bool grow = mx > m_run + kRescaleLog2, wgrow = wx > w_run + kRescaleLog2;
+      if (__builtin_amdgcn_ballot_w64(grow || wgrow) != 0) {
+        const float mnew = grow ? mx : m_run, wnew = wgrow ? wx : w_run;
+        const float corr = exp2f(w_run - wnew);
+        l_run *= exp2f(m_run - mnew);
+        m_run = mnew;
+        w_run = wnew;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) acc[d] *= corr;
+      }
+      i32x8 p[3];
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float f = __builtin_amdgcn_exp2f(fminf(m_run + vs[half] - w_run + kP, 120.0f));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float pv[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            pv[e] = __builtin_amdgcn_exp2f(fmaf(st[half][j][e], c[half], -m_run));
+            sum[e] += pv[e];
+          }
+          uint32_t word[3];
+          split3(pv[0] * f, pv[1] * f, pv[2] * f, pv[3] * f, word);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) p[k][4 * half + j] = (int)word[k];
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        const unsigned vat = opaque(v_at + place);
+        u32x4 v[2][4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) v[half][d] = lds_read(vat, 32 * half + 16 + 4 * n + d);
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+          for (int d = 0; d < 4; ++d) acc[4 * n + d] = mfma_e4m3(join(v[0][d], v[1][d]), p[k], acc[4 * n + d], k);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+
+  // A wave has its rows whole: through LDS, for stores of whole rows, 16 bytes at f of dim 4 f to place
+  // f ^ i of row i.
+  const float l = sum_over_groups(l_run), scale = exp2f(w_run - m_run - kP);
+  const size_t slot = (size_t)a.sstart[u] + h * parts + part;
+  __syncthreads();  // every wave is done with the ring
+  f32x4* const o = &sm.o[w][0][0];
+#pragma unroll
+  for (int d = 0; d < 16; ++d) o[64 * i + ((4 * d + G) ^ i)] = acc[d] * scale;
+  if (G == 0) {
+    sm.inv[r] = l != 0.f ? 1.0f / l : 0.f;
+    sm.lim[r] = lim;
+    if (parts > 1) {
+      a.part_ml[(slot * R + r) * 2] = m_run;
+      a.part_ml[(slot * R + r) * 2 + 1] = l;
+    }
+  }
+  __syncthreads();
+  for (int k = 0; k < 16; ++k) {
+    const int rk = 16 * w + k;
+    f32x4 x = o[64 * k + (lane ^ k)];
+    x += x * 0.0f;  // infinite: NaN
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (sm.lim[rk] >= sm.nan_key[4 * lane + e]) x[e] = NAN;
+    if (parts > 1)
+      *reinterpret_cast<f32x4*>(a.part_o + (slot * R + rk) * DH + 4 * lane) = x;
+    else if (rk < rows)
+      write_out(a, un.b, row0 + rk, h, 4 * lane, x, sm.inv[rk]);
+  }
+}
+
 // ---- 3. merge ---------------------------------------------------------------------------------------
 // The workgroups' (m, l, O) of a row of a pair, WPR waves to a row: wave q takes parts q, q + WPR, ...,
 // four loads of each at a time, and the first wave merges the waves'. One wave a row where pairs
@@ -854,7 +1224,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
 
 struct PagedPlan {
   bool ok;
-  int grp, R, RG, pairs, grid, nw;
+  int grp, R, RG, pairs, grid, nw, ks;
   size_t o_qs, o_po, o_ml, o_ws, o_ss, bytes;  // q first
 };
 
@@ -865,18 +1235,19 @@ PagedPlan paged_plan(int B, int T, int q_heads, int kv_heads, int max_blocks, in
   p.grp = q_heads / kv_heads;
   const int64_t rows = (int64_t)T * p.grp;
   if (p.grp > 48 || rows > 1 << 20 || (int64_t)max_blocks * block_size > (int64_t)1 << 30) return p;
-  p.R = rows <= 16 ? 16 : (rows <= 32 ? 32 : 48);
+  p.R = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 ? 48 : kRows;
   p.RG = (int)((rows + p.R - 1) / p.R);
   const int64_t pairs = (int64_t)B * p.RG * kv_heads;
   const int64_t keys = (int64_t)max_blocks * block_size;
   if (pairs > 65535 || pairs * ((keys + KS - 1) / KS) >= (int64_t)1 << 30) return p;
   p.pairs = (int)pairs;
-  p.nw = p.R == 16 ? 8 : 4;
-  p.grid = most_workgroups(p.pairs);
-  const size_t slots = pairs <= 192 ? 256 : kSlots;
+  p.nw = p.R == 16 ? 8 : p.R == kRows ? 1 : 4;
+  p.ks = p.R == kRows ? 2 * KS : KS;
+  p.grid = max(most_workgroups(p.R, p.pairs, 1), most_workgroups(p.R, p.pairs, 2));
+  const size_t slots = p.grid == 256 ? 256 : kSlots;
   const size_t units = (size_t)B * p.RG;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  p.o_qs = up((size_t)pairs * p.R * DH * 2);
+  p.o_qs = up((size_t)pairs * p.R * DH * (p.R == kRows ? 3 : 2));
   p.o_po = p.o_qs + up((size_t)pairs * p.R * sizeof(float));
   p.o_ml = p.o_po + up(slots * p.R * DH * sizeof(float));
   p.o_ws = p.o_ml + up(slots * p.R * 2 * sizeof(float));
@@ -917,17 +1288,17 @@ extern "C" int npn_gqa_tail_verify_paged(
                     reinterpret_cast<float*>(ws + p.o_qs), reinterpret_cast<float*>(ws + p.o_po),
                     reinterpret_cast<float*>(ws + p.o_ml), reinterpret_cast<int32_t*>(ws + p.o_ws),
                     reinterpret_cast<int32_t*>(ws + p.o_ss), positions, B, T, q_heads, kv_heads, p.grp,
-                    p.R, p.RG, max_blocks, n_blocks, sh, p.nw, (1ull << 32) / p.grp + 1};
+                    p.R, p.RG, max_blocks, n_blocks, sh, p.nw, p.ks, (1ull << 32) / p.grp + 1};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int nrt = p.R / 16;
-  hipLaunchKernelGGL(paged_prep_kernel, dim3(1 + (p.pairs * nrt * 16 + kPrepWaves - 1) / kPrepWaves),
-                     dim3(kPrepWaves * 64), 0, s, a);
-  if (nrt == 1)
+  hipLaunchKernelGGL(paged_prep_kernel, dim3(1 + p.pairs * p.R / kPrepWaves), dim3(kPrepWaves * 64), 0, s, a);
+  if (p.R == 16)
     hipLaunchKernelGGL((paged_attn_kernel<1, 8>), dim3(p.grid), dim3(512), 0, s, a);
-  else if (nrt == 2)
+  else if (p.R == 32)
     hipLaunchKernelGGL((paged_attn_kernel<2, 4>), dim3(p.grid), dim3(256), 0, s, a);
-  else
+  else if (p.R == 48)
     hipLaunchKernelGGL((paged_attn_kernel<3, 4>), dim3(p.grid), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(paged_rows_kernel, dim3(p.grid), dim3(512), 0, s, a);
   if (p.pairs < 32)
     hipLaunchKernelGGL(paged_merge_kernel<4>, dim3(p.R, p.pairs), dim3(256), 0, s, a);
   else

@@ -321,10 +321,13 @@ def test_tail_verify_paged_missing_pages(ops):
 @pytest.mark.parametrize("B,T,n", [(2, 1, [1, 1]), (2, 8, [8, 5]), (1, 40, [40])])
 def test_tail_verify_paged_scales_far_apart(ops, B, T, n):
     """Value scales from 2^-100 to 2^20 among a request's pages, row by row against the oracle's row: a
-    row's largest product of weight and scale may lie in any page. Scores have a deviation of about 5.6,
-    so q's rounding (2^-11, 0.0003 in the root mean square) moves a weight by 0.0017 in the root mean
-    square, which a row of few large weights shows in full beside its output's 0.0017: 0.0024 together,
-    and three times that is no row's by chance."""
+    row's largest product of weight and scale may lie in any page.
+
+    Keys' codes up to 0x48 have a root mean square of 1.17, |q'| is 16: over key scales of up to 8 a
+    score, their product over 16, deviates by 9.4. Rounding q' to f16 (0.0002 relative in the root mean
+    square) moves it by 0.0019, the difference of two keys' by 0.0027, and with it in full a row that
+    lies in two keys. Of 480 rows with a few such pairs each the largest is near 3.5 deviations; four
+    are 0.0108, with the output's own 0.0017 added 0.0125."""
     kv = [700, 131][:B]
     d = _attend_inputs(B, T, 2, 6, 16, kv, n, seed=77 + T)
     rng = np.random.default_rng(T)
@@ -334,7 +337,7 @@ def test_tail_verify_paged_scales_far_apart(ops, B, T, n):
     got, ref = _attend(ops, d).float().cpu().double().numpy(), _oracle(d)
     err, size = np.linalg.norm(got - ref, axis=-1), np.linalg.norm(ref, axis=-1)
     for b in range(B):
-        assert (size[b, :n[b]] > 0).all() and (err[b, :n[b]] <= 0.0072 * size[b, :n[b]]).all()
+        assert (size[b, :n[b]] > 0).all() and (err[b, :n[b]] <= 0.0125 * size[b, :n[b]]).all()
 
 
 @pytest.mark.parametrize("where", ["k", "v"])
@@ -357,6 +360,80 @@ def test_tail_verify_paged_nan_stays_with_its_rows(ops, where):
         hit[0, 3:, grp:, 17] = True
     assert torch.isnan(got[hit]).all()
     assert torch.equal(got[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("B,T,H,grp,bs,kv,n", [
+    (1, 9, 1, 6, 16, [0], [9]),                          # 54 rows, one step
+    (3, 25, 2, 5, 128, [127, 128, 1000], [25, 0, 7]),    # 125 rows, idle and padded requests
+    (2, 64, 1, 6, 32, [255, 2], [64, 63]),               # tokens that straddle groups of 128 rows
+    (1, 3, 1, 43, 64, [513], [3]),                       # 129 rows
+    (8, 40, 4, 6, 16, [0, 5, 100, 300, 700, 1100, 64, 128], [40, 39, 1, 40, 17, 40, 0, 22]),  # 64 pairs
+    (5, 90, 4, 5, 16, [900, 0, 1500, 33, 260], [90, 90, 90, 90, 2]),  # 80 pairs: one round or two
+    (33, 30, 2, 9, 32, [7 * k for k in range(33)], [30] * 33),        # 198: some pairs cut, some not
+])
+def test_tail_verify_paged_many_rows(ops, B, T, H, grp, bs, kv, n):
+    _check(ops, _attend_inputs(B, T, H, grp, bs, kv, n, seed=B * 11 + T))
+
+
+def test_tail_verify_paged_many_rows_long(ops):
+    """Parts of more steps than a workgroup has pages of in LDS at a time; against the formula in 64-bit
+    torch on the device, which decodes the pages once for all tokens."""
+    T, H, grp, bs, kv = 340, 4, 6, 16, 17000
+    d = _attend_inputs(1, T, H, grp, bs, [kv], [T], seed=3)
+    f64 = lambda a: torch.as_tensor(a).cuda().double()  # noqa: E731
+    e4m3 = lambda c: cuda(c).view(torch.float8_e4m3fn).double()  # noqa: E731
+    table = cuda(d["table"][0]).long()
+    k = (e4m3(d["cache"][0]) * f64(d["cache"][2])[..., None, None])[table].transpose(0, 1).reshape(H, -1, 256)
+    v = (e4m3(d["cache"][1]) * f64(d["cache"][3])[..., None, None])[table].permute(1, 0, 3, 2).reshape(H, -1, 256)
+    k, v = k[:, :kv + T].contiguous(), v[:, :kv + T].contiguous()
+    q = f64(d["query"])[0]
+    q = (1 + f64(d["q_norm"])) * q * torch.rsqrt((q * q).mean(-1, keepdim=True) + 1e-6)
+    cos, sin = (f64(d[n])[kv:kv + T, None] for n in ("cos", "sin"))
+    rot = torch.cat([-q[..., 32:64], q[..., :32]], -1)
+    q = torch.cat([q[..., :64] * cos + rot * sin, q[..., 64:]], -1)
+    hidden = torch.arange(kv + T, device="cuda") > kv + torch.arange(T, device="cuda")[:, None]
+    ref = torch.empty_like(q)
+    for h in range(H * grp):
+        s = (q[:, h] @ k[h // grp].t().contiguous() / 16).masked_fill(hidden, -torch.inf)
+        ref[:, h] = torch.softmax(s, -1) @ v[h // grp]
+    ref *= torch.sigmoid(f64(d["gate"])[0])
+    assert_rel_close(_attend(ops, d)[0].double().cpu().numpy(), ref.cpu().numpy(), tol=TOL, out_unit=BF16_U)
+
+
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("at", [500, 503, 520])
+def test_tail_verify_paged_many_rows_nan(ops, where, at):
+    """Keys past the first token's: a NaN reaches the rows that see it and no others. Before it: all."""
+    B, T, H, grp, bs = 2, 24, 2, 6, 16
+    d = _attend_inputs(B, T, H, grp, bs, [501, 30], [22, 24], seed=15)
+    clean = _attend(ops, d)
+    page, row = d["table"][0, at // bs], at % bs
+    if where == "k":
+        d["cache"][0][page, 1, row, 17] = 0x7F
+    else:
+        d["cache"][1][page, 1, [17, 200], row] = 0xFF
+        d["cache"][1][page, 1, 200, row - 1] = 0x7F
+    got = _attend(ops, d)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    if where == "k":
+        hit[0, max(at - 501, 0):22, grp:] = True
+    else:
+        hit[0, max(at - 501, 0):22, grp:, 17] = True
+        hit[0, max(at - 502, 0):22, grp:, 200] = True
+    assert torch.isnan(got[hit]).all()
+    assert torch.equal(got[~hit], clean[~hit])
+
+
+def test_tail_verify_paged_many_rows_missing_pages(ops):
+    d = _attend_inputs(3, 30, 2, 6, 16, [400, 5, 700], [30, 30, 30], seed=16)
+    d["table"][0, 1] = -1
+    d["table"][1] = len(d["cache"][0])
+    d["table"][2, [0, 3, 20, 44]] = [2**31 - 1, -2**31, -1, -1]
+    d["gate"][1] = float("nan")
+    got = _attend(ops, d).float().cpu().double().numpy()
+    d["gate"][1] = 0
+    assert not got[1].any()
+    assert_rel_close(got, _oracle(d), tol=TOL, out_unit=BF16_U, name="missing pages")
 
 
 def test_tail_verify_paged_equals_dense_op_in_values(ops):
