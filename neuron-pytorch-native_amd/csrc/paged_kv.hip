@@ -30,7 +30,9 @@ constexpr int kMinScaleExp = -100;  // the least scale is 2^-100: an all-zero pa
 //   slots       slot[b][t] = block * bs + offset of position kv_len_b + t for t < granted[b], else -1.
 // One workgroup: the prefix sums over the requests are its scans, and the block moves are dealt to
 // its threads one block each by a search in those sums, so one long prompt does not hold up a
-// thread. The slots go with it when there are few, else to a second launch over the whole chip.
+// thread. The slots go with it when there are few (up to four to a thread), else to a second launch over
+// the whole chip, which takes 4 us for 512 K slots. Bound by one workgroup's dependent loads, scans and
+// searches: 5 us for a step of 64 requests, 13 for 256 prompts of up to 2048 tokens in blocks of 16.
 struct PlanArgs {
   const int32_t* kv_len;
   const int32_t* new_len;
@@ -224,6 +226,9 @@ __global__ __launch_bounds__(256) void paged_slots_kernel(PlanArgs a) {
 // One workgroup per (request, block touched, head, K or V): it owns the page, so the
 // scale and the older rows need no atomics. Lane l of a wave holds dims 4l..4l+3 of its rows in
 // registers from the first load to the rounding (RPW rows per wave), so each input is read once.
+// 32 requests of one to eight rows take 5 us (a launch and one chain of loads); 4 x 4096 rows of 4 heads
+// in blocks of 64 (101 MB read and written) 36 us, 2.8 TB/s: a workgroup's rows all have to arrive
+// before its scale is known, and only then can it write. (Four waves a workgroup: 62 us.)
 struct PagedAppendArgs {
   const uint16_t* key;    // [B][T][Hkv][256]
   const uint16_t* value;
