@@ -135,6 +135,9 @@ __device__ __forceinline__ int last_start(const int32_t* start, int n, int x) {
   return u;
 }
 
+// Scores' factor: at least 2^-126, so that -inf times it is -inf; NaN stays.
+__device__ __forceinline__ float not_zero(float x) { return x < 0x1p-126f ? 0x1p-126f : x; }
+
 __device__ __forceinline__ float max_over_groups(float x) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
@@ -713,7 +716,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
       f16x8 pw[NRT][2];
 #pragma unroll
       for (int nt = 0; nt < NRT; ++nt) {
-        const float c = fmaxf(ks * q_scale[nt], 0x1p-126f);  // not 0: -inf stays
+        const float c = not_zero(ks * q_scale[nt]);
         float mx = st[nt][0][0];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -1064,7 +1067,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
       float c[2], mx = -INFINITY, wx = -INFINITY;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        c[half] = fmaxf(ks[half] * q_scale, 0x1p-126f);  // not 0: -inf stays
+        c[half] = not_zero(ks[half] * q_scale);
         float x = st[half][0][0];
 #pragma unroll
         for (int j = 0; j < 4; ++j)

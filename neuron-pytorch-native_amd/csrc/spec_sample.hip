@@ -483,6 +483,8 @@ __device__ __forceinline__ void row_settings(const SampleArgs& a, int r, RowStat
   // bins over what weighs something at all, or over the row's range where that is less
   const double range = fmin(kTable * ((double)kMaxExp + 1.0), ((double)m - (double)low) * o.c);
   o.per = range > 0.0 ? -fmin(kBins / range, 1e300) : 0.0;
+  // At k = 3/4 of the groups a quarter of them has no token past the k-th maximum, so that they have ln 4 on
+  // average: a list of 1.85 k, within kCap for k up to its half.
   const bool cut_k = o.k > 0 && o.k < a.V;
   o.mode = m == -INFINITY || !(T > 0.0f) ? RowState::kDone
            : m == INFINITY ? RowState::kDigits

@@ -436,6 +436,18 @@ def test_tail_verify_paged_many_rows_missing_pages(ops):
     assert_rel_close(got, _oracle(d), tol=TOL, out_unit=BF16_U, name="missing pages")
 
 
+@pytest.mark.parametrize("T", [1, 8, 30])
+@pytest.mark.parametrize("which", [2, 3])
+def test_tail_verify_paged_nan_scale(ops, T, which):
+    """A page without a valid scale makes its head's rows that see it NaN, and no others."""
+    d = _attend_inputs(2, T, 2, 6, 16, [100, 40], [T, T], seed=21)
+    clean = _attend(ops, d)
+    d["cache"][which][d["table"][0, 2], 1] = float("nan")
+    got = _attend(ops, d)
+    assert torch.isnan(got[0, :, 6:]).all()
+    assert torch.equal(got[0, :, :6], clean[0, :, :6]) and torch.equal(got[1], clean[1])
+
+
 def test_tail_verify_paged_equals_dense_op_in_values(ops):
     """The same positions through gqa::tail_verify's dense bf16 cache of the dequantised rows."""
     B, T, H, grp, bs = 2, 8, 4, 6, 32
