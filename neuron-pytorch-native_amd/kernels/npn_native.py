@@ -131,7 +131,8 @@ def register(qualname, schema, fake):
 
 def check_all(dev, *specs):
     """specs: (tensor, name, dtype, shape, or a number of elements in any shape). `require` for all
-    of them, and that they are on `dev`."""
+    of them, that they are on `dev`, and that no gradient is expected: `register` leaves out the
+    wrapper that would refuse a backward pass through the op."""
     for t, name, dtype, shape in specs:
         if isinstance(shape, int):
             ok = t.numel() == shape
@@ -140,6 +141,9 @@ def check_all(dev, *specs):
         if not (ok and t.dtype == dtype and t.device == dev and t.is_contiguous()):
             require(t, name, dtype, **({"numel": shape} if isinstance(shape, int) else {"shape": shape}))
             raise RuntimeError(f"{name} must be on {dev}, got {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} requires grad, but the op has no backward pass: "
+                               "call it under torch.no_grad()")
 
 
 def launch(dev, name, *args):

@@ -485,3 +485,19 @@ def test_refusals(ops):
         ops.paged.update_blocks_(plan[0].long(), *plan[1:], 16, 1)
     with pytest.raises(RuntimeError):
         ops.paged.update_blocks_(i32(0, 1), *plan[1:], 16, 1)
+
+
+def test_refuses_gradients(ops):
+    """No backward pass: inputs that require grad are refused unless gradients are off."""
+    d = _attend_inputs(1, 2, 1, 6, 16, [20], [2], seed=22)
+    q = d["query"].cuda().requires_grad_()
+    args = (d["gate"].cuda(), d["q_norm"].cuda(), cuda(d["cos"]), cuda(d["sin"]), *_cuda_cache(d["cache"]),
+            cuda(d["table"]), cuda(d["kv"]), cuda(d["n"]))
+    with pytest.raises(RuntimeError, match="requires grad"):
+        ops.gqa.tail_verify_paged(q, *args)
+    with torch.no_grad():
+        out = ops.gqa.tail_verify_paged(q, *args)
+    assert not out.requires_grad and torch.equal(out, ops.gqa.tail_verify_paged(q.detach(), *args))
+    r = torch.ones(2).cuda()
+    with pytest.raises(RuntimeError, match="requires grad"):
+        ops.spec.sample(torch.zeros(2, 9).cuda().requires_grad_(), r, r.int(), r, r, r)
