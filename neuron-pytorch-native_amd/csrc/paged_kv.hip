@@ -252,8 +252,13 @@ __device__ __forceinline__ float scale_of(float amax) {
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 
-// Four values / scale -> e4m3 bytes (|x| <= 448 scale where finite; the rest become NaN, 0x7F).
-__device__ __forceinline__ uint32_t to_e4m3(const float* x, float inv) {
+// Four values / scale -> e4m3 bytes (|x| <= 448 scale where finite; the rest become NaN, 0x7F). Where all
+// of a wave's are finite, the checks, most of the instructions, are left out.
+__device__ __forceinline__ uint32_t to_e4m3(const float* x, float inv, bool all_finite = false) {
+  if (all_finite) {
+    const int q = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, q, true);
+  }
   float y[4];
   uint32_t nan = 0;
 #pragma unroll
@@ -359,7 +364,7 @@ __global__ __launch_bounds__(NW * 64, RPW == 16 ? 2 : 4) void paged_append_kerne
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           v[j] = wt[j] * (v[j] * rn);
-          y[j] = __shfl_xor(v[j], 8, 64);  // dim d ^ 32
+          y[j] = __uint_as_float(npn::dpp32<0x128>(__float_as_uint(v[j])));  // dim d ^ 32: 8 lanes round the 16
         }
         const float sg = lane < ROPE / 8 ? -1.0f : 1.0f;
         const float t[4] = {v[0] * c[k].x + sg * y[0] * s[k].x, v[1] * c[k].y + sg * y[1] * s[k].y,
@@ -369,12 +374,25 @@ __global__ __launch_bounds__(NW * 64, RPW == 16 ? 2 : 4) void paged_append_kerne
       }
     }
   }
-  float amax = 0.f;
+  float amax = 0.f, none = 0.f;
 #pragma unroll
   for (int i = 0; i < RPW; ++i)
+    if (row_of(i) < rows) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      amax = fmaxf(amax, row_of(i) < rows && finite(x[i][j]) ? fabsf(x[i][j]) : 0.f);
+      for (int j = 0; j < 4; ++j) {
+        amax = fmaxf(amax, fabsf(x[i][j]));
+        none = fmaf(x[i][j], 0.0f, none);  // NaN from the first that is not finite
+      }
+    }
+  const bool all_finite = __builtin_amdgcn_ballot_w64(none != none) == 0;
+  if (!all_finite) {
+    amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < RPW; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        amax = fmaxf(amax, row_of(i) < rows && finite(x[i][j]) ? fabsf(x[i][j]) : 0.f);
+  }
   amax = npn::wave_max(amax);
   if (lane == 0) s_amax[w] = amax;
   __syncthreads();
@@ -399,7 +417,7 @@ __global__ __launch_bounds__(NW * 64, RPW == 16 ? 2 : 4) void paged_append_kerne
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
       const int r = row_of(i);
-      if (r < rows) *reinterpret_cast<uint32_t*>(page + (size_t)(off + r) * DH) = to_e4m3(x[i], inv);
+      if (r < rows) *reinterpret_cast<uint32_t*>(page + (size_t)(off + r) * DH) = to_e4m3(x[i], inv, all_finite);
     }
     return;
   }
@@ -412,15 +430,15 @@ __global__ __launch_bounds__(NW * 64, RPW == 16 ? 2 : 4) void paged_append_kerne
   if constexpr (RPW < 4) {
 #pragma unroll
     for (int i = 0; i < RPW; ++i) {
-      const uint32_t q = to_e4m3(x[i], inv);
+      const uint32_t q = to_e4m3(x[i], inv, all_finite);
 #pragma unroll
       for (int j = 0; j < 4; ++j) bytes[(64 * j + lane) * kLine * 4 + w + NW * i] = (uint8_t)(q >> (8 * j));
     }
   } else {
 #pragma unroll
     for (int i = 0; i < RPW; i += 4) {
-      const uint32_t q0 = to_e4m3(x[i], inv), q1 = to_e4m3(x[i + 1], inv);
-      const uint32_t q2 = to_e4m3(x[i + 2], inv), q3 = to_e4m3(x[i + 3], inv);
+      const uint32_t q0 = to_e4m3(x[i], inv, all_finite), q1 = to_e4m3(x[i + 1], inv, all_finite);
+      const uint32_t q2 = to_e4m3(x[i + 2], inv, all_finite), q3 = to_e4m3(x[i + 3], inv, all_finite);
       const uint32_t a0 = __builtin_amdgcn_perm(q1, q0, 0x05010400u);  // rows 0, 1 of dims 0, 1
       const uint32_t a1 = __builtin_amdgcn_perm(q1, q0, 0x07030602u);  // and of dims 2, 3
       const uint32_t b0 = __builtin_amdgcn_perm(q3, q2, 0x05010400u);
