@@ -227,8 +227,10 @@ __global__ __launch_bounds__(256) void paged_slots_kernel(PlanArgs a) {
 // scale and the older rows need no atomics. Lane l of a wave holds dims 4l..4l+3 of its rows in
 // registers from the first load to the rounding (RPW rows per wave), so each input is read once.
 // 32 requests of one to eight rows take 5 us (a launch and one chain of loads); 4 x 4096 rows of 4 heads
-// in blocks of 64 (101 MB read and written) 36 us, 2.8 TB/s: a workgroup's rows all have to arrive
-// before its scale is known, and only then can it write. (Four waves a workgroup: 62 us.)
+// in blocks of 64 (101 MB read and written) 30 us, 3.4 TB/s, bound by instructions to a row and by a
+// workgroup's rows all having to arrive before its scale is known: only then can it write. (Checks for
+// infinities at each conversion: 36 us. Four waves a workgroup of 16 rows each: 62, and 16 of 4 rows,
+// more of which fit a CU: 32. Blocks of 128 with 8 waves of 16 rows 43, with 16 of 8 rows 35.)
 struct PagedAppendArgs {
   const uint16_t* key;    // [B][T][Hkv][256]
   const uint16_t* value;
@@ -295,7 +297,7 @@ __device__ __forceinline__ float wave_sum_valu(float v) {
 // NW waves, RPW rows each: below 4 rows w, w + NW, ..; from 4 on blocks of four rows w, w + NW, .., whose 4 x 4
 // bytes a lane turns from rows into dims in registers.
 template <int RPW, int NW>
-__global__ __launch_bounds__(NW * 64, RPW == 16 ? 2 : 4) void paged_append_kernel(PagedAppendArgs a) {
+__global__ __launch_bounds__(NW * 64, 4) void paged_append_kernel(PagedAppendArgs a) {
   const int b = blockIdx.z, h = blockIdx.y >> 1;
   const bool is_v = blockIdx.y & 1;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -548,6 +550,6 @@ extern "C" int npn_gqa_kv_append_paged(const uint16_t* key, const uint16_t* valu
   else if (rows <= 16) launch(paged_append_kernel<4, 4>, 4);
   else if (rows <= 32) launch(paged_append_kernel<4, 8>, 8);
   else if (rows <= 64) launch(paged_append_kernel<8, 8>, 8);
-  else launch(paged_append_kernel<16, 8>, 8);
+  else launch(paged_append_kernel<8, 16>, 16);
   return npn_launch_status();
 }
