@@ -208,3 +208,50 @@ def test_verify_slice_with_a_paged_cache(bs):
         ids += graph.pages["free"][:int(graph.pages["count"])].tolist()
         assert sorted(ids) == list(range(B * -(-512 // bs)))
     assert torch.equal(eager.kv_len, graph.kv_len)
+
+
+def test_chunk_and_sampling_replayed_beside_each_other(ops):
+    """A prompt chunk's attention captured in one graph and sampling in another, replayed on two streams
+    at once with lengths, pages and settings that change in place, against eager calls."""
+    from test_gpu_paged import _attend_inputs, _cuda_cache
+    from test_gpu_sample import _settings
+    T, V = 70, 30011
+    inputs = [_attend_inputs(3, T, 2, 6, 32, kv, n, seed=5 + k, spare_pages=spare) for k, (kv, n, spare) in enumerate(
+        [([300, 0, 77], [70, 70, 3], 30), ([0, 900, 0], [0, 70, 70], 6), ([5, 5, 640], [70, 1, 64], 25)])]
+    N = min(len(d["cache"][0]) for d in inputs)
+    P = max(d["table"].shape[1] for d in inputs)
+    cases = []
+    for d in inputs:
+        assert d["table"].max() < len(d["cache"][0])
+        table = np.full((3, P), -1, np.int32)
+        table[:, :d["table"].shape[1]] = np.where(d["table"] < N, d["table"], -1)
+        cases.append([d["query"].cuda(), d["gate"].cuda(), *(c[:N].clone() for c in _cuda_cache(d["cache"])),
+                      *(torch.from_numpy(a).cuda() for a in (table, d["kv"], d["n"]))])
+    cos, sin = (torch.from_numpy(np.ascontiguousarray(inputs[1][k])).float().cuda() for k in ("cos", "sin"))
+    norm = inputs[0]["q_norm"].cuda()
+    rng = np.random.default_rng(3)
+    rows = []
+    for _ in range(3):
+        s = _settings(40, rng)
+        rows.append([torch.randn(40, V, device="cuda")] + [torch.from_numpy(s[k]).cuda() for k in
+                                                           ("temperature", "top_k", "top_p", "min_p", "u")])
+    live, srow = [t.clone() for t in cases[0]], [t.clone() for t in rows[0]]
+    attend = lambda c: ops.gqa.tail_verify_paged(c[0], c[1], norm, cos, sin, *c[2:])  # noqa: E731
+    want = [(attend(c), ops.spec.sample(*r)) for c, r in zip(cases, rows)]
+    torch.cuda.synchronize()
+    ga, gs = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(ga):
+        out = attend(live)
+    with torch.cuda.graph(gs):
+        ids = ops.spec.sample(*srow)
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for k in (0, 1, 2, 1, 0):
+        for dst, src in zip(live + srow, cases[k] + rows[k]):
+            dst.copy_(src)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(one):
+            ga.replay()
+        with torch.cuda.stream(two):
+            gs.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[k][0]) and torch.equal(ids, want[k][1])
