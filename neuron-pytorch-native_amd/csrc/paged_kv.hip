@@ -126,11 +126,12 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
   __shared__ int s_at[kPlanThreads];  // first entry of the request's row to move
   const int tid = threadIdx.x;
   const int count0 = min(max(a.free_count[0], 0), a.N);
+  const Req r0 = load_req(a, tid);  // kept: most batches have no request past these
 
   // blocks given back by all requests
   int given = 0;
   for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
-    const Req r = load_req(a, b0 + tid);
+    const Req r = b0 == 0 ? r0 : load_req(a, b0 + tid);
     int total;
     plan_scan(max(r.held - r.want, 0), s_wave, total);
     given += total;
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
   if (given > 0) {
     int run = 0;  // given back by earlier groups of requests
     for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
-      const Req r = load_req(a, b0 + tid);
+      const Req r = b0 == 0 ? r0 : load_req(a, b0 + tid);
       const int mine = max(r.held - r.want, 0);
       int total;
       const int upto = plan_scan(mine, s_wave, total);
@@ -162,7 +163,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PlanArgs a) {
   int taken = 0;
   for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
-    const Req r = load_req(a, b);
+    const Req r = b0 == 0 ? r0 : load_req(a, b);
     const bool room = r.want <= a.P;
     const int need = room ? max(r.want - r.held, 0) : 0;
     int total;
