@@ -276,12 +276,14 @@ constexpr int kPrepWaves = 8;
 constexpr int kPlanUnits = 4096;  // units whose steps the plan keeps in LDS
 
 // One workgroup per CU where the pairs with steps are few enough to be cut so; else one each and 512
-// more for the longest. Groups of 128 rows are few and long, so that a second round of workgroups may
-// pay where the first leaves many CUs idle (96 pairs make 192): the plan takes the cheaper by the steps
-// of 128 keys that the rounds last, with 1.5 for a workgroup's start and end and 2.5 for writing and
-// merging the parts of 256.
+// more for the longest. Requests of 100 to 16384 keys, 4 kv heads: 128 pairs 119 us in 256 workgroups and
+// 129 in 640, 180 pairs of 48 rows 214 and 201, 240 pairs 232 and 209. Groups of 128 rows are few and long,
+// so that a second round of workgroups may pay where the first leaves many CUs idle: 512 x 6 rows over
+// 16384 keys, 96 pairs, take 330 us in 192 workgroups and 290 in 480. The plan takes the cheaper by the
+// steps of 128 keys that the rounds last, with 1.5 for a workgroup's start and end and 2.5 for writing
+// and merging the parts of 256.
 __host__ __device__ constexpr int most_workgroups(int R, int pairs, int rounds) {
-  return R == kRows && rounds == 2 && pairs > 64 && pairs <= 448 ? 512 : pairs <= 192 ? 256 : pairs + 512;
+  return R == kRows && rounds == 2 && pairs > 64 && pairs <= 448 ? 512 : pairs <= 160 ? 256 : pairs + 512;
 }
 // Split pairs' workgroups: all of 256 or 512, or, as a pair of c >= 2 has c - 1 of the 512 more, twice
 // those.
@@ -1161,9 +1163,10 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
 
 // ---- 3. merge ---------------------------------------------------------------------------------------
 // The workgroups' (m, l, O) of a row of a pair, WPR waves to a row: wave q takes parts q, q + WPR, ...,
-// four loads of each at a time, and the first wave merges the waves'. One wave a row where pairs
-// have few parts, four where one pair has most of the chip (25 us for one sequence of 32768 keys
-// with one wave walking its 64 parts a load at a time).
+// four loads of each at a time, and the first wave merges the waves'. Four waves where rows are few and so
+// have many parts, else one. With both launches before it, four waves and one: 4 pairs of 16 rows with
+// 64 parts each 27.5 and 37.2 us, 32 pairs 62.6 and 66.2, 64 pairs 57.9 and 59.0, 96 pairs 91.1 and 90.8,
+// 96 pairs of 48 rows 115.3 and 113.4.
 template <int WPR>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
   const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -1238,6 +1241,9 @@ PagedPlan paged_plan(int B, int T, int q_heads, int kv_heads, int max_blocks, in
   p.grp = q_heads / kv_heads;
   const int64_t rows = (int64_t)T * p.grp;
   if (p.grp > 48 || rows > 1 << 20 || (int64_t)max_blocks * block_size > (int64_t)1 << 30) return p;
+  // Groups of 128 against groups of 48: 32 requests of 54 rows 46 and 53 us, one of 54 27 and 31, 8 of 384 75
+  // and 98, 2 of 1536 128 and 165; 16 of 96 146 and 148; but 4 of 192 59 and 54, one of 1536 over an empty
+  // cache 35 and 30.
   p.R = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 ? 48 : kRows;
   p.RG = (int)((rows + p.R - 1) / p.R);
   const int64_t pairs = (int64_t)B * p.RG * kv_heads;
@@ -1302,7 +1308,7 @@ extern "C" int npn_gqa_tail_verify_paged(
     hipLaunchKernelGGL((paged_attn_kernel<3, 4>), dim3(p.grid), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL(paged_rows_kernel, dim3(p.grid), dim3(512), 0, s, a);
-  if (p.pairs < 32)
+  if (p.pairs < 32 || p.pairs * p.R < 96 * 16)
     hipLaunchKernelGGL(paged_merge_kernel<4>, dim3(p.R, p.pairs), dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL(paged_merge_kernel<1>, dim3(p.R / 4, p.pairs), dim3(256), 0, s, a);
