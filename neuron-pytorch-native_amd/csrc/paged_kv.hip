@@ -514,6 +514,8 @@ extern "C" int npn_paged_update_blocks(const int32_t* kv_len, const int32_t* new
               NPN_ERR_SHAPE);
   NPN_REQUIRE(NPN_ALIGNED16(slots), NPN_ERR_ALIGN);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  // In a graph, without moves: 4.2 us for 512 slots in the plan's launch, 4.9 for 2048, 5.9 for 4096 and 7.8
+  // for 8192; with a launch for them 5.8 for any of these.
   const int here = (int64_t)B * T <= 4 * kPlanThreads;
   const PlanArgs a{kv_len, new_len, block_table, num_blocks, free_blocks, free_count, slots, granted,
                    B, max_blocks, n_blocks, T, sh, here};
