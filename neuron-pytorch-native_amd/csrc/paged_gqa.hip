@@ -46,9 +46,10 @@
 //     the 16x16x128 products as they are, and q' and P as three e4m3 parts of four bits each, 2^-4
 //     and 2^-8 in the product's scale operand: 12 bits, for 1.5 times the f16 products' time. 2 chunks of
 //     256 x 6 rows over up to 8192 keys: 128 us (157 with groups of 48 rows; 142 with 128 rows in f16),
-//     616 TFLOP/s by the formula's operations. Matrix units 51 %, vector units 55 % busy, and they do
-//     not overlap: priorities for one wave of each SIMD, or its V products half a step behind the
-//     other's, changed nothing.
+//     616 TFLOP/s by the formula's operations. Matrix units 51 %, vector units 55 % busy, which
+//     overlap little: without the softmax 100 us would remain, without V's products 100, without the DMAs
+//     123. Priorities for one wave of each SIMD, its V products half a step behind the other's, or LDS
+//     reads ahead of the products before them changed nothing.
 //  3. merge: the log-sum-exp merge of the other pairs' workgroups, times sigmoid(gate), to bf16.
 // prep takes 4 to 9 us and merge 5 to 10 for these.
 #include "npn_common.h"
