@@ -298,6 +298,14 @@ def test_tail_verify_paged_long(ops):
     _check(ops, _attend_inputs(2, 8, 4, 6, 128, [32768 - 8, 17000], [8, 8], seed=5))
 
 
+def test_tail_verify_paged_more_requests_than_the_plan_keeps(ops):
+    """4300 units, some without a step: the plan reads the lengths past its 4096 again."""
+    rng = np.random.default_rng(4)
+    kv, n = rng.integers(0, 50, 4300), rng.integers(0, 2, 4300)
+    kv[4200] = 700
+    _check(ops, _attend_inputs(4300, 1, 1, 2, 16, kv, n, seed=44))
+
+
 def test_tail_verify_paged_all_idle(ops):
     d = _attend_inputs(3, 2, 2, 6, 16, [5, 0, 40], [0, 0, 0], seed=9)
     assert not _attend(ops, d).any()
