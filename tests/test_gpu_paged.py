@@ -509,3 +509,33 @@ def test_refuses_gradients(ops):
     r = torch.ones(2).cuda()
     with pytest.raises(RuntimeError, match="requires grad"):
         ops.spec.sample(torch.zeros(2, 9).cuda().requires_grad_(), r, r.int(), r, r, r)
+
+
+@pytest.mark.parametrize("T", [1, 8, 40])
+def test_pages_past_32_bit_offsets(ops, T):
+    """A pool of 5 GB for K and for V, of which the request holds the last blocks: the appended bytes and
+    the attention over them are those of a pool with these blocks alone."""
+    H, bs, N, held = 4, 128, 40000, 4
+    g = torch.Generator(device="cuda").manual_seed(T)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    kv = torch.tensor([held * bs - T - 3], dtype=torch.int32, device="cuda")
+    n = torch.tensor([T], dtype=torch.int32, device="cuda")
+    cos, sin = (cuda(a) for a in og.rope_cos_sin(np.arange(held * bs)))
+    norm = r(256) * 0.1
+    past = [r(1, held * bs - T - 3, H, 256).to(BF) for _ in range(2)]
+    new = [r(1, T, H, 256).to(BF) for _ in range(2)]
+    q, gate = r(1, T, 6 * H, 256).to(BF), r(1, T, 6 * H, 256).to(BF)
+    outs, pages = [], []
+    for blocks in (N, held):
+        cache = (torch.zeros(blocks, H, bs, 256, dtype=torch.int8, device="cuda"),
+                 torch.zeros(blocks, H, 256, bs, dtype=torch.int8, device="cuda"),
+                 torch.ones(blocks, H, device="cuda"), torch.ones(blocks, H, device="cuda"))
+        table = torch.arange(blocks - held, blocks, dtype=torch.int32, device="cuda")[None]
+        slots = (blocks - held) * bs + torch.arange(held * bs, device="cuda")[None]
+        ops.gqa.kv_append_paged(*past, norm, cos, sin, torch.zeros_like(kv), slots[:, :-T - 3].contiguous(), *cache)
+        ops.gqa.kv_append_paged(*new, norm, cos, sin, kv, slots[:, -T - 3:-3].contiguous(), *cache)
+        outs.append(ops.gqa.tail_verify_paged(q, gate, norm, cos, sin, *cache, table, kv, n))
+        pages.append([c[-held:].clone() for c in cache])
+        assert not cache[0][:-held].any() and not cache[1][:-held].any()
+    assert all(torch.equal(a, b) for a, b in zip(*pages))
+    assert torch.equal(*outs) and outs[0].isfinite().all() and outs[0].any()

@@ -135,3 +135,17 @@ def test_sample_top_k_wherever_the_largest_lie(ops, R, V, kind):
     s["temperature"][:] = rng.choice([0.3, 1.0, 5.0], R)
     s["top_k"] = np.resize(np.array([1, 7, 64, 700, 1200, 1201, 2047, 2048, 2049, 3100, 4095, 4096, 4097], np.int32), R)
     _check(ops, torch.from_numpy(x), s)
+
+
+def test_sample_past_32_bit_offsets(ops):
+    """More logits than 2^31: rows from all over the batch give what they give alone."""
+    R, V = 8700, 248320
+    assert R * V > 2**31
+    x = torch.empty(R, V, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator("cuda").manual_seed(2))
+    s = _settings(R, np.random.default_rng(2))
+    s["top_k"][s["top_k"] > 1000] = 0
+    args = [torch.from_numpy(s[k]).cuda() for k in ("temperature", "top_k", "top_p", "min_p", "u")]
+    got = ops.spec.sample(x, *args)
+    for r in (0, 2047, 2048, 4321, 8648, 8649, R - 1):
+        assert got[r] == ops.spec.sample(x[r:r + 1].clone(), *[a[r:r + 1].clone() for a in args])[0]
+    assert ((got >= 0) & (got < V)).all() and got.unique().numel() > R // 2
