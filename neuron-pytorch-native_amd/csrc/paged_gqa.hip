@@ -43,10 +43,15 @@
 //  2b. rows, R = 128: eight waves of 16 rows share the steps, which pass once through LDS, two steps in
 //     all there. Half of the instructions above made f16 of K's and V's bytes, for 16 to 48 rows at
 //     a time, and the matrix units were busy for a quarter of the time. Here the bytes go into
-//     the 16x16x128 products as they are, and q' and P as three e4m3 parts of four bits each, 2^-4
-//     and 2^-8 in the product's scale operand: 12 bits, for 1.5 times the f16 products' time. 2 chunks of
-//     256 x 6 rows over up to 8192 keys: 128 us (157 with groups of 48 rows; 142 with 128 rows in f16),
-//     616 TFLOP/s by the formula's operations. Matrix units 51 %, vector units 55 % busy, which
+//     the 16x16x128 products as they are, and q' as three e4m3 parts of four bits each, 2^-4
+//     and 2^-8 in the product's scale operand: 12 bits, for 1.5 times the f16 products' time. P goes in
+//     parts too, two of e4m3 and one of e5m2, over a power of two of its own for each 32 keys of a row,
+//     which is what that operand holds one number for: 13 bits of the weights down to 2^-13 of the 32's
+//     largest, and some of those down to 2^-40 of it. (With three e4m3 parts over one power of two a
+//     row, 2^-17 was the least step: a row's other weights were off by 6 % at 2^-20 of its largest and
+//     gone at 2^-22, which is all there is where the largest one's value is near 0. 1 us less.) 2 chunks of
+//     256 x 6 rows over up to 8192 keys: 130 us (157 with groups of 48 rows; 142 with 128 rows in f16),
+//     608 TFLOP/s by the formula's operations. Matrix units 51 %, vector units 55 % busy, which
 //     overlap little: without the softmax 100 us would remain, without V's products 100, without the DMAs
 //     123. Priorities for one wave of each SIMD, its V products half a step behind the other's, or LDS
 //     reads ahead of the products before them changed nothing.
@@ -139,12 +144,16 @@ __device__ __forceinline__ int last_start(const int32_t* start, int n, int x) {
 // Scores' factor: at least 2^-126, so that -inf times it is -inf; NaN stays.
 __device__ __forceinline__ float not_zero(float x) { return x < 0x1p-126f ? 0x1p-126f : x; }
 
-__device__ __forceinline__ float max_over_groups(float x) {
+// Maxima over the lanes (i, G) of a column: of G and G ^ 2, of G and G ^ 1, of all.
+__device__ __forceinline__ float max_over_halves(float x) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
+__device__ __forceinline__ float max_over_pair(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float max_over_groups(float x) { return max_over_pair(max_over_halves(x)); }
 __device__ __forceinline__ float sum_over_groups(float x) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -218,6 +227,13 @@ __device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b) {
 __device__ __forceinline__ f32x4 mfma_e4m3(i32x8 a, i32x8 b, f32x4 c, int part) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 127, 0, 127 - 4 * part);
 }
+// The same with a part of P as B: e5m2 for the last, and byte `part` of `scales`, the biased exponents of
+// the powers of two that a block of 32 k is times. Of a lane's 32 bytes the first 16 are k 16 G + [0, 16),
+// the others 64 more; block n of k, [32 n, + 32), takes its exponent from the lanes with G = n.
+template <int PART>
+__device__ __forceinline__ f32x4 mfma_p(i32x8 a, i32x8 b, f32x4 c, int scales) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, PART == 2 ? 1 : 0, 0, 127, PART, scales);
+}
 
 // LDS by address, element k of 16 bytes (1 KB apart: one per lane) from a per-lane base. The bases are
 // hidden from the optimiser (opaque): left to itself it kept some hundred of base + offset sums,
@@ -256,7 +272,8 @@ __device__ __forceinline__ void write_out(const PagedArgs& a, int b, int row, in
 }
 
 // Four numbers of at most 448 as a word each of three e4m3 parts, x = p0 + p1 / 16 + p2 / 256: each part
-// takes 4 bits of what the ones before leave, 12 in all, down to steps of 2^-17.
+// takes 4 bits of what the ones before leave, 12 in all, down to steps of 2^-17. For q', whose small
+// elements count by what they add to the row's large ones.
 __device__ __forceinline__ void split3(float x0, float x1, float x2, float x3, uint32_t (&part)[3]) {
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
@@ -271,6 +288,29 @@ __device__ __forceinline__ void split3(float x0, float x1, float x2, float x3, u
     x3 = (x3 - hi[1]) * 16.0f;
   }
 }
+
+// Four weights of at most 2^8, x = p0 + 2^-5 p1 + 2^-17 p2, p0 and p1 in e4m3 and p2 in e5m2, which has 3 bits
+// instead of 4 but reaches 2^-16 instead of 2^-9. What p0 and p1 leave is at most 2^-9 of x's power of two, or
+// half of p1's least step, 2^-15; p2 has it to 2^-4 of its own: x to 2^-13 down to 2^-6, to 2^-19 below that,
+// and where it is p2 alone, to 2^-3 of itself down to 2^-31, with steps of 2^-33 to the end.
+__device__ __forceinline__ void split_p(float x0, float x1, float x2, float x3, uint32_t (&part)[3]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, w, true);
+    part[k] = (uint32_t)w;
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    const float by = k == 0 ? 0x1p5f : 0x1p12f;
+    x0 = (x0 - lo[0]) * by;
+    x1 = (x1 - lo[1]) * by;
+    x2 = (x2 - hi[0]) * by;
+    x3 = (x3 - hi[1]) * by;
+  }
+  int w = __builtin_amdgcn_cvt_pk_bf8_f32(x0, x1, 0, false);
+  w = __builtin_amdgcn_cvt_pk_bf8_f32(x2, x3, w, true);
+  part[2] = (uint32_t)w;
+}
+constexpr int kPartExp[3] = {0, 5, 17};
 
 // ---- 1. prep ----------------------------------------------------------------------------------------
 constexpr int kPrepWaves = 8;
@@ -888,7 +928,7 @@ struct RowsSmem {
 
 __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
   constexpr int R = kRows, KR = 128, kSteps = kChunk * KS / KR;
-  constexpr float kP = 4.0f;  // P is at most 2^(4 + 4), under e4m3's 448
+  constexpr int kTop = 7;  // a block's largest weight is taken to [2^kTop, 2^(kTop + 1))
   __shared__ __attribute__((aligned(1024))) RowsSmem sm;
   const int tid = threadIdx.x;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -1067,7 +1107,9 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
               if (!held[half] || k0 + KS * half + 16 * G + 4 * j + e > lim) st[half][j][e] = -INFINITY;
       }
 
-      float c[2], mx = -INFINITY, wx = -INFINITY;
+      // Beside the row's maxima, `top` of each block of 32 keys that its products take as one: those of
+      // the lanes G and G ^ 1 in a half.
+      float c[2], mx = -INFINITY, top[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         c[half] = not_zero(ks[half] * q_scale);
@@ -1077,9 +1119,9 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) x = fmaxf(x, st[half][j][e]);
         mx = fmaxf(mx, x * c[half]);
-        wx = fmaxf(wx, x * c[half] + vs[half]);
+        top[half] = max_over_pair(x * c[half] + vs[half]);
       }
-      wx = max_over_groups(wx);
+      const float wx = max_over_halves(fmaxf(top[0], top[1]));
       mx = max_over_groups(mx);
       const bool grow = mx > m_run + kRescaleLog2, wgrow = wx > w_run + kRescaleLog2;
       if (__builtin_amdgcn_ballot_w64(grow || wgrow) != 0) {
@@ -1091,11 +1133,13 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
 #pragma unroll
         for (int d = 0; d < 16; ++d) acc[d] *= corr;
       }
+      // Each block's weights over a power of two of their own: whole, 2^-100 of the row's at least.
       i32x8 p[3];
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      float sum[4] = {0.f, 0.f, 0.f, 0.f}, block[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const float f = __builtin_amdgcn_exp2f(fminf(m_run + vs[half] - w_run + kP, 120.0f));
+        block[half] = fminf(fmaxf(floorf(top[half] - w_run), -100.0f), kRescaleLog2);
+        const float f = __builtin_amdgcn_exp2f(fminf(m_run + vs[half] - w_run + (kTop - block[half]), 120.0f));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float pv[4];
@@ -1105,13 +1149,17 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
             sum[e] += pv[e];
           }
           uint32_t word[3];
-          split3(pv[0] * f, pv[1] * f, pv[2] * f, pv[3] * f, word);
+          split_p(pv[0] * f, pv[1] * f, pv[2] * f, pv[3] * f, word);
 #pragma unroll
           for (int k = 0; k < 3; ++k) p[k][4 * half + j] = (int)word[k];
           __builtin_amdgcn_sched_barrier(0);
         }
       }
       l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      // Lanes G = 0, 1, 2, 3 hand over the exponents of half 0's first and second block and half 1's.
+      const auto lo_hi = __builtin_amdgcn_permlane32_swap((int)block[0], (int)block[1], false, false);
+      int scales = (127 - kTop + (int)((G & 1) ? lo_hi[1] : lo_hi[0])) * 0x010101;
+      scales -= kPartExp[1] << 8 | kPartExp[2] << 16;
 
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
@@ -1122,9 +1170,11 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
 #pragma unroll
           for (int d = 0; d < 4; ++d) v[half][d] = lds_read(vat, 32 * half + 16 + 4 * n + d);
 #pragma unroll
-        for (int k = 0; k < 3; ++k)
+        for (int d = 0; d < 4; ++d) acc[4 * n + d] = mfma_p<0>(join(v[0][d], v[1][d]), p[0], acc[4 * n + d], scales);
 #pragma unroll
-          for (int d = 0; d < 4; ++d) acc[4 * n + d] = mfma_e4m3(join(v[0][d], v[1][d]), p[k], acc[4 * n + d], k);
+        for (int d = 0; d < 4; ++d) acc[4 * n + d] = mfma_p<1>(join(v[0][d], v[1][d]), p[1], acc[4 * n + d], scales);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) acc[4 * n + d] = mfma_p<2>(join(v[0][d], v[1][d]), p[2], acc[4 * n + d], scales);
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -1133,7 +1183,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
 
   // A wave has its rows whole: through LDS, for stores of whole rows, 16 bytes at f of dim 4 f to place
   // f ^ i of row i.
-  const float l = sum_over_groups(l_run), scale = exp2f(w_run - m_run - kP);
+  const float l = sum_over_groups(l_run), scale = exp2f(w_run - m_run);
   const size_t slot = (size_t)a.sstart[u] + h * parts + part;
   __syncthreads();  // every wave is done with the ring
   f32x4* const o = &sm.o[w][0][0];

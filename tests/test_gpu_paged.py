@@ -5,7 +5,9 @@ normed K value apart, attention within its roundings.
 Attention's tolerance: the kernel rounds q' to f16 relative to the row's largest element (at most
 2^-11, 0.0002 in the root mean square), the softmax weights to f16 (2^-11 as well) and its output to
 bf16, at most 2^-8 relative and 0.43 * 2^-8 = 0.0017 in the root mean square over a binade:
-2e-3 in the norm, and for an element its own rounding (BF16_U) beside 2e-3 of the largest.
+2e-3 in the norm, and for an element its own rounding (BF16_U) beside 2e-3 of the largest. Above
+48 rows of a kv head q' has three e4m3 parts (2^-13 at most) and a weight three parts over its 32 keys'
+largest (2^-13, or 2^-26 of that largest): less than f16's.
 """
 import numpy as np
 import pytest
@@ -406,6 +408,48 @@ def test_tail_verify_paged_many_rows_long(ops):
         ref[:, h] = torch.softmax(s, -1) @ v[h // grp]
     ref *= torch.sigmoid(f64(d["gate"])[0])
     assert_rel_close(_attend(ops, d)[0].double().cpu().numpy(), ref.cpu().numpy(), tol=TOL, out_unit=BF16_U)
+
+
+@pytest.mark.parametrize("T", [8, 40])
+@pytest.mark.parametrize("at", [0, 9001])
+def test_tail_verify_paged_dominating_key(ops, T, at):
+    """One key 11 to 18 nats above 16000 others that are all alike, its value 0: a row's output is what
+    the small weights leave, row by row against the formula in 64 bits. As many pairs as leave each
+    whole (T = 40), requests over the same pages.
+
+    Beside the output's rounding (0.43 * 2^-8 = 0.0017 of a row in the root mean square, 0.0023 where all
+    its elements lie at the bottom of a binade) such a row has, in full, the weights' rounding, alike for
+    equal weights: 2^-11 in f16, 2^-13 in three parts. Those of the key's own 32 in the parts are off by
+    up to 2^-3, 31 of 16000: 0.0002. And the key's score, at most 18 nats of 128 products of one sign, each
+    with q's rounding of 0.0002: 18 * 0.0002 / (0.8 * sqrt(128)) = 0.0004, four deviations 0.0016. In all
+    0.0046."""
+    B, grp, bs, kv = 264, 6, 64, 16000 - 17
+    S = kv + T
+    P = -(-S // bs)
+    g = torch.Generator().manual_seed(T + at)
+    cache = [np.zeros((P, 1, bs, 256), np.uint8),
+             torch.randint(0x30, 0x41, (P, 1, 256, bs), generator=g).numpy().astype(np.uint8),  # 0.5 to 2
+             np.ones((P, 1), np.float32), np.exp2(np.arange(P) % 3).astype(np.float32).reshape(P, 1)]
+    cache[0][at // bs, 0, at % bs, 128:] = 0x41  # 2.25
+    cache[1][at // bs, 0, :, at % bs] = 0
+    q = torch.randn(1, T, grp, 256, generator=g).abs().to(BF)
+    gate = torch.randn(1, T, grp, 256, generator=g).to(BF)
+    i32 = lambda v: torch.full((B,), v, dtype=torch.int32, device="cuda")  # noqa: E731
+    table = torch.arange(P, dtype=torch.int32, device="cuda").expand(B, P).contiguous()
+    out = ops.gqa.tail_verify_paged(q.cuda().expand(B, -1, -1, -1).contiguous(),
+                                    gate.cuda().expand(B, -1, -1, -1).contiguous(), torch.zeros(256).cuda(),
+                                    *(cuda(a) for a in og.rope_cos_sin(np.arange(S))), *_cuda_cache(cache), table,
+                                    i32(kv), i32(T))
+    v = cuda(cache[1]).view(torch.float8_e4m3fn).double() * cuda(cache[3]).double()[..., None, None]
+    v = v[:, 0].transpose(1, 2).reshape(-1, 256).cumsum(0)[kv:kv + T]  # up to each token's last key
+    x = q[0].double()
+    gap = (x * torch.rsqrt((x * x).mean(-1, keepdim=True) + 1e-6))[..., 128:].sum(-1) * 2.25 / 16  # [T, grp]
+    assert 10 < gap.min() and gap.max() < 18
+    z = torch.arange(kv, kv + T)[:, None] + gap.exp()
+    ref = v.cpu()[:, None] / z[..., None] * torch.sigmoid(gate[0].double())
+    for b in (0, B - 1):
+        err = (out[b].cpu().double() - ref).norm(dim=-1) / ref.norm(dim=-1)
+        assert err.max() <= 0.0046, float(err.max())
 
 
 @pytest.mark.parametrize("where", ["k", "v"])
