@@ -141,8 +141,11 @@ __device__ __forceinline__ int last_start(const int32_t* start, int n, int x) {
   return u;
 }
 
-// Scores' factor: at least 2^-126, so that -inf times it is -inf; NaN stays.
+// Scores' factor: at least 2^-126, so that -inf times it is -inf; NaN stays. (A row that sees none of a
+// lane's 16 keys takes 1, and 0 as their values' logarithm: their page's scales are not its business.)
 __device__ __forceinline__ float not_zero(float x) { return x < 0x1p-126f ? 0x1p-126f : x; }
+// 2^x for x up to 120, and 2^120 above; NaN stays.
+__device__ __forceinline__ float exp2_bounded(float x) { return __builtin_amdgcn_exp2f(x > 120.0f ? 120.0f : x); }
 
 // Maxima over the lanes (i, G) of a column: of G and G ^ 2, of G and G ^ 1, of all.
 __device__ __forceinline__ float max_over_halves(float x) {
@@ -759,14 +762,15 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
       f16x8 pw[NRT][2];
 #pragma unroll
       for (int nt = 0; nt < NRT; ++nt) {
-        const float c = not_zero(ks * q_scale[nt]);
+        const bool hidden = tail && k0 + 16 * G > lim[nt];  // all 16 keys of the lane
+        const float c = hidden ? 1.0f : not_zero(ks * q_scale[nt]), vsn = hidden ? 0.0f : vs;
         float mx = st[nt][0][0];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[nt][j][r]);
         mx *= c;
-        const float wx = max_over_groups(mx + vs);
+        const float wx = max_over_groups(mx + vsn);
         mx = max_over_groups(mx);
         const bool grow = mx > m_run[nt] + kRescaleLog2, wgrow = wx > w_run[nt] + kRescaleLog2;
         if (__builtin_amdgcn_ballot_w64(grow || wgrow) != 0) {
@@ -781,7 +785,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
             if constexpr (NW == 4) pin(acc[nt][d]);
           }
         }
-        const float f = __builtin_amdgcn_exp2f(fminf(m_run[nt] + vs - w_run[nt] + kPLog2, 120.0f));
+        const float f = exp2_bounded(m_run[nt] + vsn - w_run[nt] + kPLog2);
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -1112,7 +1116,9 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
       float c[2], mx = -INFINITY, top[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        c[half] = not_zero(ks[half] * q_scale);
+        const bool hidden = tail && k0 + KS * half + 16 * G > lim;
+        c[half] = hidden ? 1.0f : not_zero(ks[half] * q_scale);
+        vs[half] = hidden ? 0.0f : vs[half];
         float x = st[half][0][0];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -1139,7 +1145,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         block[half] = fminf(fmaxf(floorf(top[half] - w_run), -100.0f), kRescaleLog2);
-        const float f = __builtin_amdgcn_exp2f(fminf(m_run + vs[half] - w_run + (kTop - block[half]), 120.0f));
+        const float f = exp2_bounded(m_run + vs[half] - w_run + (kTop - block[half]));
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float pv[4];

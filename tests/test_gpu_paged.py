@@ -500,6 +500,22 @@ def test_tail_verify_paged_nan_scale(ops, T, which):
     assert torch.equal(got[0, :, :6], clean[0, :, :6]) and torch.equal(got[1], clean[1])
 
 
+@pytest.mark.parametrize("which", [2, 3])
+@pytest.mark.parametrize("T,grp,bs", [(8, 2, 16), (8, 4, 16), (8, 6, 16), (40, 6, 16), (40, 6, 64), (100, 2, 32)])
+def test_tail_verify_paged_nan_scale_behind_the_first_rows(ops, which, T, grp, bs):
+    """A page without a valid scale that only a request's later tokens reach: NaN from its first position
+    on, and the tokens before it as they were, in every tile width."""
+    kv = 2 * bs - 4
+    d = _attend_inputs(2, T, 2, grp, bs, [kv, 40], [T, T], seed=23)
+    clean = _attend(ops, d)
+    d["cache"][which][d["table"][0, 2], 1] = float("nan")  # positions from 2 bs on: the tokens from 4 on
+    got = _attend(ops, d)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[0, 4:, grp:] = True
+    assert torch.isnan(got[hit]).all()
+    assert torch.equal(got[~hit], clean[~hit])
+
+
 def test_tail_verify_paged_equals_dense_op_in_values(ops):
     """The same positions through gqa::tail_verify's dense bf16 cache of the dequantised rows."""
     B, T, H, grp, bs = 2, 8, 4, 6, 32
