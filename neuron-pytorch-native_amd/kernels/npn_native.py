@@ -9,6 +9,8 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 PKG_DIR = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(PKG_DIR, "libnpn_spec_verify.so")
@@ -74,6 +76,8 @@ SIGNATURES = {
 }
 
 _lib = None
+_libraries = []  # registrations last as long as these
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, int))  # of tensors, a kernel sees all there is
 
 
 def lib():
@@ -117,39 +121,87 @@ def call(name, *args):
         raise RuntimeError(f"{name} failed with status {status}: {text}")
 
 
+def _refuse_gradients(name, tensors):
+    """Raise if a backward pass (t requires grad while gradients are on) or a forward one (t has a
+    tangent) is expected through an op that has none."""
+    if torch.is_grad_enabled():
+        for arg, t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{arg} requires grad, but {name} has no backward pass: call it under "
+                                   "torch.no_grad() or with detached inputs")
+    if forward_ad._current_level >= 0:
+        for arg, t in tensors:
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{arg} has a tangent, but {name} has no forward-mode derivative")
+
+
 def register(qualname, schema, fake):
     """Decorator: registers the function as torch.ops.<qualname> for HIP tensors with `schema` and
     the shape propagation `fake`. Like torch.library.custom_op, minus its autograd wrapper, which
-    costs 8 us a call: more than these ops' kernels take at their smallest sizes."""
+    costs 8 us a call: more than these ops' kernels take at their smallest sizes. In the wrapper's
+    place a kernel above the op's own refuses inputs that a gradient is expected of, in eager, compiled
+    and torch.func code alike, and calls the function at once where nothing else (a mode, a
+    transform, a tensor subclass) has a part in the call; tensors that the op writes count as written."""
+    namespace, name = qualname.split("::")
+
     def wrap(fn):
         torch.library.define(qualname, schema)
-        torch.library.impl(qualname, "cuda", fn)
         torch.library.register_fake(qualname, fake)
+        op = getattr(getattr(torch.ops, namespace), name).default
+        specs = op._schema.arguments
+        names = [(i, a.name) for i, a in enumerate(specs) if str(a.type) == "Tensor"]
+        first = names[0][0]
+        written = [i for i, a in enumerate(specs) if a.alias_info is not None and a.alias_info.is_write]
+
+        def count_as_written(args):
+            tensors = [args[i] for i in written]
+            try:
+                increment_version(tensors)
+            except RuntimeError:  # inference tensors among them, which have no version
+                increment_version([t for t in tensors if not t.is_inference()])
+
+        def below_autograd(keyset, *args):
+            count_as_written(args)
+            return op.redispatch(keyset & torch._C._after_ADInplaceOrView_keyset, *args)
+
+        def autograd(*args):
+            if torch._C._any_requires_grad(*args) or forward_ad._current_level >= 0:
+                _refuse_gradients(qualname, [(arg, args[i]) for i, arg in names])
+            plain = (args[first].is_cuda and _PLAIN.issuperset(map(type, args))
+                     and torch._C._len_torch_dispatch_stack() == 0
+                     and torch._C._functorch.peek_interpreter_stack() is None)
+            if plain:
+                if written:
+                    count_as_written(args)
+                return fn(*args)
+            with torch._C._AutoDispatchBelowAutograd():
+                return op(*args)
+
+        torch.library.impl(qualname, "cuda", fn)
+        library = torch.library.Library(namespace, "FRAGMENT")
+        library.impl(name, autograd, "Autograd")
+        if written:
+            library.impl(name, below_autograd, "ADInplaceOrView", with_keyset=True)
+        _libraries.append(library)
         return fn
     return wrap
 
 
 def check_all(dev, *specs):
     """specs: (tensor, name, dtype, shape, or a number of elements in any shape). `require` for all
-    of them, that they are on `dev`, and that no gradient is expected: `register` leaves out the
-    wrapper that would refuse a backward pass through the op."""
+    of them, and that they are on `dev`."""
+    index = dev.index
     for t, name, dtype, shape in specs:
-        if isinstance(shape, int):
-            ok = t.numel() == shape
-        else:
-            ok = t.shape == shape
-        if not (ok and t.dtype == dtype and t.device == dev and t.is_contiguous()):
+        if not ((t.numel() if type(shape) is int else t.shape) == shape and t.dtype is dtype
+                and t.get_device() == index and t.is_contiguous()):
             require(t, name, dtype, **({"numel": shape} if isinstance(shape, int) else {"shape": shape}))
             raise RuntimeError(f"{name} must be on {dev}, got {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{name} requires grad, but the op has no backward pass: "
-                               "call it under torch.no_grad()")
 
 
 def launch(dev, name, *args):
     """`call` of an entry point that ends with a stream, on dev's current stream and with dev as the
     current device; the tensors' devices have been checked."""
-    raw = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    raw = [a if type(a) is int else a.data_ptr() for a in args]
     fn = getattr(lib(), name)
     if dev.index == torch.cuda.current_device():
         status = fn(*raw, torch._C._cuda_getCurrentRawStream(dev.index))

@@ -571,6 +571,34 @@ def test_refuses_gradients(ops):
         ops.spec.sample(torch.zeros(2, 9).cuda().requires_grad_(), r, r.int(), r, r, r)
 
 
+def test_refuses_gradients_under_transforms(ops):
+    """The same through torch.func, forward mode and compiled code; without a gradient of theirs these run."""
+    import torch._dynamo
+    torch._dynamo.reset()
+    d = _attend_inputs(1, 2, 1, 6, 16, [20], [2], seed=22)
+    q = d["query"].cuda()
+    args = (d["gate"].cuda(), d["q_norm"].cuda(), cuda(d["cos"]), cuda(d["sin"]), *_cuda_cache(d["cache"]),
+            cuda(d["table"]), cuda(d["kv"]), cuda(d["n"]))
+    fn = lambda x: ops.gqa.tail_verify_paged(x, *args)  # noqa: E731
+    want, compiled = fn(q), torch.compile(fn, fullgraph=True, backend="aot_eager")
+    with pytest.raises(RuntimeError, match="requires grad"):
+        torch.func.grad(lambda x: fn(x).float().sum())(q)
+    with pytest.raises(RuntimeError, match="tangent"):
+        torch.func.jvp(fn, (q,), (q,))
+    with pytest.raises(Exception, match="requires grad"):
+        compiled(q.clone().requires_grad_())
+    assert torch.equal(compiled(q), want)
+    w = torch.ones((), device="cuda")
+    assert torch.equal(torch.func.grad(lambda x: (x * fn(q)).sum())(w), want.sum())
+    with torch.inference_mode():
+        assert torch.equal(fn(q), want) and torch.equal(fn(q.clone()), want)
+    # an append counts as a write of the cache
+    old = args[6]._version
+    key = torch.randn(1, 2, 1, 256, device="cuda").to(BF)
+    ops.gqa.kv_append_paged(key, key, *args[1:4], args[9], torch.full((1, 2), -1, device="cuda"), *args[4:8])
+    assert args[6]._version > old
+
+
 @pytest.mark.parametrize("T", [1, 8, 40])
 def test_pages_past_32_bit_offsets(ops, T):
     """A pool of 5 GB for K and for V, of which the request holds the last blocks: the appended bytes and
