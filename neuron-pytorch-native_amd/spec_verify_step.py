@@ -116,9 +116,10 @@ class VerifySlice:
     def __init__(self, B, K, kv_lens, s_max, pattern="DDDG", seed=0, device="cuda",
                  fuse_splitk=True, fuse_swiglu=True, fuse_launches=True, paged_block=None):
         """paged_block: None for dense bf16 KV caches, or the block size of a paged e4m3 cache
-        with one block table for all GQA layers, planned on the device at every step."""
+        with one block table for all GQA layers, planned on the device at every step. A step with
+        pages raises where a sequence has fewer than K + 1 rows left of its s_max."""
         self.B, self.K, self.T = B, K, K + 1
-        self.paged_block = paged_block
+        self.paged_block, self.s_max = paged_block, s_max
         self.fuse_splitk = fuse_splitk
         self.fuse_swiglu = fuse_swiglu
         self.fuse_launches = fuse_launches
@@ -172,6 +173,7 @@ class VerifySlice:
                           "free": torch.randperm(B * P, generator=g, device=device).int(),
                           "count": torch.full((1,), B * P, **i32)}
             self.new_len = torch.full((B,), self.T, **i32)
+            self.longest = int(self.kv_len.max())  # no sequence is longer
             self._plan_pages(torch.zeros(B, **i32))  # the blocks of the rows that are there
         # RoPE table of every cache position, built once (the reference's _init_rope); each
         # step gathers the rows of its T positions.
@@ -187,6 +189,19 @@ class VerifySlice:
         p = self.pages
         return torch.ops.paged.update_blocks_(self.kv_len, new_len, p["table"], p["held"], p["free"],
                                               p["count"], self.paged_block, self.T)
+
+    def _take_rows(self):
+        """Before a step with pages: every sequence has room for its T rows. The step cannot go on
+        without: a sequence that is refused its blocks would be committed all the same. The host
+        counts T rows a step for all and looks at the lengths (a wait) only where that is too many."""
+        if self.paged_block is None or "G" not in self.pattern or torch.cuda.is_current_stream_capturing():
+            return
+        if self.longest + self.T > self.s_max:
+            self.longest = int(self.kv_len.max())
+            if self.longest + self.T > self.s_max:
+                raise RuntimeError(f"a sequence of {self.longest} rows has no room for {self.T} more: "
+                                   f"s_max is {self.s_max}")
+        self.longest += self.T
 
     # ---- layers: each takes the normed input and returns the residual delta -------------
     def _deltanet(self, L, h):
@@ -287,6 +302,7 @@ class VerifySlice:
         if self.paged_block is not None and "G" in self.pattern:
             if cos is not None:
                 raise ValueError("the paged cache takes its RoPE rows from the tables")
+            self._take_rows()
             self.plan = self.timer("paged.update_blocks", self._plan_pages, self.new_len)
         elif cos is None and not self.fuse_launches and "G" in self.pattern:
             cos, sin = self.timer("gqa.rope_rows", torch.ops.gqa.rope_rows, self.rope_cos,
@@ -390,6 +406,7 @@ class VerifySlice:
         i = self.next_graph
         if (self.graph_parity0 + i) % 2 != self.parity:
             raise RuntimeError("graph replay out of step with the checkpoint-buffer parity")
+        self._take_rows()
         self.graphs[i].replay()
         self.parity ^= 1
         self.next_graph = (i + 1) % len(self.graphs)

@@ -210,6 +210,34 @@ def test_verify_slice_with_a_paged_cache(bs):
     assert torch.equal(eager.kv_len, graph.kv_len)
 
 
+@pytest.mark.parametrize("replayed", [False, True])
+@pytest.mark.parametrize("s_max", [64, 72])
+def test_verify_slice_stops_where_its_pages_end(s_max, replayed):
+    """A step whose rows would pass s_max is refused before it runs, eager or replayed: every step that
+    runs has all its rows granted, and the refused one changes nothing."""
+    from spec_verify_step import HIDDEN, VerifySlice, synthetic_logits
+    B, K, V = 2, 3, 500
+    m = VerifySlice(B, K, [s_max - 12, 5], s_max, pattern="DG", seed=1, paged_block=16)
+    x = torch.randn(B * (K + 1), HIDDEN, device="cuda").to(BF)
+    sets = [synthetic_logits(B, K, V, 30 + i, "cuda") for i in range(2)]
+    m.step(x, *sets[0])
+    if replayed:
+        m.capture(x, sets)
+    for n in range(20):
+        before = [m.kv_len.clone()] + [m.pages[k].clone() for k in ("table", "held", "free", "count")]
+        full = int(m.kv_len.max()) + K + 1 > s_max
+        if full:
+            with pytest.raises(RuntimeError, match="s_max"):
+                m.replay() if replayed else m.step(x, *sets[n % 2])
+            torch.cuda.synchronize()
+            after = [m.kv_len] + [m.pages[k] for k in ("table", "held", "free", "count")]
+            assert all(torch.equal(a, b) for a, b in zip(before, after))
+            break
+        m.replay() if replayed else m.step(x, *sets[n % 2])
+        assert torch.equal(m.pages["held"], (before[0] + K + 1 + 15) // 16)  # granted, which is to have its blocks
+    assert full
+
+
 def test_chunk_and_sampling_replayed_beside_each_other(ops):
     """A prompt chunk's attention captured in one graph and sampling in another, replayed on two streams
     at once with lengths, pages and settings that change in place, against eager calls."""
