@@ -255,13 +255,15 @@ int npn_paged_update_blocks(const int32_t* kv_len, const int32_t* new_len, int32
  * partial RoPE with the table rows kv_len[b] + t, clamped to [0, positions)), into e4m3 pages:
  *   key, value [B, T, Hkv, 256] bf16; k_norm [256]; cos_table, sin_table [positions, 64];
  *   slots [B, T] int64 as npn_paged_update_blocks makes them: a request's rows in order, -1
- *   from its last one on. A row whose slot is out of [0, n_blocks * block_size) is skipped.
+ *   from its last one on. The first slot's place in its block says with which rows the next blocks
+ *   begin; of a block's rows those before the first whose slot is out of [0, n_blocks *
+ *   block_size), or does not follow the slot before it, are appended, and the others skipped.
  * Per (block, head) that gets rows: need = the least power of two with amax <= 448 need over
  * the finite new values; the scale becomes need if row 0 of the block is among the new ones,
  * else max(scale, need), and the block's older rows are moved to it (rounded to nearest even,
  * exact but for e4m3 subnormals). New rows are e4m3(x / scale), nearest even; NaN and
- * infinities are stored as NaN. Other rows keep their bytes. No two requests of a call may
- * append to one block. */
+ * infinities are stored as NaN. Other rows keep their bytes. A call may append to a block at
+ * one place only: neither two of its requests nor two entries of a request's table may name it. */
 int npn_gqa_kv_append_paged(const uint16_t* key, const uint16_t* value, const float* k_norm,
                             const float* cos_table, const float* sin_table, int positions,
                             const int32_t* kv_len, const int64_t* slots, int8_t* cache_k,

@@ -305,12 +305,12 @@ __global__ __launch_bounds__(NW * 64, 4) void paged_append_kernel(PagedAppendArg
   const int bs = 1 << a.sh;
   const int64_t* slots = a.slots + (size_t)b * a.T;
 
-  // The rows [t0, t1) of this block: the request's first slot says where its blocks end.
+  // The rows [t0, t1) of this block: the request's first slot says where its blocks end, also where
+  // its block is none (id -1: a slot of -bs + its row). A request without rows has -1 throughout.
   const int64_t first = slots[0];
-  if (first < 0) return;
   const int off0 = (int)(first & (bs - 1));
   const int t0 = blockIdx.x == 0 ? 0 : bs - off0 + ((int)blockIdx.x - 1) * bs;
-  if (t0 >= a.T) return;
+  if (t0 >= a.T || (first < 0 && slots[t0] < 0)) return;
   const int room = min(blockIdx.x == 0 ? bs - off0 : bs, a.T - t0);
   auto row_of = [&](int i) { return RPW < 4 ? w + NW * i : 4 * (w + NW * (i >> 2)) + (i & 3); };
 

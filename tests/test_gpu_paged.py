@@ -219,6 +219,28 @@ def test_kv_append_paged_non_finite_and_foreign_slots(ops):
     _same_cache(dev, cache)
 
 
+def test_kv_append_paged_rows_behind_a_block_that_is_none(ops):
+    """A request's first block is none in its table: its rows there go nowhere, those in the blocks behind
+    it are appended, as where a block's id is past the pool."""
+    rng = np.random.default_rng(8)
+    H, bs, N, T = 2, 16, 8, 40
+    for none in (-1, N):
+        for kv0 in (0, 5, 15):
+            cache = _empty_cache(N, H, bs, rng)
+            dev = _cuda_cache(cache)
+            table = np.array([[none, 3, 1, 6], [none, none, 2, none]], np.int32)
+            kv = np.array([kv0, kv0], np.int32)
+            pos = kv[:, None] + np.arange(T)
+            slots = np.take_along_axis(table, pos // bs, 1).astype(np.int64) * bs + pos % bs
+            key, value = torch.randn(2, T, H, 256).to(BF), torch.randn(2, T, H, 256).to(BF)
+            cos, sin = og.rope_cos_sin(np.arange(64))
+            z = torch.zeros(256)
+            _append(ops, key.cuda(), value.cuda(), z.cuda(), cuda(cos), cuda(sin), cuda(kv), cuda(slots), dev)
+            torch.cuda.synchronize()
+            op.kv_append(key.double().numpy(), value.double().numpy(), z.double().numpy(), cos, sin, kv, slots, cache)
+            _same_cache(dev, cache)
+
+
 # ---- attention -----------------------------------------------------------------------------------------------
 
 def _attend_inputs(B, T, H, grp, bs, kv, n, seed, spare_pages=2):
