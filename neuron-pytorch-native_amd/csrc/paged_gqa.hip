@@ -451,8 +451,9 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagedArgs a
   const int row = min((u - b * a.RG) * a.R + r, a.T * a.grp - 1);
   const int t = a.token_of(row), qh = h * a.grp + row - t * a.grp;
   const uint2 q = *reinterpret_cast<const uint2*>(a.query + (((size_t)b * a.T + t) * a.Hq + qh) * DH + 4 * lane);
-  const int kv = min(max(a.kv_len[b], 0), a.P << a.sh);
-  const size_t pos = (size_t)min(kv + t, a.positions - 1) * ROPE + 4 * (lane & 15);
+  // The row's own position, also where the table ends before it.
+  const int64_t at = min((int64_t)max(a.kv_len[b], 0) + t, (int64_t)a.positions - 1);
+  const size_t pos = (size_t)at * ROPE + 4 * (lane & 15);
   const float4 c = *reinterpret_cast<const float4*>(a.cos + pos);
   const float4 s = *reinterpret_cast<const float4*>(a.sin + pos);
   const float4 nw = *reinterpret_cast<const float4*>(a.q_norm + 4 * lane);

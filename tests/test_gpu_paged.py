@@ -538,6 +538,18 @@ def test_tail_verify_paged_nan_scale_behind_the_first_rows(ops, which, T, grp, b
     assert torch.equal(got[~hit], clean[~hit])
 
 
+@pytest.mark.parametrize("T", [1, 8, 40])
+def test_tail_verify_paged_rotates_by_the_length_past_the_table(ops, T):
+    """A length past what the table's row holds: all of the row's positions are seen, and the query's
+    RoPE rows are those of its own position (clamped to the RoPE tables alone)."""
+    d = _attend_inputs(2, T, 2, 6, 16, [70, 20], [T, T], seed=24)
+    d["cos"], d["sin"] = og.rope_cos_sin(np.arange(70 + T - 1))  # the last token's clamps
+    d["table"] = np.ascontiguousarray(d["table"][:, :3])  # 48 positions
+    d["cache"][0] &= 0xF7  # finite bytes throughout
+    d["cache"][1] &= 0xF7
+    _check(ops, d)
+
+
 def test_tail_verify_paged_equals_dense_op_in_values(ops):
     """The same positions through gqa::tail_verify's dense bf16 cache of the dequantised rows."""
     B, T, H, grp, bs = 2, 8, 4, 6, 32
