@@ -252,7 +252,8 @@ int npn_paged_update_blocks(const int32_t* kv_len, const int32_t* new_len, int32
                             int n_blocks, int block_size, int T, void* stream);
 
 /* torch.ops.gqa.kv_append_paged -- npn_gqa_kv_append's k-side math in fp32 (RMSNorm (1+w) and
- * partial RoPE with the table rows kv_len[b] + t, clamped to [0, positions)), into e4m3 pages:
+ * partial RoPE with the table rows kv_len[b] + t, at most positions - 1; negative kv_len counts
+ * as 0), into e4m3 pages:
  *   key, value [B, T, Hkv, 256] bf16; k_norm [256]; cos_table, sin_table [positions, 64];
  *   slots [B, T] int64 as npn_paged_update_blocks makes them: a request's rows in order, -1
  *   from its last one on. The first slot's place in its block says with which rows the next blocks

@@ -346,7 +346,7 @@ __global__ __launch_bounds__(NW * 64, 4) void paged_append_kernel(PagedAppendArg
   if (!is_v) {
     const float4 nw = *reinterpret_cast<const float4*>(a.k_norm + 4 * lane);
     const float wt[4] = {1.0f + nw.x, 1.0f + nw.y, 1.0f + nw.z, 1.0f + nw.w};
-    const int64_t pos0 = (int64_t)a.kv_len[b] + t0;
+    const int64_t pos0 = (int64_t)max(a.kv_len[b], 0) + t0;
     constexpr int BATCH = RPW < 4 ? RPW : 4;  // rows whose RoPE rows are loaded at a time, without branches
 #pragma unroll
     for (int i0 = 0; i0 < RPW; i0 += BATCH) {
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(NW * 64, 4) void paged_append_kernel(PagedAppendArg
 #pragma unroll
       for (int k = 0; k < BATCH; ++k) {
         int64_t pos = pos0 + min(row_of(i0 + k), most - 1);
-        pos = pos < 0 ? 0 : (pos >= a.positions ? a.positions - 1 : pos);
+        pos = pos >= a.positions ? a.positions - 1 : pos;
         c[k] = *reinterpret_cast<const float4*>(a.cos + pos * ROPE + 4 * (lane & 15));
         s[k] = *reinterpret_cast<const float4*>(a.sin + pos * ROPE + 4 * (lane & 15));
       }

@@ -75,7 +75,7 @@ def kv_append(key, value, k_norm, cos_table, sin_table, kv_len, slots, cache):
     N, H, bs, _ = cache_k.shape
     B, T = slots.shape
     for b in range(B):
-        pos = np.clip(int(kv_len[b]) + np.arange(T), 0, len(cos_table) - 1)
+        pos = np.minimum(max(int(kv_len[b]), 0) + np.arange(T), len(cos_table) - 1)
         k = norm_rope(key[b], k_norm, cos_table[pos][:, None].astype(np.float64),
                       sin_table[pos][:, None].astype(np.float64))
         rows = {}

@@ -241,6 +241,27 @@ def test_kv_append_paged_rows_behind_a_block_that_is_none(ops):
             _same_cache(dev, cache)
 
 
+def test_kv_append_paged_negative_length(ops):
+    """A negative length counts as 0 here too, so that the rows that update_blocks_ places from position
+    0 on are rotated by these positions."""
+    rng = np.random.default_rng(9)
+    H, bs, N, T = 1, 16, 3, 20
+    slots = np.arange(T, dtype=np.int64)[None]
+    key, value = torch.randn(1, T, H, 256).to(BF), torch.randn(1, T, H, 256).to(BF)
+    cos, sin = og.rope_cos_sin(np.arange(64))
+    z = torch.zeros(256)
+    cache = _empty_cache(N, H, bs, rng)
+    for kv in (-3, -2**31):
+        dev = _cuda_cache(cache)
+        kv = np.array([kv], np.int32)
+        _append(ops, key.cuda(), value.cuda(), z.cuda(), cuda(cos), cuda(sin), cuda(kv), cuda(slots), dev)
+        torch.cuda.synchronize()
+        ref = [a.copy() for a in cache]
+        op.kv_append(key.double().numpy(), value.double().numpy(), z.double().numpy(), cos, sin, np.zeros(1, np.int32),
+                     slots, ref)
+        _same_cache(dev, ref)
+
+
 # ---- attention -----------------------------------------------------------------------------------------------
 
 def _attend_inputs(B, T, H, grp, bs, kv, n, seed, spare_pages=2):
