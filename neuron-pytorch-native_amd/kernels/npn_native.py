@@ -75,6 +75,7 @@ SIGNATURES = {
     "npn_deltanet_full_fp8": (_I, [_P] * 19 + [_I] * 3 + [_P, _Z, _P]),
 }
 
+_INT_MAX = 2 ** 31 - 1
 _lib = None
 _libraries = []  # registrations last as long as these
 _PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, int))  # of tensors, a kernel sees all there is
@@ -214,7 +215,10 @@ def launch(dev, name, *args):
 
 
 def query(name, *args):
-    """Call a size-query entry point and return its value."""
+    """Call a size-query entry point and return its value; 0 (unsupported) for sizes past a C int,
+    which ctypes would take modulo 2^32."""
+    if max(args) > _INT_MAX:
+        return 0
     return int(getattr(lib(), name)(*args))
 
 

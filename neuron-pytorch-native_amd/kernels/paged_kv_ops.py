@@ -67,6 +67,8 @@ def update_blocks_(kv_len, new_len, block_table, num_blocks, free_blocks, free_c
         raise RuntimeError(f"T must be at least 1, got {T}")
     B, P = _dims(block_table, "block_table", 2)
     n = free_blocks.numel()
+    if max(B * T, B * P) > 2 ** 30 or n >= 2 ** 31:
+        raise RuntimeError(f"unsupported update_blocks_ sizes B={B} T={T} P={P} N={n}")
     dev = kv_len.device
     check_all(dev, (kv_len, "kv_len", I32, B), (new_len, "new_len", I32, B),
               (block_table, "block_table", I32, (B, P)), (num_blocks, "num_blocks", I32, B),

@@ -610,6 +610,18 @@ def test_refusals(ops):
         ops.paged.update_blocks_(i32(0, 1), *plan[1:], 16, 1)
 
 
+def test_update_blocks_refuses_sizes_past_the_limits(ops):
+    """T past 32 bits: refused before anything is allocated, not taken modulo 2^32."""
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    plan = [i32(0), i32(1), i32(-1, -1).reshape(1, 2), i32(0), i32(0, 1), i32(2)]
+    held = torch.cuda.memory_allocated()
+    for T in (2**32 + 8, 2**31, 2**30 + 1):
+        with pytest.raises(RuntimeError):
+            ops.paged.update_blocks_(*plan, 16, T)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() < held + 2**33 and int(plan[3]) == 0
+
+
 def test_refuses_gradients(ops):
     """No backward pass: inputs that require grad are refused unless gradients are off."""
     d = _attend_inputs(1, 2, 1, 6, 16, [20], [2], seed=22)

@@ -62,6 +62,16 @@ def test_size_queries():
     assert q("npn_deltanet_full_fp8_workspace_size", 5120, 5, 48) == 0         # Hv % Hk
 
 
+def test_size_queries_past_32_bits():
+    """Sizes that a C int does not hold are unsupported, not taken modulo 2^32."""
+    import npn_native
+    q = npn_native.query
+    for big in (2 ** 31, 2 ** 32 + 5, 2 ** 33 + 4096):
+        assert q("npn_sample_workspace_size", 1, big) == 0 and q("npn_sample_workspace_size", big, 5) == 0
+        assert q("npn_gqa_tail_verify_paged_workspace_size", 1, 1, 6, 1, big, 16) == 0
+    assert q("npn_sample_workspace_size", 1, 5) > 0
+
+
 def test_ops_register_and_propagate_shapes():
     import npn_ops  # noqa: F401
     from torch._subclasses.fake_tensor import FakeTensorMode
