@@ -109,9 +109,8 @@ __device__ __forceinline__ uint64_t row_sum_dpp(uint64_t v) {
 // scratch SGPR, sets the base, and restores m0 after the issue (the instruction reads m0
 // when it issues). GFX9 needs one wait state between an SALU write of m0 and an LDS DMA
 // that reads it, hence the s_nop.
-__device__ __forceinline__ void lds_dma16(const void* g, const void* lds_base) {
-  const unsigned base = __builtin_amdgcn_readfirstlane(
-      (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)lds_base);
+// lds is the wave-uniform LDS address; the forms below make it of what they are given.
+__device__ __forceinline__ void lds_dma16_uniform(const void* g, unsigned lds) {
   unsigned saved;
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
@@ -120,17 +119,13 @@ __device__ __forceinline__ void lds_dma16(const void* g, const void* lds_base) {
       "global_load_lds_dwordx4 %1, off\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)
-      : "v"(g), "s"(base)
+      : "v"(g), "s"(lds)
       : "memory");
 }
 
-// Same DMA with a wave-uniform global base (SGPR pair), a 32-bit per-lane byte offset (one
-// VGPR per lane live instead of a 64-bit address) and the LDS base as a wave-uniform LDS
-// address (no generic-to-LDS pointer conversion, whose null check costs four scalar
-// instructions per DMA).
-__device__ __forceinline__ void lds_dma16_soff(const void* sbase, unsigned voff,
-                                               unsigned lds_addr) {
-  const unsigned base = __builtin_amdgcn_readfirstlane(lds_addr);
+// Same DMA with a wave-uniform global base (SGPR pair) and a 32-bit per-lane byte offset (one
+// VGPR per lane live instead of a 64-bit address).
+__device__ __forceinline__ void lds_dma16_soff_uniform(const void* sbase, unsigned voff, unsigned lds) {
   unsigned saved;
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
@@ -139,7 +134,7 @@ __device__ __forceinline__ void lds_dma16_soff(const void* sbase, unsigned voff,
       "global_load_lds_dwordx4 %1, %2\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)
-      : "v"(voff), "s"(sbase), "s"(base)
+      : "v"(voff), "s"(sbase), "s"(lds)
       : "memory");
 }
 
@@ -148,19 +143,17 @@ __device__ __forceinline__ unsigned lds_addr(const void* p) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }
 
-__device__ __forceinline__ void lds_dma16_soff(const void* sbase, unsigned voff,
-                                               const void* lds_base) {
-  const unsigned base = __builtin_amdgcn_readfirstlane(lds_addr(lds_base));
-  unsigned saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %3\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, %2\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "v"(voff), "s"(sbase), "s"(base)
-      : "memory");
+__device__ __forceinline__ void lds_dma16(const void* g, const void* lds_base) {
+  lds_dma16_uniform(g, __builtin_amdgcn_readfirstlane(lds_addr(lds_base)));
+}
+
+// By LDS address (no generic-to-LDS pointer conversion, whose null check costs four scalar
+// instructions per DMA), and by pointer.
+__device__ __forceinline__ void lds_dma16_soff(const void* sbase, unsigned voff, unsigned lds_addr) {
+  lds_dma16_soff_uniform(sbase, voff, __builtin_amdgcn_readfirstlane(lds_addr));
+}
+__device__ __forceinline__ void lds_dma16_soff(const void* sbase, unsigned voff, const void* lds_base) {
+  lds_dma16_soff(sbase, voff, lds_addr(lds_base));
 }
 
 }  // namespace npn

@@ -194,34 +194,10 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return t * 0xFFu;
 }
 
-// 16 bytes per lane from g into LDS at lds + 16 * lane (global_load_lds_dwordx4, its LDS base in m0:
-// see npn::lds_dma16); lds is wave-uniform. The caller waits with vmcnt.
-__device__ __forceinline__ void dma16(const void* g, unsigned lds) {
-  unsigned saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %2\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, off\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "v"(g), "s"(lds)
-      : "memory");
-}
-
-// The same with a wave-uniform address and a per-lane byte offset.
-__device__ __forceinline__ void dma16_soff(const void* base, unsigned voff, unsigned lds) {
-  unsigned saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %3\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, %2\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "v"(voff), "s"(base), "s"(lds)
-      : "memory");
-}
+// 16 bytes per lane into LDS at a wave-uniform address, from a per-lane address or an offset. The
+// caller waits with vmcnt.
+using npn::lds_dma16_soff_uniform;
+using npn::lds_dma16_uniform;
 
 __device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b) {
   return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
@@ -564,7 +540,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
   } else {
 #pragma unroll
     for (int k = 0; k < 2 * NRT; ++k)
-      dma16(qsrc + 64 * (w * 2 * NRT + k),
+      lds_dma16_uniform(qsrc + 64 * (w * 2 * NRT + k),
             __builtin_amdgcn_readfirstlane(npn::lds_addr(&sm.q[0][0][0])) + (w * 2 * NRT + k) * 1024u);
   }
 
@@ -591,7 +567,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
     for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int j = 0; j < 2; ++j)
-        dma16_soff(pg[k] + (2 * n + j) * 4 * DH, src ^ (k << 6),
+        lds_dma16_soff_uniform(pg[k] + (2 * n + j) * 4 * DH, src ^ (k << 6),
                    ring_lds + (unsigned)(at * 8192 + (k * 2 + j) * 1024));
   };
   auto v_page = [&](int s) {  // the lane's place, dim i, in the page of its 16 keys of a step
@@ -602,7 +578,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
   auto load_v = [&](const uint8_t* pg, int n, int at) {  // dims 128 n .. + 127
 #pragma unroll
     for (int d = 0; d < 8; ++d)
-      dma16(pg + ((size_t)(8 * n + d) << (a.sh + 4)), ring_lds + (unsigned)(at * 8192 + d * 1024));
+      lds_dma16_uniform(pg + ((size_t)(8 * n + d) << (a.sh + 4)), ring_lds + (unsigned)(at * 8192 + d * 1024));
   };
   auto begin_chunk = [&](int c0) {
     cn = min(kChunk, steps - c0);
@@ -982,13 +958,13 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
       const int kid = __builtin_amdgcn_readfirstlane(max(sm.page[(kk >> a.sh) - page0], 0));
       const uint8_t* const kp =
           a.cache_k + ((((size_t)kid * a.Hkv + h) << a.sh) + (kk & (bs - 1))) * DH + (w & 1) * 4 * DH;
-      dma16_soff(kp, ksrc, at);
-      dma16_soff(kp + 8 * DH, ksrc, at + 8192);
+      lds_dma16_soff_uniform(kp, ksrc, at);
+      lds_dma16_soff_uniform(kp + 8 * DH, ksrc, at + 8192);
       const int vid = max(sm.page[(kv >> a.sh) - page0], 0);
       const uint8_t* const vp =
           a.cache_v + ((((size_t)vid * a.Hkv + h) * DH + 16 * w + i) << a.sh) + (kv & (bs - 1));
-      dma16(vp, at + 2 * 8192);
-      dma16(vp + ((size_t)128 << a.sh), at + 3 * 8192);
+      lds_dma16_uniform(vp, at + 2 * 8192);
+      lds_dma16_uniform(vp + ((size_t)128 << a.sh), at + 3 * 8192);
     }
   };
   // V bytes of keys that no row sees are cleared (0 times NaN is NaN), each wave those that it sent for. So
