@@ -51,7 +51,7 @@
 //     row, 2^-17 was the least step: a row's other weights were off by 6 % at 2^-20 of its largest and
 //     gone at 2^-22, which is all there is where the largest one's value is near 0. 1 us less.) 2 chunks of
 //     256 x 6 rows over up to 8192 keys: 130 us (157 with groups of 48 rows; 142 with 128 rows in f16),
-//     608 TFLOP/s by the formula's operations. Matrix units 51 %, vector units 55 % busy, which
+//     608 TFLOP/s by the formula's operations. Matrix units 48 %, vector units 54 % busy, which
 //     overlap little: without the softmax 100 us would remain, without V's products 100, without the DMAs
 //     123. Priorities for one wave of each SIMD, its V products half a step behind the other's, or LDS
 //     reads ahead of the products before them changed nothing.

@@ -227,7 +227,8 @@ __global__ __launch_bounds__(256) void paged_slots_kernel(PlanArgs a) {
 // One workgroup per (request, block touched, head, K or V): it owns the page, so the
 // scale and the older rows need no atomics. Lane l of a wave holds dims 4l..4l+3 of its rows in
 // registers from the first load to the rounding (RPW rows per wave), so each input is read once.
-// 32 requests of one to eight rows take 5 us (a launch and one chain of loads); 4 x 4096 rows of 4 heads
+// 32 requests of one to eight rows take 5 us (a launch and one chain of loads), whether their pages' scales
+// hold already or all grow, older rows moved with them; 4 x 4096 rows of 4 heads
 // in blocks of 64 (101 MB read and written) 30 us, 3.4 TB/s, bound by instructions to a row and by a
 // workgroup's rows all having to arrive before its scale is known: only then can it write. (Checks for
 // infinities at each conversion: 36 us. Four waves a workgroup of 16 rows each: 62, and 16 of 4 rows,

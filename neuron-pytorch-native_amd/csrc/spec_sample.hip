@@ -32,9 +32,9 @@
 //     (thousands of equal logits), or a longer top-k, is searched by the digits of its keys instead,
 //     which reads it some ten times.
 //
-// Measured on 256 rows of 248320 bf16 logits (127 MB), settings mixed: 25 + 43 + 38 + 12 us for the four
-// launches, where one reading takes 21 from HBM at 6.15 TB/s; on 32 rows of 151936 in float 7 + 11 + 12 +
-// 11 us, on one 4.4 + 5.4 + 7 + 4.4. The first pass runs at 5.1 TB/s. The others are bound by instructions:
+// Measured on 256 rows of 248320 bf16 logits (127 MB), settings mixed: 25 + 38 + 35 + 12 us for the four
+// launches, where one reading takes 21 from HBM at 6.15 TB/s; on 32 rows of 151936 in float 7 + 11 + 13 +
+// 11 us, on one 4.4 + 5.4 + 7 + 4.3. The first pass runs at 5.1 TB/s. The others are bound by instructions:
 // three loads in flight instead of one made them slower (all rows without top-k: histogram 66 -> 110 us),
 // while loads without the cleaning of NaN and -0, maxima by groups of 16 bytes, and one t for both weight
 // and bin made them 1.3 times faster. Weights are the longest, 66 us when no row has a top-k, next the
@@ -1022,7 +1022,7 @@ SamplePlan sample_plan(int R, int V) {
   R = R < kRows ? R : kRows;
   // Workgroups per row: two per CU in all (what their registers let run at once), chunks of 4096 tokens at
   // least, a load or two a thread; and of many long rows chunks of 32768 at most, since greedy rows are
-  // done at once: 256 rows of 248320 took 119 us so, 160 with 65536, 173 with 131072.
+  // done at once: 256 rows of 248320 take 107 us so, 146 with 65536, 171 with 131072.
   p.C = max(1, max(min(512 / R, (V + 4095) / 4096), V / 32768));
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   const size_t chunks = up((size_t)R * p.C * 4);
