@@ -281,6 +281,10 @@ size_t npn_gqa_tail_verify_paged_workspace_size(int B, int T, int q_heads, int k
  * kv_len[b] + t clamped to them. Table entries out of [0, n_blocks) hide their positions; a row
  * without any is 0. A row does not depend on the cache behind its last position, NaN included.
  * T = 1 is plain decode; T may be long (a prompt's chunk).
+ * Roundings beside fp32's and the output's to bf16: q' to 2^-11. A softmax weight times its value
+ * scale, with Hq/Hkv * T up to 48: to 2^-11 down to 2^-25 of the row's largest, below that to
+ * 2^-36 of it; with more: to 2^-13 down to 2^-13 of the largest of its block's (32 keys from a multiple
+ * of 32 on), below that to 2^-26 of it and to 2^-3 down to 2^-38 of it.
  * Limits: Hq/Hkv <= 48, Hq/Hkv * T <= 2^20, max_blocks * block_size <= 2^30, and with the
  * Hq/Hkv * T rows of a kv head in groups of 128 (one group up to 48), B * Hkv * groups <= 65535
  * and that times max_blocks * block_size / 64 < 2^30. */

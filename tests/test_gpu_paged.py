@@ -614,6 +614,7 @@ def test_update_blocks_refuses_sizes_past_the_limits(ops):
     """T past 32 bits: refused before anything is allocated, not taken modulo 2^32."""
     i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
     plan = [i32(0), i32(1), i32(-1, -1).reshape(1, 2), i32(0), i32(0, 1), i32(2)]
+    torch.cuda.reset_peak_memory_stats()  # of the tests before
     held = torch.cuda.memory_allocated()
     for T in (2**32 + 8, 2**31, 2**30 + 1):
         with pytest.raises(RuntimeError):

@@ -90,5 +90,8 @@ def test_in_place_arguments_count_as_written():
         version = kept._version
         fill_(kept, X)
         assert kept._version > version
-    with torch.inference_mode():  # tensors without a version
-        fill_(torch.ones(4), X)
+    with torch.inference_mode():
+        fill_(torch.ones(4), X)  # a tensor without a version
+        version = kept._version
+        fill_(kept, X)
+    assert kept._version > version
