@@ -581,6 +581,95 @@ int npn_deltanet_rollback_commit(const uint16_t* const* mixed_qkv, uint16_t* con
                                  int v_heads, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Trees of drafted tokens (new ops; the reference drafts no tokens,
+ * contrib/qwen3.6-27b/static_decode.py:1313 is its one-token step).
+ *   parent [B, T] int32, 1 <= T <= 64: node t of request b hangs on node parent[b, t] where
+ *   that lies in [0, t), else on the committed tokens alone. Node 0 is the last committed
+ *   token. A node sees the committed tokens, its ancestors and itself, and lies at position
+ *   kv_len[b] + its number of ancestors. What a node gets depends on nothing of other nodes,
+ *   NaN included. A chain (parent[t] = t - 1) is what the verify calls above take.
+ * A step: npn_paged_update_blocks for T rows; per layer npn_deltanet_verify_tree or
+ * npn_gqa_tree_verify_paged; the target's token of every node (npn_sample: lossless, or
+ * npn_argmax_parts); npn_accept_tree; npn_deltanet_commit_tree, npn_gqa_compact_paged and
+ * npn_spec_commit.
+ *   path [B, T] int32: the accepted nodes in order, -1 behind. Its entries count from the
+ *   first on as long as they are nodes of [0, T) in ascending order.
+ * ------------------------------------------------------------------------- */
+
+/* Workspace bytes for npn_gqa_tree_verify_paged with these sizes (0: unsupported sizes). */
+size_t npn_gqa_tree_verify_paged_workspace_size(int B, int T, int q_heads, int kv_heads,
+                                                int max_blocks, int block_size);
+
+/* torch.ops.gqa.tree_verify_paged -- npn_gqa_kv_append_paged of the nodes' rows (key, value
+ * [B, T, Hkv, 256] bf16 to slots [B, T]) with the positions of the tree, and
+ * npn_gqa_tail_verify_paged's attention over the pages, node t < q_len[b] seeing the keys
+ * [0, kv_len[b]) and of those behind its ancestors and itself (node s's row is the one at
+ * kv_len[b] + s of the block table). Rows t >= q_len[b] are 0. Other arguments, roundings and
+ * limits as in those two; T <= 64. With a chain equal to them bit for bit. */
+int npn_gqa_tree_verify_paged(const uint16_t* query, const uint16_t* gate, const uint16_t* key,
+                              const uint16_t* value, const float* q_norm, const float* k_norm,
+                              const float* cos_table, const float* sin_table, int positions,
+                              int8_t* cache_k, int8_t* cache_v, float* k_scale, float* v_scale,
+                              const int32_t* block_table, const int32_t* kv_len,
+                              const int64_t* slots, const int32_t* q_len, const int32_t* parent,
+                              uint16_t* out, int B, int T, int q_heads, int kv_heads,
+                              int n_blocks, int max_blocks, int block_size, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/* torch.ops.deltanet.verify_tree -- npn_deltanet_verify's token step of every node from the state and
+ * conv window behind its parent, without forming a state per node (64 KB each for every head).
+ *   state [B, Hv, 128, 128] f32 and conv_state [B, QKV, 3] bf16: the committed ones;
+ *   the other inputs as npn_deltanet_verify's, T <= 64; B * Hv <= 2^22.
+ * Outputs: out [B, T, Hv, 128] bf16; records, B * T * ((Hk + Hv) * 128 + Hv) f32, what
+ * npn_deltanet_commit_tree needs of every node: k [B, T, Hk, 128] (normalised), u [B, T, Hv, 128]
+ * and decay [B, T, Hv], S_t = decay_t S_parent + k_t u_t^T. */
+int npn_deltanet_verify_tree(const float* state, const int32_t* parent,
+                             const uint16_t* mixed_qkv, const uint16_t* conv_state,
+                             const float* conv_weight, const float* conv_bias,
+                             const float* a_out, const float* b_out, const uint16_t* z,
+                             const float* A_log, const float* dt_bias,
+                             const float* norm_weight, uint16_t* out, float* records, int B,
+                             int T, int k_heads, int v_heads, void* stream);
+
+/* torch.ops.spec.accept_tree -- the walk: from node 0 to the first child (lowest index) whose
+ * draft token is the target's token of the node, until there is none.
+ *   target_ids, draft_ids [B, T] int64 (draft_ids[b, 0] is not read as a draft; negative ids
+ *   match nothing), q_len [B] int32: nodes from q_len[b] on are none.
+ * Outputs: accepted [B] int32 = drafts accepted, -1 where q_len[b] < 1; path [B, T] int32;
+ * out_ids [B, T] int64: the accepted drafts, the target's token of the last node, then -1. */
+int npn_accept_tree(const int64_t* target_ids, const int64_t* draft_ids, const int32_t* parent,
+                    const int32_t* q_len, int32_t* accepted, int32_t* path, int64_t* out_ids,
+                    int B, int T, void* stream);
+
+/* torch.ops.deltanet.commit_tree_ -- every DeltaNet layer's state and conv window moved along the
+ * path, in place and in one launch for up to 64 layers; requests with an empty path keep theirs.
+ *   state, conv_state, mixed_qkv, records: host arrays of `layers` device pointers, layer l's
+ *   [B, Hv, 128, 128] f32 state and [B, QKV, 3] bf16 window (both updated), the [B, T, QKV]
+ *   bf16 inputs and records of its npn_deltanet_verify_tree. The layers' states and windows must
+ *   not overlap (NPN_ERR_VALUE where two are the same). */
+int npn_deltanet_commit_tree(float* const* state, uint16_t* const* conv_state,
+                             const uint16_t* const* mixed_qkv, const float* const* records,
+                             int layers, const int32_t* path, int B, int T, int k_heads,
+                             int v_heads, void* stream);
+
+/* torch.ops.gqa.compact_paged_ -- the accepted path's rows of every attention layer's cache to the
+ * front of the tree's: row path[b, d]'s, at slots[b, path[b, d]], to slots[b, d], where the row behind
+ * the last committed one is slots[b, 0]. One launch for up to 32 layers.
+ *   cache_k, cache_v, k_scale, v_scale: host arrays of `layers` device pointers;
+ *   slots [B, T] int64 as npn_paged_update_blocks made them (a path ends where one of its two slots
+ *   is out of [0, n_blocks * block_size)); a block may belong to one request only.
+ * A row that comes from a block of another scale is rounded to its new block's, nearest even, which
+ * first grows to the least power of two s with amax <= 448 s over the finite values of the rows
+ * that move there, if that is more; the block's rows up to the path's last one are moved to it.
+ * Rows that stay in a block whose scale stays, or come from one of the same scale, keep their
+ * bytes; so do the rows behind the path. The layers' caches must not overlap (NPN_ERR_VALUE
+ * where two are the same). */
+int npn_gqa_compact_paged(const int32_t* path, const int64_t* slots, int8_t* const* cache_k,
+                          int8_t* const* cache_v, float* const* k_scale, float* const* v_scale,
+                          int layers, int B, int T, int kv_heads, int n_blocks, int block_size,
+                          void* stream);
+
+/* ---------------------------------------------------------------------------
  * Sampling.
  * ------------------------------------------------------------------------- */
 

@@ -58,6 +58,8 @@
 //  3. merge: the log-sum-exp merge of the other pairs' workgroups, times sigmoid(gate), to bf16.
 // prep takes 4 to 9 us and merge 5 to 10 for these.
 #include "npn_common.h"
+#include "paged_append.h"
+#include "tree.h"
 
 namespace {
 
@@ -99,6 +101,7 @@ struct PagedArgs {
   float* q_scale;          // [pairs][R]
   float* part_o;           // [slots][R][256] O of the workgroups of split pairs
   float* part_ml;          // [slots][R][2]
+  uint64_t* anc;           // trees: [B][T] each node and its ancestors as bits
   int32_t* wstart;         // [U + 1] first workgroup of each unit
   int32_t* sstart;         // [U] first slot of each unit
   int positions, B, T, Hq, Hkv, grp, R, RG, P, N, sh, nw, ks;  // ks: keys of a step
@@ -413,12 +416,9 @@ __device__ void plan_block(const PagedArgs& a) {
 // q' of one padded row per wave (rows that are none repeat the pair's last), over the least power of
 // two above the row's largest element. In f16 dim d = 64 c + 16 g + 8 h + e is element e of lane group
 // g in k step 2 c + h; in e4m3 parts d = 128 m + 64 x + 16 g + e is byte 16 x + e of group g in step m.
-__global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagedArgs a) {
-  if (blockIdx.x == 0) {
-    plan_block(a);
-    return;
-  }
-  const int64_t wave = (int64_t)(blockIdx.x - 1) * kPrepWaves + (threadIdx.x >> 6);
+// TREE: the row's position is its node's depth behind the committed ones.
+template <bool TREE>
+__device__ __forceinline__ void prep_row(const PagedArgs& a, const int32_t* parent, int64_t wave) {
   const int lane = threadIdx.x & 63;
   const int pair = (int)(wave / a.R), r = (int)(wave - (int64_t)pair * a.R);
   if (pair >= a.units() * a.Hkv) return;
@@ -427,8 +427,15 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagedArgs a
   const int row = min((u - b * a.RG) * a.R + r, a.T * a.grp - 1);
   const int t = a.token_of(row), qh = h * a.grp + row - t * a.grp;
   const uint2 q = *reinterpret_cast<const uint2*>(a.query + (((size_t)b * a.T + t) * a.Hq + qh) * DH + 4 * lane);
+  int behind = t;
+  if constexpr (TREE) {
+    const uint64_t anc =
+        npn::tree_ancestors(npn::tree_parent(parent + (size_t)b * a.T, a.T, lane), a.T, lane);
+    behind = __popcll(npn::tree_bits(anc, __builtin_amdgcn_readfirstlane(t))) - 1;
+    if (qh == 0 && lane == t) a.anc[(size_t)b * a.T + t] = anc;  // (rows that repeat the last write the same)
+  }
   // The row's own position, also where the table ends before it.
-  const int64_t at = min((int64_t)max(a.kv_len[b], 0) + t, (int64_t)a.positions - 1);
+  const int64_t at = min((int64_t)max(a.kv_len[b], 0) + behind, (int64_t)a.positions - 1);
   const size_t pos = (size_t)at * ROPE + 4 * (lane & 15);
   const float4 c = *reinterpret_cast<const float4*>(a.cos + pos);
   const float4 s = *reinterpret_cast<const float4*>(a.sin + pos);
@@ -479,8 +486,48 @@ __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagedArgs a
   *reinterpret_cast<uint2*>(reinterpret_cast<uint32_t*>(dst) + ((d & 4) >> 1)) = make_uint2(two[0], two[1]);
 }
 
+__global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagedArgs a) {
+  if (blockIdx.x == 0) plan_block(a);
+  else prep_row<false>(a, nullptr, (int64_t)(blockIdx.x - 1) * kPrepWaves + (threadIdx.x >> 6));
+}
+
+// The same for a tree, and in the workgroups behind the append of its nodes' rows, which the attention's
+// launch reads: none of the three parts reads what another writes.
+template <int RPW>
+__global__ __launch_bounds__(kPrepWaves * 64) void tree_prep_kernel(PagedArgs a, append::PagedAppendArgs ap,
+                                                                    const int32_t* parent, int rows, int per) {
+  const int x = (int)blockIdx.x - 1 - rows;
+  if (blockIdx.x == 0) {
+    plan_block(a);
+  } else if (x < 0) {
+    prep_row<true>(a, parent, (int64_t)(blockIdx.x - 1) * kPrepWaves + (threadIdx.x >> 6));
+  } else {
+    const int bh = x / per, b = bh / (2 * ap.Hkv), hv = bh - b * 2 * ap.Hkv, lane = threadIdx.x & 63;
+    const uint64_t anc =
+        npn::tree_ancestors(npn::tree_parent(parent + (size_t)b * ap.T, ap.T, lane), ap.T, lane);
+    const int64_t kv = max(ap.kv_len[b], 0);
+    append::append_block<RPW, kPrepWaves>(ap, x - bh * per, b, hv >> 1, hv & 1, [&](int t) {
+      return kv + __popcll(npn::tree_bits(anc, __builtin_amdgcn_readfirstlane(t))) - 1;
+    });
+  }
+}
+
 // ---- 2. attn ----------------------------------------------------------------------------------------
-template <int NRT, int NW>
+// Trees: which of a lane's 16 keys a row sees, as bits: of those up to its last one, `left` from the lane's first
+// on, the committed ones and the nodes `anc`. The first is `at` places behind the committed ones.
+__device__ __forceinline__ uint32_t seen16(uint64_t anc, int at, int left) {
+  const uint32_t upto = left >= 16 ? 0xFFFFu : (left <= 0 ? 0u : (1u << left) - 1);
+  const uint32_t nodes = at >= 64 ? 0u : at >= 0 ? (uint32_t)(anc >> at)
+                         : at <= -16 ? ~0u : ((uint32_t)anc << -at) | ((1u << -at) - 1);
+  return nodes & upto;
+}
+// x where bit k of `bits` is set, else -inf.
+__device__ __forceinline__ float if_seen(uint32_t bits, int k, float x) {
+  const int keep = (int)(bits << (31 - k)) >> 31;
+  return __uint_as_float((__float_as_uint(x) & keep) | (0xFF800000u & ~keep));
+}
+
+template <int NRT, int NW, bool TREE>
 struct PagedSmem {
   static constexpr int DR = NRT == 3 ? 8 : 16;  // 16-dim tiles of O that all waves have in LDS at once
   union {
@@ -491,14 +538,15 @@ struct PagedSmem {
   float m[NW][NRT * 16], l[NW][NRT * 16], inv[NRT * 16];
   int page[kPages];                             // -1: none
   float ks[kPages], vs[kPages];                 // the keys' scales, the logarithms of the values'
+  uint64_t anc[TREE ? NRT * 16 : 1];            // what a row sees of the nodes
 };
 
-template <int NRT, int NW>
+template <int NRT, int NW, bool TREE>
 __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a) {
   constexpr int R = NRT * 16;
   constexpr int NR = 16 / NW;  // groups in a wave's ring
   constexpr int kThreads = NW * 64;
-  using Smem = PagedSmem<NRT, NW>;
+  using Smem = PagedSmem<NRT, NW, TREE>;
   __shared__ __attribute__((aligned(1024))) Smem sm;
   const int tid = threadIdx.x;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -525,12 +573,14 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
   for (int nt = 0; nt < NRT; ++nt) {
     const int r = 16 * nt + i, t = a.token_of(row0 + r);
     lim[nt] = r < rows && t < a.q_len[un.b] ? min(un.kv + t, un.kend - 1) : -1;
+    if constexpr (TREE)
+      if (w == 0 && G == 0) sm.anc[r] = a.anc[(size_t)un.b * a.T + min(t, a.T - 1)];
     q_scale[nt] = a.q_scale[(size_t)pair * R + r];
     m_run[nt] = kNegBig;
     w_run[nt] = kNegBig;
     l_run[nt] = 0.f;
   }
-  const int lim0 = un.kv + un.t0;  // no row of the group sees less
+  const int lim0 = TREE ? un.kv - 1 : un.kv + un.t0;  // every row of the group sees the keys up to here
   const unsigned ring_lds = __builtin_amdgcn_readfirstlane(npn::lds_addr(&sm.ring[w][0][0]));
   const u32x4* qsrc = a.q + (size_t)pair * 8 * NRT * 64 + lane;
   u32x4 qreg[NW == 8 ? 8 : 1];
@@ -725,21 +775,29 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
 
       // A step with keys past the group's first limit, or past a page that is none, is masked.
       const bool tail = k0 + KS - 1 > lim0 || __builtin_amdgcn_ballot_w64(!held) != 0;
+      auto seen = [&](int nt) {
+        return seen16(sm.anc[TREE ? 16 * nt + i : 0], k0 + 16 * G - un.kv, lim[nt] + 1 - (k0 + 16 * G));
+      };
+      uint32_t see_bits[NRT];  // trees
       if (tail) {
         const int kb = k0 + 16 * G;
 #pragma unroll
-        for (int nt = 0; nt < NRT; ++nt)
+        for (int nt = 0; nt < NRT; ++nt) {
+          if constexpr (TREE) see_bits[nt] = seen(nt);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (!held || kb + 4 * j + r > lim[nt]) st[nt][j][r] = -INFINITY;
+            for (int r = 0; r < 4; ++r) {
+              if constexpr (TREE) st[nt][j][r] = if_seen(held ? see_bits[nt] : 0u, 4 * j + r, st[nt][j][r]);
+              else if (!held || kb + 4 * j + r > lim[nt]) st[nt][j][r] = -INFINITY;
+            }
+        }
       }
 
       f16x8 pw[NRT][2];
 #pragma unroll
       for (int nt = 0; nt < NRT; ++nt) {
-        const bool hidden = tail && k0 + 16 * G > lim[nt];  // all 16 keys of the lane
+        const bool hidden = tail && (TREE ? see_bits[nt] == 0 : k0 + 16 * G > lim[nt]);  // all 16 keys of the lane
         const float c = hidden ? 1.0f : not_zero(ks * q_scale[nt]), vsn = hidden ? 0.0f : vs;
         float mx = st[nt][0][0];
 #pragma unroll
@@ -802,7 +860,8 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
             for (int nt = 0; nt < NRT; ++nt)
 #pragma unroll
               for (int e = 0; e < 16; ++e)
-                see[nt][e >> 3][e & 7] = (__bf16)(k0 + 16 * G + e <= lim[nt] ? 0x1p100f : 0.0f);
+                see[nt][e >> 3][e & 7] =
+                    (__bf16)((TREE ? seen(nt) >> e & 1 : k0 + 16 * G + e <= lim[nt]) ? 0x1p100f : 0.0f);
 #pragma unroll
             for (int d = 0; d < 8; ++d) {
               u32x4 is;
@@ -895,6 +954,7 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
 }
 
 // ---- 2b. attn of many rows ----------------------------------------------------------------------------
+template <bool TREE>
 struct RowsSmem {
   union {
     uint8_t ring[2][65536];  // two steps of 128 keys: for each half two groups of K and two of V, as above
@@ -902,15 +962,18 @@ struct RowsSmem {
   };
   float inv[kRows];
   int lim[kRows];
-  int nan_key[DH];         // the first key past lim0 whose value at a dim is NaN
+  int nan_key[TREE ? 1 : DH];        // the first key past lim0 whose value at a dim is NaN
+  uint64_t anc[TREE ? kRows : 1];    // what a row sees of the nodes; 0: not even the committed keys
+  uint64_t nan_node[TREE ? DH : 1];  // the nodes whose value at a dim is NaN; all where a committed key's is
   int page[kPages];
   float ks[kPages], vs[kPages];
 };
 
+template <bool TREE>
 __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
   constexpr int R = kRows, KR = 128, kSteps = kChunk * KS / KR;
   constexpr int kTop = 7;  // a block's largest weight is taken to [2^kTop, 2^(kTop + 1))
-  __shared__ __attribute__((aligned(1024))) RowsSmem sm;
+  __shared__ __attribute__((aligned(1024))) RowsSmem<TREE> sm;
   const int tid = threadIdx.x;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int i = lane & 15, G = lane >> 4;
@@ -930,9 +993,10 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
 
   const int r = 16 * w + i, t = a.token_of(row0 + r);  // this lane's row and its last key, or -1
   int lim = r < rows && t < a.q_len[un.b] ? min(un.kv + t, un.kend - 1) : -1;
+  uint64_t anc = TREE ? a.anc[(size_t)un.b * a.T + min(t, a.T - 1)] : 0;
   float q_scale = a.q_scale[(size_t)pair * R + r];
   float m_run = kNegBig, w_run = kNegBig, l_run = 0.f;
-  const int lim0 = un.kv + un.t0;
+  const int lim0 = TREE ? un.kv - 1 : un.kv + un.t0;
   i32x8 q[2][3];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -984,7 +1048,18 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
           v[k] &= keep_bytes(live - 4 * k);
           const uint32_t nan = nan_bytes(v[k]);
           if (nan != 0) {
-            atomicMin(&sm.nan_key[16 * (w + 8 * n) + i], k1 + 4 * k + (__ffs(nan) - 1) / 8);
+            const int dim = 16 * (w + 8 * n) + i, key = k1 + 4 * k;
+            if constexpr (TREE) {
+              uint64_t nodes = 0;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int at = key + e - un.kv;  // below 64: behind kend they have been cleared
+                if ((nan >> (8 * e)) & 1) nodes |= at < 0 ? ~0ull : 1ull << at;
+              }
+              atomicOr(reinterpret_cast<unsigned long long*>(&sm.nan_node[dim]), (unsigned long long)nodes);
+            } else {
+              atomicMin(&sm.nan_key[dim], key + (__ffs(nan) - 1) / 8);
+            }
             v[k] &= ~nan;
           }
         }
@@ -1012,10 +1087,14 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
     }
     __syncthreads();
   };
-  if (tid < DH) sm.nan_key[tid] = 0x7FFFFFFF;
+  if (tid < DH) {
+    if constexpr (TREE) sm.nan_node[tid] = 0;
+    else sm.nan_key[tid] = 0x7FFFFFFF;
+  }
   begin_chunk(0);
   // What was loaded so far is waited for before the first DMAs.
   asm volatile("" : "+v"(lim), "+v"(q_scale));
+  if constexpr (TREE) asm volatile("" : "+v"(anc));
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -1078,14 +1157,20 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
           __builtin_amdgcn_sched_barrier(0);
         }
 
+      uint32_t see_bits[2];  // trees
       if (tail) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int half = 0; half < 2; ++half) {
+          const int kb = k0 + KS * half + 16 * G;
+          if constexpr (TREE) see_bits[half] = seen16(anc, kb - un.kv, lim + 1 - kb);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (!held[half] || k0 + KS * half + 16 * G + 4 * j + e > lim) st[half][j][e] = -INFINITY;
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (TREE) st[half][j][e] = if_seen(held[half] ? see_bits[half] : 0u, 4 * j + e, st[half][j][e]);
+              else if (!held[half] || kb + 4 * j + e > lim) st[half][j][e] = -INFINITY;
+            }
+        }
       }
 
       // Beside the row's maxima, `top` of each block of 32 keys that its products take as one: those of
@@ -1093,7 +1178,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
       float c[2], mx = -INFINITY, top[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const bool hidden = tail && k0 + KS * half + 16 * G > lim;
+        const bool hidden = tail && (TREE ? see_bits[half] == 0 : k0 + KS * half + 16 * G > lim);
         c[half] = hidden ? 1.0f : not_zero(ks[half] * q_scale);
         vs[half] = hidden ? 0.0f : vs[half];
         float x = st[half][0][0];
@@ -1175,6 +1260,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
   if (G == 0) {
     sm.inv[r] = l != 0.f ? 1.0f / l : 0.f;
     sm.lim[r] = lim;
+    if constexpr (TREE) sm.anc[r] = lim >= 0 ? anc : 0;
     if (parts > 1) {
       a.part_ml[(slot * R + r) * 2] = m_run;
       a.part_ml[(slot * R + r) * 2 + 1] = l;
@@ -1187,7 +1273,9 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
     x += x * 0.0f;  // infinite: NaN
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (sm.lim[rk] >= sm.nan_key[4 * lane + e]) x[e] = NAN;
+      if (TREE ? (sm.anc[TREE ? rk : 0] & sm.nan_node[TREE ? 4 * lane + e : 0]) != 0
+               : sm.lim[rk] >= sm.nan_key[TREE ? 0 : 4 * lane + e])
+        x[e] = NAN;
     if (parts > 1)
       *reinterpret_cast<f32x4*>(a.part_o + (slot * R + rk) * DH + 4 * lane) = x;
     else if (rk < rows)
@@ -1265,11 +1353,12 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedArgs a) {
 struct PagedPlan {
   bool ok;
   int grp, R, RG, pairs, grid, nw, ks;
-  size_t o_qs, o_po, o_ml, o_ws, o_ss, bytes;  // q first
+  size_t o_qs, o_po, o_ml, o_an, o_ws, o_ss, bytes;  // q first
 };
 
-PagedPlan paged_plan(int B, int T, int q_heads, int kv_heads, int max_blocks, int block_size) {
+PagedPlan paged_plan(int B, int T, int q_heads, int kv_heads, int max_blocks, int block_size, bool tree) {
   PagedPlan p{};
+  if (tree && T > npn::kMaxNodes) return p;
   if (B < 1 || T < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || max_blocks < 1) return p;
   if (block_size != 16 && block_size != 32 && block_size != 64 && block_size != 128) return p;
   p.grp = q_heads / kv_heads;
@@ -1293,18 +1382,56 @@ PagedPlan paged_plan(int B, int T, int q_heads, int kv_heads, int max_blocks, in
   p.o_qs = up((size_t)pairs * p.R * DH * (p.R == kRows ? 3 : 2));
   p.o_po = p.o_qs + up((size_t)pairs * p.R * sizeof(float));
   p.o_ml = p.o_po + up(slots * p.R * DH * sizeof(float));
-  p.o_ws = p.o_ml + up(slots * p.R * 2 * sizeof(float));
+  p.o_an = p.o_ml + up(slots * p.R * 2 * sizeof(float));
+  p.o_ws = p.o_an + (tree ? up((size_t)B * T * sizeof(uint64_t)) : 0);
   p.o_ss = p.o_ws + up((units + 1) * sizeof(int32_t));
   p.bytes = p.o_ss + up(units * sizeof(int32_t));
   p.ok = true;
   return p;
 }
 
+int block_shift(int block_size) { return block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7; }
+
+PagedArgs paged_args(const PagedPlan& p, const uint16_t* query, const uint16_t* gate, const float* q_norm,
+                     const float* cos_table, const float* sin_table, int positions, const int8_t* cache_k,
+                     const int8_t* cache_v, const float* k_scale, const float* v_scale,
+                     const int32_t* block_table, const int32_t* kv_len, const int32_t* q_len, uint16_t* out,
+                     int B, int T, int q_heads, int kv_heads, int n_blocks, int max_blocks, int block_size,
+                     void* workspace) {
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  return PagedArgs{query, gate, q_norm, cos_table, sin_table,
+                   reinterpret_cast<const uint8_t*>(cache_k),
+                   reinterpret_cast<const uint8_t*>(cache_v), k_scale, v_scale, block_table,
+                   kv_len, q_len, out, reinterpret_cast<u32x4*>(ws),
+                   reinterpret_cast<float*>(ws + p.o_qs), reinterpret_cast<float*>(ws + p.o_po),
+                   reinterpret_cast<float*>(ws + p.o_ml), reinterpret_cast<uint64_t*>(ws + p.o_an),
+                   reinterpret_cast<int32_t*>(ws + p.o_ws), reinterpret_cast<int32_t*>(ws + p.o_ss), positions,
+                   B, T, q_heads, kv_heads, p.grp, p.R, p.RG, max_blocks, n_blocks, block_shift(block_size),
+                   p.nw, p.ks, (1ull << 32) / p.grp + 1};
+}
+
+// The launches after the prep's.
+template <bool TREE>
+void launch_attn(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
+  if (p.R == 16)
+    hipLaunchKernelGGL((paged_attn_kernel<1, 8, TREE>), dim3(p.grid), dim3(512), 0, s, a);
+  else if (p.R == 32)
+    hipLaunchKernelGGL((paged_attn_kernel<2, 4, TREE>), dim3(p.grid), dim3(256), 0, s, a);
+  else if (p.R == 48)
+    hipLaunchKernelGGL((paged_attn_kernel<3, 4, TREE>), dim3(p.grid), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(paged_rows_kernel<TREE>, dim3(p.grid), dim3(512), 0, s, a);
+  if (p.pairs < 32 || p.pairs * p.R < 96 * 16)
+    hipLaunchKernelGGL(paged_merge_kernel<4>, dim3(p.R, p.pairs), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(paged_merge_kernel<1>, dim3(p.R / 4, p.pairs), dim3(256), 0, s, a);
+}
+
 }  // namespace
 
 extern "C" size_t npn_gqa_tail_verify_paged_workspace_size(int B, int T, int q_heads, int kv_heads,
                                                            int max_blocks, int block_size) {
-  return paged_plan(B, T, q_heads, kv_heads, max_blocks, block_size).bytes;
+  return paged_plan(B, T, q_heads, kv_heads, max_blocks, block_size, false).bytes;
 }
 
 extern "C" int npn_gqa_tail_verify_paged(
@@ -1315,36 +1442,63 @@ extern "C" int npn_gqa_tail_verify_paged(
     int max_blocks, int block_size, void* workspace, size_t workspace_bytes, void* stream) {
   NPN_REQUIRE(query && gate && q_norm && cos_table && sin_table && cache_k && cache_v && k_scale &&
                   v_scale && block_table && kv_len && q_len && out, NPN_ERR_NULL);
-  const PagedPlan p = paged_plan(B, T, q_heads, kv_heads, max_blocks, block_size);
+  const PagedPlan p = paged_plan(B, T, q_heads, kv_heads, max_blocks, block_size, false);
   NPN_REQUIRE(p.ok && n_blocks >= 1 && positions >= 1, NPN_ERR_SHAPE);
   NPN_REQUIRE(NPN_ALIGNED16(query) && NPN_ALIGNED16(gate) && NPN_ALIGNED16(q_norm) &&
                   NPN_ALIGNED16(cos_table) && NPN_ALIGNED16(sin_table) && NPN_ALIGNED16(cache_k) &&
                   NPN_ALIGNED16(cache_v) && NPN_ALIGNED16(out) && NPN_ALIGNED16(workspace),
               NPN_ERR_ALIGN);
   NPN_REQUIRE(workspace != nullptr && workspace_bytes >= p.bytes, NPN_ERR_WORKSPACE);
-  uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const int sh = block_size == 16 ? 4 : block_size == 32 ? 5 : block_size == 64 ? 6 : 7;
-  const PagedArgs a{query, gate, q_norm, cos_table, sin_table,
-                    reinterpret_cast<const uint8_t*>(cache_k),
-                    reinterpret_cast<const uint8_t*>(cache_v), k_scale, v_scale, block_table,
-                    kv_len, q_len, out, reinterpret_cast<u32x4*>(ws),
-                    reinterpret_cast<float*>(ws + p.o_qs), reinterpret_cast<float*>(ws + p.o_po),
-                    reinterpret_cast<float*>(ws + p.o_ml), reinterpret_cast<int32_t*>(ws + p.o_ws),
-                    reinterpret_cast<int32_t*>(ws + p.o_ss), positions, B, T, q_heads, kv_heads, p.grp,
-                    p.R, p.RG, max_blocks, n_blocks, sh, p.nw, p.ks, (1ull << 32) / p.grp + 1};
+  const PagedArgs a = paged_args(p, query, gate, q_norm, cos_table, sin_table, positions, cache_k, cache_v,
+                                 k_scale, v_scale, block_table, kv_len, q_len, out, B, T, q_heads, kv_heads,
+                                 n_blocks, max_blocks, block_size, workspace);
   hipStream_t s = static_cast<hipStream_t>(stream);
   hipLaunchKernelGGL(paged_prep_kernel, dim3(1 + p.pairs * p.R / kPrepWaves), dim3(kPrepWaves * 64), 0, s, a);
-  if (p.R == 16)
-    hipLaunchKernelGGL((paged_attn_kernel<1, 8>), dim3(p.grid), dim3(512), 0, s, a);
-  else if (p.R == 32)
-    hipLaunchKernelGGL((paged_attn_kernel<2, 4>), dim3(p.grid), dim3(256), 0, s, a);
-  else if (p.R == 48)
-    hipLaunchKernelGGL((paged_attn_kernel<3, 4>), dim3(p.grid), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL(paged_rows_kernel, dim3(p.grid), dim3(512), 0, s, a);
-  if (p.pairs < 32 || p.pairs * p.R < 96 * 16)
-    hipLaunchKernelGGL(paged_merge_kernel<4>, dim3(p.R, p.pairs), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL(paged_merge_kernel<1>, dim3(p.R / 4, p.pairs), dim3(256), 0, s, a);
+  launch_attn<false>(p, a, s);
+  return npn_launch_status();
+}
+
+extern "C" size_t npn_gqa_tree_verify_paged_workspace_size(int B, int T, int q_heads, int kv_heads,
+                                                           int max_blocks, int block_size) {
+  return paged_plan(B, T, q_heads, kv_heads, max_blocks, block_size, true).bytes;
+}
+
+extern "C" int npn_gqa_tree_verify_paged(
+    const uint16_t* query, const uint16_t* gate, const uint16_t* key, const uint16_t* value,
+    const float* q_norm, const float* k_norm, const float* cos_table, const float* sin_table, int positions,
+    int8_t* cache_k, int8_t* cache_v, float* k_scale, float* v_scale, const int32_t* block_table,
+    const int32_t* kv_len, const int64_t* slots, const int32_t* q_len, const int32_t* parent, uint16_t* out,
+    int B, int T, int q_heads, int kv_heads, int n_blocks, int max_blocks, int block_size, void* workspace,
+    size_t workspace_bytes, void* stream) {
+  NPN_REQUIRE(query && gate && key && value && q_norm && k_norm && cos_table && sin_table && cache_k &&
+                  cache_v && k_scale && v_scale && block_table && kv_len && slots && q_len && parent && out,
+              NPN_ERR_NULL);
+  const PagedPlan p = paged_plan(B, T, q_heads, kv_heads, max_blocks, block_size, true);
+  NPN_REQUIRE(p.ok && n_blocks >= 1 && positions >= 1 && kv_heads <= 1024, NPN_ERR_SHAPE);
+  NPN_REQUIRE(NPN_ALIGNED16(query) && NPN_ALIGNED16(gate) && NPN_ALIGNED16(key) && NPN_ALIGNED16(value) &&
+                  NPN_ALIGNED16(q_norm) && NPN_ALIGNED16(k_norm) && NPN_ALIGNED16(cos_table) &&
+                  NPN_ALIGNED16(sin_table) && NPN_ALIGNED16(cache_k) && NPN_ALIGNED16(cache_v) &&
+                  NPN_ALIGNED16(out) && NPN_ALIGNED16(workspace),
+              NPN_ERR_ALIGN);
+  NPN_REQUIRE(workspace != nullptr && workspace_bytes >= p.bytes, NPN_ERR_WORKSPACE);
+  const PagedArgs a = paged_args(p, query, gate, q_norm, cos_table, sin_table, positions, cache_k, cache_v,
+                                 k_scale, v_scale, block_table, kv_len, q_len, out, B, T, q_heads, kv_heads,
+                                 n_blocks, max_blocks, block_size, workspace);
+  const append::PagedAppendArgs ap{key, value, k_norm, cos_table, sin_table, kv_len, slots,
+                                   reinterpret_cast<uint8_t*>(cache_k), reinterpret_cast<uint8_t*>(cache_v),
+                                   k_scale, v_scale, B, T, kv_heads, n_blocks, a.sh, positions};
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int rows = p.pairs * p.R / kPrepWaves;               // workgroups of q'
+  const int per = 1 + (T - 1 + block_size - 1) / block_size;  // a request's rows touch at most so many blocks
+  const int at_once = T < block_size ? T : block_size;
+  auto prep = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(1 + rows + per * 2 * kv_heads * B), dim3(kPrepWaves * 64), 0, s, a, ap, parent,
+                       rows, per);
+  };
+  if (at_once <= 8) prep(tree_prep_kernel<1>);
+  else if (at_once <= 16) prep(tree_prep_kernel<2>);
+  else if (at_once <= 32) prep(tree_prep_kernel<4>);
+  else prep(tree_prep_kernel<8>);
+  launch_attn<true>(p, a, s);
   return npn_launch_status();
 }

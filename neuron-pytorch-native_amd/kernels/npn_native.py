@@ -69,6 +69,12 @@ SIGNATURES = {
     "npn_gqa_kv_append_paged": (_I, [_P] * 5 + [_I] + [_P] * 6 + [_I] * 5 + [_P]),
     "npn_gqa_tail_verify_paged_workspace_size": (_Z, [_I] * 6),
     "npn_gqa_tail_verify_paged": (_I, [_P] * 5 + [_I] + [_P] * 8 + [_I] * 7 + [_P, _Z, _P]),
+    "npn_gqa_tree_verify_paged_workspace_size": (_Z, [_I] * 6),
+    "npn_gqa_tree_verify_paged": (_I, [_P] * 8 + [_I] + [_P] * 10 + [_I] * 7 + [_P, _Z, _P]),
+    "npn_gqa_compact_paged": (_I, [_P] * 6 + [_I] * 6 + [_P]),
+    "npn_deltanet_verify_tree": (_I, [_P] * 14 + [_I] * 4 + [_P]),
+    "npn_deltanet_commit_tree": (_I, [_P] * 4 + [_I, _P] + [_I] * 4 + [_P]),
+    "npn_accept_tree": (_I, [_P] * 7 + [_I] * 2 + [_P]),
     "npn_sample_workspace_size": (_Z, [_I] * 2),
     "npn_sample": (_I, [_P, _I] + [_P] * 6 + [_I] * 2 + [_P, _Z, _P]),
     "npn_deltanet_full_fp8_workspace_size": (_Z, [_I] * 3),
@@ -151,11 +157,16 @@ def register(qualname, schema, fake):
         op = getattr(getattr(torch.ops, namespace), name).default
         specs = op._schema.arguments
         names = [(i, a.name) for i, a in enumerate(specs) if str(a.type) == "Tensor"]
+        lists = [(i, a.name) for i, a in enumerate(specs) if str(a.type) == "List[Tensor]"]
         first = names[0][0]
         written = [i for i, a in enumerate(specs) if a.alias_info is not None and a.alias_info.is_write]
 
+        def flat(args):
+            """The arguments with the lists' tensors in the lists' places."""
+            return [t for a in args for t in (a if isinstance(a, list) else (a,))]
+
         def count_as_written(args):
-            tensors = [args[i] for i in written]
+            tensors = flat([args[i] for i in written])
             try:
                 increment_version(tensors)
             except RuntimeError:  # inference tensors among them, which have no version
@@ -167,8 +178,9 @@ def register(qualname, schema, fake):
 
         def autograd(*args):
             if torch._C._any_requires_grad(*args) or forward_ad._current_level >= 0:
-                _refuse_gradients(qualname, [(arg, args[i]) for i, arg in names])
-            plain = (args[first].is_cuda and _PLAIN.issuperset(map(type, args))
+                _refuse_gradients(qualname, [(arg, args[i]) for i, arg in names] +
+                                  [(arg, t) for i, arg in lists for t in args[i]])
+            plain = (args[first].is_cuda and _PLAIN.issuperset(map(type, flat(args) if lists else args))
                      and torch._C._len_torch_dispatch_stack() == 0
                      and torch._C._functorch.peek_interpreter_stack() is None)
             if plain:
@@ -199,10 +211,15 @@ def check_all(dev, *specs):
             raise RuntimeError(f"{name} must be on {dev}, got {t.device}")
 
 
+def addresses(tensors):
+    """Host array of the tensors' device pointers, for an entry point that takes one."""
+    return (_P * max(len(tensors), 1))(*[t.data_ptr() for t in tensors])
+
+
 def launch(dev, name, *args):
     """`call` of an entry point that ends with a stream, on dev's current stream and with dev as the
-    current device; the tensors' devices have been checked."""
-    raw = [a if type(a) is int else a.data_ptr() for a in args]
+    current device; the tensors' devices have been checked. Arguments: tensors, ints and `addresses`."""
+    raw = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
     fn = getattr(lib(), name)
     if dev.index == torch.cuda.current_device():
         status = fn(*raw, torch._C._cuda_getCurrentRawStream(dev.index))

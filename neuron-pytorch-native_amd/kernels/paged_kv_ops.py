@@ -22,11 +22,23 @@ One block table serves all layers. Lengths stay on the device, so a step plans i
       gqa::tail_verify over the pages: row (b, t, h) attends positions [0, kv_len[b] + t]; rows
       t >= q_len[b] are 0 (pass granted). T = 1 decodes, a long T is a prompt's chunk.
 
+For a tree of drafted tokens (parent [B, T] int32: deltanet_tree_ops.py):
+
+  gqa::tree_verify_paged(query, gate [B, T, Hq, 256] bf16, key, value [B, T, Hkv, 256] bf16, q_norm,
+                         k_norm, cos_table, sin_table, cache_k, cache_v, k_scale, v_scale, block_table,
+                         kv_len, slots [B, T] int64, q_len, parent) -> out [B, T, Hq, 256] bf16
+      Both of the above for the nodes of a tree: their rows appended at the positions of the tree, and
+      attention of each node t < q_len[b] over [0, kv_len[b]), its ancestors and itself.
+  gqa::compact_paged_(path [B, T] int32, slots [B, T] int64, cache_ks, cache_vs, k_scales, v_scales) -> ()
+      Lists of every layer's tensors; the accepted path's rows go to the front of the tree's, slots[b, path[b, d]]
+      to slots[b, d]. paged::update_blocks_ then gives back the blocks behind them.
+
 include/npn_spec_verify.h has the details and limits.
 """
 import torch
 
-from npn_native import check_all, launch, query as size_query, register
+from deltanet_tree_ops import tree_shape
+from npn_native import addresses, check_all, launch, query as size_query, register
 
 HEAD_DIM = 256
 ROPE_DIM = 64
@@ -136,3 +148,65 @@ def tail_verify_paged(query, gate, q_norm, cos_table, sin_table, cache_k, cache_
            cache_k, cache_v, k_scale, v_scale, block_table, kv_len, q_len, out, B, T, hq, hkv, n, P,
            bs, ws, n_ws)
     return out
+
+
+def _tree_verify_fake(query, gate, key, value, q_norm, k_norm, cos_table, sin_table, cache_k, cache_v, k_scale,
+                      v_scale, block_table, kv_len, slots, q_len, parent):
+    return torch.empty_like(query)
+
+
+@register("gqa::tree_verify_paged",
+          "(Tensor query, Tensor gate, Tensor key, Tensor value, Tensor q_norm, Tensor k_norm, "
+          "Tensor cos_table, Tensor sin_table, Tensor(a!) cache_k, Tensor(b!) cache_v, "
+          "Tensor(c!) k_scale, Tensor(d!) v_scale, Tensor block_table, Tensor kv_len, Tensor slots, "
+          "Tensor q_len, Tensor parent) -> Tensor", _tree_verify_fake)
+def tree_verify_paged(query, gate, key, value, q_norm, k_norm, cos_table, sin_table, cache_k, cache_v, k_scale,
+                      v_scale, block_table, kv_len, slots, q_len, parent):
+    n, hkv, bs = _cache_sizes(cache_k)
+    B, T = tree_shape(parent, "parent")
+    hq = _dims(query, "query", 4)[2]
+    P, positions = _dims(block_table, "block_table", 2)[1], cos_table.shape[0]
+    dev, table = query.device, (positions, ROPE_DIM)
+    rows, kv_rows = (B, T, hq, HEAD_DIM), (B, T, hkv, HEAD_DIM)
+    check_all(dev, (query, "query", BF16, rows), (gate, "gate", BF16, rows), (key, "key", BF16, kv_rows),
+              (value, "value", BF16, kv_rows), (q_norm, "q_norm", F32, HEAD_DIM),
+              (k_norm, "k_norm", F32, HEAD_DIM), (cos_table, "cos_table", F32, table),
+              (sin_table, "sin_table", F32, table), (cache_k, "cache_k", I8, (n, hkv, bs, HEAD_DIM)),
+              (cache_v, "cache_v", I8, (n, hkv, HEAD_DIM, bs)), (k_scale, "k_scale", F32, (n, hkv)),
+              (v_scale, "v_scale", F32, (n, hkv)), (block_table, "block_table", I32, (B, P)),
+              (kv_len, "kv_len", I32, B), (slots, "slots", I64, (B, T)), (q_len, "q_len", I32, B),
+              (parent, "parent", I32, (B, T)))
+    n_ws = size_query("npn_gqa_tree_verify_paged_workspace_size", B, T, hq, hkv, P, bs)
+    if n_ws == 0:
+        raise RuntimeError(f"unsupported tree_verify_paged sizes B={B} T={T} Hq={hq} Hkv={hkv} "
+                           f"P={P} bs={bs}")
+    ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
+    out = torch.empty_like(query)
+    launch(dev, "npn_gqa_tree_verify_paged", query, gate, key, value, q_norm, k_norm, cos_table, sin_table,
+           positions, cache_k, cache_v, k_scale, v_scale, block_table, kv_len, slots, q_len, parent, out,
+           B, T, hq, hkv, n, P, bs, ws, n_ws)
+    return out
+
+
+def _compact_fake(path, slots, cache_ks, cache_vs, k_scales, v_scales):
+    return None
+
+
+@register("gqa::compact_paged_",
+          "(Tensor path, Tensor slots, Tensor(a!)[] cache_ks, Tensor(b!)[] cache_vs, "
+          "Tensor(c!)[] k_scales, Tensor(d!)[] v_scales) -> ()", _compact_fake)
+def compact_paged_(path, slots, cache_ks, cache_vs, k_scales, v_scales):
+    layers = len(cache_ks)
+    if not layers == len(cache_vs) == len(k_scales) == len(v_scales):
+        raise RuntimeError("compact_paged_: one cache_v, k_scale and v_scale for each cache_k")
+    B, T = tree_shape(path, "path")
+    dev = path.device
+    check_all(dev, (path, "path", I32, (B, T)), (slots, "slots", I64, (B, T)))
+    if layers == 0:
+        return
+    n, hkv, bs = _cache_sizes(cache_ks[0])
+    for specs in zip(cache_ks, cache_vs, k_scales, v_scales):
+        check_all(dev, *zip(specs, ("cache_ks", "cache_vs", "k_scales", "v_scales"), (I8, I8, F32, F32),
+                            ((n, hkv, bs, HEAD_DIM), (n, hkv, HEAD_DIM, bs), (n, hkv), (n, hkv))))
+    launch(dev, "npn_gqa_compact_paged", path, slots, addresses(cache_ks), addresses(cache_vs),
+           addresses(k_scales), addresses(v_scales), layers, B, T, hkv, n, bs)

@@ -14,6 +14,12 @@ contrib/qwen3.6-27b/static_decode.py:1313).
                                  u_sample, inv_temperature)
       -> (accepted, out_ids, target_logits [B, K+1, V] bf16)
 
+  spec::accept_tree(target_ids, draft_ids [B, T] int64, parent [B, T] int32, q_len [B] int32)
+      -> (accepted [B] int32, path [B, T] int32, out_ids [B, T] int64)
+      The walk through a tree of drafted tokens (deltanet_tree_ops.py): from node 0 to the first child
+      whose draft is the target's token of the node. path holds the nodes, -1 behind; accepted is -1,
+      and out_ids -1 throughout, where a request has no node (q_len[b] < 1).
+
 accepted[b] is the number of accepted drafts (0..K); out_ids[b] holds those drafts,
 then the correction (or bonus) token, then -1. Rejection sampling follows Leviathan
 et al. 2023 (Alg. 1) under the library's integer softmax contract (chunk-relative exponentials
@@ -22,7 +28,8 @@ are bit-identical to the CPU restatement for the same logits and uniforms.
 """
 import torch
 
-from npn_native import call, query, require, stream_of
+from deltanet_tree_ops import tree_shape
+from npn_native import call, check_all, launch, query, register, require, stream_of
 
 
 def _workspace(B, K, V, device):
@@ -176,3 +183,19 @@ def _(hidden, lm_head_w, lm_head_scale, draft_logits, draft_ids, u_accept, u_sam
     B, K, V = draft_logits.shape
     return (hidden.new_empty(B, dtype=torch.int32), hidden.new_empty((B, K + 1), dtype=torch.int64),
             hidden.new_empty((B, K + 1, V), dtype=torch.bfloat16))
+
+
+def _accept_tree_fake(target_ids, draft_ids, parent, q_len):
+    return torch.empty_like(q_len), torch.empty_like(parent), torch.empty_like(target_ids)
+
+
+@register("spec::accept_tree", "(Tensor target_ids, Tensor draft_ids, Tensor parent, Tensor q_len) "
+          "-> (Tensor, Tensor, Tensor)", _accept_tree_fake)
+def accept_tree(target_ids, draft_ids, parent, q_len):
+    B, T = tree_shape(parent, "parent")
+    dev = parent.device
+    check_all(dev, (target_ids, "target_ids", torch.int64, (B, T)), (draft_ids, "draft_ids", torch.int64, (B, T)),
+              (parent, "parent", torch.int32, (B, T)), (q_len, "q_len", torch.int32, B))
+    accepted, path, out_ids = q_len.new_empty(B), torch.empty_like(parent), torch.empty_like(target_ids)
+    launch(dev, "npn_accept_tree", target_ids, draft_ids, parent, q_len, accepted, path, out_ids, B, T)
+    return accepted, path, out_ids
