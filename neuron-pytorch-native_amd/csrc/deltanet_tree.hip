@@ -41,139 +41,371 @@ struct TreeArgs {
   int B, T, Hk, Hv;
 };
 
-// One workgroup a (b, h), thread (c, p) for column c of the state: p = 0 the rows of k, p = 1 those of q.
-template <int TMAX>
-__global__ __launch_bounds__(256) void dn_tree_verify_kernel(TreeArgs a) {
-  __shared__ float s_q[TMAX][D], s_k[TMAX][D], s_u[TMAX][D];
-  __shared__ float s_kk[TMAX][TMAX + 1], s_qk[TMAX][TMAX + 1];
-  __shared__ double s_g[TMAX];
-  __shared__ float s_begun[TMAX], s_beta[TMAX], s_sum[TMAX][2];
-  __shared__ uint64_t s_anc[TMAX];
-  __shared__ int s_tap[TMAX][3];
-  const int T = a.T, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+typedef _Float16 f16x8 __attribute__((__vector_size__(8 * sizeof(_Float16))));
+typedef _Float16 f16x2 __attribute__((__vector_size__(2 * sizeof(_Float16))));
+typedef float f32x4 __attribute__((__vector_size__(4 * sizeof(float))));
+
+// One workgroup of four waves a (b, h); NT tiles of 16 nodes; wave w has columns 32 w + 2 i + {0, 1} of everything that
+// has the state's columns (lane (i, G): i = lane % 16, G = lane / 16), so that the products' results are the next ones'
+// operands where they are. Steps, with a barrier between them:
+//   1. conv, SiLU and norms, a row of 128 channels to a wave at a time, two channels a lane, into LDS;
+//   2. K S0, Q S0 and, tile by tile of the lower triangle, K K^T and Q K^T. In f16 MFMAs: a number is the sum of two
+//      f16 (x 2^12, the state's columns over a power of two of their own), of whose four products the
+//      smallest is left out: 22 bits each, accumulated in fp32, a fifth of fp32 MFMAs' time;
+//   3. the inverses of the NT diagonal 16 x 16 blocks of 1 - low, low(t, s) = -beta_t D(t, s) (k_s . k_t) at t's
+//      ancestors s, by forward substitution (low's powers may grow where its inverse does not);
+//   4. block by block u = inverse (beta (v - e^G K S0) + low u of the blocks before), then o = e^G Q S0 + (D Q K^T) u,
+//      in fp32 MFMAs;
+//   5. the norm over the workgroup's columns, z and the output.
+// A node whose input is not finite has zeros in these sums, which reach all nodes of a tile, and is noted: NaN
+// goes to its own and its descendants' rows at the end.
+template <int NT>
+struct TreeSmem {
+  static constexpr int TM = 16 * NT;
+  _Float16 x[2][2 * TM][D + 8];  // high and low parts of k's rows, then q's
+  float v[TM][D + 4];
+  float low[TM][TM + 4], mix[TM][TM + 4];
+  float inv[NT][16][20];
+  double g[TM];  // sums of g along a node's line, base 2
+  uint64_t anc[TM];
+  uint64_t bad_kv[4], bad_q[4];  // by wave
+  unsigned long long bad_u;
+  float begun[TM], beta[TM], ss[4][TM];
+};
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// Maximum over the lanes (i, G) of a column i.
+__device__ __forceinline__ float max_over_groups(float x) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ f32x4 mfma_f16(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// Four products over k = 16: lane (i, G) has the row's (a) or column's (b) k 4 G + [0, 4), b as a result has its rows.
+__device__ __forceinline__ f32x4 mfma_f32(const float4 a, const f32x4 b, f32x4 c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x, b[0], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.y, b[1], c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.z, b[2], c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a.w, b[3], c, 0, 0, 0);
+}
+
+template <int NT>
+__global__ __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) void dn_tree_verify_kernel(TreeArgs a) {
+  constexpr int TM = 16 * NT;
+  constexpr float kUnit = 4096.0f;  // the rows' scale in f16
+  __shared__ __attribute__((aligned(16))) TreeSmem<NT> sm;
+  const int T = a.T, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, G = lane >> 4;
   const int b = blockIdx.x / a.Hv, h = blockIdx.x - b * a.Hv, kh = h / (a.Hv / a.Hk);
   const int QKV = (2 * a.Hk + a.Hv) * D;
 
+  // The state, lane (i, G): rows 32 s + 8 G + e of its two columns.
+  const float2* S0 = reinterpret_cast<const float2*>(a.state + ((size_t)b * a.Hv + h) * D * D + 32 * w + 2 * i) +
+                     (size_t)(8 * G) * (D / 2);
+  float2 s0[4][8];
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s0[s][e] = S0[(32 * s + e) * (D / 2)];
+
+  // Lane t: node t's inputs one to three back, a node or -1 .. -3 for the last to the first of conv_state.
   const int parent = npn::tree_parent(a.parent + (size_t)b * T, T, lane);
-  const uint64_t anc = npn::tree_ancestors(parent, T, lane);
-  if (w == 0) {
-    // The window's inputs one to three back: a node, or -1 .. -3 for the last to the first of conv_state.
+  int tap[3];
+  {
     int at = lane;
+#pragma unroll
     for (int j = 0; j < 3; ++j) {
       const int up = __shfl(parent, max(at, 0), 64);
       at = at < 0 ? at - 1 : up;
-      if (lane < T) s_tap[lane][j] = at;
+      tap[j] = at;
     }
+  }
+  uint64_t bad_kv = 0, bad_q = 0;  // wave-uniform
+  if (w == 0) {
+    float beta = 0.f;
     double g = 0.0;
+    bool bad = false;
     if (lane < T) {
       const size_t gi = ((size_t)b * T + lane) * a.Hv + h;
       const float gf = -__expf(a.A_log[h]) * npn::softplus(a.a_out[gi] + a.dt_bias[h]);
       a.rec_decay[gi] = __expf(gf);
-      s_beta[lane] = npn::sigmoid(a.b_out[gi]);
-      g = gf < -256.0f ? -256.0 : (double)gf;
-      s_anc[lane] = anc;
+      beta = npn::sigmoid(a.b_out[gi]);
+      bad = gf != gf || beta != beta;
+      g = bad ? 0.0 : (double)fmaxf(gf, -256.0f) * 1.4426950408889634;
+      beta = bad ? 0.f : beta;
     }
-    double total = 0.0;
-    for (int t = 0; t < T; ++t) {
-      const double x = __longlong_as_double(npn::tree_bits(__double_as_longlong(g), t));
-      total += (anc >> t) & 1 ? x : 0.0;
+    bad_kv = __builtin_amdgcn_ballot_w64(bad);
+    const uint64_t anc = npn::tree_ancestors(parent, T, lane);
+    double total = g;
+    int up = parent;
+    for (int n = 1; n < T; n <<= 1) {
+      const int from = up < 0 ? lane : up;
+      const uint64_t bits = (uint64_t)__double_as_longlong(total);
+      const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)bits, from, 64);
+      const uint32_t hi = (uint32_t)__shfl((int)(uint32_t)(bits >> 32), from, 64);
+      const int next = __shfl(up, from, 64);
+      total += up < 0 ? 0.0 : __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+      up = up < 0 ? up : next;
     }
-    if (lane < T) {
-      s_g[lane] = total;
-      s_begun[lane] = __expf((float)total);
+    if (lane < TM) {
+      sm.anc[lane] = anc;
+      sm.beta[lane] = beta;
+      sm.g[lane] = total;
+      sm.begun[lane] = __builtin_amdgcn_exp2f((float)total);
+    }
+    if (lane == 0) sm.bad_u = 0;
+  }
+
+  // 1. rows q, k, v (0, 1, 2), node t = w + 4 n, four of them in flight
+#pragma unroll
+  for (int which = 0; which < 3; ++which) {
+    const int c = (which == 0 ? kh : which == 1 ? a.Hk + kh : 2 * a.Hk + h) * D + 2 * lane;
+    const float4 w0 = *reinterpret_cast<const float4*>(a.conv_weight + 4 * c);
+    const float4 w1 = *reinterpret_cast<const float4*>(a.conv_weight + 4 * c + 4);
+    const float2 bias = make_float2(a.conv_bias[c], a.conv_bias[c + 1]);
+    const uint16_t* cs = a.conv_state + ((size_t)b * QKV + c) * 3;
+    uint32_t old[3];  // both channels' inputs one to three back from the first
+#pragma unroll
+    for (int j = 0; j < 3; ++j) old[j] = cs[2 - j] | ((uint32_t)cs[5 - j] << 16);
+    const uint16_t* xb = a.mixed_qkv + (size_t)b * T * QKV + c;
+    for (int t0 = w; t0 < TM; t0 += 16) {
+      uint32_t x[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = min(t0 + 4 * k, T - 1);
+        x[k][0] = *reinterpret_cast<const uint32_t*>(xb + (size_t)t * QKV);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          const int at = __builtin_amdgcn_readlane(tap[j], t);
+          x[k][j + 1] = *reinterpret_cast<const uint32_t*>(xb + (size_t)max(at, 0) * QKV);
+          x[k][j + 1] = at >= 0 ? x[k][j + 1] : at == -1 ? old[0] : at == -2 ? old[1] : old[2];
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int t = t0 + 4 * k;
+        float y0 = bias.x, y1 = bias.y;
+        y0 += w0.x * npn::bf16lo(x[k][3]) + w0.y * npn::bf16lo(x[k][2]) + w0.z * npn::bf16lo(x[k][1]) +
+              w0.w * npn::bf16lo(x[k][0]);
+        y1 += w1.x * npn::bf16hi(x[k][3]) + w1.y * npn::bf16hi(x[k][2]) + w1.z * npn::bf16hi(x[k][1]) +
+              w1.w * npn::bf16hi(x[k][0]);
+        y0 = npn::silu(y0);
+        y1 = npn::silu(y1);
+        const bool in = t < T, bad = in && __builtin_amdgcn_ballot_w64(!finite(y0) || !finite(y1)) != 0;
+        if (which < 2) {
+          const float ss = npn::wave_sum(y0 * y0 + y1 * y1);
+          const float n = rsqrtf(ss + kEps) * (which == 0 ? 0.08838834764831845f : 1.0f);  // q: / sqrt(128)
+          y0 *= n;
+          y1 *= n;
+          if (which == 1 && in && h == kh * (a.Hv / a.Hk))
+            *reinterpret_cast<float2*>(a.rec_k + (((size_t)b * T + t) * a.Hk + kh) * D + 2 * lane) = make_float2(y0, y1);
+        }
+        if (!in || bad) y0 = y1 = 0.f;
+        if (bad && which == 0) bad_q |= 1ull << t;
+        if (bad && which != 0) bad_kv |= 1ull << t;
+        if (which < 2) {
+          const f16x2 hi = {(_Float16)(y0 * kUnit), (_Float16)(y1 * kUnit)};
+          const f16x2 lo = {(_Float16)(y0 * kUnit - (float)hi[0]), (_Float16)(y1 * kUnit - (float)hi[1])};
+          const int row = which == 0 ? TM + t : t;
+          *reinterpret_cast<f16x2*>(&sm.x[0][row][2 * lane]) = hi;
+          *reinterpret_cast<f16x2*>(&sm.x[1][row][2 * lane]) = lo;
+        } else {
+          *reinterpret_cast<float2*>(&sm.v[t][2 * lane]) = make_float2(y0, y1);
+        }
+      }
+    }
+  }
+  if (lane == 0) {
+    sm.bad_kv[w] = bad_kv;
+    sm.bad_q[w] = bad_q;
+  }
+  __syncthreads();
+
+  // 2. the pairs' products, tile (a, s) with s <= a of k's rows and of q's
+  auto rows_of = [&](int part, int tile, int step) {
+    return *reinterpret_cast<const f16x8*>(&sm.x[part][16 * tile + i][32 * step + 8 * G]);
+  };
+  int turn = 0;
+#pragma unroll
+  for (int ta = 0; ta < NT; ++ta)
+#pragma unroll
+    for (int ts = 0; ts <= ta; ++ts)
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        if ((turn++ & 3) != w) continue;
+        f32x4 p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+          const f16x8 xh = rows_of(0, q * NT + ta, step), xl = rows_of(1, q * NT + ta, step);
+          const f16x8 kh8 = rows_of(0, ts, step), kl8 = rows_of(1, ts, step);
+          p = mfma_f16(xl, kh8, p);
+          p = mfma_f16(xh, kl8, p);
+          p = mfma_f16(xh, kh8, p);
+        }
+        const int s = 16 * ts + i;
+        const double gs = sm.g[s];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int t = 16 * ta + 4 * G + r;
+          const bool sees = (sm.anc[t] >> s & 1) && (q || s != t);
+          const float f = __builtin_amdgcn_exp2f((float)(sm.g[t] - gs)) * (1.0f / (kUnit * kUnit));
+          (q ? sm.mix : sm.low)[t][s] = sees ? p[r] * f * (q ? 1.0f : -sm.beta[t]) : 0.f;
+        }
+      }
+  // and the state's
+  float inv_scale[2];
+  f32x4 ks[NT][2], qs[NT][2];
+  {
+    float scale[2], big[2] = {0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        big[0] = fmaxf(big[0], fabsf(s0[s][e].x));
+        big[1] = fmaxf(big[1], fabsf(s0[s][e].y));
+      }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      // to [2^11, 2^12); of a column that is not finite some product is not either
+      const uint32_t e = min(max(__float_as_uint(max_over_groups(big[c])) >> 23, 12u), 254u);
+      scale[c] = __uint_as_float((265u - e) << 23);
+      inv_scale[c] = __uint_as_float((e - 11u) << 23) * (1.0f / kUnit);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) ks[n][c] = qs[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      f16x8 hi[2], lo[2];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x0 = s0[s][e].x * scale[0], x1 = s0[s][e].y * scale[1];
+        hi[0][e] = (_Float16)x0;
+        hi[1][e] = (_Float16)x1;
+        lo[0][e] = (_Float16)(x0 - (float)hi[0][e]);
+        lo[1][e] = (_Float16)(x1 - (float)hi[1][e]);
+      }
+#pragma unroll
+      for (int n = 0; n < 2 * NT; ++n) {
+        const f16x8 xh = rows_of(0, n, s), xl = rows_of(1, n, s);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          f32x4& p = n < NT ? ks[n % NT][c] : qs[n % NT][c];
+          p = mfma_f16(xl, hi[c], p);
+          p = mfma_f16(xh, lo[c], p);
+          p = mfma_f16(xh, hi[c], p);
+        }
+      }
     }
   }
   __syncthreads();
 
-  const uint16_t* xb = a.mixed_qkv + (size_t)b * T * QKV;
-  const uint16_t* csb = a.conv_state + (size_t)b * QKV * 3;
-  for (int idx = tid; idx < T * 3 * D; idx += 256) {
-    const int t = idx / (3 * D), ch = idx - t * 3 * D, which = ch / D, i = ch - which * D;
-    const int c = which == 0 ? kh * D + i : which == 1 ? (a.Hk + kh) * D + i : (2 * a.Hk + h) * D + i;
-    float y = a.conv_bias[c];
-    for (int j = 2; j >= 0; --j) {
-      const int at = s_tap[t][j];
-      const uint16_t x = at >= 0 ? xb[(size_t)at * QKV + c] : csb[(size_t)c * 3 + 3 + at];
-      y += a.conv_weight[c * 4 + 2 - j] * npn::bf16_to_f32(x);
+  // 3. column i of the inverse of block w
+  if (w < NT) {
+    float x[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float y = r == i ? 1.0f : 0.f;
+#pragma unroll
+      for (int q = 0; q < r; ++q) y = fmaf(sm.low[16 * w + r][16 * w + q], x[q], y);
+      x[r] = y;
+      if (G == 0) sm.inv[w][r][i] = y;
     }
-    y += a.conv_weight[c * 4 + 3] * npn::bf16_to_f32(xb[(size_t)t * QKV + c]);
-    (which == 0 ? s_q : which == 1 ? s_k : s_u)[t][i] = npn::silu(y);
-  }
-  __syncthreads();
-  for (int r = w; r < 2 * T; r += 4) {
-    float* x = r < T ? s_q[r] : s_k[r - T];
-    const float x0 = x[lane], x1 = x[lane + 64];
-    const float n = rsqrtf(npn::wave_sum(x0 * x0 + x1 * x1) + kEps) * (r < T ? 0.08838834764831845f : 1.0f);
-    x[lane] = x0 * n;
-    x[lane + 64] = x1 * n;
-    if (r >= T && h == kh * (a.Hv / a.Hk)) {
-      float* k = a.rec_k + (((size_t)b * T + r - T) * a.Hk + kh) * D;
-      k[lane] = x0 * n;
-      k[lane + 64] = x1 * n;
-    }
-  }
-  __syncthreads();
-  for (int idx = tid; idx < 2 * T * T; idx += 256) {
-    const int which = idx / (T * T), t = (idx - which * T * T) / T, s = idx % T;
-    if (!((s_anc[t] >> s) & 1)) continue;
-    const float* x = which ? s_q[t] : s_k[t];
-    float dot = 0.f;
-    for (int i = 0; i < D; ++i) dot += x[i] * s_k[s][i];
-    (which ? s_qk : s_kk)[t][s] = dot * __expf((float)(s_g[t] - s_g[s]));
   }
   __syncthreads();
 
-  const int c = tid & (D - 1), p = tid >> 7;
-  const float* S0 = a.state + ((size_t)b * a.Hv + h) * D * D + c;
-  const float (*x)[D] = p ? s_q : s_k;
-  float acc[TMAX];
+  // 4.
+  // Rows' entries that are not finite count as 0 from here on, and their nodes as bad.
+  auto clear = [&](f32x4 (&x)[2], int tile) {
 #pragma unroll
-  for (int t = 0; t < TMAX; ++t) acc[t] = 0.f;
-  for (int i = 0; i < D; ++i) {
-    const float s = S0[(size_t)i * D];
-#pragma unroll
-    for (int t = 0; t < TMAX; ++t)
-      if (t < T) acc[t] += x[t][i] * s;
-  }
-  if (p == 0) {
-#pragma unroll
-    for (int t = 0; t < TMAX; ++t)
-      if (t < T) {
-        float r = s_u[t][c] - s_begun[t] * acc[t];
-        for (uint64_t m = s_anc[t] & ~(1ull << t); m; m &= m - 1) {
-          const int s = __builtin_ctzll(m);
-          r -= s_kk[t][s] * s_u[s][c];
-        }
-        s_u[t][c] = r * s_beta[t];
-        a.rec_u[(((size_t)b * T + t) * a.Hv + h) * D + c] = r * s_beta[t];
+    for (int r = 0; r < 4; ++r) {
+      const bool bad = !finite(x[0][r]) || !finite(x[1][r]);
+      const uint64_t lanes = __builtin_amdgcn_ballot_w64(bad);
+      if (lanes == 0) continue;
+      if (bad) {
+        x[0][r] = x[1][r] = 0.f;
+        atomicOr(&sm.bad_u, 1ull << (16 * tile + 4 * G + r));
       }
+    }
+  };
+  f32x4 u[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    f32x4 rhs[2];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int t = 16 * n + 4 * G + r;
+      const float2 v = *reinterpret_cast<const float2*>(&sm.v[t][32 * w + 2 * i]);
+      const float begun = sm.begun[t], beta = sm.beta[t];
+      rhs[0][r] = beta * (v.x - begun * (ks[n][0][r] * inv_scale[0]));
+      rhs[1][r] = beta * (v.y - begun * (ks[n][1][r] * inv_scale[1]));
+    }
+#pragma unroll
+    for (int s = 0; s < n; ++s) {
+      const float4 f = *reinterpret_cast<const float4*>(&sm.low[16 * n + i][16 * s + 4 * G]);
+      rhs[0] = mfma_f32(f, u[s][0], rhs[0]);
+      rhs[1] = mfma_f32(f, u[s][1], rhs[1]);
+    }
+    clear(rhs, n);
+    const float4 f = *reinterpret_cast<const float4*>(&sm.inv[n][i][4 * G]);
+    u[n][0] = mfma_f32(f, rhs[0], f32x4{0.f, 0.f, 0.f, 0.f});
+    u[n][1] = mfma_f32(f, rhs[1], f32x4{0.f, 0.f, 0.f, 0.f});
+    clear(u[n], n);
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float begun = sm.begun[16 * n + 4 * G + r];
+      qs[n][0][r] *= begun * inv_scale[0];
+      qs[n][1][r] *= begun * inv_scale[1];
+    }
+#pragma unroll
+    for (int s = 0; s <= n; ++s) {
+      const float4 f = *reinterpret_cast<const float4*>(&sm.mix[16 * n + i][16 * s + 4 * G]);
+      qs[n][0] = mfma_f32(f, u[s][0], qs[n][0]);
+      qs[n][1] = mfma_f32(f, u[s][1], qs[n][1]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float ss = qs[n][0][r] * qs[n][0][r] + qs[n][1][r] * qs[n][1][r];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t bits = __float_as_uint(ss);
+        ss += __uint_as_float(k == 0 ? npn::dpp32<npn::kDppStep[0]>(bits) : k == 1 ? npn::dpp32<npn::kDppStep[1]>(bits)
+                              : k == 2 ? npn::dpp32<npn::kDppStep[2]>(bits) : npn::dpp32<npn::kDppStep[3]>(bits));
+      }
+      if (i == 0) sm.ss[w][16 * n + 4 * G + r] = ss;
+    }
   }
   __syncthreads();
-  if (p == 1) {
+
+  // 5.
+  const uint64_t kv = sm.bad_kv[0] | sm.bad_kv[1] | sm.bad_kv[2] | sm.bad_kv[3] | sm.bad_u;
+  const uint64_t bq = sm.bad_q[0] | sm.bad_q[1] | sm.bad_q[2] | sm.bad_q[3];
+  const float2 nw = *reinterpret_cast<const float2*>(a.norm_weight + 32 * w + 2 * i);
 #pragma unroll
-    for (int t = 0; t < TMAX; ++t)
-      if (t < T) {
-        float o = s_begun[t] * acc[t];
-        for (uint64_t m = s_anc[t]; m; m &= m - 1) {
-          const int s = __builtin_ctzll(m);
-          o += s_qk[t][s] * s_u[s][c];
-        }
-        acc[t] = o;
-        const float sum = npn::wave_sum(o * o);
-        if (lane == 0) s_sum[t][w & 1] = sum;
-      }
-  }
-  __syncthreads();
-  if (p == 1) {
-    const float nw = a.norm_weight[c];
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int t = 0; t < TMAX; ++t)
-      if (t < T) {
-        const size_t oi = (((size_t)b * T + t) * a.Hv + h) * D + c;
-        const float r = rsqrtf((s_sum[t][0] + s_sum[t][1]) * (1.0f / D) + kEps);
-        a.out[oi] = npn::f32_to_bf16(acc[t] * r * nw * npn::silu(npn::bf16_to_f32(a.z[oi])));
-      }
-  }
+    for (int r = 0; r < 4; ++r) {
+      const int t = 16 * n + 4 * G + r;
+      if (t >= T) continue;
+      const size_t at = (((size_t)b * T + t) * a.Hv + h) * D + 32 * w + 2 * i;
+      const bool nan = (sm.anc[t] & kv) != 0;
+      const float ss = (sm.ss[0][t] + sm.ss[1][t]) + (sm.ss[2][t] + sm.ss[3][t]);
+      const float f = nan || (bq >> t & 1) ? NAN : rsqrtf(ss * (1.0f / D) + kEps);
+      const uint32_t z = *reinterpret_cast<const uint32_t*>(a.z + at);
+      const float o0 = qs[n][0][r] * f * nw.x * npn::silu(npn::bf16lo(z));
+      const float o1 = qs[n][1][r] * f * nw.y * npn::silu(npn::bf16hi(z));
+      *reinterpret_cast<uint32_t*>(a.out + at) = npn::f32_to_bf16(o0) | ((uint32_t)npn::f32_to_bf16(o1) << 16);
+      *reinterpret_cast<float2*>(a.rec_u + at) = nan ? make_float2(NAN, NAN) : make_float2(u[n][0][r], u[n][1][r]);
+    }
 }
 
 // ---- commit -----------------------------------------------------------------------------------------
@@ -272,9 +504,10 @@ extern "C" int npn_deltanet_verify_tree(const float* state, const int32_t* paren
                    dt_bias, norm_weight, out, records, rec_u, rec_decay, B, T, k_heads, v_heads};
   const dim3 grid(B * v_heads), block(256);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (T <= 16) hipLaunchKernelGGL(dn_tree_verify_kernel<16>, grid, block, 0, s, a);
-  else if (T <= 32) hipLaunchKernelGGL(dn_tree_verify_kernel<32>, grid, block, 0, s, a);
-  else hipLaunchKernelGGL(dn_tree_verify_kernel<64>, grid, block, 0, s, a);
+  if (T <= 16) hipLaunchKernelGGL(dn_tree_verify_kernel<1>, grid, block, 0, s, a);
+  else if (T <= 32) hipLaunchKernelGGL(dn_tree_verify_kernel<2>, grid, block, 0, s, a);
+  else if (T <= 48) hipLaunchKernelGGL(dn_tree_verify_kernel<3>, grid, block, 0, s, a);
+  else hipLaunchKernelGGL(dn_tree_verify_kernel<4>, grid, block, 0, s, a);
   return npn_launch_status();
 }
 
@@ -286,7 +519,7 @@ extern "C" int npn_deltanet_commit_tree(float* const* state, uint16_t* const* co
   NPN_REQUIRE(layers >= 0 && heads_ok(B, T, k_heads, v_heads), NPN_ERR_SHAPE);
   for (int l = 0; l < layers; ++l) {
     NPN_REQUIRE(state[l] && conv_state[l] && mixed_qkv[l] && records[l], NPN_ERR_NULL);
-    NPN_REQUIRE(NPN_ALIGNED16(state[l]) && NPN_ALIGNED16(records[l]), NPN_ERR_ALIGN);
+    NPN_REQUIRE(NPN_ALIGNED16(state[l]), NPN_ERR_ALIGN);
     for (int k = 0; k < l; ++k) NPN_REQUIRE(state[k] != state[l] && conv_state[k] != conv_state[l], NPN_ERR_VALUE);
   }
   const int per = ((2 * k_heads + v_heads) * D + 255) / 256;

@@ -180,6 +180,8 @@ def test_commit_tree_matches_oracle(ops, L, B, T, Hk, Hv):
         path[1] = -1                      # a request that sits out
         path[2, :3] = [2, 1, 5][:3]       # ends where it no longer ascends
     recs = [_verify(ops, f, cuda(parent))[1] for _, f in ds]
+    stack = torch.stack([torch.cat([r[:1], r]) for r in recs])  # kept in one tensor: off 16 bytes, as odd heads leave them
+    recs = [r[1:] for r in stack]
     states, convs = [f["state"].clone() for _, f in ds], [f["conv_state"].clone() for _, f in ds]
     ops.deltanet.commit_tree_(states, convs, [f["mixed_qkv"] for _, f in ds], recs, cuda(path), Hv)
     torch.cuda.synchronize()
