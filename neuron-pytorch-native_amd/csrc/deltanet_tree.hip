@@ -59,7 +59,7 @@ typedef float f32x4 __attribute__((__vector_size__(4 * sizeof(float))));
 //   5. the norm over the workgroup's columns, z and the output.
 // A node whose input is not finite has zeros in these sums, which reach all nodes of a tile, and is noted: NaN
 // goes to its own and its descendants' rows at the end.
-template <int NT>
+template <int NT, int NW>
 struct TreeSmem {
   static constexpr int TM = 16 * NT;
   _Float16 x[2][2 * TM][D + 8];  // high and low parts of k's rows, then q's
@@ -68,9 +68,9 @@ struct TreeSmem {
   float inv[NT][16][20];
   double g[TM];  // sums of g along a node's line, base 2
   uint64_t anc[TM];
-  uint64_t bad_kv[4], bad_q[4];  // by wave
+  uint64_t bad_kv[NW], bad_q[NW];  // by wave
   unsigned long long bad_u;
-  float begun[TM], beta[TM], ss[4][TM];
+  float begun[TM], beta[TM], ss[NW][TM];
 };
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
@@ -81,6 +81,20 @@ __device__ __forceinline__ float max_over_groups(float x) {
   x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// Sum over a row of 16 lanes.
+__device__ __forceinline__ float row_sum(float x) {
+  x += __uint_as_float(npn::dpp32<npn::kDppStep[0]>(__float_as_uint(x)));
+  x += __uint_as_float(npn::dpp32<npn::kDppStep[1]>(__float_as_uint(x)));
+  x += __uint_as_float(npn::dpp32<npn::kDppStep[2]>(__float_as_uint(x)));
+  return x + __uint_as_float(npn::dpp32<npn::kDppStep[3]>(__float_as_uint(x)));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+  x = row_sum(x);
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 __device__ __forceinline__ f32x4 mfma_f16(f16x8 a, f16x8 b, f32x4 c) {
@@ -94,27 +108,67 @@ __device__ __forceinline__ f32x4 mfma_f32(const float4 a, const f32x4 b, f32x4 c
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a.w, b[3], c, 0, 0, 0);
 }
 
-template <int NT>
-__global__ __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) void dn_tree_verify_kernel(TreeArgs a) {
+// N neighbouring floats.
+template <int N>
+struct Floats {
+  float x[N];
+};
+
+template <int NT, int NW>
+__global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_verify_kernel(TreeArgs a) {
   constexpr int TM = 16 * NT;
-  constexpr float kUnit = 4096.0f;  // the rows' scale in f16
-  __shared__ __attribute__((aligned(16))) TreeSmem<NT> sm;
+  constexpr int CT = 8 / NW;              // column tiles of a wave
+  constexpr int RW = TM / NW;             // rows of a wave in step 1
+  constexpr float kUnit = 4096.0f;        // the rows' scale in f16
+  __shared__ __attribute__((aligned(16))) TreeSmem<NT, NW> sm;
   const int T = a.T, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, G = lane >> 4;
   const int b = blockIdx.x / a.Hv, h = blockIdx.x - b * a.Hv, kh = h / (a.Hv / a.Hk);
   const int QKV = (2 * a.Hk + a.Hv) * D;
+  const int col = CT * (16 * w + i);      // this lane's first column
 
-  // The state, lane (i, G): rows 32 s + 8 G + e of its two columns.
-  const float2* S0 = reinterpret_cast<const float2*>(a.state + ((size_t)b * a.Hv + h) * D * D + 32 * w + 2 * i) +
-                     (size_t)(8 * G) * (D / 2);
-  float2 s0[4][8];
+  // Loads return in order: what is needed first goes first, the state last.
+  const int parent = npn::tree_parent(a.parent + (size_t)b * T, T, lane);
+  constexpr int kGates = NW - 1;          // the wave that has the gates
+  float in_a = 0.f, in_b = 0.f, in_log = 0.f, in_dt = 0.f;
+  if (w == kGates) {
+    const size_t gi = ((size_t)b * T + min(lane, T - 1)) * a.Hv + h;
+    in_a = a.a_out[gi];
+    in_b = a.b_out[gi];
+    in_log = a.A_log[h];
+    in_dt = a.dt_bias[h];
+  }
+  uint32_t raw[3][RW];                    // node w + NW k's inputs of two channels, q, k, v; then what they become
+  float v1[RW];
+  float4 wt[3][2];
+  float2 bias[3];
+  uint32_t old[3][3];                     // conv_state's, one to three back from the first node
+#pragma unroll
+  for (int which = 0; which < 3; ++which) {
+    const int c = (which == 0 ? kh : which == 1 ? a.Hk + kh : 2 * a.Hk + h) * D + 2 * lane;
+    const uint16_t* xb = a.mixed_qkv + (size_t)b * T * QKV + c;
+#pragma unroll
+    for (int k = 0; k < RW; ++k)
+      raw[which][k] = *reinterpret_cast<const uint32_t*>(xb + (size_t)min(w + NW * k, T - 1) * QKV);
+    wt[which][0] = *reinterpret_cast<const float4*>(a.conv_weight + 4 * c);
+    wt[which][1] = *reinterpret_cast<const float4*>(a.conv_weight + 4 * c + 4);
+    bias[which] = make_float2(a.conv_bias[c], a.conv_bias[c + 1]);
+    const uint16_t* cs = a.conv_state + ((size_t)b * QKV + c) * 3;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) old[which][j] = cs[2 - j] | ((uint32_t)cs[5 - j] << 16);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  // The state, lane (i, G): rows 32 s + 8 G + e of its columns.
+  const Floats<CT>* S0 = reinterpret_cast<const Floats<CT>*>(a.state + ((size_t)b * a.Hv + h) * D * D +
+                                                             (size_t)(8 * G) * D + col);
+  Floats<CT> s0[4][8];
 #pragma unroll
   for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s0[s][e] = S0[(32 * s + e) * (D / 2)];
+    for (int e = 0; e < 8; ++e) s0[s][e] = S0[(32 * s + e) * (D / CT)];
+  __builtin_amdgcn_sched_barrier(0);
 
   // Lane t: node t's inputs one to three back, a node or -1 .. -3 for the last to the first of conv_state.
-  const int parent = npn::tree_parent(a.parent + (size_t)b * T, T, lane);
   int tap[3];
   {
     int at = lane;
@@ -125,23 +179,25 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) void dn_tree_ve
       tap[j] = at;
     }
   }
+  // 1. A node's inputs wait in the places that its row's low parts, or the row of v, will have.
+  auto place = [&](int which, int t) {
+    return which == 2 ? reinterpret_cast<uint32_t*>(&sm.v[t][2 * lane])
+                      : reinterpret_cast<uint32_t*>(&sm.x[1][which == 0 ? TM + t : t][2 * lane]);
+  };
+#pragma unroll
+  for (int which = 0; which < 3; ++which)
+#pragma unroll
+    for (int k = 0; k < RW; ++k) *place(which, w + NW * k) = raw[which][k];
   uint64_t bad_kv = 0, bad_q = 0;  // wave-uniform
-  if (w == 0) {
-    float beta = 0.f;
-    double g = 0.0;
-    bool bad = false;
-    if (lane < T) {
-      const size_t gi = ((size_t)b * T + lane) * a.Hv + h;
-      const float gf = -__expf(a.A_log[h]) * npn::softplus(a.a_out[gi] + a.dt_bias[h]);
-      a.rec_decay[gi] = __expf(gf);
-      beta = npn::sigmoid(a.b_out[gi]);
-      bad = gf != gf || beta != beta;
-      g = bad ? 0.0 : (double)fmaxf(gf, -256.0f) * 1.4426950408889634;
-      beta = bad ? 0.f : beta;
-    }
-    bad_kv = __builtin_amdgcn_ballot_w64(bad);
+  if (w == kGates) {
+    const float gf = -__expf(in_log) * npn::softplus(in_a + in_dt);
+    float beta = npn::sigmoid(in_b);
+    if (lane < T) a.rec_decay[((size_t)b * T + lane) * a.Hv + h] = __expf(gf);
+    const bool bad = gf != gf || beta != beta;
+    bad_kv = __builtin_amdgcn_ballot_w64(bad && lane < T);
+    beta = bad || lane >= T ? 0.f : beta;
+    double total = bad || lane >= T ? 0.0 : (double)fmaxf(gf, -256.0f) * 1.4426950408889634;
     const uint64_t anc = npn::tree_ancestors(parent, T, lane);
-    double total = g;
     int up = parent;
     for (int n = 1; n < T; n <<= 1) {
       const int from = up < 0 ? lane : up;
@@ -160,69 +216,59 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) void dn_tree_ve
     }
     if (lane == 0) sm.bad_u = 0;
   }
-
-  // 1. rows q, k, v (0, 1, 2), node t = w + 4 n, four of them in flight
+  __syncthreads();
 #pragma unroll
-  for (int which = 0; which < 3; ++which) {
-    const int c = (which == 0 ? kh : which == 1 ? a.Hk + kh : 2 * a.Hk + h) * D + 2 * lane;
-    const float4 w0 = *reinterpret_cast<const float4*>(a.conv_weight + 4 * c);
-    const float4 w1 = *reinterpret_cast<const float4*>(a.conv_weight + 4 * c + 4);
-    const float2 bias = make_float2(a.conv_bias[c], a.conv_bias[c + 1]);
-    const uint16_t* cs = a.conv_state + ((size_t)b * QKV + c) * 3;
-    uint32_t old[3];  // both channels' inputs one to three back from the first
+  for (int k = 0; k < RW; ++k) {
+    const int t = w + NW * k;
+    const bool in = t < T;
 #pragma unroll
-    for (int j = 0; j < 3; ++j) old[j] = cs[2 - j] | ((uint32_t)cs[5 - j] << 16);
-    const uint16_t* xb = a.mixed_qkv + (size_t)b * T * QKV + c;
-    for (int t0 = w; t0 < TM; t0 += 16) {
-      uint32_t x[4][4];
+    for (int which = 0; which < 3; ++which) {
+      uint32_t x[3];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int t = min(t0 + 4 * k, T - 1);
-        x[k][0] = *reinterpret_cast<const uint32_t*>(xb + (size_t)t * QKV);
-#pragma unroll
-        for (int j = 0; j < 3; ++j) {
-          const int at = __builtin_amdgcn_readlane(tap[j], t);
-          x[k][j + 1] = *reinterpret_cast<const uint32_t*>(xb + (size_t)max(at, 0) * QKV);
-          x[k][j + 1] = at >= 0 ? x[k][j + 1] : at == -1 ? old[0] : at == -2 ? old[1] : old[2];
-        }
+      for (int j = 0; j < 3; ++j) {
+        const int at = __builtin_amdgcn_readlane(tap[j], t);
+        x[j] = *place(which, max(at, 0));
+        x[j] = at >= 0 ? x[j] : at == -1 ? old[which][0] : at == -2 ? old[which][1] : old[which][2];
       }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int t = t0 + 4 * k;
-        float y0 = bias.x, y1 = bias.y;
-        y0 += w0.x * npn::bf16lo(x[k][3]) + w0.y * npn::bf16lo(x[k][2]) + w0.z * npn::bf16lo(x[k][1]) +
-              w0.w * npn::bf16lo(x[k][0]);
-        y1 += w1.x * npn::bf16hi(x[k][3]) + w1.y * npn::bf16hi(x[k][2]) + w1.z * npn::bf16hi(x[k][1]) +
-              w1.w * npn::bf16hi(x[k][0]);
-        y0 = npn::silu(y0);
-        y1 = npn::silu(y1);
-        const bool in = t < T, bad = in && __builtin_amdgcn_ballot_w64(!finite(y0) || !finite(y1)) != 0;
-        if (which < 2) {
-          const float ss = npn::wave_sum(y0 * y0 + y1 * y1);
-          const float n = rsqrtf(ss + kEps) * (which == 0 ? 0.08838834764831845f : 1.0f);  // q: / sqrt(128)
-          y0 *= n;
-          y1 *= n;
-          if (which == 1 && in && h == kh * (a.Hv / a.Hk))
-            *reinterpret_cast<float2*>(a.rec_k + (((size_t)b * T + t) * a.Hk + kh) * D + 2 * lane) = make_float2(y0, y1);
-        }
-        if (!in || bad) y0 = y1 = 0.f;
-        if (bad && which == 0) bad_q |= 1ull << t;
-        if (bad && which != 0) bad_kv |= 1ull << t;
-        if (which < 2) {
-          const f16x2 hi = {(_Float16)(y0 * kUnit), (_Float16)(y1 * kUnit)};
-          const f16x2 lo = {(_Float16)(y0 * kUnit - (float)hi[0]), (_Float16)(y1 * kUnit - (float)hi[1])};
-          const int row = which == 0 ? TM + t : t;
-          *reinterpret_cast<f16x2*>(&sm.x[0][row][2 * lane]) = hi;
-          *reinterpret_cast<f16x2*>(&sm.x[1][row][2 * lane]) = lo;
-        } else {
-          *reinterpret_cast<float2*>(&sm.v[t][2 * lane]) = make_float2(y0, y1);
-        }
+      const float4 w0 = wt[which][0], w1 = wt[which][1];
+      float y0 = bias[which].x + w0.x * npn::bf16lo(x[2]) + w0.y * npn::bf16lo(x[1]) + w0.z * npn::bf16lo(x[0]) +
+                 w0.w * npn::bf16lo(raw[which][k]);
+      float y1 = bias[which].y + w1.x * npn::bf16hi(x[2]) + w1.y * npn::bf16hi(x[1]) + w1.z * npn::bf16hi(x[0]) +
+                 w1.w * npn::bf16hi(raw[which][k]);
+      y0 = npn::silu_bf16(y0);  // (its 2 ulp)
+      y1 = npn::silu_bf16(y1);
+      const bool bad = in && __builtin_amdgcn_ballot_w64(!finite(y0) || !finite(y1)) != 0;
+      if (which < 2) {
+        const float n = rsqrtf(wave_sum(y0 * y0 + y1 * y1) + kEps) * (which == 0 ? 0.08838834764831845f : 1.0f);
+        y0 *= n;  // q: / sqrt(128)
+        y1 *= n;
+        if (which == 1 && in && h == kh * (a.Hv / a.Hk))
+          *reinterpret_cast<float2*>(a.rec_k + (((size_t)b * T + t) * a.Hk + kh) * D + 2 * lane) = make_float2(y0, y1);
+      }
+      if (!in || bad) y0 = y1 = 0.f;
+      if (bad && which == 0) bad_q |= 1ull << t;
+      if (bad && which != 0) bad_kv |= 1ull << t;
+      if (which < 2) {
+        const f16x2 hi = {(_Float16)(y0 * kUnit), (_Float16)(y1 * kUnit)};
+        const f16x2 lo = {(_Float16)(y0 * kUnit - (float)hi[0]), (_Float16)(y1 * kUnit - (float)hi[1])};
+        *reinterpret_cast<f16x2*>(&sm.x[0][which == 0 ? TM + t : t][2 * lane]) = hi;
+        raw[which][k] = __builtin_bit_cast(uint32_t, lo);
+      } else {
+        raw[2][k] = __float_as_uint(y0);
+        v1[k] = y1;
       }
     }
   }
   if (lane == 0) {
     sm.bad_kv[w] = bad_kv;
     sm.bad_q[w] = bad_q;
+  }
+  __syncthreads();  // the inputs have been read
+#pragma unroll
+  for (int k = 0; k < RW; ++k) {
+    *place(0, w + NW * k) = raw[0][k];
+    *place(1, w + NW * k) = raw[1][k];
+    *reinterpret_cast<float2*>(place(2, w + NW * k)) = make_float2(__uint_as_float(raw[2][k]), v1[k]);
   }
   __syncthreads();
 
@@ -237,7 +283,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) void dn_tree_ve
     for (int ts = 0; ts <= ta; ++ts)
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        if ((turn++ & 3) != w) continue;
+        if ((turn++ & (NW - 1)) != w) continue;
         f32x4 p = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
@@ -258,44 +304,40 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) void dn_tree_ve
         }
       }
   // and the state's
-  float inv_scale[2];
-  f32x4 ks[NT][2], qs[NT][2];
+  float inv_scale[CT];
+  f32x4 ks[NT][CT], qs[NT][CT];
   {
-    float scale[2], big[2] = {0.f, 0.f};
+    float scale[CT], big[CT];
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+    for (int c = 0; c < CT; ++c) {
+      big[c] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        big[0] = fmaxf(big[0], fabsf(s0[s][e].x));
-        big[1] = fmaxf(big[1], fabsf(s0[s][e].y));
-      }
+      for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+        for (int e = 0; e < 8; ++e) big[c] = fmaxf(big[c], fabsf(s0[s][e].x[c]));
       // to [2^11, 2^12); of a column that is not finite some product is not either
       const uint32_t e = min(max(__float_as_uint(max_over_groups(big[c])) >> 23, 12u), 254u);
       scale[c] = __uint_as_float((265u - e) << 23);
       inv_scale[c] = __uint_as_float((e - 11u) << 23) * (1.0f / kUnit);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) ks[n][c] = qs[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) ks[n][c] = qs[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
     for (int s = 0; s < 4; ++s) {
-      f16x8 hi[2], lo[2];
+      f16x8 hi[CT], lo[CT];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x0 = s0[s][e].x * scale[0], x1 = s0[s][e].y * scale[1];
-        hi[0][e] = (_Float16)x0;
-        hi[1][e] = (_Float16)x1;
-        lo[0][e] = (_Float16)(x0 - (float)hi[0][e]);
-        lo[1][e] = (_Float16)(x1 - (float)hi[1][e]);
-      }
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x = s0[s][e].x[c] * scale[c];
+          hi[c][e] = (_Float16)x;
+          lo[c][e] = (_Float16)(x - (float)hi[c][e]);
+        }
 #pragma unroll
       for (int n = 0; n < 2 * NT; ++n) {
         const f16x8 xh = rows_of(0, n, s), xl = rows_of(1, n, s);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < CT; ++c) {
           f32x4& p = n < NT ? ks[n % NT][c] : qs[n % NT][c];
           p = mfma_f16(xl, hi[c], p);
           p = mfma_f16(xh, lo[c], p);
@@ -304,6 +346,16 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) void dn_tree_ve
       }
     }
   }
+  // z is on its way by the time it is needed.
+  const size_t node0 = ((size_t)b * T * a.Hv + h) * D + col;  // row t: t * Hv * 128 behind
+  uint32_t z[NT][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint16_t* p = a.z + node0 + (size_t)min(16 * n + 4 * G + r, T - 1) * a.Hv * D;
+      z[n][r] = CT == 2 ? *reinterpret_cast<const uint32_t*>(p) : *p;
+    }
   __syncthreads();
 
   // 3. column i of the inverse of block w
@@ -322,40 +374,42 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) void dn_tree_ve
 
   // 4.
   // Rows' entries that are not finite count as 0 from here on, and their nodes as bad.
-  auto clear = [&](f32x4 (&x)[2], int tile) {
+  auto clear = [&](f32x4 (&x)[CT], int tile) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const bool bad = !finite(x[0][r]) || !finite(x[1][r]);
-      const uint64_t lanes = __builtin_amdgcn_ballot_w64(bad);
-      if (lanes == 0) continue;
+      bool bad = false;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) bad |= !finite(x[c][r]);
+      if (__builtin_amdgcn_ballot_w64(bad) == 0) continue;
       if (bad) {
-        x[0][r] = x[1][r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < CT; ++c) x[c][r] = 0.f;
         atomicOr(&sm.bad_u, 1ull << (16 * tile + 4 * G + r));
       }
     }
   };
-  f32x4 u[NT][2];
+  f32x4 u[NT][CT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    f32x4 rhs[2];
+    f32x4 rhs[CT];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * n + 4 * G + r;
-      const float2 v = *reinterpret_cast<const float2*>(&sm.v[t][32 * w + 2 * i]);
+      const Floats<CT> v = *reinterpret_cast<const Floats<CT>*>(&sm.v[t][col]);
       const float begun = sm.begun[t], beta = sm.beta[t];
-      rhs[0][r] = beta * (v.x - begun * (ks[n][0][r] * inv_scale[0]));
-      rhs[1][r] = beta * (v.y - begun * (ks[n][1][r] * inv_scale[1]));
+#pragma unroll
+      for (int c = 0; c < CT; ++c) rhs[c][r] = beta * (v.x[c] - begun * (ks[n][c][r] * inv_scale[c]));
     }
 #pragma unroll
     for (int s = 0; s < n; ++s) {
       const float4 f = *reinterpret_cast<const float4*>(&sm.low[16 * n + i][16 * s + 4 * G]);
-      rhs[0] = mfma_f32(f, u[s][0], rhs[0]);
-      rhs[1] = mfma_f32(f, u[s][1], rhs[1]);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) rhs[c] = mfma_f32(f, u[s][c], rhs[c]);
     }
     clear(rhs, n);
     const float4 f = *reinterpret_cast<const float4*>(&sm.inv[n][i][4 * G]);
-    u[n][0] = mfma_f32(f, rhs[0], f32x4{0.f, 0.f, 0.f, 0.f});
-    u[n][1] = mfma_f32(f, rhs[1], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+    for (int c = 0; c < CT; ++c) u[n][c] = mfma_f32(f, rhs[c], f32x4{0.f, 0.f, 0.f, 0.f});
     clear(u[n], n);
   }
 #pragma unroll
@@ -363,48 +417,57 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : NT == 2 ? 2 : 1) void dn_tree_ve
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float begun = sm.begun[16 * n + 4 * G + r];
-      qs[n][0][r] *= begun * inv_scale[0];
-      qs[n][1][r] *= begun * inv_scale[1];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) qs[n][c][r] *= begun * inv_scale[c];
     }
 #pragma unroll
     for (int s = 0; s <= n; ++s) {
       const float4 f = *reinterpret_cast<const float4*>(&sm.mix[16 * n + i][16 * s + 4 * G]);
-      qs[n][0] = mfma_f32(f, u[s][0], qs[n][0]);
-      qs[n][1] = mfma_f32(f, u[s][1], qs[n][1]);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) qs[n][c] = mfma_f32(f, u[s][c], qs[n][c]);
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      float ss = qs[n][0][r] * qs[n][0][r] + qs[n][1][r] * qs[n][1][r];
+      float ss = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t bits = __float_as_uint(ss);
-        ss += __uint_as_float(k == 0 ? npn::dpp32<npn::kDppStep[0]>(bits) : k == 1 ? npn::dpp32<npn::kDppStep[1]>(bits)
-                              : k == 2 ? npn::dpp32<npn::kDppStep[2]>(bits) : npn::dpp32<npn::kDppStep[3]>(bits));
-      }
+      for (int c = 0; c < CT; ++c) ss += qs[n][c][r] * qs[n][c][r];
+      ss = row_sum(ss);
       if (i == 0) sm.ss[w][16 * n + 4 * G + r] = ss;
     }
   }
   __syncthreads();
 
   // 5.
-  const uint64_t kv = sm.bad_kv[0] | sm.bad_kv[1] | sm.bad_kv[2] | sm.bad_kv[3] | sm.bad_u;
-  const uint64_t bq = sm.bad_q[0] | sm.bad_q[1] | sm.bad_q[2] | sm.bad_q[3];
-  const float2 nw = *reinterpret_cast<const float2*>(a.norm_weight + 32 * w + 2 * i);
+  uint64_t kv = sm.bad_u, bq = 0;
+#pragma unroll
+  for (int k = 0; k < NW; ++k) {
+    kv |= sm.bad_kv[k];
+    bq |= sm.bad_q[k];
+  }
+  const Floats<CT> nw = *reinterpret_cast<const Floats<CT>*>(a.norm_weight + col);
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * n + 4 * G + r;
       if (t >= T) continue;
-      const size_t at = (((size_t)b * T + t) * a.Hv + h) * D + 32 * w + 2 * i;
+      const size_t at = node0 + (size_t)t * a.Hv * D;
       const bool nan = (sm.anc[t] & kv) != 0;
-      const float ss = (sm.ss[0][t] + sm.ss[1][t]) + (sm.ss[2][t] + sm.ss[3][t]);
+      float ss = 0.f;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) ss += sm.ss[k][t];
       const float f = nan || (bq >> t & 1) ? NAN : rsqrtf(ss * (1.0f / D) + kEps);
-      const uint32_t z = *reinterpret_cast<const uint32_t*>(a.z + at);
-      const float o0 = qs[n][0][r] * f * nw.x * npn::silu(npn::bf16lo(z));
-      const float o1 = qs[n][1][r] * f * nw.y * npn::silu(npn::bf16hi(z));
-      *reinterpret_cast<uint32_t*>(a.out + at) = npn::f32_to_bf16(o0) | ((uint32_t)npn::f32_to_bf16(o1) << 16);
-      *reinterpret_cast<float2*>(a.rec_u + at) = nan ? make_float2(NAN, NAN) : make_float2(u[n][0][r], u[n][1][r]);
+      Floats<CT> rec;
+      uint32_t o = 0;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const float y = qs[n][c][r] * f * nw.x[c] * npn::silu_bf16(c == 0 ? npn::bf16lo(z[n][r]) : npn::bf16hi(z[n][r]));
+        o |= (uint32_t)npn::f32_to_bf16(y) << (16 * c);
+        rec.x[c] = nan ? NAN : u[n][c][r];
+      }
+      if constexpr (CT == 2) *reinterpret_cast<uint32_t*>(a.out + at) = o;
+      else a.out[at] = (uint16_t)o;
+      *reinterpret_cast<Floats<CT>*>(a.rec_u + at) = rec;
     }
 }
 
@@ -502,12 +565,12 @@ extern "C" int npn_deltanet_verify_tree(const float* state, const int32_t* paren
   float* rec_decay = rec_u + (size_t)B * T * v_heads * D;
   const TreeArgs a{state, parent, mixed_qkv, conv_state, conv_weight, conv_bias, a_out, b_out, z, A_log,
                    dt_bias, norm_weight, out, records, rec_u, rec_decay, B, T, k_heads, v_heads};
-  const dim3 grid(B * v_heads), block(256);
+  const dim3 grid(B * v_heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (T <= 16) hipLaunchKernelGGL(dn_tree_verify_kernel<1>, grid, block, 0, s, a);
-  else if (T <= 32) hipLaunchKernelGGL(dn_tree_verify_kernel<2>, grid, block, 0, s, a);
-  else if (T <= 48) hipLaunchKernelGGL(dn_tree_verify_kernel<3>, grid, block, 0, s, a);
-  else hipLaunchKernelGGL(dn_tree_verify_kernel<4>, grid, block, 0, s, a);
+  if (T <= 16) hipLaunchKernelGGL((dn_tree_verify_kernel<1, 4>), grid, dim3(256), 0, s, a);
+  else if (T <= 32) hipLaunchKernelGGL((dn_tree_verify_kernel<2, 8>), grid, dim3(512), 0, s, a);
+  else if (T <= 48) hipLaunchKernelGGL((dn_tree_verify_kernel<3, 8>), grid, dim3(512), 0, s, a);
+  else hipLaunchKernelGGL((dn_tree_verify_kernel<4, 8>), grid, dim3(512), 0, s, a);
   return npn_launch_status();
 }
 
