@@ -66,14 +66,19 @@ struct TreeSmem {
   float v[TM][D + 4];
   float low[TM][TM + 4], mix[TM][TM + 4];
   float inv[NT][16][20];
+  float begun[TM], beta[TM], ss[NW][TM];
   double g[TM];  // sums of g along a node's line, base 2
   uint64_t anc[TM];
   uint64_t bad_kv[NW], bad_q[NW];  // by wave
   unsigned long long bad_u;
-  float begun[TM], beta[TM], ss[NW][TM];
+  uint32_t old[3][3][64];        // conv_state's inputs of q, k, v, one to three back from the first node
 };
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+// x sigmoid(x) to 2 ulp: the reciprocal's one and the product's. (0 where e^-x overflows.)
+__device__ __forceinline__ float silu(float x) {
+  return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
+}
 
 // Maximum over the lanes (i, G) of a column i.
 __device__ __forceinline__ float max_over_groups(float x) {
@@ -138,8 +143,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
     in_log = a.A_log[h];
     in_dt = a.dt_bias[h];
   }
-  uint32_t raw[3][RW];                    // node w + NW k's inputs of two channels, q, k, v; then what they become
-  float v1[RW];
+  uint32_t raw[3][RW];                    // node w + NW k's inputs of two channels, q, k, v
   float4 wt[3][2];
   float2 bias[3];
   uint32_t old[3][3];                     // conv_state's, one to three back from the first node
@@ -153,9 +157,9 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
     wt[which][0] = *reinterpret_cast<const float4*>(a.conv_weight + 4 * c);
     wt[which][1] = *reinterpret_cast<const float4*>(a.conv_weight + 4 * c + 4);
     bias[which] = make_float2(a.conv_bias[c], a.conv_bias[c + 1]);
-    const uint16_t* cs = a.conv_state + ((size_t)b * QKV + c) * 3;
+    const uint32_t* cs = reinterpret_cast<const uint32_t*>(a.conv_state + ((size_t)b * QKV + c) * 3);
 #pragma unroll
-    for (int j = 0; j < 3; ++j) old[which][j] = cs[2 - j] | ((uint32_t)cs[5 - j] << 16);
+    for (int j = 0; j < 3; ++j) old[which][j] = cs[j];
   }
   __builtin_amdgcn_sched_barrier(0);
   // The state, lane (i, G): rows 32 s + 8 G + e of its columns.
@@ -179,6 +183,19 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
       tap[j] = at;
     }
   }
+#pragma unroll
+  for (int which = 0; which < 3; ++which) {  // [c0 c0][c0 c1][c1 c1], oldest first, to a word a step back
+    const uint32_t x = old[which][0], y = old[which][1], v = old[which][2];
+    old[which][0] = (y & 0xFFFFu) | (v & 0xFFFF0000u);
+    old[which][1] = (x >> 16) | (v << 16);
+    old[which][2] = (x & 0xFFFFu) | (y & 0xFFFF0000u);
+  }
+  if (w == 0) {
+#pragma unroll
+    for (int which = 0; which < 3; ++which)
+#pragma unroll
+      for (int j = 0; j < 3; ++j) sm.old[which][j][lane] = old[which][j];
+  }
   // 1. A node's inputs wait in the places that its row's low parts, or the row of v, will have.
   auto place = [&](int which, int t) {
     return which == 2 ? reinterpret_cast<uint32_t*>(&sm.v[t][2 * lane])
@@ -197,17 +214,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
     bad_kv = __builtin_amdgcn_ballot_w64(bad && lane < T);
     beta = bad || lane >= T ? 0.f : beta;
     double total = bad || lane >= T ? 0.0 : (double)fmaxf(gf, -256.0f) * 1.4426950408889634;
-    const uint64_t anc = npn::tree_ancestors(parent, T, lane);
-    int up = parent;
-    for (int n = 1; n < T; n <<= 1) {
-      const int from = up < 0 ? lane : up;
-      const uint64_t bits = (uint64_t)__double_as_longlong(total);
-      const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)bits, from, 64);
-      const uint32_t hi = (uint32_t)__shfl((int)(uint32_t)(bits >> 32), from, 64);
-      const int next = __shfl(up, from, 64);
-      total += up < 0 ? 0.0 : __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
-      up = up < 0 ? up : next;
-    }
+    const uint64_t anc = npn::tree_ancestors(parent, T, lane, total);
     if (lane < TM) {
       sm.anc[lane] = anc;
       sm.beta[lane] = beta;
@@ -217,47 +224,53 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
     if (lane == 0) sm.bad_u = 0;
   }
   __syncthreads();
+  float y[3][RW][2];
+#pragma unroll
+  for (int k = 0; k < RW; ++k) {
+    const int t = w + NW * k;
+    int at[3];
+#pragma unroll
+    for (int j = 0; j < 3; ++j) at[j] = __builtin_amdgcn_readlane(tap[j], t);
+#pragma unroll
+    for (int which = 0; which < 3; ++which) {
+      uint32_t x[3];
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        x[j] = at[j] >= 0 ? *place(which, at[j]) : sm.old[which][-1 - at[j]][lane];
+      }
+      const float4 w0 = wt[which][0], w1 = wt[which][1];
+      const float y0 = bias[which].x + w0.x * npn::bf16lo(x[2]) + w0.y * npn::bf16lo(x[1]) +
+                       w0.z * npn::bf16lo(x[0]) + w0.w * npn::bf16lo(raw[which][k]);
+      const float y1 = bias[which].y + w1.x * npn::bf16hi(x[2]) + w1.y * npn::bf16hi(x[1]) +
+                       w1.z * npn::bf16hi(x[0]) + w1.w * npn::bf16hi(raw[which][k]);
+      y[which][k][0] = silu(y0);
+      y[which][k][1] = silu(y1);
+    }
+  }
 #pragma unroll
   for (int k = 0; k < RW; ++k) {
     const int t = w + NW * k;
     const bool in = t < T;
 #pragma unroll
     for (int which = 0; which < 3; ++which) {
-      uint32_t x[3];
-#pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        const int at = __builtin_amdgcn_readlane(tap[j], t);
-        x[j] = *place(which, max(at, 0));
-        x[j] = at >= 0 ? x[j] : at == -1 ? old[which][0] : at == -2 ? old[which][1] : old[which][2];
-      }
-      const float4 w0 = wt[which][0], w1 = wt[which][1];
-      float y0 = bias[which].x + w0.x * npn::bf16lo(x[2]) + w0.y * npn::bf16lo(x[1]) + w0.z * npn::bf16lo(x[0]) +
-                 w0.w * npn::bf16lo(raw[which][k]);
-      float y1 = bias[which].y + w1.x * npn::bf16hi(x[2]) + w1.y * npn::bf16hi(x[1]) + w1.z * npn::bf16hi(x[0]) +
-                 w1.w * npn::bf16hi(raw[which][k]);
-      y0 = npn::silu_bf16(y0);  // (its 2 ulp)
-      y1 = npn::silu_bf16(y1);
-      const bool bad = in && __builtin_amdgcn_ballot_w64(!finite(y0) || !finite(y1)) != 0;
+      float &y0 = y[which][k][0], &y1 = y[which][k][1];
+      const float none = fmaf(y0, 0.f, y1 * 0.f);  // NaN if one is not finite
+      const bool bad = in && __builtin_amdgcn_ballot_w64(none != none) != 0;
+      (which == 0 ? bad_q : bad_kv) |= bad ? 1ull << t : 0ull;
       if (which < 2) {
-        const float n = rsqrtf(wave_sum(y0 * y0 + y1 * y1) + kEps) * (which == 0 ? 0.08838834764831845f : 1.0f);
-        y0 *= n;  // q: / sqrt(128)
+        const float n = __builtin_amdgcn_rsqf(wave_sum(y0 * y0 + y1 * y1) + kEps) *
+                        (which == 0 ? 0.08838834764831845f * kUnit : kUnit);  // q: / sqrt(128)
+        y0 *= n;
         y1 *= n;
-        if (which == 1 && in && h == kh * (a.Hv / a.Hk))
-          *reinterpret_cast<float2*>(a.rec_k + (((size_t)b * T + t) * a.Hk + kh) * D + 2 * lane) = make_float2(y0, y1);
-      }
-      if (!in || bad) y0 = y1 = 0.f;
-      if (bad && which == 0) bad_q |= 1ull << t;
-      if (bad && which != 0) bad_kv |= 1ull << t;
-      if (which < 2) {
-        const f16x2 hi = {(_Float16)(y0 * kUnit), (_Float16)(y1 * kUnit)};
-        const f16x2 lo = {(_Float16)(y0 * kUnit - (float)hi[0]), (_Float16)(y1 * kUnit - (float)hi[1])};
-        *reinterpret_cast<f16x2*>(&sm.x[0][which == 0 ? TM + t : t][2 * lane]) = hi;
-        raw[which][k] = __builtin_bit_cast(uint32_t, lo);
-      } else {
-        raw[2][k] = __float_as_uint(y0);
-        v1[k] = y1;
       }
     }
+  }
+  if (h == kh * (a.Hv / a.Hk)) {
+#pragma unroll
+    for (int k = 0; k < RW; ++k)
+      if (w + NW * k < T)
+        *reinterpret_cast<float2*>(a.rec_k + (((size_t)b * T + w + NW * k) * a.Hk + kh) * D + 2 * lane) =
+            make_float2(y[1][k][0] * (1.0f / kUnit), y[1][k][1] * (1.0f / kUnit));
   }
   if (lane == 0) {
     sm.bad_kv[w] = bad_kv;
@@ -266,9 +279,20 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
   __syncthreads();  // the inputs have been read
 #pragma unroll
   for (int k = 0; k < RW; ++k) {
-    *place(0, w + NW * k) = raw[0][k];
-    *place(1, w + NW * k) = raw[1][k];
-    *reinterpret_cast<float2*>(place(2, w + NW * k)) = make_float2(__uint_as_float(raw[2][k]), v1[k]);
+    const int t = w + NW * k;
+#pragma unroll
+    for (int which = 0; which < 3; ++which) {
+      const bool none = t >= T || ((which == 0 ? bad_q : bad_kv) >> t & 1);
+      const float y0 = none ? 0.f : y[which][k][0], y1 = none ? 0.f : y[which][k][1];
+      if (which < 2) {
+        const f16x2 hi = {(_Float16)y0, (_Float16)y1};
+        const f16x2 lo = {(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])};
+        *reinterpret_cast<f16x2*>(&sm.x[0][which == 0 ? TM + t : t][2 * lane]) = hi;
+        *reinterpret_cast<f16x2*>(place(which, t)) = lo;
+      } else {
+        *reinterpret_cast<float2*>(place(2, t)) = make_float2(y0, y1);
+      }
+    }
   }
   __syncthreads();
 
@@ -356,6 +380,21 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
       const uint16_t* p = a.z + node0 + (size_t)min(16 * n + 4 * G + r, T - 1) * a.Hv * D;
       z[n][r] = CT == 2 ? *reinterpret_cast<const uint32_t*>(p) : *p;
     }
+  const Floats<CT> nw = *reinterpret_cast<const Floats<CT>*>(a.norm_weight + col);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const f32x4 begun = *reinterpret_cast<const f32x4*>(&sm.begun[16 * n + 4 * G]);
+    const f32x4 beta = *reinterpret_cast<const f32x4*>(&sm.beta[16 * n + 4 * G]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const Floats<CT> v = *reinterpret_cast<const Floats<CT>*>(&sm.v[16 * n + 4 * G + r][col]);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        ks[n][c][r] = beta[r] * (v.x[c] - begun[r] * (ks[n][c][r] * inv_scale[c]));
+        qs[n][c][r] *= begun[r] * inv_scale[c];
+      }
+    }
+  }
   __syncthreads();
 
   // 3. column i of the inverse of block w
@@ -375,12 +414,17 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
   // 4.
   // Rows' entries that are not finite count as 0 from here on, and their nodes as bad.
   auto clear = [&](f32x4 (&x)[CT], int tile) {
+    float none = 0.f;  // NaN from the first that is not finite
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) none = fmaf(x[c][r], 0.f, none);
+    if (__builtin_amdgcn_ballot_w64(none != none) == 0) return;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       bool bad = false;
 #pragma unroll
       for (int c = 0; c < CT; ++c) bad |= !finite(x[c][r]);
-      if (__builtin_amdgcn_ballot_w64(bad) == 0) continue;
       if (bad) {
 #pragma unroll
         for (int c = 0; c < CT; ++c) x[c][r] = 0.f;
@@ -391,84 +435,82 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
   f32x4 u[NT][CT];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    f32x4 rhs[CT];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = 16 * n + 4 * G + r;
-      const Floats<CT> v = *reinterpret_cast<const Floats<CT>*>(&sm.v[t][col]);
-      const float begun = sm.begun[t], beta = sm.beta[t];
-#pragma unroll
-      for (int c = 0; c < CT; ++c) rhs[c][r] = beta * (v.x[c] - begun * (ks[n][c][r] * inv_scale[c]));
-    }
 #pragma unroll
     for (int s = 0; s < n; ++s) {
       const float4 f = *reinterpret_cast<const float4*>(&sm.low[16 * n + i][16 * s + 4 * G]);
 #pragma unroll
-      for (int c = 0; c < CT; ++c) rhs[c] = mfma_f32(f, u[s][c], rhs[c]);
+      for (int c = 0; c < CT; ++c) ks[n][c] = mfma_f32(f, u[s][c], ks[n][c]);
     }
-    clear(rhs, n);
+    clear(ks[n], n);
     const float4 f = *reinterpret_cast<const float4*>(&sm.inv[n][i][4 * G]);
 #pragma unroll
-    for (int c = 0; c < CT; ++c) u[n][c] = mfma_f32(f, rhs[c], f32x4{0.f, 0.f, 0.f, 0.f});
+    for (int c = 0; c < CT; ++c) u[n][c] = mfma_f32(f, ks[n][c], f32x4{0.f, 0.f, 0.f, 0.f});
     clear(u[n], n);
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float begun = sm.begun[16 * n + 4 * G + r];
-#pragma unroll
-      for (int c = 0; c < CT; ++c) qs[n][c][r] *= begun * inv_scale[c];
-    }
 #pragma unroll
     for (int s = 0; s <= n; ++s) {
       const float4 f = *reinterpret_cast<const float4*>(&sm.mix[16 * n + i][16 * s + 4 * G]);
 #pragma unroll
       for (int c = 0; c < CT; ++c) qs[n][c] = mfma_f32(f, u[s][c], qs[n][c]);
     }
+    f32x4 ss = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      float ss = 0.f;
 #pragma unroll
-      for (int c = 0; c < CT; ++c) ss += qs[n][c][r] * qs[n][c][r];
-      ss = row_sum(ss);
-      if (i == 0) sm.ss[w][16 * n + 4 * G + r] = ss;
+      for (int c = 0; c < CT; ++c) ss[r] += qs[n][c][r] * qs[n][c][r];
+      ss[r] = row_sum(ss[r]);
     }
+    if (i == 0) *reinterpret_cast<f32x4*>(&sm.ss[w][16 * n + 4 * G]) = ss;
   }
   __syncthreads();
 
-  // 5.
-  uint64_t kv = sm.bad_u, bq = 0;
+  // 5. A row's factor: NaN where the node or one before it is bad; of its record 0 or NaN.
+  if (tid < TM) {
+    uint64_t kv = sm.bad_u, bq = 0;
+    float ss = 0.f;
 #pragma unroll
-  for (int k = 0; k < NW; ++k) {
-    kv |= sm.bad_kv[k];
-    bq |= sm.bad_q[k];
+    for (int k = 0; k < NW; ++k) {
+      kv |= sm.bad_kv[k];
+      bq |= sm.bad_q[k];
+      ss += sm.ss[k][tid];
+    }
+    const bool nan = (sm.anc[tid] & kv) != 0;
+    sm.begun[tid] = nan || (bq >> tid & 1) ? NAN : __builtin_amdgcn_rsqf(ss * (1.0f / D) + kEps);
+    sm.beta[tid] = nan ? NAN : 0.f;
   }
-  const Floats<CT> nw = *reinterpret_cast<const Floats<CT>*>(a.norm_weight + col);
+  float gate[NT][4][CT];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+        gate[n][r][c] = nw.x[c] * silu(c == 0 ? npn::bf16lo(z[n][r]) : npn::bf16hi(z[n][r]));
+  __syncthreads();
+
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const f32x4 f = *reinterpret_cast<const f32x4*>(&sm.begun[16 * n + 4 * G]);
+    const f32x4 none = *reinterpret_cast<const f32x4*>(&sm.beta[16 * n + 4 * G]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * n + 4 * G + r;
       if (t >= T) continue;
       const size_t at = node0 + (size_t)t * a.Hv * D;
-      const bool nan = (sm.anc[t] & kv) != 0;
-      float ss = 0.f;
-#pragma unroll
-      for (int k = 0; k < NW; ++k) ss += sm.ss[k][t];
-      const float f = nan || (bq >> t & 1) ? NAN : rsqrtf(ss * (1.0f / D) + kEps);
       Floats<CT> rec;
       uint32_t o = 0;
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        const float y = qs[n][c][r] * f * nw.x[c] * npn::silu_bf16(c == 0 ? npn::bf16lo(z[n][r]) : npn::bf16hi(z[n][r]));
-        o |= (uint32_t)npn::f32_to_bf16(y) << (16 * c);
-        rec.x[c] = nan ? NAN : u[n][c][r];
+        o |= (uint32_t)npn::f32_to_bf16(qs[n][c][r] * f[r] * gate[n][r][c]) << (16 * c);
+        rec.x[c] = u[n][c][r] + none[r];
       }
       if constexpr (CT == 2) *reinterpret_cast<uint32_t*>(a.out + at) = o;
       else a.out[at] = (uint16_t)o;
       *reinterpret_cast<Floats<CT>*>(a.rec_u + at) = rec;
     }
+  }
 }
 
 // ---- commit -----------------------------------------------------------------------------------------
@@ -558,7 +600,8 @@ extern "C" int npn_deltanet_verify_tree(const float* state, const int32_t* paren
                   A_log && dt_bias && norm_weight && out && records,
               NPN_ERR_NULL);
   NPN_REQUIRE(heads_ok(B, T, k_heads, v_heads), NPN_ERR_SHAPE);
-  NPN_REQUIRE(NPN_ALIGNED16(state) && NPN_ALIGNED16(mixed_qkv) && NPN_ALIGNED16(conv_weight) &&
+  NPN_REQUIRE(NPN_ALIGNED16(state) && NPN_ALIGNED16(mixed_qkv) && NPN_ALIGNED16(conv_state) &&
+                  NPN_ALIGNED16(conv_weight) && NPN_ALIGNED16(conv_bias) && NPN_ALIGNED16(norm_weight) &&
                   NPN_ALIGNED16(z) && NPN_ALIGNED16(out) && NPN_ALIGNED16(records),
               NPN_ERR_ALIGN);
   float* rec_u = records + (size_t)B * T * k_heads * D;

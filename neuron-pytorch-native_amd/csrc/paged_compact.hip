@@ -29,11 +29,6 @@ struct CompactArgs {
   int T, Hkv, N, sh;
 };
 
-__device__ __forceinline__ int64_t shfl64(int64_t x, int from) {
-  const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)x, from, 64);
-  return (int64_t)(((uint64_t)(uint32_t)__shfl((int)(x >> 32), from, 64) << 32) | lo);
-}
-
 __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(CompactArgs a) {
   constexpr int kRows = npn::kMaxNodes, kWaves = kCompactThreads / 64;
   __shared__ uint32_t s_row[kRows][DH / 4];  // the rows that move
@@ -50,7 +45,7 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(CompactA
   const size_t at = (size_t)b * a.T + lane;
   const int node = lane < a.T ? a.path[at] : -1;
   const int64_t dst = lane < a.T ? a.slots[at] : -1;
-  const int64_t src = shfl64(dst, min(max(node, 0), a.T - 1));
+  const int64_t src = (int64_t)npn::shfl64(dst, min(max(node, 0), a.T - 1));
   const int n = npn::path_length(node, a.T, lane, dst >= 0 && dst < end && src >= 0 && src < end);
   const bool row = lane < n, moves = row && src != dst;
   const uint64_t moving = __builtin_amdgcn_ballot_w64(moves);
@@ -118,7 +113,7 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(CompactA
     }
     uint64_t left = __builtin_amdgcn_ballot_w64(row);
     while (left != 0) {  // page by page
-      const bool here = row && dst_page == shfl64(dst_page, __builtin_ctzll(left));
+      const bool here = row && dst_page == (int64_t)npn::shfl64(dst_page, __builtin_ctzll(left));
       const float top = npn::wave_max(here ? fmaxf(d_old, need) : 0.f);
       if (here) now = top;
       left &= ~__builtin_amdgcn_ballot_w64(here);
@@ -129,11 +124,11 @@ __global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(CompactA
   __syncthreads();  // rows, factors and old scales have been read
   while (grown != 0) {  // a grown page's rows up to the path's last in it move to the new scale
     const int first = __builtin_ctzll(grown);
-    const int64_t page = shfl64(dst_page, first);
+    const int64_t page = (int64_t)npn::shfl64(dst_page, first);
     const bool here = row && dst_page == page;
     const uint64_t in = __builtin_amdgcn_ballot_w64(here);
     const int last = 63 - __builtin_clzll(in);
-    const int upto = (int)(shfl64(dst, last) & (bs - 1));
+    const int upto = (int)(npn::shfl64(dst, last) & (bs - 1));
     const float by = __shfl(d_old, first, 64) / __shfl(now, first, 64);
     uint8_t* p = cache + (page * a.Hkv + h) * ((int64_t)DH << a.sh);
     if (!is_v) {

@@ -17,20 +17,29 @@ __device__ __forceinline__ int tree_parent(const int32_t* parent, int T, int lan
   return p >= 0 && p < lane ? p : -1;
 }
 
+__device__ __forceinline__ uint64_t shfl64(uint64_t x, int from) {
+  const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)x, from, kWave);
+  return ((uint64_t)(uint32_t)__shfl((int)(x >> 32), from, kWave) << 32) | lo;
+}
+
 // Node `lane` and its ancestors as bits, by pointer doubling: after k steps a lane knows 2^k nodes up and
-// the next one.
-__device__ __forceinline__ uint64_t tree_ancestors(int parent, int T, int lane) {
-  uint32_t lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
+// the next one. `sum`, the lane's number, becomes the sum over those nodes'.
+__device__ __forceinline__ uint64_t tree_ancestors(int parent, int T, int lane, double& sum) {
+  uint64_t bits = 1ull << lane;
   int up = parent;
   for (int n = 1; n < T; n <<= 1) {
     const int from = up < 0 ? lane : up;
-    const uint32_t l = (uint32_t)__shfl((int)lo, from, kWave), h = (uint32_t)__shfl((int)hi, from, kWave);
+    const uint64_t other = shfl64(bits, from), more = shfl64((uint64_t)__double_as_longlong(sum), from);
     const int next = __shfl(up, from, kWave);
-    lo |= l;
-    hi |= h;
+    bits |= other;
+    sum += up < 0 ? 0.0 : __longlong_as_double((long long)more);
     up = up < 0 ? up : next;
   }
-  return ((uint64_t)hi << 32) | lo;
+  return bits;
+}
+__device__ __forceinline__ uint64_t tree_ancestors(int parent, int T, int lane) {
+  double none = 0.0;
+  return tree_ancestors(parent, T, lane, none);
 }
 
 // Lane `from`'s bits (wave-uniform `from`).
