@@ -516,10 +516,11 @@ __global__ __launch_bounds__(kPrepWaves * 64) void tree_prep_kernel(PagedArgs a,
 // Trees: which of a lane's 16 keys a row sees, as bits: of those up to its last one, `left` from the lane's first
 // on, the committed ones and the nodes `anc`. The first is `at` places behind the committed ones.
 __device__ __forceinline__ uint32_t seen16(uint64_t anc, int at, int left) {
-  const uint32_t upto = left >= 16 ? 0xFFFFu : (left <= 0 ? 0u : (1u << left) - 1);
-  const uint32_t nodes = at >= 64 ? 0u : at >= 0 ? (uint32_t)(anc >> at)
-                         : at <= -16 ? ~0u : ((uint32_t)anc << -at) | ((1u << -at) - 1);
-  return nodes & upto;
+  // bits [at + 32, at + 48) of 32 committed keys, the nodes and nothing
+  const int s = min(max(at + 32, 0), 96), k = s >> 5;
+  const uint32_t lo = (uint32_t)anc, hi = (uint32_t)(anc >> 32);
+  const uint32_t a = k == 0 ? ~0u : k == 1 ? lo : k == 2 ? hi : 0u, b = k == 0 ? lo : k == 1 ? hi : 0u;
+  return __builtin_amdgcn_alignbit(b, a, s & 31) & (0xFFFFu >> (16 - min(max(left, 0), 16)));
 }
 // x where bit k of `bits` is set, else -inf.
 __device__ __forceinline__ float if_seen(uint32_t bits, int k, float x) {
@@ -539,6 +540,7 @@ struct PagedSmem {
   int page[kPages];                             // -1: none
   float ks[kPages], vs[kPages];                 // the keys' scales, the logarithms of the values'
   uint64_t anc[TREE ? NRT * 16 : 1];            // what a row sees of the nodes
+  int lim[TREE ? NRT * 16 : 1];
 };
 
 template <int NRT, int NW, bool TREE>
@@ -573,8 +575,12 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
   for (int nt = 0; nt < NRT; ++nt) {
     const int r = 16 * nt + i, t = a.token_of(row0 + r);
     lim[nt] = r < rows && t < a.q_len[un.b] ? min(un.kv + t, un.kend - 1) : -1;
-    if constexpr (TREE)
-      if (w == 0 && G == 0) sm.anc[r] = a.anc[(size_t)un.b * a.T + min(t, a.T - 1)];
+    if constexpr (TREE) {
+      if (w == 0 && G == 0) {
+        sm.anc[r] = a.anc[(size_t)un.b * a.T + min(t, a.T - 1)];
+        sm.lim[r] = lim[nt];
+      }
+    }
     q_scale[nt] = a.q_scale[(size_t)pair * R + r];
     m_run[nt] = kNegBig;
     w_run[nt] = kNegBig;
@@ -776,19 +782,24 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
       // A step with keys past the group's first limit, or past a page that is none, is masked.
       const bool tail = k0 + KS - 1 > lim0 || __builtin_amdgcn_ballot_w64(!held) != 0;
       auto seen = [&](int nt) {
-        return seen16(sm.anc[TREE ? 16 * nt + i : 0], k0 + 16 * G - un.kv, lim[nt] + 1 - (k0 + 16 * G));
+        const int r = TREE ? 16 * nt + i : 0, kb = k0 + 16 * G;
+        return seen16(sm.anc[r], kb - un.kv, sm.lim[r] + 1 - kb);
       };
-      uint32_t see_bits[NRT];  // trees
+      uint32_t bits[TREE ? NRT : 1];
+      if constexpr (TREE) {
+        // In every step: computed where it is needed, in the branch below, it had thirty registers spilled.
+#pragma unroll
+        for (int nt = 0; nt < NRT; ++nt) bits[nt] = held ? seen(nt) : 0u;
+      }
       if (tail) {
         const int kb = k0 + 16 * G;
 #pragma unroll
         for (int nt = 0; nt < NRT; ++nt) {
-          if constexpr (TREE) see_bits[nt] = seen(nt);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              if constexpr (TREE) st[nt][j][r] = if_seen(held ? see_bits[nt] : 0u, 4 * j + r, st[nt][j][r]);
+              if constexpr (TREE) st[nt][j][r] = if_seen(bits[nt], 4 * j + r, st[nt][j][r]);
               else if (!held || kb + 4 * j + r > lim[nt]) st[nt][j][r] = -INFINITY;
             }
         }
@@ -797,13 +808,14 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
       f16x8 pw[NRT][2];
 #pragma unroll
       for (int nt = 0; nt < NRT; ++nt) {
-        const bool hidden = tail && (TREE ? see_bits[nt] == 0 : k0 + 16 * G > lim[nt]);  // all 16 keys of the lane
-        const float c = hidden ? 1.0f : not_zero(ks * q_scale[nt]), vsn = hidden ? 0.0f : vs;
         float mx = st[nt][0][0];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r) mx = fmaxf(mx, st[nt][j][r]);
+        // All 16 keys of the lane. (Scores are not infinite; masked ones beside a NaN do no harm: it stays.)
+        const bool hidden = TREE ? mx == -INFINITY : tail && k0 + 16 * G > lim[nt];
+        const float c = hidden ? 1.0f : not_zero(ks * q_scale[nt]), vsn = hidden ? 0.0f : vs;
         mx *= c;
         const float wx = max_over_groups(mx + vsn);
         mx = max_over_groups(mx);
