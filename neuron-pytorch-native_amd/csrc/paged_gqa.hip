@@ -416,91 +416,103 @@ __device__ void plan_block(const PagedArgs& a) {
 // q' of one padded row per wave (rows that are none repeat the pair's last), over the least power of
 // two above the row's largest element. In f16 dim d = 64 c + 16 g + 8 h + e is element e of lane group
 // g in k step 2 c + h; in e4m3 parts d = 128 m + 64 x + 16 g + e is byte 16 x + e of group g in step m.
-// TREE: the row's position is its node's depth behind the committed ones.
-template <bool TREE>
-__device__ __forceinline__ void prep_row(const PagedArgs& a, const int32_t* parent, int64_t wave) {
+// A wave has RW rows in turn, whose loads go out together. TREE: a row's position is its node's depth behind the
+// committed ones.
+template <bool TREE, int RW>
+__device__ __forceinline__ void prep_rows(const PagedArgs& a, const int32_t* parent, int64_t wave) {
   const int lane = threadIdx.x & 63;
-  const int pair = (int)(wave / a.R), r = (int)(wave - (int64_t)pair * a.R);
+  const int64_t first = wave * RW;
+  const int pair = (int)(first / a.R), r0 = (int)(first - (int64_t)pair * a.R);
   if (pair >= a.units() * a.Hkv) return;
   const int u = pair / a.Hkv, h = pair - u * a.Hkv;
   const int b = u / a.RG;
-  const int row = min((u - b * a.RG) * a.R + r, a.T * a.grp - 1);
-  const int t = a.token_of(row), qh = h * a.grp + row - t * a.grp;
-  const uint2 q = *reinterpret_cast<const uint2*>(a.query + (((size_t)b * a.T + t) * a.Hq + qh) * DH + 4 * lane);
-  int behind = t;
-  if constexpr (TREE) {
-    const uint64_t anc =
-        npn::tree_ancestors(npn::tree_parent(parent + (size_t)b * a.T, a.T, lane), a.T, lane);
-    behind = __popcll(npn::tree_bits(anc, __builtin_amdgcn_readfirstlane(t))) - 1;
-    if (qh == 0 && lane == t) a.anc[(size_t)b * a.T + t] = anc;  // (rows that repeat the last write the same)
-  }
-  // The row's own position, also where the table ends before it.
-  const int64_t at = min((int64_t)max(a.kv_len[b], 0) + behind, (int64_t)a.positions - 1);
-  const size_t pos = (size_t)at * ROPE + 4 * (lane & 15);
-  const float4 c = *reinterpret_cast<const float4*>(a.cos + pos);
-  const float4 s = *reinterpret_cast<const float4*>(a.sin + pos);
+  uint64_t anc = 0;
+  if constexpr (TREE) anc = npn::tree_ancestors(npn::tree_parent(parent + (size_t)b * a.T, a.T, lane), a.T, lane);
   const float4 nw = *reinterpret_cast<const float4*>(a.q_norm + 4 * lane);
-  float v[4] = {npn::bf16lo(q.x), npn::bf16hi(q.x), npn::bf16lo(q.y), npn::bf16hi(q.y)};
-  const float ss = npn::wave_sum(v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3]);
-  const float rn = rsqrtf(ss * (1.0f / DH) + kEps);
-  v[0] = (1.0f + nw.x) * (v[0] * rn);
-  v[1] = (1.0f + nw.y) * (v[1] * rn);
-  v[2] = (1.0f + nw.z) * (v[2] * rn);
-  v[3] = (1.0f + nw.w) * (v[3] * rn);
-  float y[4];
+  uint2 q[RW];
+  float4 cs[RW], sn[RW];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) y[j] = __shfl_xor(v[j], 8, 64);  // dim d ^ 32
-  if (lane < ROPE / 4) {
-    const float sg = lane < ROPE / 8 ? -1.0f : 1.0f;
-    v[0] = v[0] * c.x + sg * y[0] * s.x;
-    v[1] = v[1] * c.y + sg * y[1] * s.y;
-    v[2] = v[2] * c.z + sg * y[2] * s.z;
-    v[3] = v[3] * c.w + sg * y[3] * s.w;
+  for (int k = 0; k < RW; ++k) {
+    const int row = min((u - b * a.RG) * a.R + r0 + k, a.T * a.grp - 1);
+    const int t = a.token_of(row), qh = h * a.grp + row - t * a.grp;
+    q[k] = *reinterpret_cast<const uint2*>(a.query + (((size_t)b * a.T + t) * a.Hq + qh) * DH + 4 * lane);
+    int behind = t;
+    if constexpr (TREE) {
+      behind = __popcll(npn::tree_bits(anc, __builtin_amdgcn_readfirstlane(t))) - 1;
+      if (qh == 0 && lane == t) a.anc[(size_t)b * a.T + t] = anc;  // (rows that repeat the last write the same)
+    }
+    // The row's own position, also where the table ends before it.
+    const int64_t at = min((int64_t)max(a.kv_len[b], 0) + behind, (int64_t)a.positions - 1);
+    const size_t pos = (size_t)at * ROPE + 4 * (lane & 15);
+    cs[k] = *reinterpret_cast<const float4*>(a.cos + pos);
+    sn[k] = *reinterpret_cast<const float4*>(a.sin + pos);
   }
-  const float big = npn::wave_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
-  const uint32_t e = min(max(__float_as_uint(big) >> 23, 64u), 190u);  // 2^-63 to 2^63
-  float inv = __uint_as_float((253u - e) << 23);                      // 2^-(e - 126)
-  float q_scale = __uint_as_float((e + 1) << 23) * (kLog2e / 16.0f);
-  const int d = 4 * lane;
-  if (a.R == kRows) {  // three e4m3 parts of 256 times as much
-    inv *= 256.0f;
-    q_scale *= 1.0f / 256;
+#pragma unroll
+  for (int k = 0; k < RW; ++k) {
+    const int r = r0 + k;
+    const float4 c = cs[k], s = sn[k];
+    float v[4] = {npn::bf16lo(q[k].x), npn::bf16hi(q[k].x), npn::bf16lo(q[k].y), npn::bf16hi(q[k].y)};
+    const float ss = npn::wave_sum(v[0] * v[0] + v[1] * v[1] + v[2] * v[2] + v[3] * v[3]);
+    const float rn = rsqrtf(ss * (1.0f / DH) + kEps);
+    v[0] = (1.0f + nw.x) * (v[0] * rn);
+    v[1] = (1.0f + nw.y) * (v[1] * rn);
+    v[2] = (1.0f + nw.z) * (v[2] * rn);
+    v[3] = (1.0f + nw.w) * (v[3] * rn);
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = __shfl_xor(v[j], 8, 64);  // dim d ^ 32
+    if (lane < ROPE / 4) {
+      const float sg = lane < ROPE / 8 ? -1.0f : 1.0f;
+      v[0] = v[0] * c.x + sg * y[0] * s.x;
+      v[1] = v[1] * c.y + sg * y[1] * s.y;
+      v[2] = v[2] * c.z + sg * y[2] * s.z;
+      v[3] = v[3] * c.w + sg * y[3] * s.w;
+    }
+    const float big = npn::wave_max(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+    const uint32_t e = min(max(__float_as_uint(big) >> 23, 64u), 190u);  // 2^-63 to 2^63
+    float inv = __uint_as_float((253u - e) << 23);                      // 2^-(e - 126)
+    float q_scale = __uint_as_float((e + 1) << 23) * (kLog2e / 16.0f);
+    const int d = 4 * lane;
+    if (a.R == kRows) {  // three e4m3 parts of 256 times as much
+      inv *= 256.0f;
+      q_scale *= 1.0f / 256;
+      if (lane == 0) a.q_scale[(size_t)pair * a.R + r] = q_scale;
+      uint32_t part[3];
+      split3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv, part);
+      const size_t at = ((((size_t)pair * 8 + (r >> 4)) * 2 + (d >> 7)) * 3 * 2 + ((d >> 6) & 1)) * 64;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(a.q + at + 16 * ((d >> 4) & 3) + (r & 15));
+#pragma unroll
+      for (int k = 0; k < 3; ++k) dst[k * 512 + ((d >> 2) & 3)] = part[k];
+      continue;
+    }
     if (lane == 0) a.q_scale[(size_t)pair * a.R + r] = q_scale;
-    uint32_t part[3];
-    split3(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv, part);
-    const size_t at = ((((size_t)pair * 8 + (r >> 4)) * 2 + (d >> 7)) * 3 * 2 + ((d >> 6) & 1)) * 64;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(a.q + at + 16 * ((d >> 4) & 3) + (r & 15));
+    uint32_t two[2];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) dst[k * 512 + ((d >> 2) & 3)] = part[k];
-    return;
+    for (int j = 0; j < 2; ++j) {
+      const f16x2 x = {(_Float16)(v[2 * j] * inv), (_Float16)(v[2 * j + 1] * inv)};
+      two[j] = __builtin_bit_cast(uint32_t, x);
+    }
+    const int step = 2 * (d >> 6) + ((d >> 3) & 1), g = (d >> 4) & 3;
+    u32x4* dst = a.q + (((size_t)pair * 8 + step) * (a.R / 16) + (r >> 4)) * 64 + 16 * g + (r & 15);
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint32_t*>(dst) + ((d & 4) >> 1)) = make_uint2(two[0], two[1]);
   }
-  if (lane == 0) a.q_scale[(size_t)pair * a.R + r] = q_scale;
-  uint32_t two[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const f16x2 x = {(_Float16)(v[2 * j] * inv), (_Float16)(v[2 * j + 1] * inv)};
-    two[j] = __builtin_bit_cast(uint32_t, x);
-  }
-  const int step = 2 * (d >> 6) + ((d >> 3) & 1), g = (d >> 4) & 3;
-  u32x4* dst = a.q + (((size_t)pair * 8 + step) * (a.R / 16) + (r >> 4)) * 64 + 16 * g + (r & 15);
-  *reinterpret_cast<uint2*>(reinterpret_cast<uint32_t*>(dst) + ((d & 4) >> 1)) = make_uint2(two[0], two[1]);
 }
 
 __global__ __launch_bounds__(kPrepWaves * 64) void paged_prep_kernel(PagedArgs a) {
   if (blockIdx.x == 0) plan_block(a);
-  else prep_row<false>(a, nullptr, (int64_t)(blockIdx.x - 1) * kPrepWaves + (threadIdx.x >> 6));
+  else prep_rows<false, 1>(a, nullptr, (int64_t)(blockIdx.x - 1) * kPrepWaves + (threadIdx.x >> 6));
 }
 
-// The same for a tree, and in the workgroups behind the append of its nodes' rows, which the attention's
+// The same for a tree, and before it, in `appends` workgroups, the append of its nodes' rows, which the attention's
 // launch reads: none of the three parts reads what another writes.
-template <int RPW>
+template <int RPW, int QR>
 __global__ __launch_bounds__(kPrepWaves * 64) void tree_prep_kernel(PagedArgs a, append::PagedAppendArgs ap,
-                                                                    const int32_t* parent, int rows, int per) {
-  const int x = (int)blockIdx.x - 1 - rows;
-  if (blockIdx.x == 0) {
+                                                                    const int32_t* parent, int appends, int per) {
+  const int x = (int)blockIdx.x - 1;
+  if (x < 0) {
     plan_block(a);
-  } else if (x < 0) {
-    prep_row<true>(a, parent, (int64_t)(blockIdx.x - 1) * kPrepWaves + (threadIdx.x >> 6));
+  } else if (x >= appends) {
+    prep_rows<true, QR>(a, parent, (int64_t)(x - appends) * kPrepWaves + (threadIdx.x >> 6));
   } else {
     const int bh = x / per, b = bh / (2 * ap.Hkv), hv = bh - b * 2 * ap.Hkv, lane = threadIdx.x & 63;
     const uint64_t anc =
@@ -1288,9 +1300,10 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
       if (TREE ? (sm.anc[TREE ? rk : 0] & sm.nan_node[TREE ? 4 * lane + e : 0]) != 0
                : sm.lim[rk] >= sm.nan_key[TREE ? 0 : 4 * lane + e])
         x[e] = NAN;
+    if (rk >= rows) break;
     if (parts > 1)
       *reinterpret_cast<f32x4*>(a.part_o + (slot * R + rk) * DH + 4 * lane) = x;
-    else if (rk < rows)
+    else
       write_out(a, un.b, row0 + rk, h, 4 * lane, x, sm.inv[rk]);
   }
 }
@@ -1380,6 +1393,11 @@ PagedPlan paged_plan(int B, int T, int q_heads, int kv_heads, int max_blocks, in
   // and 98, 2 of 1536 128 and 165; 16 of 96 146 and 148; but 4 of 192 59 and 54, one of 1536 over an empty
   // cache 35 and 30.
   p.R = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 ? 48 : kRows;
+  // Trees have groups of 48, nearly full, where those of 128 are a quarter empty or more: 16 requests of 144 rows over
+  // up to 16384 keys 207 us and 251 with groups of 128, 2 of them 49 and 59; one of 96 rows over 32768 47 and 50, of 192
+  // over 16384 47.1 and 48.4; but 16 of 96 159 and 152, and one of 60, half empty in both, 47 and 42.
+  const int64_t by48 = (rows + 47) / 48 * 48, by128 = (rows + kRows - 1) / kRows * kRows;
+  if (tree && by48 * 4 <= by128 * 3 && rows * 8 >= by48 * 7) p.R = rows <= 48 ? p.R : 48;
   p.RG = (int)((rows + p.R - 1) / p.R);
   const int64_t pairs = (int64_t)B * p.RG * kv_heads;
   const int64_t keys = (int64_t)max_blocks * block_size;
@@ -1500,17 +1518,21 @@ extern "C" int npn_gqa_tree_verify_paged(
                                    reinterpret_cast<uint8_t*>(cache_k), reinterpret_cast<uint8_t*>(cache_v),
                                    k_scale, v_scale, B, T, kv_heads, n_blocks, a.sh, positions};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int rows = p.pairs * p.R / kPrepWaves;               // workgroups of q'
   const int per = 1 + (T - 1 + block_size - 1) / block_size;  // a request's rows touch at most so many blocks
+  const int appends = per * 2 * kv_heads * B;
   const int at_once = T < block_size ? T : block_size;
+  // Four rows of q' to a wave where one each would be more waves than run at once: 24576 rows with their append 19 us
+  // instead of 32, 6144 8.3 instead of 10.5; 512 rows with four to a wave 6.0 instead of 5.0.
+  const int qr = p.pairs * p.R > 4096 ? 4 : 1;
+  const int rows = p.pairs * p.R / (kPrepWaves * qr) + (p.pairs * p.R % (kPrepWaves * qr) != 0);  // workgroups of q'
   auto prep = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(1 + rows + per * 2 * kv_heads * B), dim3(kPrepWaves * 64), 0, s, a, ap, parent,
-                       rows, per);
+    hipLaunchKernelGGL(kernel, dim3(1 + appends + rows), dim3(kPrepWaves * 64), 0, s, a, ap, parent, appends, per);
   };
-  if (at_once <= 8) prep(tree_prep_kernel<1>);
-  else if (at_once <= 16) prep(tree_prep_kernel<2>);
-  else if (at_once <= 32) prep(tree_prep_kernel<4>);
-  else prep(tree_prep_kernel<8>);
+  auto by_rows = [&](auto one, auto four) { qr == 4 ? prep(four) : prep(one); };
+  if (at_once <= 8) by_rows(tree_prep_kernel<1, 1>, tree_prep_kernel<1, 4>);
+  else if (at_once <= 16) by_rows(tree_prep_kernel<2, 1>, tree_prep_kernel<2, 4>);
+  else if (at_once <= 32) by_rows(tree_prep_kernel<4, 1>, tree_prep_kernel<4, 4>);
+  else by_rows(tree_prep_kernel<8, 1>, tree_prep_kernel<8, 4>);
   launch_attn<true>(p, a, s);
   return npn_launch_status();
 }

@@ -302,7 +302,11 @@ def test_tree_verify_paged_of_a_chain_is_append_and_verify(ops, T):
     args, out = _check(ops, d)
     query, gate, key, value, qn, kn, cos, sin, *cache, table, kv, slots, n, _ = _args(d)
     ops.gqa.kv_append_paged(key, value, kn, cos, sin, kv, slots, *cache)
-    assert torch.equal(out, ops.gqa.tail_verify_paged(query, gate, qn, cos, sin, *cache, table, kv, n))
+    want = ops.gqa.tail_verify_paged(query, gate, qn, cos, sin, *cache, table, kv, n)
+    if T == 30:  # groups of other sizes: both within the tolerance of the formula, so within twice that of each other
+        assert_rel_close(out.float().cpu().numpy(), want.float().cpu().numpy(), tol=4e-3, out_unit=2 * BF16_U)
+    else:
+        assert torch.equal(out, want)
     assert all(torch.equal(a, b) for a, b in zip(args[8:12], cache))
 
 
