@@ -5,9 +5,15 @@
 // A page's scale is the page's own: a row that comes from a page of another scale is rounded to its new
 // page's, which grows first where the row needs it (as an append's does), the page's older rows with it.
 //
-// One workgroup per (layer, request, head, K or V): all rows that move go through its LDS before the first
-// is written, since one row's place is another's source. Bound by a chain of loads: path and slots, scales
-// and rows.
+// K: a wave has the rows of one (layer, request, head), 256 bytes each. It takes them in order, a batch into registers and
+// then to their places: a row's place is no later row's source, so nothing waits for other waves.
+// V: rows are columns of their page, bytes a line apart. A thread of a workgroup has one dim: it loads the 16 rows of each
+// piece of the tree that has a part in it, up to five, at once, moves bytes between them in LDS of its own and
+// stores the pieces that rows went to.
+// Bound by a chain of loads (path and slots, scales and rows) where there is little to move, one layer of one request
+// 4.2 us, and by lines of the pages, which V's bytes take whole, where there is much: 16 layers of 64 requests of 64
+// nodes over blocks of 16, whose paths touch four pieces of five, 39 us for some 100 MB. (There V's bytes moved one by
+// one: 51 us by a wave for all dims, 39 by a workgroup with all rows in LDS, which took 5.2 for the one request.)
 #include "paged_append.h"
 #include "tree.h"
 
@@ -16,8 +22,10 @@ namespace {
 using append::DH;
 
 constexpr int kCompactLayers = 32;
-constexpr int kCompactThreads = 256;
-static_assert(kCompactThreads == DH, "a thread for each dim of V");
+constexpr int kCompactWaves = 4;  // of a workgroup; for K they share nothing
+constexpr int kBatch = 8;         // K's rows in registers
+constexpr int kPieces = 5;        // 64 rows from any place on lie in at most so many pieces of 16
+static_assert(64 * kCompactWaves == DH, "a thread for each dim of V");
 
 struct CompactArgs {
   uint8_t* cache_k[kCompactLayers];
@@ -29,137 +37,260 @@ struct CompactArgs {
   int T, Hkv, N, sh;
 };
 
-__global__ __launch_bounds__(kCompactThreads) void paged_compact_kernel(CompactArgs a) {
-  constexpr int kRows = npn::kMaxNodes, kWaves = kCompactThreads / 64;
-  __shared__ uint32_t s_row[kRows][DH / 4];  // the rows that move
-  __shared__ int64_t s_src[kRows], s_dst[kRows];
-  __shared__ float s_by[kRows];
-  __shared__ int s_max[kRows];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int h = blockIdx.x >> 1, b = blockIdx.y, layer = blockIdx.z;
-  const bool is_v = blockIdx.x & 1;
-  const int bs = 1 << a.sh;
+// A path as a wave has it: lane d row d.
+struct Path {
+  int node, off;       // and where the first row lies in its piece of 16 positions
+  int64_t src, dst, dst_page;
+  bool row, moves;
+  uint64_t moving;     // bits of the rows that move
+  float s_old, d_old;  // the scales of the row where it lies and of the page that it goes to
+};
 
-  // Every wave has the whole path, lane d its row d.
+__device__ __forceinline__ Path path_of(const CompactArgs& a, const float* scale, int b, int h) {
+  const int lane = threadIdx.x & 63;
   const int64_t end = (int64_t)a.N << a.sh;
   const size_t at = (size_t)b * a.T + lane;
-  const int node = lane < a.T ? a.path[at] : -1;
-  const int64_t dst = lane < a.T ? a.slots[at] : -1;
-  const int64_t src = (int64_t)npn::shfl64(dst, min(max(node, 0), a.T - 1));
-  const int n = npn::path_length(node, a.T, lane, dst >= 0 && dst < end && src >= 0 && src < end);
-  const bool row = lane < n, moves = row && src != dst;
-  const uint64_t moving = __builtin_amdgcn_ballot_w64(moves);
-  if (moving == 0) return;  // the same in all waves
-  const int m = __popcll(moving), mine = __popcll(moving & ((1ull << lane) - 1));  // of those that move
-  float* scale = is_v ? a.v_scale[layer] : a.k_scale[layer];
-  uint8_t* cache = is_v ? a.cache_v[layer] : a.cache_k[layer];
-  const int64_t dst_page = dst >> a.sh;
-  const float s_old = row ? scale[(src >> a.sh) * a.Hkv + h] : 0.f;  // of the row where it lies
-  const float d_old = row ? scale[dst_page * a.Hkv + h] : 0.f;       // and of the page that it goes to
-  // Byte offset of a slot's row (K), of its place in the first dim's line (V).
-  auto place = [&](int64_t slot) {
-    return ((slot >> a.sh) * a.Hkv + h) * ((int64_t)DH << a.sh) +
-           (is_v ? (slot & (bs - 1)) : (slot & (bs - 1)) * DH);
-  };
-  if (w == 0 && moves) {
-    s_src[mine] = place(src);
-    s_dst[mine] = place(dst);
-  }
-  __syncthreads();
-  uint8_t* bytes = reinterpret_cast<uint8_t*>(s_row);
-  constexpr int kBatch = 8;  // loads in flight
-  if (!is_v) {
-    for (int i0 = w; i0 < m; i0 += kBatch * kWaves) {
-      uint32_t x[kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        x[j] = *reinterpret_cast<const uint32_t*>(cache + s_src[min(i0 + j * kWaves, m - 1)] + 4 * lane);
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        if (i0 + j * kWaves < m) s_row[i0 + j * kWaves][lane] = x[j];
-    }
-  } else {
-    for (int i0 = 0; i0 < m; i0 += kBatch) {
-      uint8_t x[kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) x[j] = cache[s_src[min(i0 + j, m - 1)] + ((int64_t)tid << a.sh)];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        if (i0 + j < m) bytes[(i0 + j) * DH + tid] = x[j];
-    }
-  }
-  __syncthreads();
+  Path p;
+  p.node = lane < a.T ? a.path[at] : -1;
+  p.dst = lane < a.T ? a.slots[at] : -1;
+  p.src = (int64_t)npn::shfl64((uint64_t)p.dst, min(max(p.node, 0), a.T - 1));
+  // A row's place counted from the beginning of the first one's piece of 16 positions tells where its own piece begins.
+  p.off = (int)(npn::tree_bits((uint64_t)p.dst, 0) & 15);
+  const int first = max(16 * ((p.off + lane) >> 4) - p.off, 0);
+  const bool run = p.dst == (int64_t)npn::shfl64((uint64_t)p.dst, first) + lane - first &&
+                   (int)(p.dst & 15) == ((p.off + lane) & 15);
+  const bool both = run && __shfl((int)run, min(max(p.node, 0), a.T - 1), 64);
+  const bool in = p.dst >= 0 && p.dst < end && p.src >= 0 && p.src < end;
+  const int n = npn::path_length(p.node, a.T, lane, in && both);
+  p.dst_page = p.dst >> a.sh;
+  p.row = lane < n;
+  p.moves = p.row && p.src != p.dst;
+  p.moving = __builtin_amdgcn_ballot_w64(p.moves);
+  p.s_old = p.moves ? scale[(p.src >> a.sh) * a.Hkv + h] : 0.f;
+  p.d_old = p.row && p.moving ? scale[p.dst_page * a.Hkv + h] : 0.f;
+  return p;
+}
 
-  // The pages' new scales. Where no row comes from a larger one they stay.
-  float now = d_old;
-  if (__builtin_amdgcn_ballot_w64(moves && s_old > d_old) != 0) {
-    for (int i = w; i < m; i += kWaves) {
-      const uint32_t x = s_row[i][lane];
-      int big = 0;
+// The largest magnitude among a word's bytes that is not NaN.
+__device__ __forceinline__ int largest_byte(uint32_t x) {
+  int big = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int mag = (int)(x >> (8 * j)) & 0x7F;
-        big = max(big, mag == 0x7F ? 0 : mag);
-      }
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) big = max(big, __shfl_xor(big, off, 64));
-      if (lane == 0) s_max[i] = big;
-    }
-    __syncthreads();
-    float need = 0.f;
-    if (moves) {
-      const auto v = __builtin_amdgcn_cvt_pk_f32_fp8(s_max[mine], false);
-      need = v[0] > 0.f ? append::scale_of(v[0] * s_old) : 0.f;
-    }
-    uint64_t left = __builtin_amdgcn_ballot_w64(row);
-    while (left != 0) {  // page by page
-      const bool here = row && dst_page == (int64_t)npn::shfl64(dst_page, __builtin_ctzll(left));
-      const float top = npn::wave_max(here ? fmaxf(d_old, need) : 0.f);
-      if (here) now = top;
-      left &= ~__builtin_amdgcn_ballot_w64(here);
-    }
+  for (int j = 0; j < 4; ++j) {
+    const int mag = (int)(x >> (8 * j)) & 0x7F;
+    big = max(big, mag == 0x7F ? 0 : mag);
   }
-  if (w == 0 && moves) s_by[mine] = s_old / now;
-  uint64_t grown = __builtin_amdgcn_ballot_w64(row && now > d_old);
-  __syncthreads();  // rows, factors and old scales have been read
-  while (grown != 0) {  // a grown page's rows up to the path's last in it move to the new scale
+  return big;
+}
+__device__ __forceinline__ int wave_max_int(int x) {
+  x = max(x, (int)npn::dpp32<npn::kDppStep[0]>((uint32_t)x));
+  x = max(x, (int)npn::dpp32<npn::kDppStep[1]>((uint32_t)x));
+  x = max(x, (int)npn::dpp32<npn::kDppStep[2]>((uint32_t)x));
+  x = max(x, (int)npn::dpp32<npn::kDppStep[3]>((uint32_t)x));
+  const auto a = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+  x = max((int)a[0], (int)a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+  return max((int)b[0], (int)b[1]);
+}
+// The scale that a row needs whose largest byte this is.
+__device__ __forceinline__ float need_of(int big, float scale) {
+  const auto v = __builtin_amdgcn_cvt_pk_f32_fp8(big, false);
+  return v[0] > 0.f ? append::scale_of(v[0] * scale) : 0.f;
+}
+// The new scale of each row's page, from what its rows need.
+__device__ __forceinline__ float grown_scale(const Path& p, float need) {
+  float now = p.d_old;
+  uint64_t left = __builtin_amdgcn_ballot_w64(p.row);
+  while (left != 0) {  // page by page
+    const bool here = p.row && p.dst_page == (int64_t)npn::tree_bits((uint64_t)p.dst_page, __builtin_ctzll(left));
+    const float top = npn::wave_max(here ? fmaxf(p.d_old, need) : 0.f);
+    if (here) now = top;
+    left &= ~__builtin_amdgcn_ballot_w64(here);
+  }
+  return now;
+}
+// For each grown page: f(page, its first row of the path, its last one's place in it, factor, new scale). Of its rows up
+// to that place those move to the new scale that the path does not overwrite. No source is among them: where its
+// place is one of the path's, another row moves there.
+template <class F>
+__device__ __forceinline__ void each_grown(const CompactArgs& a, const Path& p, float now, F&& f) {
+  uint64_t grown = __builtin_amdgcn_ballot_w64(p.row && now > p.d_old);
+  while (grown != 0) {
     const int first = __builtin_ctzll(grown);
-    const int64_t page = (int64_t)npn::shfl64(dst_page, first);
-    const bool here = row && dst_page == page;
-    const uint64_t in = __builtin_amdgcn_ballot_w64(here);
-    const int last = 63 - __builtin_clzll(in);
-    const int upto = (int)(npn::shfl64(dst, last) & (bs - 1));
-    const float by = __shfl(d_old, first, 64) / __shfl(now, first, 64);
-    uint8_t* p = cache + (page * a.Hkv + h) * ((int64_t)DH << a.sh);
-    if (!is_v) {
-      for (int r = w; r <= upto; r += kWaves) {
-        uint32_t* word = reinterpret_cast<uint32_t*>(p + (size_t)r * DH) + lane;
-        *word = append::rescale_e4m3(*word, by);
-      }
-    } else {
-      for (int r = 0; r <= upto; r += 4) {
-        uint32_t* word = reinterpret_cast<uint32_t*>(p + ((size_t)tid << a.sh) + r);
-        const uint32_t keep = upto - r >= 3 ? 0u : ~0u << (8 * (upto - r + 1));
-        *word = (*word & keep) | (append::rescale_e4m3(*word, by) & ~keep);
-      }
-    }
-    if (tid == first) scale[page * a.Hkv + h] = now;
+    const int64_t page = (int64_t)npn::tree_bits((uint64_t)p.dst_page, first);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(p.row && p.dst_page == page);
+    const int upto = (int)(npn::tree_bits((uint64_t)p.dst, 63 - __builtin_clzll(in)) & ((1 << a.sh) - 1));
+    const float old = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p.d_old), first));
+    const float to = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(now), first));
+    f(page, first, upto, old / to, to);
     grown &= ~in;
   }
-  __syncthreads();  // the rows that move are written over those
-  if (!is_v) {
-    for (int i = w; i < m; i += kWaves) {
-      const uint32_t x = s_row[i][lane];
-      const float by = s_by[i];
-      *reinterpret_cast<uint32_t*>(cache + s_dst[i] + 4 * lane) = by == 1.0f ? x : append::rescale_e4m3(x, by);
+}
+// Whether the path moves a row to this slot (wave-uniform).
+__device__ __forceinline__ bool moved_to(const Path& p, int64_t slot) {
+  return __builtin_amdgcn_ballot_w64(p.moves && p.dst == slot) != 0;
+}
+
+__device__ __forceinline__ void compact_k(const CompactArgs& a, uint8_t* cache, float* scale, int b, int h) {
+  const int lane = threadIdx.x & 63;
+  const Path p = path_of(a, scale, b, h);
+  if (p.moving == 0) return;
+  auto place = [&](int64_t slot) {  // a slot's row
+    return ((slot >> a.sh) * a.Hkv + h) * ((int64_t)DH << a.sh) + (slot & ((1 << a.sh) - 1)) * DH;
+  };
+  const int64_t from = place(p.src), to = place(p.dst);  // of lanes that have no row: not used
+  // The rows that move, kBatch at a time from `left` on: which, and the lane's bytes of them.
+  auto take = [&](uint64_t& left, int (&d)[kBatch], uint32_t (&x)[kBatch]) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      d[k] = left ? __builtin_ctzll(left) : -1;
+      left &= left - 1;
     }
-  } else {
-    for (int i = 0; i < m; ++i) {
-      const uint32_t x = bytes[i * DH + tid];
-      const float by = s_by[i];
-      cache[s_dst[i] + ((int64_t)tid << a.sh)] = (uint8_t)(by == 1.0f ? x : append::rescale_e4m3(x, by));
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (d[k] >= 0)
+        x[k] = *reinterpret_cast<const uint32_t*>(cache + (int64_t)npn::tree_bits((uint64_t)from, d[k]) + 4 * lane);
+  };
+  // The pages' new scales. Where no row comes from a larger one they stay.
+  float now = p.d_old;
+  if (__builtin_amdgcn_ballot_w64(p.moves && p.s_old > p.d_old) != 0) {
+    float need = 0.f;
+    uint64_t left = p.moving;
+    while (left != 0) {
+      int d[kBatch];
+      uint32_t x[kBatch];
+      take(left, d, x);
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (d[k] < 0) continue;
+        const int big = wave_max_int(largest_byte(x[k]));
+        if (lane == d[k]) need = need_of(big, p.s_old);
+      }
+    }
+    now = grown_scale(p, need);
+    each_grown(a, p, now, [&](int64_t page, int, int upto, float by, float to_scale) {
+      uint32_t* rows = reinterpret_cast<uint32_t*>(cache + (page * a.Hkv + h) * ((int64_t)DH << a.sh)) + lane;
+      for (int r0 = 0; r0 <= upto; r0 += kBatch) {
+        uint32_t x[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) x[k] = rows[min(r0 + k, upto) * (DH / 4)];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (r0 + k <= upto && !moved_to(p, (page << a.sh) + r0 + k))
+            rows[(r0 + k) * (DH / 4)] = append::rescale_e4m3(x[k], by);
+      }
+      if (lane == 0) scale[page * a.Hkv + h] = to_scale;
+    });
+  }
+  const float by = p.s_old / now;
+  uint64_t left = p.moving;
+  while (left != 0) {
+    int d[kBatch];
+    uint32_t x[kBatch];
+    take(left, d, x);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (d[k] < 0) continue;
+      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), d[k]));
+      *reinterpret_cast<uint32_t*>(cache + (int64_t)npn::tree_bits((uint64_t)to, d[k]) + 4 * lane) =
+          f == 1.0f ? x[k] : append::rescale_e4m3(x[k], f);
     }
   }
+}
+
+__device__ __forceinline__ void compact_v(const CompactArgs& a, uint8_t* cache, float* scale, int b, int h) {
+  __shared__ uint4 s_piece[kPieces][DH];
+  __shared__ int s_big[kCompactWaves][npn::kMaxNodes];
+  const int dim = threadIdx.x, lane = dim & 63, w = __builtin_amdgcn_readfirstlane(dim >> 6);
+  const Path p = path_of(a, scale, b, h);  // the same in every wave
+  if (p.moving == 0) return;
+  uint8_t* line = cache + (size_t)h * ((size_t)DH << a.sh) + ((size_t)dim << a.sh);  // of this dim in block 0
+  const int64_t block = (int64_t)a.Hkv * DH << a.sh;
+  const int mask = (1 << a.sh) - 1;
+  const int src_at = p.off + p.node, dst_at = p.off + lane;
+
+  // The pieces up to the last row's and those of the sources, all in flight.
+  const bool grows = __builtin_amdgcn_ballot_w64(p.moves && p.s_old > p.d_old) != 0;  // some may
+  unsigned load = 0, store = 0;
+  uint4 x[kPieces];
+  uint8_t* at[kPieces];
+#pragma unroll
+  for (int c = kPieces - 1; c >= 0; --c) {
+    const bool to = __builtin_amdgcn_ballot_w64(p.moves && dst_at >> 4 == c) != 0;
+    if (to || (grows && store != 0)) store |= 1u << c;
+    if (__builtin_amdgcn_ballot_w64(p.moves && src_at >> 4 == c) != 0) load |= 1u << c;
+    load |= store;
+    if (!(load >> c & 1)) continue;
+    const int64_t slot = (int64_t)npn::tree_bits((uint64_t)p.dst, max(16 * c - p.off, 0)) & ~15ll;
+    at[c] = line + (slot >> a.sh) * block + (slot & mask);
+    x[c] = *reinterpret_cast<const uint4*>(at[c]);
+  }
+#pragma unroll
+  for (int c = 0; c < kPieces; ++c)
+    if (load >> c & 1) s_piece[c][dim] = x[c];
+  auto byte_of = [&](int place) {
+    return reinterpret_cast<uint8_t*>(s_piece) + ((place >> 4) * DH + dim) * 16 + (place & 15);
+  };
+
+  float now = p.d_old;
+  if (grows) {
+    for (uint64_t left = p.moving; left != 0; left &= left - 1) {
+      const int d = __builtin_ctzll(left);
+      const int big = wave_max_int(largest_byte(*byte_of(__builtin_amdgcn_readlane(src_at, d))));
+      if (lane == 0) s_big[w][d] = big;
+    }
+    __syncthreads();
+    int big = 0;
+#pragma unroll
+    for (int k = 0; k < kCompactWaves; ++k) big = max(big, p.moves ? s_big[k][lane] : 0);
+    now = grown_scale(p, need_of(big, p.s_old));
+    each_grown(a, p, now, [&](int64_t page, int first, int upto, float by, float to_scale) {
+      const int first_at = (int)(npn::tree_bits((uint64_t)p.dst, first) & mask);
+      for (int r = 0; r <= upto; r += 4) {
+        uint32_t change = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (r + j <= upto && !moved_to(p, (page << a.sh) + r + j)) change |= 0xFFu << (8 * j);
+        const int place = p.off + first + r - first_at;  // below 0: before the pieces
+        uint32_t* word = place >= 0 ? reinterpret_cast<uint32_t*>(byte_of(place))
+                                    : reinterpret_cast<uint32_t*>(line + page * block + r);
+        const uint32_t old = *word;
+        *word = (old & ~change) | (append::rescale_e4m3(old, by) & change);
+      }
+      if (dim == 0) scale[page * a.Hkv + h] = to_scale;  // every wave has read the old one
+    });
+  }
+
+  const float by = p.s_old / now;
+  uint64_t left = p.moving;
+  while (left != 0) {
+    int d[kBatch];
+    uint32_t y[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      d[k] = left ? __builtin_ctzll(left) : -1;
+      left &= left - 1;
+      if (d[k] >= 0) y[k] = *byte_of(__builtin_amdgcn_readlane(src_at, d[k]));
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (d[k] < 0) continue;
+      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), d[k]));
+      *byte_of(p.off + d[k]) = (uint8_t)(f == 1.0f ? y[k] : append::rescale_e4m3(y[k], f));
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kPieces; ++c)
+    if (store >> c & 1) *reinterpret_cast<uint4*>(at[c]) = s_piece[c][dim];
+}
+
+__global__ __launch_bounds__(64 * kCompactWaves) void paged_compact_kernel(CompactArgs a) {
+  const int b = blockIdx.y, layer = blockIdx.z, x = blockIdx.x;
+  if (x < a.Hkv) {
+    compact_v(a, a.cache_v[layer], a.v_scale[layer], b, x);
+    return;
+  }
+  const int h = __builtin_amdgcn_readfirstlane((x - a.Hkv) * kCompactWaves + ((int)threadIdx.x >> 6));
+  if (h < a.Hkv) compact_k(a, a.cache_k[layer], a.k_scale[layer], b, h);
 }
 
 }  // namespace
@@ -193,7 +324,8 @@ extern "C" int npn_gqa_compact_paged(const int32_t* path, const int64_t* slots, 
     a.Hkv = kv_heads;
     a.N = n_blocks;
     a.sh = sh;
-    hipLaunchKernelGGL(paged_compact_kernel, dim3(2 * kv_heads, B, n), dim3(kCompactThreads), 0,
+    hipLaunchKernelGGL(paged_compact_kernel, dim3(kv_heads + (kv_heads + kCompactWaves - 1) / kCompactWaves, B, n),
+                       dim3(64 * kCompactWaves), 0,
                        static_cast<hipStream_t>(stream), a);
     const int st = npn_launch_status();
     if (st != NPN_OK) return st;
