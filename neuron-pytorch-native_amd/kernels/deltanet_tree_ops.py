@@ -20,7 +20,7 @@ include/npn_spec_verify.h has the details and limits.
 import torch
 
 from deltanet_full_batched_ops import K_DIM, V_DIM, heads_from_shapes
-from npn_native import addresses, check_all, launch, register
+from npn_native import check_all, check_lists, launch, register
 
 MAX_NODES = 64
 I32, F32, BF16 = torch.int32, torch.float32, torch.bfloat16
@@ -90,9 +90,7 @@ def commit_tree_(states, conv_states, mixed_qkvs, records, path, v_heads):
         return
     qkv = conv_states[0].shape[0] // B
     hk, hv = heads_from_shapes(qkv, v_heads)
-    for specs in zip(states, conv_states, mixed_qkvs, records):
-        check_all(dev, *zip(specs, ("states", "conv_states", "mixed_qkvs", "records"),
-                            (F32, BF16, BF16, F32),
-                            ((B * hv * K_DIM, V_DIM), (B * qkv, 3), B * T * qkv, _records(B, T, hk, hv))))
-    launch(dev, "npn_deltanet_commit_tree", addresses(states), addresses(conv_states),
-           addresses(mixed_qkvs), addresses(records), layers, path, B, T, hk, hv)
+    lists = check_lists(dev, (states, "states", F32, (B * hv * K_DIM, V_DIM)),
+                        (conv_states, "conv_states", BF16, (B * qkv, 3)), (mixed_qkvs, "mixed_qkvs", BF16, B * T * qkv),
+                        (records, "records", F32, _records(B, T, hk, hv)))
+    launch(dev, "npn_deltanet_commit_tree", *lists, layers, path, B, T, hk, hv)

@@ -5,7 +5,9 @@ This is the only place Python crosses into native code. Each op module calls
 and a non-zero npn_status becomes a RuntimeError carrying the library's text.
 There is no fallback: if the library is missing the first call raises.
 """
+import array
 import ctypes
+import operator
 import os
 
 import torch
@@ -211,15 +213,40 @@ def check_all(dev, *specs):
             raise RuntimeError(f"{name} must be on {dev}, got {t.device}")
 
 
-def addresses(tensors):
-    """Host array of the tensors' device pointers, for an entry point that takes one."""
-    return (_P * max(len(tensors), 1))(*[t.data_ptr() for t in tensors])
+class Addresses:
+    """Host array of device pointers, as an argument of `launch`."""
+
+    def __init__(self, tensors):
+        pointers = array.array("Q", map(torch.Tensor.data_ptr, tensors))
+        self.pointers = pointers if pointers else array.array("Q", (0,))
+
+    def data_ptr(self):
+        return self.pointers.buffer_info()[0]
+
+
+_DTYPE = operator.attrgetter("dtype")
+
+
+def check_lists(dev, *specs):
+    """specs: (list of tensors, name, dtype, shape, or a number of elements in any shape), one tensor a layer:
+    `check_all` for each, the shape by the first and the others' number of elements. Returns their `Addresses`."""
+    out = []
+    for ts, name, dtype, shape in specs:
+        if ts:
+            check_all(dev, (ts[0], name, dtype, shape))
+            if len(ts) > 1 and not (
+                    set(map(torch.Tensor.numel, ts)) == {ts[0].numel()} and set(map(_DTYPE, ts)) == {dtype}
+                    and set(map(torch.Tensor.get_device, ts)) == {dev.index}
+                    and all(map(torch.Tensor.is_contiguous, ts))):
+                check_all(dev, *[(t, f"{name}[{i}]", dtype, ts[0].numel()) for i, t in enumerate(ts)])
+        out.append(Addresses(ts))
+    return out
 
 
 def launch(dev, name, *args):
     """`call` of an entry point that ends with a stream, on dev's current stream and with dev as the
-    current device; the tensors' devices have been checked. Arguments: tensors, ints and `addresses`."""
-    raw = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    current device; the tensors' devices have been checked. Arguments: tensors, ints and `Addresses`."""
+    raw = [a if type(a) is int else a.data_ptr() for a in args]
     fn = getattr(lib(), name)
     if dev.index == torch.cuda.current_device():
         status = fn(*raw, torch._C._cuda_getCurrentRawStream(dev.index))

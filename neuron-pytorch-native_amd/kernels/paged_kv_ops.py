@@ -38,7 +38,7 @@ include/npn_spec_verify.h has the details and limits.
 import torch
 
 from deltanet_tree_ops import tree_shape
-from npn_native import addresses, check_all, launch, query as size_query, register
+from npn_native import check_all, check_lists, launch, query as size_query, register
 
 HEAD_DIM = 256
 ROPE_DIM = 64
@@ -205,8 +205,7 @@ def compact_paged_(path, slots, cache_ks, cache_vs, k_scales, v_scales):
     if layers == 0:
         return
     n, hkv, bs = _cache_sizes(cache_ks[0])
-    for specs in zip(cache_ks, cache_vs, k_scales, v_scales):
-        check_all(dev, *zip(specs, ("cache_ks", "cache_vs", "k_scales", "v_scales"), (I8, I8, F32, F32),
-                            ((n, hkv, bs, HEAD_DIM), (n, hkv, HEAD_DIM, bs), (n, hkv), (n, hkv))))
-    launch(dev, "npn_gqa_compact_paged", path, slots, addresses(cache_ks), addresses(cache_vs),
-           addresses(k_scales), addresses(v_scales), layers, B, T, hkv, n, bs)
+    lists = check_lists(dev, (cache_ks, "cache_ks", I8, (n, hkv, bs, HEAD_DIM)),
+                        (cache_vs, "cache_vs", I8, (n, hkv, HEAD_DIM, bs)), (k_scales, "k_scales", F32, (n, hkv)),
+                        (v_scales, "v_scales", F32, (n, hkv)))
+    launch(dev, "npn_gqa_compact_paged", path, slots, *lists, layers, B, T, hkv, n, bs)
