@@ -59,12 +59,21 @@ typedef float f32x4 __attribute__((__vector_size__(4 * sizeof(float))));
 //   5. the norm over the workgroup's columns, z and the output.
 // A node whose input is not finite has zeros in these sums, which reach all nodes of a tile, and is noted: NaN
 // goes to its own and its descendants' rows at the end.
-template <int NT, int NW>
+// APART: q's rows take k's place once those have been used, and v's after them, so that two workgroups of 64 nodes fit a CU.
+template <int NT, int NW, bool APART>
 struct TreeSmem {
-  static constexpr int TM = 16 * NT;
-  _Float16 x[2][2 * TM][D + 8];  // high and low parts of k's rows, then q's
-  float v[TM][D + 4];
-  float low[TM][TM + 4], mix[TM][TM + 4];
+  static constexpr int TM = 16 * NT, kTiles = NT * (NT + 1) / 2;
+  union {
+    struct {
+      union {
+        _Float16 x[2][APART ? TM : 2 * TM][D + 8];  // high and low parts of k's rows, then q's
+        float v_apart[APART ? TM : 1][D + 4];
+      };
+      float low[kTiles][16][20], mix[kTiles][16][20];  // tile (a, s), s <= a, at a (a + 1) / 2 + s
+    };
+    uint32_t raw[APART ? 3 : 1][APART ? TM : 1][64];   // the nodes' inputs of q, k, v
+  };
+  float v[APART ? 1 : TM][D + 4];
   float inv[NT][16][20];
   float begun[TM], beta[TM], ss[NW][TM];
   double g[TM];  // sums of g along a node's line, base 2
@@ -73,6 +82,7 @@ struct TreeSmem {
   unsigned long long bad_u;
   uint32_t old[3][3][64];        // conv_state's inputs of q, k, v, one to three back from the first node
 };
+constexpr int tile_at(int a, int s) { return a * (a + 1) / 2 + s; }
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
 // x sigmoid(x) to 2 ulp: the reciprocal's one and the product's. (0 where e^-x overflows.)
@@ -119,13 +129,13 @@ struct Floats {
   float x[N];
 };
 
-template <int NT, int NW>
-__global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_verify_kernel(TreeArgs a) {
+template <int NT, int NW, bool APART>
+__global__ __launch_bounds__(64 * NW, NT == 1 || APART ? NW / 2 : NW / 4) void dn_tree_verify_kernel(TreeArgs a) {
   constexpr int TM = 16 * NT;
   constexpr int CT = 8 / NW;              // column tiles of a wave
   constexpr int RW = TM / NW;             // rows of a wave in step 1
   constexpr float kUnit = 4096.0f;        // the rows' scale in f16
-  __shared__ __attribute__((aligned(16))) TreeSmem<NT, NW> sm;
+  __shared__ __attribute__((aligned(16))) TreeSmem<NT, NW, APART> sm;
   const int T = a.T, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, G = lane >> 4;
   const int b = blockIdx.x / a.Hv, h = blockIdx.x - b * a.Hv, kh = h / (a.Hv / a.Hk);
@@ -166,11 +176,14 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
   const Floats<CT>* S0 = reinterpret_cast<const Floats<CT>*>(a.state + ((size_t)b * a.Hv + h) * D * D +
                                                              (size_t)(8 * G) * D + col);
   Floats<CT> s0[4][8];
+  auto load_state = [&]() {
 #pragma unroll
-  for (int s = 0; s < 4; ++s)
+    for (int s = 0; s < 4; ++s)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s0[s][e] = S0[(32 * s + e) * (D / CT)];
-  __builtin_amdgcn_sched_barrier(0);
+      for (int e = 0; e < 8; ++e) s0[s][e] = S0[(32 * s + e) * (D / CT)];
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if constexpr (!APART) load_state();
 
   // Lane t: node t's inputs one to three back, a node or -1 .. -3 for the last to the first of conv_state.
   int tap[3];
@@ -196,10 +209,12 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
 #pragma unroll
       for (int j = 0; j < 3; ++j) sm.old[which][j][lane] = old[which][j];
   }
-  // 1. A node's inputs wait in the places that its row's low parts, or the row of v, will have.
+  // 1. A node's inputs wait in the places that its row's low parts, or the row of v, will have (APART: in theirs).
   auto place = [&](int which, int t) {
-    return which == 2 ? reinterpret_cast<uint32_t*>(&sm.v[t][2 * lane])
-                      : reinterpret_cast<uint32_t*>(&sm.x[1][which == 0 ? TM + t : t][2 * lane]);
+    if constexpr (APART) return &sm.raw[which][t][lane];
+    else
+      return which == 2 ? reinterpret_cast<uint32_t*>(&sm.v[t][2 * lane])
+                        : reinterpret_cast<uint32_t*>(&sm.x[1][which == 0 ? TM + t : t][2 * lane]);
   };
 #pragma unroll
   for (int which = 0; which < 3; ++which)
@@ -276,29 +291,57 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
     sm.bad_kv[w] = bad_kv;
     sm.bad_q[w] = bad_q;
   }
+  if constexpr (APART) load_state();
   __syncthreads();  // the inputs have been read
+  auto write_rows = [&](int which) {
 #pragma unroll
-  for (int k = 0; k < RW; ++k) {
-    const int t = w + NW * k;
-#pragma unroll
-    for (int which = 0; which < 3; ++which) {
+    for (int k = 0; k < RW; ++k) {
+      const int t = w + NW * k;
       const bool none = t >= T || ((which == 0 ? bad_q : bad_kv) >> t & 1);
       const float y0 = none ? 0.f : y[which][k][0], y1 = none ? 0.f : y[which][k][1];
       if (which < 2) {
         const f16x2 hi = {(_Float16)y0, (_Float16)y1};
         const f16x2 lo = {(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])};
-        *reinterpret_cast<f16x2*>(&sm.x[0][which == 0 ? TM + t : t][2 * lane]) = hi;
-        *reinterpret_cast<f16x2*>(place(which, t)) = lo;
+        const int row = which == 0 && !APART ? TM + t : t;
+        *reinterpret_cast<f16x2*>(&sm.x[0][row][2 * lane]) = hi;
+        *reinterpret_cast<f16x2*>(&sm.x[1][row][2 * lane]) = lo;
       } else {
-        *reinterpret_cast<float2*>(place(2, t)) = make_float2(y0, y1);
+        *reinterpret_cast<float2*>(APART ? &sm.v_apart[APART ? t : 0][2 * lane] : &sm.v[APART ? 0 : t][2 * lane]) =
+            make_float2(y0, y1);
       }
     }
+  };
+  write_rows(1);
+  if constexpr (!APART) {
+    write_rows(0);
+    write_rows(2);
   }
   __syncthreads();
 
-  // 2. the pairs' products, tile (a, s) with s <= a of k's rows and of q's
+  // 2. the pairs' products, tile (a, s) with s <= a of k's rows and of q's, k's rows of tile s by `keys`
   auto rows_of = [&](int part, int tile, int step) {
     return *reinterpret_cast<const f16x8*>(&sm.x[part][16 * tile + i][32 * step + 8 * G]);
+  };
+  auto pair_tile = [&](int q, int ta, int ts, auto&& keys) {
+    f32x4 p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      const int rows = q && !APART ? NT + ta : ta;
+      const f16x8 xh = rows_of(0, rows, step), xl = rows_of(1, rows, step);
+      const f16x8 kh8 = keys(0, step), kl8 = keys(1, step);
+      p = mfma_f16(xl, kh8, p);
+      p = mfma_f16(xh, kl8, p);
+      p = mfma_f16(xh, kh8, p);
+    }
+    const int s = 16 * ts + i;
+    const double gs = sm.g[s];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int t = 16 * ta + 4 * G + r;
+      const bool sees = (sm.anc[t] >> s & 1) && (q || s != t);
+      const float f = __builtin_amdgcn_exp2f((float)(sm.g[t] - gs)) * (1.0f / (kUnit * kUnit));
+      (q ? sm.mix : sm.low)[tile_at(ta, ts)][4 * G + r][i] = sees ? p[r] * f * (q ? 1.0f : -sm.beta[t]) : 0.f;
+    }
   };
   int turn = 0;
 #pragma unroll
@@ -306,68 +349,78 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
 #pragma unroll
     for (int ts = 0; ts <= ta; ++ts)
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        if ((turn++ & (NW - 1)) != w) continue;
-        f32x4 p = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          const f16x8 xh = rows_of(0, q * NT + ta, step), xl = rows_of(1, q * NT + ta, step);
-          const f16x8 kh8 = rows_of(0, ts, step), kl8 = rows_of(1, ts, step);
-          p = mfma_f16(xl, kh8, p);
-          p = mfma_f16(xh, kl8, p);
-          p = mfma_f16(xh, kh8, p);
-        }
-        const int s = 16 * ts + i;
-        const double gs = sm.g[s];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int t = 16 * ta + 4 * G + r;
-          const bool sees = (sm.anc[t] >> s & 1) && (q || s != t);
-          const float f = __builtin_amdgcn_exp2f((float)(sm.g[t] - gs)) * (1.0f / (kUnit * kUnit));
-          (q ? sm.mix : sm.low)[t][s] = sees ? p[r] * f * (q ? 1.0f : -sm.beta[t]) : 0.f;
-        }
-      }
+      for (int q = 0; q < (APART ? 1 : 2); ++q)
+        if ((turn++ & (NW - 1)) == w) pair_tile(q, ta, ts, [&](int part, int step) { return rows_of(part, ts, step); });
   // and the state's
-  float inv_scale[CT];
+  float scale[CT], inv_scale[CT];
   f32x4 ks[NT][CT], qs[NT][CT];
-  {
-    float scale[CT], big[CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    float big = 0.f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(s0[s][e].x[c]));
+    // to [2^11, 2^12); of a column that is not finite some product is not either
+    const uint32_t e = min(max(__float_as_uint(max_over_groups(big)) >> 23, 12u), 254u);
+    scale[c] = __uint_as_float((265u - e) << 23);
+    inv_scale[c] = __uint_as_float((e - 11u) << 23) * (1.0f / kUnit);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) ks[n][c] = qs[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  auto state_parts = [&](int s, f16x8 (&hi)[CT], f16x8 (&lo)[CT]) {
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = s0[s][e].x[c] * scale[c];
+        hi[c][e] = (_Float16)x;
+        lo[c][e] = (_Float16)(x - (float)hi[c][e]);
+      }
+  };
+  auto state_tile = [&](int rows, int s, const f16x8 (&hi)[CT], const f16x8 (&lo)[CT], f32x4 (&p)[CT]) {
+    const f16x8 xh = rows_of(0, rows, s), xl = rows_of(1, rows, s);
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      big[c] = 0.f;
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) big[c] = fmaxf(big[c], fabsf(s0[s][e].x[c]));
-      // to [2^11, 2^12); of a column that is not finite some product is not either
-      const uint32_t e = min(max(__float_as_uint(max_over_groups(big[c])) >> 23, 12u), 254u);
-      scale[c] = __uint_as_float((265u - e) << 23);
-      inv_scale[c] = __uint_as_float((e - 11u) << 23) * (1.0f / kUnit);
-#pragma unroll
-      for (int n = 0; n < NT; ++n) ks[n][c] = qs[n][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+      p[c] = mfma_f16(xl, hi[c], p[c]);
+      p[c] = mfma_f16(xh, lo[c], p[c]);
+      p[c] = mfma_f16(xh, hi[c], p[c]);
     }
+  };
+  if constexpr (APART) {
+    f16x8 hi[4][CT], lo[4][CT], key[2][4];  // wave w has tile w of k's rows when q's come
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      state_parts(s, hi[s], lo[s]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) state_tile(n, s, hi[s], lo[s], ks[n]);
+    }
+    const int mine = min(w, NT - 1);
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+      for (int s = 0; s < 4; ++s) key[part][s] = rows_of(part, mine, s);
+    __syncthreads();
+    write_rows(0);
+    __syncthreads();
+#pragma unroll
+    for (int ta = 0; ta < NT; ++ta)
+      if (ta >= w) pair_tile(1, ta, w, [&](int part, int step) { return key[part][step]; });
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) state_tile(n, s, hi[s], lo[s], qs[n]);
+    __syncthreads();
+    write_rows(2);
+  } else {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       f16x8 hi[CT], lo[CT];
+      state_parts(s, hi, lo);
 #pragma unroll
-      for (int c = 0; c < CT; ++c)
+      for (int n = 0; n < NT; ++n) state_tile(n, s, hi, lo, ks[n]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = s0[s][e].x[c] * scale[c];
-          hi[c][e] = (_Float16)x;
-          lo[c][e] = (_Float16)(x - (float)hi[c][e]);
-        }
-#pragma unroll
-      for (int n = 0; n < 2 * NT; ++n) {
-        const f16x8 xh = rows_of(0, n, s), xl = rows_of(1, n, s);
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          f32x4& p = n < NT ? ks[n % NT][c] : qs[n % NT][c];
-          p = mfma_f16(xl, hi[c], p);
-          p = mfma_f16(xh, lo[c], p);
-          p = mfma_f16(xh, hi[c], p);
-        }
-      }
+      for (int n = 0; n < NT; ++n) state_tile(NT + n, s, hi, lo, qs[n]);
     }
   }
   // z is on its way by the time it is needed.
@@ -381,35 +434,44 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
       z[n][r] = CT == 2 ? *reinterpret_cast<const uint32_t*>(p) : *p;
     }
   const Floats<CT> nw = *reinterpret_cast<const Floats<CT>*>(a.norm_weight + col);
+  auto right_sides = [&]() {
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const f32x4 begun = *reinterpret_cast<const f32x4*>(&sm.begun[16 * n + 4 * G]);
-    const f32x4 beta = *reinterpret_cast<const f32x4*>(&sm.beta[16 * n + 4 * G]);
+    for (int n = 0; n < NT; ++n) {
+      const f32x4 begun = *reinterpret_cast<const f32x4*>(&sm.begun[16 * n + 4 * G]);
+      const f32x4 beta = *reinterpret_cast<const f32x4*>(&sm.beta[16 * n + 4 * G]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const Floats<CT> v = *reinterpret_cast<const Floats<CT>*>(&sm.v[16 * n + 4 * G + r][col]);
+      for (int r = 0; r < 4; ++r) {
+        const int t = 16 * n + 4 * G + r;
+        const Floats<CT> v =
+            *reinterpret_cast<const Floats<CT>*>(APART ? &sm.v_apart[APART ? t : 0][col] : &sm.v[APART ? 0 : t][col]);
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        ks[n][c][r] = beta[r] * (v.x[c] - begun[r] * (ks[n][c][r] * inv_scale[c]));
-        qs[n][c][r] *= begun[r] * inv_scale[c];
+        for (int c = 0; c < CT; ++c) {
+          ks[n][c][r] = beta[r] * (v.x[c] - begun[r] * (ks[n][c][r] * inv_scale[c]));
+          qs[n][c][r] *= begun[r] * inv_scale[c];
+        }
       }
     }
+  };
+  if constexpr (!APART) {
+    right_sides();
+    __syncthreads();
   }
-  __syncthreads();
 
   // 3. column i of the inverse of block w
   if (w < NT) {
+    const float (*low)[20] = sm.low[tile_at(w, w)];
     float x[16];
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       float y = r == i ? 1.0f : 0.f;
 #pragma unroll
-      for (int q = 0; q < r; ++q) y = fmaf(sm.low[16 * w + r][16 * w + q], x[q], y);
+      for (int q = 0; q < r; ++q) y = fmaf(low[r][q], x[q], y);
       x[r] = y;
       if (G == 0) sm.inv[w][r][i] = y;
     }
   }
   __syncthreads();
+  if constexpr (APART) right_sides();
 
   // 4.
   // Rows' entries that are not finite count as 0 from here on, and their nodes as bad.
@@ -437,7 +499,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int s = 0; s < n; ++s) {
-      const float4 f = *reinterpret_cast<const float4*>(&sm.low[16 * n + i][16 * s + 4 * G]);
+      const float4 f = *reinterpret_cast<const float4*>(&sm.low[tile_at(n, s)][i][4 * G]);
 #pragma unroll
       for (int c = 0; c < CT; ++c) ks[n][c] = mfma_f32(f, u[s][c], ks[n][c]);
     }
@@ -451,7 +513,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 ? NW / 2 : NW / 4) void dn_tree_ve
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int s = 0; s <= n; ++s) {
-      const float4 f = *reinterpret_cast<const float4*>(&sm.mix[16 * n + i][16 * s + 4 * G]);
+      const float4 f = *reinterpret_cast<const float4*>(&sm.mix[tile_at(n, s)][i][4 * G]);
 #pragma unroll
       for (int c = 0; c < CT; ++c) qs[n][c] = mfma_f32(f, u[s][c], qs[n][c]);
     }
@@ -610,10 +672,12 @@ extern "C" int npn_deltanet_verify_tree(const float* state, const int32_t* paren
                    dt_bias, norm_weight, out, records, rec_u, rec_decay, B, T, k_heads, v_heads};
   const dim3 grid(B * v_heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (T <= 16) hipLaunchKernelGGL((dn_tree_verify_kernel<1, 4>), grid, dim3(256), 0, s, a);
-  else if (T <= 32) hipLaunchKernelGGL((dn_tree_verify_kernel<2, 8>), grid, dim3(512), 0, s, a);
-  else if (T <= 48) hipLaunchKernelGGL((dn_tree_verify_kernel<3, 8>), grid, dim3(512), 0, s, a);
-  else hipLaunchKernelGGL((dn_tree_verify_kernel<4, 8>), grid, dim3(512), 0, s, a);
+  const bool apart = B * v_heads > 256;
+  auto launch = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, s, a); };
+  if (T <= 16) launch(dn_tree_verify_kernel<1, 4, false>, 4);
+  else if (T <= 32) launch(dn_tree_verify_kernel<2, 8, false>, 8);
+  else if (T <= 48) apart ? launch(dn_tree_verify_kernel<3, 4, true>, 4) : launch(dn_tree_verify_kernel<3, 8, false>, 8);
+  else apart ? launch(dn_tree_verify_kernel<4, 4, true>, 4) : launch(dn_tree_verify_kernel<4, 8, false>, 8);
   return npn_launch_status();
 }
 

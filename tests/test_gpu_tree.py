@@ -89,6 +89,34 @@ def test_verify_tree_matches_oracle(ops, B, T, Hk, Hv, reach):
     out_close(out, ref)
 
 
+@pytest.mark.parametrize("T", [33, 47, 48, 49, 64])
+def test_verify_tree_more_heads_than_compute_units(ops, T):
+    """Which has a kernel of its own above 32 nodes: one request against the oracle, all against one by one; a node
+    that is not a number in the middle stays on its branch."""
+    B, Hk, Hv = 9, 1, 29
+    d, f = _dn(B, T, Hk, Hv, seed=T, state_std=0.1)
+    parent = trees(B, T, 5, seed=T, wild=True)
+    out, rec = _verify(ops, f, cuda(parent))
+    got = _records(rec, B, T, Hk, Hv)
+    out = out.reshape(B, T, Hv, 128)
+    one = lambda b: {k: v[b:b + 1] if v.shape[0] == B else v for k, v in d.items()}  # noqa: E731
+    ref, *want, _ = ot.deltanet_verify(deltanet_oracle_args(one(4)), parent[4:5], Hk, Hv)
+    out_close(out[4:5], ref)
+    for g, r in zip(got, want):
+        assert_rel_close(g[4:5], r, tol=F32_TOL)
+    for b in range(B):
+        o, r = _verify(ops, deltanet_flat_device(one(b)), cuda(parent[b:b + 1]))
+        for g, w in zip(got, _records(r, 1, T, Hk, Hv)):
+            assert_rel_close(g[b:b + 1], w, tol=2 * F32_TOL)
+        assert_rel_close(out[b].float().cpu().numpy(), o.float().cpu().double().numpy().reshape(T, Hv, 128), tol=4e-3, out_unit=2 * BF16_U)
+    d["mixed_qkv"][3, T // 2, 128 + 5] = float("nan")
+    bad, brec = _verify(ops, deltanet_flat_device(d), cuda(parent))
+    hit = torch.zeros(B, T, Hv, 128, dtype=torch.bool, device="cuda")
+    hit[3, torch.tensor([T // 2 in ot.line(parent[3], t) for t in range(T)])] = True
+    bad = bad.reshape(hit.shape)
+    assert torch.isnan(bad[hit]).all() and torch.equal(bad[~hit], out[~hit])
+
+
 def test_verify_tree_takes_odd_parents(ops):
     """Parents that are none, the node itself, later or out of range hang the node on the committed tokens."""
     B, T = 3, 40
