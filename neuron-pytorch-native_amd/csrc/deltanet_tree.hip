@@ -43,6 +43,7 @@ struct TreeArgs {
 
 typedef _Float16 f16x8 __attribute__((__vector_size__(8 * sizeof(_Float16))));
 typedef _Float16 f16x2 __attribute__((__vector_size__(2 * sizeof(_Float16))));
+typedef __bf16 bf16x2 __attribute__((__vector_size__(2 * sizeof(__bf16))));
 typedef float f32x4 __attribute__((__vector_size__(4 * sizeof(float))));
 
 // One workgroup of four waves a (b, h); NT tiles of 16 nodes; wave w has columns 32 w + 2 i + {0, 1} of everything that
@@ -71,7 +72,7 @@ struct TreeSmem {
       };
       float low[kTiles][16][20], mix[kTiles][16][20];  // tile (a, s), s <= a, at a (a + 1) / 2 + s
     };
-    uint32_t raw[APART ? 3 : 1][APART ? TM : 1][64];   // the nodes' inputs of q, k, v
+    uint32_t raw[3][3 + TM][64];  // the inputs of q, k, v: conv_state's, then the nodes'
   };
   float v[APART ? 1 : TM][D + 4];
   float inv[NT][16][20];
@@ -80,7 +81,6 @@ struct TreeSmem {
   uint64_t anc[TM];
   uint64_t bad_kv[NW], bad_q[NW];  // by wave
   unsigned long long bad_u;
-  uint32_t old[3][3][64];        // conv_state's inputs of q, k, v, one to three back from the first node
 };
 constexpr int tile_at(int a, int s) { return a * (a + 1) / 2 + s; }
 
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * NW, NT == 1 || APART ? NW / 2 : NW / 4) void d
   uint32_t raw[3][RW];                    // node w + NW k's inputs of two channels, q, k, v
   float4 wt[3][2];
   float2 bias[3];
-  uint32_t old[3][3];                     // conv_state's, one to three back from the first node
+  uint32_t old[3][3];                     // conv_state's
 #pragma unroll
   for (int which = 0; which < 3; ++which) {
     const int c = (which == 0 ? kh : which == 1 ? a.Hk + kh : 2 * a.Hk + h) * D + 2 * lane;
@@ -173,19 +173,19 @@ __global__ __launch_bounds__(64 * NW, NT == 1 || APART ? NW / 2 : NW / 4) void d
   }
   __builtin_amdgcn_sched_barrier(0);
   // The state, lane (i, G): rows 32 s + 8 G + e of its columns.
-  const Floats<CT>* S0 = reinterpret_cast<const Floats<CT>*>(a.state + ((size_t)b * a.Hv + h) * D * D +
-                                                             (size_t)(8 * G) * D + col);
+  const float* S0 = a.state + ((size_t)b * a.Hv + h) * D * D;
+  const unsigned s_at = 8 * G * D + col;
   Floats<CT> s0[4][8];
   auto load_state = [&]() {
 #pragma unroll
     for (int s = 0; s < 4; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s0[s][e] = S0[(32 * s + e) * (D / CT)];
+      for (int e = 0; e < 8; ++e) s0[s][e] = *reinterpret_cast<const Floats<CT>*>(S0 + 32 * s * D + (s_at + e * D));
     __builtin_amdgcn_sched_barrier(0);
   };
   if constexpr (!APART) load_state();
 
-  // Lane t: node t's inputs one to three back, a node or -1 .. -3 for the last to the first of conv_state.
+  // Lane t: the rows below of node t's inputs one to three back.
   int tap[3];
   {
     int at = lane;
@@ -193,33 +193,23 @@ __global__ __launch_bounds__(64 * NW, NT == 1 || APART ? NW / 2 : NW / 4) void d
     for (int j = 0; j < 3; ++j) {
       const int up = __shfl(parent, max(at, 0), 64);
       at = at < 0 ? at - 1 : up;
-      tap[j] = at;
+      tap[j] = 3 + at;
+    }
+  }
+  // 1. The inputs wait in LDS, a node t's in row 3 + t, those before the first node's in rows 0 to 2.
+  if (w == 0) {
+#pragma unroll
+    for (int which = 0; which < 3; ++which) {  // [c0 c0][c0 c1][c1 c1], oldest first, to a word a step
+      const uint32_t x = old[which][0], y = old[which][1], v = old[which][2];
+      sm.raw[which][0][lane] = (x & 0xFFFFu) | (y & 0xFFFF0000u);
+      sm.raw[which][1][lane] = (x >> 16) | (v << 16);
+      sm.raw[which][2][lane] = (y & 0xFFFFu) | (v & 0xFFFF0000u);
     }
   }
 #pragma unroll
-  for (int which = 0; which < 3; ++which) {  // [c0 c0][c0 c1][c1 c1], oldest first, to a word a step back
-    const uint32_t x = old[which][0], y = old[which][1], v = old[which][2];
-    old[which][0] = (y & 0xFFFFu) | (v & 0xFFFF0000u);
-    old[which][1] = (x >> 16) | (v << 16);
-    old[which][2] = (x & 0xFFFFu) | (y & 0xFFFF0000u);
-  }
-  if (w == 0) {
-#pragma unroll
-    for (int which = 0; which < 3; ++which)
-#pragma unroll
-      for (int j = 0; j < 3; ++j) sm.old[which][j][lane] = old[which][j];
-  }
-  // 1. A node's inputs wait in the places that its row's low parts, or the row of v, will have (APART: in theirs).
-  auto place = [&](int which, int t) {
-    if constexpr (APART) return &sm.raw[which][t][lane];
-    else
-      return which == 2 ? reinterpret_cast<uint32_t*>(&sm.v[t][2 * lane])
-                        : reinterpret_cast<uint32_t*>(&sm.x[1][which == 0 ? TM + t : t][2 * lane]);
-  };
-#pragma unroll
   for (int which = 0; which < 3; ++which)
 #pragma unroll
-    for (int k = 0; k < RW; ++k) *place(which, w + NW * k) = raw[which][k];
+    for (int k = 0; k < RW; ++k) sm.raw[which][3 + w + NW * k][lane] = raw[which][k];
   uint64_t bad_kv = 0, bad_q = 0;  // wave-uniform
   if (w == kGates) {
     const float gf = -__expf(in_log) * npn::softplus(in_a + in_dt);
@@ -239,47 +229,50 @@ __global__ __launch_bounds__(64 * NW, NT == 1 || APART ? NW / 2 : NW / 4) void d
     if (lane == 0) sm.bad_u = 0;
   }
   __syncthreads();
-  float y[3][RW][2];
+  float y[3][RW][2], none = 0.f;  // NaN from the first number that is not finite
 #pragma unroll
   for (int k = 0; k < RW; ++k) {
-    const int t = w + NW * k;
-    int at[3];
+    uint32_t x[3][3];
 #pragma unroll
-    for (int j = 0; j < 3; ++j) at[j] = __builtin_amdgcn_readlane(tap[j], t);
+    for (int j = 0; j < 3; ++j) {
+      const uint32_t* row = &sm.raw[0][0][lane] + 64 * __builtin_amdgcn_readlane(tap[j], w + NW * k);
+#pragma unroll
+      for (int which = 0; which < 3; ++which) x[which][j] = row[which * (3 + TM) * 64];
+    }
 #pragma unroll
     for (int which = 0; which < 3; ++which) {
-      uint32_t x[3];
-#pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        x[j] = at[j] >= 0 ? *place(which, at[j]) : sm.old[which][-1 - at[j]][lane];
-      }
       const float4 w0 = wt[which][0], w1 = wt[which][1];
-      const float y0 = bias[which].x + w0.x * npn::bf16lo(x[2]) + w0.y * npn::bf16lo(x[1]) +
-                       w0.z * npn::bf16lo(x[0]) + w0.w * npn::bf16lo(raw[which][k]);
-      const float y1 = bias[which].y + w1.x * npn::bf16hi(x[2]) + w1.y * npn::bf16hi(x[1]) +
-                       w1.z * npn::bf16hi(x[0]) + w1.w * npn::bf16hi(raw[which][k]);
+      const float y0 = bias[which].x + w0.x * npn::bf16lo(x[which][2]) + w0.y * npn::bf16lo(x[which][1]) +
+                       w0.z * npn::bf16lo(x[which][0]) + w0.w * npn::bf16lo(raw[which][k]);
+      const float y1 = bias[which].y + w1.x * npn::bf16hi(x[which][2]) + w1.y * npn::bf16hi(x[which][1]) +
+                       w1.z * npn::bf16hi(x[which][0]) + w1.w * npn::bf16hi(raw[which][k]);
       y[which][k][0] = silu(y0);
       y[which][k][1] = silu(y1);
+      none = fmaf(y[which][k][0], 0.f, none);
+      none = fmaf(y[which][k][1], 0.f, none);
     }
   }
+  const bool some = __builtin_amdgcn_ballot_w64(none != none) != 0;
+  if (some) {
 #pragma unroll
-  for (int k = 0; k < RW; ++k) {
-    const int t = w + NW * k;
-    const bool in = t < T;
+    for (int k = 0; k < RW; ++k)
 #pragma unroll
-    for (int which = 0; which < 3; ++which) {
-      float &y0 = y[which][k][0], &y1 = y[which][k][1];
-      const float none = fmaf(y0, 0.f, y1 * 0.f);  // NaN if one is not finite
-      const bool bad = in && __builtin_amdgcn_ballot_w64(none != none) != 0;
-      (which == 0 ? bad_q : bad_kv) |= bad ? 1ull << t : 0ull;
-      if (which < 2) {
-        const float n = __builtin_amdgcn_rsqf(wave_sum(y0 * y0 + y1 * y1) + kEps) *
-                        (which == 0 ? 0.08838834764831845f * kUnit : kUnit);  // q: / sqrt(128)
-        y0 *= n;
-        y1 *= n;
+      for (int which = 0; which < 3; ++which) {
+        const bool bad = w + NW * k < T &&
+                         __builtin_amdgcn_ballot_w64(!finite(y[which][k][0]) || !finite(y[which][k][1])) != 0;
+        (which == 0 ? bad_q : bad_kv) |= bad ? 1ull << (w + NW * k) : 0ull;
       }
-    }
   }
+#pragma unroll
+  for (int k = 0; k < RW; ++k)
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float &y0 = y[which][k][0], &y1 = y[which][k][1];
+      const float n = __builtin_amdgcn_rsqf(wave_sum(y0 * y0 + y1 * y1) + kEps) *
+                      (which == 0 ? 0.08838834764831845f * kUnit : kUnit);  // q: / sqrt(128)
+      y0 *= n;
+      y1 *= n;
+    }
   if (h == kh * (a.Hv / a.Hk)) {
 #pragma unroll
     for (int k = 0; k < RW; ++k)
@@ -291,14 +284,20 @@ __global__ __launch_bounds__(64 * NW, NT == 1 || APART ? NW / 2 : NW / 4) void d
     sm.bad_kv[w] = bad_kv;
     sm.bad_q[w] = bad_q;
   }
+  if (some) {  // zeros in the sums
+#pragma unroll
+    for (int k = 0; k < RW; ++k)
+#pragma unroll
+      for (int which = 0; which < 3; ++which)
+        if ((which == 0 ? bad_q : bad_kv) >> (w + NW * k) & 1) y[which][k][0] = y[which][k][1] = 0.f;
+  }
   if constexpr (APART) load_state();
   __syncthreads();  // the inputs have been read
   auto write_rows = [&](int which) {
 #pragma unroll
     for (int k = 0; k < RW; ++k) {
       const int t = w + NW * k;
-      const bool none = t >= T || ((which == 0 ? bad_q : bad_kv) >> t & 1);
-      const float y0 = none ? 0.f : y[which][k][0], y1 = none ? 0.f : y[which][k][1];
+      const float y0 = t < T ? y[which][k][0] : 0.f, y1 = t < T ? y[which][k][1] : 0.f;
       if (which < 2) {
         const f16x2 hi = {(_Float16)y0, (_Float16)y1};
         const f16x2 lo = {(_Float16)(y0 - (float)hi[0]), (_Float16)(y1 - (float)hi[1])};
@@ -424,13 +423,14 @@ __global__ __launch_bounds__(64 * NW, NT == 1 || APART ? NW / 2 : NW / 4) void d
     }
   }
   // z is on its way by the time it is needed.
-  const size_t node0 = ((size_t)b * T * a.Hv + h) * D + col;  // row t: t * Hv * 128 behind
+  const size_t node0 = (size_t)b * T * a.Hv * D;
+  const unsigned node_at = h * D + col, node_step = a.Hv * D;  // node t: t steps behind
   uint32_t z[NT][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const uint16_t* p = a.z + node0 + (size_t)min(16 * n + 4 * G + r, T - 1) * a.Hv * D;
+      const uint16_t* p = a.z + node0 + (node_at + min(16 * n + 4 * G + r, T - 1) * node_step);
       z[n][r] = CT == 2 ? *reinterpret_cast<const uint32_t*>(p) : *p;
     }
   const Floats<CT> nw = *reinterpret_cast<const Floats<CT>*>(a.norm_weight + col);
@@ -560,17 +560,21 @@ __global__ __launch_bounds__(64 * NW, NT == 1 || APART ? NW / 2 : NW / 4) void d
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * n + 4 * G + r;
       if (t >= T) continue;
-      const size_t at = node0 + (size_t)t * a.Hv * D;
+      const unsigned at = node_at + t * node_step;
       Floats<CT> rec;
-      uint32_t o = 0;
+      __bf16 o[CT];
 #pragma unroll
       for (int c = 0; c < CT; ++c) {
-        o |= (uint32_t)npn::f32_to_bf16(qs[n][c][r] * f[r] * gate[n][r][c]) << (16 * c);
+        o[c] = (__bf16)(qs[n][c][r] * f[r] * gate[n][r][c]);
         rec.x[c] = u[n][c][r] + none[r];
       }
-      if constexpr (CT == 2) *reinterpret_cast<uint32_t*>(a.out + at) = o;
-      else a.out[at] = (uint16_t)o;
-      *reinterpret_cast<Floats<CT>*>(a.rec_u + at) = rec;
+      if constexpr (CT == 2) {
+        const bf16x2 both = {o[0], o[1]};
+        *reinterpret_cast<bf16x2*>(a.out + node0 + at) = both;
+      } else {
+        *reinterpret_cast<__bf16*>(a.out + node0 + at) = o[0];
+      }
+      *reinterpret_cast<Floats<CT>*>(a.rec_u + node0 + at) = rec;
     }
   }
 }
