@@ -89,11 +89,12 @@ def test_verify_tree_matches_oracle(ops, B, T, Hk, Hv, reach):
     out_close(out, ref)
 
 
-@pytest.mark.parametrize("T", [33, 47, 48, 49, 64])
-def test_verify_tree_more_heads_than_compute_units(ops, T):
-    """Which has a kernel of its own above 32 nodes: one request against the oracle, all against one by one; a node
-    that is not a number in the middle stays on its branch."""
-    B, Hk, Hv = 9, 1, 29
+@pytest.mark.parametrize("T,B,where", [(1, 27, "v"), (2, 27, "k"), (7, 27, "q"), (16, 27, "v"), (15, 27, "k"), (33, 9, "k"),
+                                       (47, 9, "v"), (48, 9, "q"), (49, 9, "k"), (64, 9, "v")])
+def test_verify_tree_many_heads(ops, T, B, where):
+    """More heads than run at once, which have kernels of their own up to 16 and above 32 nodes: one request against
+    the oracle, some against one by one; a node that is not a number in the middle stays on its branch."""
+    Hk, Hv = 1, 29
     d, f = _dn(B, T, Hk, Hv, seed=T, state_std=0.1)
     parent = trees(B, T, 5, seed=T, wild=True)
     out, rec = _verify(ops, f, cuda(parent))
@@ -104,15 +105,18 @@ def test_verify_tree_more_heads_than_compute_units(ops, T):
     out_close(out[4:5], ref)
     for g, r in zip(got, want):
         assert_rel_close(g[4:5], r, tol=F32_TOL)
-    for b in range(B):
+    for b in range(0, B, 4):
         o, r = _verify(ops, deltanet_flat_device(one(b)), cuda(parent[b:b + 1]))
         for g, w in zip(got, _records(r, 1, T, Hk, Hv)):
             assert_rel_close(g[b:b + 1], w, tol=2 * F32_TOL)
         assert_rel_close(out[b].float().cpu().numpy(), o.float().cpu().double().numpy().reshape(T, Hv, 128), tol=4e-3, out_unit=2 * BF16_U)
-    d["mixed_qkv"][3, T // 2, 128 + 5] = float("nan")
+    d["mixed_qkv"][3, T // 2, {"q": 5, "k": 128 + 5, "v": 256 + 17 * 128 + 5}[where]] = float("nan")
     bad, brec = _verify(ops, deltanet_flat_device(d), cuda(parent))
     hit = torch.zeros(B, T, Hv, 128, dtype=torch.bool, device="cuda")
-    hit[3, torch.tensor([T // 2 in ot.line(parent[3], t) for t in range(T)])] = True
+    # a query: the nodes whose window has it; a key: all below; a value: all below, its head
+    lines = [ot.line(parent[3], t) for t in range(T)]
+    below = torch.tensor([T // 2 in (mine[-4:] if where == "q" else mine) for mine in lines])
+    hit[3, below, 17 if where == "v" else 0:18 if where == "v" else Hv] = True
     bad = bad.reshape(hit.shape)
     assert torch.isnan(bad[hit]).all() and torch.equal(bad[~hit], out[~hit])
 
