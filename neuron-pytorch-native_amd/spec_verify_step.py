@@ -16,6 +16,10 @@ per sequence instead of one:
   rollback: DeltaNet state = checkpoint[accepted] (read in place by the next step),
             conv window rolled back, KV length += accepted + 1.
 
+A step over a tree of drafted tokens (step_tree, with a paged cache) runs the same layers with
+deltanet::verify_tree and gqa::tree_verify_paged, walks the tree (spec::accept_tree) and commits the path:
+deltanet::commit_tree_, gqa::compact_paged_ and spec::commit_.
+
 Dimensions are the 27B model's whole-model widths on one GPU: hidden 5120, DeltaNet 16 k /
 48 v heads of 128, GQA 24 q / 4 kv heads of 256 with a 64-dim partial RoPE (theta 1e7),
 MLP intermediate 17408. Weights are random (e4m3fn, per-output-channel fp32 scales).
@@ -180,6 +184,8 @@ class VerifySlice:
         self.rope_cos, self.rope_sin = rope_tables(torch.arange(s_max, device=device))
         self.prev_accepted = None
         self.timer = _untimed
+        self.nodes = self.tree = self.tree_graph = None  # how many nodes and the parents of the nodes of a step_tree; its graph
+        self.committed, self.last_accepted = torch.zeros(2, B, dtype=torch.int32, device=device)
         self.persistent = False
         self.parity = 0
         self.graphs = None
@@ -216,6 +222,13 @@ class VerifySlice:
             mixed, z, a, b = self.timer("glue.deltanet_split", torch.ops.glue.deltanet_split,
                                         proj, DN_QKV, DN_VAL, DN_HV)
         mixed = mixed.reshape(-1)
+        if self.tree is not None:
+            out, records = self.timer("deltanet.verify_tree", torch.ops.deltanet.verify_tree, L["state"], self.tree,
+                                      mixed, L["conv_state"], L["conv_w"], L["conv_b"], a.reshape(-1), b.reshape(-1),
+                                      z.reshape(B * T * DN_HV, DN_D), L["A_log"], L["dt_bias"], L["norm_w"])
+            L["pending"] = (records, mixed)
+            return fp8_project(out.reshape(B * T, DN_VAL), L["out_proj"], self.timer,
+                               f"fp8.matmul[{B * T}x{DN_VAL}x{HIDDEN}]", self.fuse_splitk)
         args = (mixed, L["conv_state"], L["conv_w"], L["conv_b"], a.reshape(-1), b.reshape(-1),
                 z.reshape(B * T * DN_HV, DN_D), L["A_log"], L["dt_bias"], L["norm_w"])
         if self.persistent:  # previous checkpoints in ckbuf[parity], new ones into the other
@@ -252,6 +265,11 @@ class VerifySlice:
         if self.paged_block is not None:
             slots, granted = self.plan
             pages = (L["cache_k"], L["cache_v"], L["k_scale"], L["v_scale"])
+        if self.tree is not None:
+            attn = self.timer("gqa.tree_verify_paged", torch.ops.gqa.tree_verify_paged, query, gate, key, value,
+                              L["q_norm"], L["k_norm"], self.rope_cos, self.rope_sin, *pages, self.pages["table"],
+                              self.kv_len, slots, granted, self.tree)
+        elif self.paged_block is not None:
             self.timer("gqa.kv_append_paged", torch.ops.gqa.kv_append_paged, key, value, L["k_norm"],
                        self.rope_cos, self.rope_sin, self.kv_len, slots, *pages)
             attn = self.timer("gqa.tail_verify_paged", torch.ops.gqa.tail_verify_paged, query, gate,
@@ -303,7 +321,8 @@ class VerifySlice:
             if cos is not None:
                 raise ValueError("the paged cache takes its RoPE rows from the tables")
             self._take_rows()
-            self.plan = self.timer("paged.update_blocks", self._plan_pages, self.new_len)
+            self.plan = self.timer("paged.update_blocks", self._plan_pages,
+                                   self.new_len if self.nodes is None else self.nodes)
         elif cos is None and not self.fuse_launches and "G" in self.pattern:
             cos, sin = self.timer("gqa.rope_rows", torch.ops.gqa.rope_rows, self.rope_cos,
                                   self.rope_sin, self.kv_len, self.T)
@@ -425,6 +444,49 @@ class VerifySlice:
                                            draft_logits, draft_ids, u_accept, u_sample, 1.0)
         self.accept_and_rollback(accepted)
         return h, accepted, out_ids
+
+    # ---- a step over a tree of drafted tokens ----------------------------------------------
+    def step_tree(self, x, parent, draft_ids, target_ids, n_nodes=None, trace=None):
+        """One verify + accept + commit step over trees of T = K + 1 nodes: x [B*T, 5120], parent [B, T] int32,
+        draft_ids and target_ids [B, T] int64 (the target's token of each node), n_nodes [B] int32 where
+        some have fewer than T (nodes [0, n_nodes[b]) count; 0: the sequence sits out). All state is
+        updated in place. Returns (hidden, accepted, path, out_ids). Steps over chains (step) leave
+        their DeltaNet states as checkpoints, so a slice takes steps of the one kind only."""
+        if self.paged_block is None and "G" in self.pattern:
+            raise ValueError("a tree needs the paged cache")
+        if self.prev_accepted is not None:
+            raise RuntimeError("step_tree after step: the states are in the chain's checkpoints")
+        self.tree, self.nodes = parent, n_nodes
+        try:
+            hidden = self.forward(x, trace=trace)
+        finally:
+            self.tree = self.nodes = None
+        attn = [L for L in self.layers if L["kind"] == "G"]
+        dn = [L for L in self.layers if L["kind"] == "D"]
+        granted = self.plan[1] if attn else self.new_len if n_nodes is None else n_nodes
+        accepted, path, out_ids = self.timer("spec.accept_tree", torch.ops.spec.accept_tree, target_ids, draft_ids,
+                                             parent, granted)
+        if dn:
+            pend = [L.pop("pending") for L in dn]
+            self.timer("deltanet.commit_tree", torch.ops.deltanet.commit_tree_, [L["state"] for L in dn],
+                       [L["conv_state"] for L in dn], [m for _, m in pend], [r for r, _ in pend], path, DN_HV)
+        if attn:
+            self.timer("gqa.compact_paged", torch.ops.gqa.compact_paged_, path, self.plan[0],
+                       *[[L[k] for L in attn] for k in ("cache_k", "cache_v", "k_scale", "v_scale")])
+        self.timer("spec.commit", torch.ops.spec.commit_, accepted, self.last_accepted, self.kv_len, self.committed)
+        return hidden, accepted, path, out_ids
+
+    def capture_tree(self, x, parent, draft_ids, target_ids, n_nodes=None):
+        """Capture step_tree over these tensors, which keep their addresses, as a HIP graph. Run one
+        eager step_tree before. replay_tree() runs it and returns the same four tensors every time."""
+        self.tree_graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.tree_graph):
+            self.tree_outputs = self.step_tree(x, parent, draft_ids, target_ids, n_nodes)
+
+    def replay_tree(self):
+        self._take_rows()
+        self.tree_graph.replay()
+        return self.tree_outputs
 
 
 def synthetic_logits(B, K, V, seed, device, rho=0.8):
