@@ -621,7 +621,7 @@ int npn_gqa_tree_verify_paged(const uint16_t* query, const uint16_t* gate, const
 /* torch.ops.deltanet.verify_tree -- npn_deltanet_verify's token step of every node from the state and
  * conv window behind its parent, without forming a state per node (64 KB each for every head).
  *   state [B, Hv, 128, 128] f32 and conv_state [B, QKV, 3] bf16: the committed ones;
- *   the other inputs as npn_deltanet_verify's, T <= 64; B * Hv <= 2^22.
+ *   the other inputs as npn_deltanet_verify's, T <= 64; Hv <= 4096, B <= 65536, B * Hv <= 2^22.
  * Outputs: out [B, T, Hv, 128] bf16; records, B * T * ((Hk + Hv) * 128 + Hv) f32, what
  * npn_deltanet_commit_tree needs of every node: k [B, T, Hk, 128] (normalised), u [B, T, Hv, 128]
  * and decay [B, T, Hv], S_t = decay_t S_parent + k_t u_t^T. */
@@ -647,8 +647,8 @@ int npn_accept_tree(const int64_t* target_ids, const int64_t* draft_ids, const i
  * path, in place and in one launch for up to 64 layers; requests with an empty path keep theirs.
  *   state, conv_state, mixed_qkv, records: host arrays of `layers` device pointers, layer l's
  *   [B, Hv, 128, 128] f32 state and [B, QKV, 3] bf16 window (both updated), the [B, T, QKV]
- *   bf16 inputs and records of its npn_deltanet_verify_tree. The layers' states and windows must
- *   not overlap (NPN_ERR_VALUE where two are the same). */
+ *   bf16 inputs and records of its npn_deltanet_verify_tree. Two layers' states or windows must
+ *   not overlap (NPN_ERR_VALUE). */
 int npn_deltanet_commit_tree(float* const* state, uint16_t* const* conv_state,
                              const uint16_t* const* mixed_qkv, const float* const* records,
                              int layers, const int32_t* path, int B, int T, int k_heads,
@@ -665,8 +665,8 @@ int npn_deltanet_commit_tree(float* const* state, uint16_t* const* conv_state,
  * first grows to the least power of two s with amax <= 448 s over the finite values of the rows
  * that move there, if that is more; the block's rows up to the path's last one are moved to it.
  * Rows that stay in a block whose scale stays, or come from one of the same scale, keep their
- * bytes; so do the rows behind the path. The layers' caches must not overlap (NPN_ERR_VALUE
- * where two are the same). */
+ * bytes; so do the rows behind the path. The layers' keys, values and scales must not
+ * overlap (NPN_ERR_VALUE). */
 int npn_gqa_compact_paged(const int32_t* path, const int64_t* slots, int8_t* const* cache_k,
                           int8_t* const* cache_v, float* const* k_scale, float* const* v_scale,
                           int layers, int B, int T, int kv_heads, int n_blocks, int block_size,

@@ -691,10 +691,14 @@ extern "C" int npn_deltanet_commit_tree(float* const* state, uint16_t* const* co
                                         int v_heads, void* stream) {
   NPN_REQUIRE(path && (layers == 0 || (state && conv_state && mixed_qkv && records)), NPN_ERR_NULL);
   NPN_REQUIRE(layers >= 0 && heads_ok(B, T, k_heads, v_heads), NPN_ERR_SHAPE);
+  const size_t states = sizeof(float) * B * v_heads * D * D;
+  const size_t windows = sizeof(uint16_t) * 3 * B * (2 * k_heads + v_heads) * D;
   for (int l = 0; l < layers; ++l) {
     NPN_REQUIRE(state[l] && conv_state[l] && mixed_qkv[l] && records[l], NPN_ERR_NULL);
     NPN_REQUIRE(NPN_ALIGNED16(state[l]), NPN_ERR_ALIGN);
-    for (int k = 0; k < l; ++k) NPN_REQUIRE(state[k] != state[l] && conv_state[k] != conv_state[l], NPN_ERR_VALUE);
+    for (int k = 0; k < l; ++k)
+      NPN_REQUIRE(npn_apart(state[k], states, state[l], states) && npn_apart(conv_state[k], windows, conv_state[l], windows),
+                  NPN_ERR_VALUE);
   }
   const int per = ((2 * k_heads + v_heads) * D + 255) / 256;
   const int64_t blocks = (int64_t)B * (v_heads + per);  // a layer's workgroups

@@ -167,6 +167,12 @@ __device__ __forceinline__ void lds_dma16_soff(const void* sbase, unsigned voff,
 
 #define NPN_ALIGNED16(p) ((reinterpret_cast<uintptr_t>(p) & 15u) == 0)
 
+// Whether n bytes at p and m bytes at q have none in common.
+static inline bool npn_apart(const void* p, size_t n, const void* q, size_t m) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b ? b - a >= n : a - b >= m;
+}
+
 static inline int npn_launch_status() {
   hipError_t e = hipGetLastError();
   return e == hipSuccess ? NPN_OK : NPN_ERR_LAUNCH;

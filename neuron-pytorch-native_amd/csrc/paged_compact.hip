@@ -304,10 +304,19 @@ extern "C" int npn_gqa_compact_paged(const int32_t* path, const int64_t* slots, 
   NPN_REQUIRE(sh >= 0 && layers >= 0 && B >= 1 && B <= 65535 && T >= 1 && T <= npn::kMaxNodes &&
                   kv_heads >= 1 && kv_heads <= 1024 && n_blocks >= 1,
               NPN_ERR_SHAPE);
+  const size_t blocks = (size_t)n_blocks * kv_heads, pages = blocks * block_size * 256, scales = 4 * blocks;
   for (int l = 0; l < layers; ++l) {
     NPN_REQUIRE(cache_k[l] && cache_v[l] && k_scale[l] && v_scale[l], NPN_ERR_NULL);
     NPN_REQUIRE(NPN_ALIGNED16(cache_k[l]) && NPN_ALIGNED16(cache_v[l]), NPN_ERR_ALIGN);
-    for (int k = 0; k < l; ++k) NPN_REQUIRE(cache_k[k] != cache_k[l] && cache_v[k] != cache_v[l], NPN_ERR_VALUE);
+    for (int k = 0; k <= l; ++k)
+      NPN_REQUIRE((k == l || (npn_apart(cache_k[k], pages, cache_k[l], pages) &&
+                              npn_apart(cache_v[k], pages, cache_v[l], pages) &&
+                              npn_apart(k_scale[k], scales, k_scale[l], scales) &&
+                              npn_apart(v_scale[k], scales, v_scale[l], scales))) &&
+                      npn_apart(cache_k[k], pages, cache_v[l], pages) && npn_apart(cache_v[k], pages, cache_k[l], pages) &&
+                      npn_apart(k_scale[k], scales, v_scale[l], scales) &&
+                      npn_apart(v_scale[k], scales, k_scale[l], scales),
+                  NPN_ERR_VALUE);
   }
   for (int l0 = 0; l0 < layers; l0 += kCompactLayers) {
     CompactArgs a{};
