@@ -46,9 +46,9 @@ typedef _Float16 f16x2 __attribute__((__vector_size__(2 * sizeof(_Float16))));
 typedef __bf16 bf16x2 __attribute__((__vector_size__(2 * sizeof(__bf16))));
 typedef float f32x4 __attribute__((__vector_size__(4 * sizeof(float))));
 
-// One workgroup of four waves a (b, h); NT tiles of 16 nodes; wave w has columns 32 w + 2 i + {0, 1} of everything that
-// has the state's columns (lane (i, G): i = lane % 16, G = lane / 16), so that the products' results are the next ones'
-// operands where they are. Steps, with a barrier between them:
+// One workgroup of NW waves a (b, h); NT tiles of 16 nodes; wave w has columns CT (16 w + i) + [0, CT), CT = 8 / NW, of
+// everything that has the state's columns (lane (i, G): i = lane % 16, G = lane / 16), so that the products' results are the
+// next ones' operands where they are. Steps, with a barrier between them:
 //   1. conv, SiLU and norms, a row of 128 channels to a wave at a time, two channels a lane, into LDS;
 //   2. K S0, Q S0 and, tile by tile of the lower triangle, K K^T and Q K^T. In f16 MFMAs: a number is the sum of two
 //      f16 (x 2^12, the state's columns over a power of two of their own), of whose four products the
@@ -61,6 +61,10 @@ typedef float f32x4 __attribute__((__vector_size__(4 * sizeof(float))));
 // A node whose input is not finite has zeros in these sums, which reach all nodes of a tile, and is noted: NaN
 // goes to its own and its descendants' rows at the end.
 // APART: q's rows take k's place once those have been used, and v's after them, so that two workgroups of 64 nodes fit a CU.
+//
+// Bound by the state and the rows' bytes where heads are many and trees small: 1536 heads of 16 nodes 37.5 us (141 MB, 27.4
+// at a copy's rate); by the length of the steps above, one behind the other with a barrier between, where a CU has a head
+// or two: 48 heads of 16 nodes 9.2 us, of 64 nodes 21.7, 384 heads of 64 nodes 37.5 (65 MB, 13 us; its products take 5).
 template <int NT, int NW, bool APART>
 struct TreeSmem {
   static constexpr int TM = 16 * NT, kTiles = NT * (NT + 1) / 2;
@@ -130,7 +134,7 @@ struct Floats {
 };
 
 template <int NT, int NW, bool APART>
-__global__ __launch_bounds__(64 * NW, NT == 1 || APART ? NW / 2 : NW / 4) void dn_tree_verify_kernel(TreeArgs a) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && (NT == 1 || APART) ? 2 : NW / 4) void dn_tree_verify_kernel(TreeArgs a) {
   constexpr int TM = 16 * NT;
   constexpr int CT = 8 / NW;              // column tiles of a wave
   constexpr int RW = TM / NW;             // rows of a wave in step 1
@@ -593,7 +597,8 @@ struct CommitArgs {
 };
 
 // One workgroup a (layer, b, h), its 128 x 128 floats in registers: thread (r, c4) has rows r + 8 i of columns
-// 4 c4 .. + 3. The workgroups behind move the conv windows, a thread a channel.
+// 4 c4 .. + 3. The workgroups behind move the conv windows, a thread a channel. Bound by the states' bytes, read and
+// written once: 48 layers of 48 heads 65 us for 316 MB, 3 layers of 32 requests 131 us for 632 MB.
 __global__ __launch_bounds__(256) void dn_tree_commit_kernel(CommitArgs a) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int QKV = (2 * a.Hk + a.Hv) * D;
@@ -676,12 +681,17 @@ extern "C" int npn_deltanet_verify_tree(const float* state, const int32_t* paren
                    dt_bias, norm_weight, out, records, rec_u, rec_decay, B, T, k_heads, v_heads};
   const dim3 grid(B * v_heads);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool apart = B * v_heads > 256;
+  // Up to a head for each of the 256 CUs, eight waves: the steps are shorter. Above, two workgroups of four share a CU and
+  // each fills the other's waits. us with four waves (APART above 32 nodes) and with eight, at 48, 240, 288 and 768 heads:
+  //   16 nodes 10.1, 11.8, 15.5, 20.7 and 9.2, 11.3, 15.2, 22.6; 48 nodes 20, 23.0, 28.4, 46 and 17, 20.6, 35.4, 57;
+  //   64 nodes 25.8, 29.0, 36.9, 61 and 21.6, 25.4, 43.9, 72.
+  // 32 nodes have eight waves at all of them: 15, 21 at 288, 34 at 768 heads with four APART and 13, 21.4, 32 with eight.
+  const bool many = B * v_heads > 256;
   auto launch = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, s, a); };
-  if (T <= 16) launch(dn_tree_verify_kernel<1, 4, false>, 4);
+  if (T <= 16) many ? launch(dn_tree_verify_kernel<1, 4, false>, 4) : launch(dn_tree_verify_kernel<1, 8, false>, 8);
   else if (T <= 32) launch(dn_tree_verify_kernel<2, 8, false>, 8);
-  else if (T <= 48) apart ? launch(dn_tree_verify_kernel<3, 4, true>, 4) : launch(dn_tree_verify_kernel<3, 8, false>, 8);
-  else apart ? launch(dn_tree_verify_kernel<4, 4, true>, 4) : launch(dn_tree_verify_kernel<4, 8, false>, 8);
+  else if (T <= 48) many ? launch(dn_tree_verify_kernel<3, 4, true>, 4) : launch(dn_tree_verify_kernel<3, 8, false>, 8);
+  else many ? launch(dn_tree_verify_kernel<4, 4, true>, 4) : launch(dn_tree_verify_kernel<4, 8, false>, 8);
   return npn_launch_status();
 }
 
