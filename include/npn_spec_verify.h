@@ -605,9 +605,8 @@ size_t npn_gqa_tree_verify_paged_workspace_size(int B, int T, int q_heads, int k
  * npn_gqa_tail_verify_paged's attention over the pages, node t < q_len[b] seeing the keys
  * [0, kv_len[b]) and of those behind its ancestors and itself (node s's row is the one at
  * kv_len[b] + s of the block table). Rows t >= q_len[b] are 0. Other arguments, roundings and
- * limits as in those two; T <= 64. (Of a chain's outputs these are the same bits where its rows are
- * cut into the same groups: up to 48 always, above where groups of 128 are more than three
- * quarters full.) */
+ * limits as in those two; T <= 64. (Of a chain's outputs these are the same bits for up to 48
+ * rows of a kv head, T * q_heads / kv_heads.) */
 int npn_gqa_tree_verify_paged(const uint16_t* query, const uint16_t* gate, const uint16_t* key,
                               const uint16_t* value, const float* q_norm, const float* k_norm,
                               const float* cos_table, const float* sin_table, int positions,

@@ -55,6 +55,15 @@
 //     overlap little: without the softmax 100 us would remain, without V's products 100, without the DMAs
 //     123. Priorities for one wave of each SIMD, its V products half a step behind the other's, or LDS
 //     reads ahead of the products before them changed nothing.
+//  2c. the same of a tree: four waves of 32 rows, one to a SIMD, share steps of 64 keys in f16, K's and V's bytes made f16 for
+//     32 rows at a time in 32x32x16 products. A lane (i, G) has 16 keys of row i in a tile of 32, in order, so that P is
+//     again the next product's operand where it is, over powers of two as in 2. The next step's scores are computed
+//     between this step's weights. Of a step's 4700 cycles its products take 2200 and the bytes' conversion 1700, in
+//     the same issue slots as the softmax's 1400 and the DMAs, the page ids and the barrier's 800; start and end 13000 each: the plan,
+//     the first bytes' way, and the parts' 128 KB. 16 requests of 64 x 6 rows over up to 8192 keys 160 us, 720 TFLOP/s
+//     by the formula's operations (2b with a tree's masks 200); 8 of 32 x 6 rows 60 (groups of 48: 73).
+//     Tried: DMAs between the products, whose branches had registers spilled (283 us for 232 in all); two chains of
+//     products at once, as fast as one; the longest workgroups first, as fast.
 //  3. merge: the log-sum-exp merge of the other pairs' workgroups, times sigmoid(gate), to bf16.
 // prep takes 4 to 9 us and merge 5 to 10 for these.
 #include "npn_common.h"
@@ -81,6 +90,7 @@ typedef _Float16 f16x8 __attribute__((__vector_size__(8 * sizeof(_Float16))));
 typedef _Float16 f16x2 __attribute__((__vector_size__(2 * sizeof(_Float16))));
 typedef float f32x4 __attribute__((__vector_size__(4 * sizeof(float))));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((__vector_size__(16 * sizeof(float))));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 struct PagedArgs {
@@ -160,9 +170,12 @@ __device__ __forceinline__ float max_over_pair(float x) {
   return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 __device__ __forceinline__ float max_over_groups(float x) { return max_over_pair(max_over_halves(x)); }
-__device__ __forceinline__ float sum_over_groups(float x) {
+__device__ __forceinline__ float sum_over_halves(float x) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ float sum_over_groups(float x) {
+  x = sum_over_halves(x);
   const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
@@ -230,6 +243,7 @@ __device__ __forceinline__ void lds_write(unsigned base, int k, u32x4 v) {
 // With a SIMD to itself a wave's accumulators stay in AGPRs: without a word at the places where VALU
 // work touches them, the compiler carried them in VGPRs and copied all of them twice a step.
 __device__ __forceinline__ void pin(f32x4& x) { asm volatile("" : "+a"(x)); }
+__device__ __forceinline__ void pin(f32x16& x) { asm volatile("" : "+a"(x)); }
 __device__ __forceinline__ unsigned opaque(unsigned x) {
   asm volatile("" : "+v"(x));
   return x;
@@ -304,7 +318,7 @@ constexpr int kPlanUnits = 4096;  // units whose steps the plan keeps in LDS
 // so that a second round of workgroups may pay where the first leaves many CUs idle: 512 x 6 rows over
 // 16384 keys, 96 pairs, take 330 us in 192 workgroups and 290 in 480. The plan takes the cheaper by the
 // steps of 128 keys that the rounds last, with 1.5 for a workgroup's start and end and 2.5 for writing
-// and merging the parts of 256.
+// and merging the parts of 256. (Of trees the steps have 64 keys, and start and end take as long as five of them.)
 __host__ __device__ constexpr int most_workgroups(int R, int pairs, int rounds) {
   return R == kRows && rounds == 2 && pairs > 64 && pairs <= 448 ? 512 : pairs <= 160 ? 256 : pairs + 512;
 }
@@ -376,7 +390,8 @@ __device__ void plan_block(const PagedArgs& a) {
   int made;
   int Q = least(most_workgroups(a.R, pairs, 1), made);
   if (a.R == kRows && most_workgroups(a.R, pairs, 2) > most_workgroups(a.R, pairs, 1)) {
-    auto cost = [&](int q, int g) { return up(g, 256) * (q + 1.5f) + g * 0.01f; };
+    const float part = a.ks == KS ? 5.0f : 1.5f, join = a.ks == KS ? 0.02f : 0.01f;
+    auto cost = [&](int q, int g) { return up(g, 256) * (q + part) + g * join; };
     const float one = cost(Q, made);
     const int Q2 = least(most_workgroups(a.R, pairs, 2), made);
     if (cost(Q2, made) < one) Q = Q2;
@@ -473,7 +488,7 @@ __device__ __forceinline__ void prep_rows(const PagedArgs& a, const int32_t* par
     float inv = __uint_as_float((253u - e) << 23);                      // 2^-(e - 126)
     float q_scale = __uint_as_float((e + 1) << 23) * (kLog2e / 16.0f);
     const int d = 4 * lane;
-    if (a.R == kRows) {  // three e4m3 parts of 256 times as much
+    if (!TREE && a.R == kRows) {  // three e4m3 parts of 256 times as much
       inv *= 256.0f;
       q_scale *= 1.0f / 256;
       if (lane == 0) a.q_scale[(size_t)pair * a.R + r] = q_scale;
@@ -492,8 +507,14 @@ __device__ __forceinline__ void prep_rows(const PagedArgs& a, const int32_t* par
       const f16x2 x = {(_Float16)(v[2 * j] * inv), (_Float16)(v[2 * j + 1] * inv)};
       two[j] = __builtin_bit_cast(uint32_t, x);
     }
-    const int step = 2 * (d >> 6) + ((d >> 3) & 1), g = (d >> 4) & 3;
-    u32x4* dst = a.q + (((size_t)pair * 8 + step) * (a.R / 16) + (r >> 4)) * 64 + 16 * g + (r & 15);
+    u32x4* dst;
+    if (TREE && a.R == kRows) {  // d = 32 c + 16 g + 8 h + e, k step 2 c + h of 16, rows 32 to a product
+      const int step = 2 * (d >> 5) + ((d >> 3) & 1), g = (d >> 4) & 1;
+      dst = a.q + (((size_t)pair * 4 + (r >> 5)) * 16 + step) * 64 + 32 * g + (r & 31);
+    } else {
+      const int step = 2 * (d >> 6) + ((d >> 3) & 1), g = (d >> 4) & 3;
+      dst = a.q + (((size_t)pair * 8 + step) * (a.R / 16) + (r >> 4)) * 64 + 16 * g + (r & 15);
+    }
     *reinterpret_cast<uint2*>(reinterpret_cast<uint32_t*>(dst) + ((d & 4) >> 1)) = make_uint2(two[0], two[1]);
   }
 }
@@ -978,7 +999,6 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
 }
 
 // ---- 2b. attn of many rows ----------------------------------------------------------------------------
-template <bool TREE>
 struct RowsSmem {
   union {
     uint8_t ring[2][65536];  // two steps of 128 keys: for each half two groups of K and two of V, as above
@@ -986,18 +1006,15 @@ struct RowsSmem {
   };
   float inv[kRows];
   int lim[kRows];
-  int nan_key[TREE ? 1 : DH];        // the first key past lim0 whose value at a dim is NaN
-  uint64_t anc[TREE ? kRows : 1];    // what a row sees of the nodes; 0: not even the committed keys
-  uint64_t nan_node[TREE ? DH : 1];  // the nodes whose value at a dim is NaN; all where a committed key's is
+  int nan_key[DH];         // the first key past lim0 whose value at a dim is NaN
   int page[kPages];
   float ks[kPages], vs[kPages];
 };
 
-template <bool TREE>
 __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
   constexpr int R = kRows, KR = 128, kSteps = kChunk * KS / KR;
   constexpr int kTop = 7;  // a block's largest weight is taken to [2^kTop, 2^(kTop + 1))
-  __shared__ __attribute__((aligned(1024))) RowsSmem<TREE> sm;
+  __shared__ __attribute__((aligned(1024))) RowsSmem sm;
   const int tid = threadIdx.x;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int i = lane & 15, G = lane >> 4;
@@ -1017,10 +1034,9 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
 
   const int r = 16 * w + i, t = a.token_of(row0 + r);  // this lane's row and its last key, or -1
   int lim = r < rows && t < a.q_len[un.b] ? min(un.kv + t, un.kend - 1) : -1;
-  uint64_t anc = TREE ? a.anc[(size_t)un.b * a.T + min(t, a.T - 1)] : 0;
   float q_scale = a.q_scale[(size_t)pair * R + r];
   float m_run = kNegBig, w_run = kNegBig, l_run = 0.f;
-  const int lim0 = TREE ? un.kv - 1 : un.kv + un.t0;
+  const int lim0 = un.kv + un.t0;
   i32x8 q[2][3];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -1072,18 +1088,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
           v[k] &= keep_bytes(live - 4 * k);
           const uint32_t nan = nan_bytes(v[k]);
           if (nan != 0) {
-            const int dim = 16 * (w + 8 * n) + i, key = k1 + 4 * k;
-            if constexpr (TREE) {
-              uint64_t nodes = 0;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int at = key + e - un.kv;  // below 64: behind kend they have been cleared
-                if ((nan >> (8 * e)) & 1) nodes |= at < 0 ? ~0ull : 1ull << at;
-              }
-              atomicOr(reinterpret_cast<unsigned long long*>(&sm.nan_node[dim]), (unsigned long long)nodes);
-            } else {
-              atomicMin(&sm.nan_key[dim], key + (__ffs(nan) - 1) / 8);
-            }
+            atomicMin(&sm.nan_key[16 * (w + 8 * n) + i], k1 + 4 * k + (__ffs(nan) - 1) / 8);
             v[k] &= ~nan;
           }
         }
@@ -1111,14 +1116,10 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
     }
     __syncthreads();
   };
-  if (tid < DH) {
-    if constexpr (TREE) sm.nan_node[tid] = 0;
-    else sm.nan_key[tid] = 0x7FFFFFFF;
-  }
+  if (tid < DH) sm.nan_key[tid] = 0x7FFFFFFF;
   begin_chunk(0);
   // What was loaded so far is waited for before the first DMAs.
   asm volatile("" : "+v"(lim), "+v"(q_scale));
-  if constexpr (TREE) asm volatile("" : "+v"(anc));
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -1181,20 +1182,14 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
           __builtin_amdgcn_sched_barrier(0);
         }
 
-      uint32_t see_bits[2];  // trees
       if (tail) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int kb = k0 + KS * half + 16 * G;
-          if constexpr (TREE) see_bits[half] = seen16(anc, kb - un.kv, lim + 1 - kb);
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if constexpr (TREE) st[half][j][e] = if_seen(held[half] ? see_bits[half] : 0u, 4 * j + e, st[half][j][e]);
-              else if (!held[half] || kb + 4 * j + e > lim) st[half][j][e] = -INFINITY;
-            }
-        }
+            for (int e = 0; e < 4; ++e)
+              if (!held[half] || k0 + KS * half + 16 * G + 4 * j + e > lim) st[half][j][e] = -INFINITY;
       }
 
       // Beside the row's maxima, `top` of each block of 32 keys that its products take as one: those of
@@ -1202,7 +1197,7 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
       float c[2], mx = -INFINITY, top[2];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const bool hidden = tail && (TREE ? see_bits[half] == 0 : k0 + KS * half + 16 * G > lim);
+        const bool hidden = tail && k0 + KS * half + 16 * G > lim;
         c[half] = hidden ? 1.0f : not_zero(ks[half] * q_scale);
         vs[half] = hidden ? 0.0f : vs[half];
         float x = st[half][0][0];
@@ -1284,7 +1279,6 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
   if (G == 0) {
     sm.inv[r] = l != 0.f ? 1.0f / l : 0.f;
     sm.lim[r] = lim;
-    if constexpr (TREE) sm.anc[r] = lim >= 0 ? anc : 0;
     if (parts > 1) {
       a.part_ml[(slot * R + r) * 2] = m_run;
       a.part_ml[(slot * R + r) * 2 + 1] = l;
@@ -1297,10 +1291,392 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
     x += x * 0.0f;  // infinite: NaN
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (TREE ? (sm.anc[TREE ? rk : 0] & sm.nan_node[TREE ? 4 * lane + e : 0]) != 0
-               : sm.lim[rk] >= sm.nan_key[TREE ? 0 : 4 * lane + e])
-        x[e] = NAN;
+      if (sm.lim[rk] >= sm.nan_key[4 * lane + e]) x[e] = NAN;
+    if (parts > 1)
+      *reinterpret_cast<f32x4*>(a.part_o + (slot * R + rk) * DH + 4 * lane) = x;
+    else if (rk < rows)
+      write_out(a, un.b, row0 + rk, h, 4 * lane, x, sm.inv[rk]);
+  }
+}
+
+// ---- 2c. attn of many rows of a tree -------------------------------------------------------------------
+// Four DMAs of 1 KB each: from a uniform base + o0, o1, o0 and o1, the later ones 1, 2 and 3 KB behind, as are their places.
+__device__ __forceinline__ void lds_dma16x4_soff(const void* sbase, unsigned o0, unsigned o1, unsigned lds) {
+  unsigned saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %4\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %3\n\t"
+      "global_load_lds_dwordx4 %2, %3 offset:1024\n\t"
+      "global_load_lds_dwordx4 %1, %3 offset:2048\n\t"
+      "global_load_lds_dwordx4 %2, %3 offset:3072\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(o0), "v"(o1), "s"(sbase), "s"(lds)
+      : "memory");
+}
+// The same from per-lane addresses, `step` bytes apart.
+__device__ __forceinline__ void lds_dma16x4(const uint8_t* g, size_t step, unsigned lds) {
+  unsigned saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %5\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off\n\t"
+      "s_add_u32 m0, m0, 0x400\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %2, off\n\t"
+      "s_add_u32 m0, m0, 0x400\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %3, off\n\t"
+      "s_add_u32 m0, m0, 0x400\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %4, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(g), "v"(g + step), "v"(g + 2 * step), "v"(g + 3 * step), "s"(lds)
+      : "memory", "scc");
+}
+
+struct TreeRowsSmem {
+  union {
+    uint8_t ring[4][32768];  // four steps of 64 keys: K, 64 rows of 256 bytes, and V, 16 groups of 16 dims
+    f32x4 o[4][32][64];      // 32 rows of 256 to a wave
+  };
+  float inv[kRows];
+  uint64_t anc[kRows];   // what a row sees of the nodes; 0: not even the committed keys
+  uint64_t nan_node[DH]; // the nodes whose value at a dim is NaN; all where a committed key's is
+  int page[kPages];
+  float ks[kPages], vs[kPages];
+};
+
+__global__ __launch_bounds__(256, 1) void paged_tree_rows_kernel(PagedArgs a) {
+  constexpr int R = kRows;
+  constexpr int NS = 4;  // steps in LDS
+  __shared__ __attribute__((aligned(1024))) TreeRowsSmem sm;
+  const int tid = threadIdx.x;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int i = lane & 31, G = lane >> 5;
+  const int bs = 1 << a.sh;
+  const int U = a.units();
+
+  if ((int)blockIdx.x >= a.wstart[U]) return;
+  const int u = last_start(a.wstart, U, (int)blockIdx.x);
+  const Unit un = unit_of(a, u);
+  const int w0 = a.wstart[u], parts = (a.wstart[u + 1] - w0) / a.Hkv;
+  const int h = ((int)blockIdx.x - w0) / parts, part = (int)blockIdx.x - w0 - h * parts;
+  const int s_lo = (int)((int64_t)part * un.steps / parts);
+  const int steps = (int)((int64_t)(part + 1) * un.steps / parts) - s_lo;
+  const int pair = u * a.Hkv + h;
+  const int row0 = (u - un.b * a.RG) * R;
+  const int rows = min(R, a.T * a.grp - row0);
+
+  const int r = 32 * w + i, t = a.token_of(row0 + r);  // this lane's row and its last key, or -1
+  int lim = r < rows && t < a.q_len[un.b] ? min(un.kv + t, un.kend - 1) : -1;
+  uint64_t anc = a.anc[(size_t)un.b * a.T + min(t, a.T - 1)];
+  float q_scale = a.q_scale[(size_t)pair * R + r];
+  float m_run = kNegBig, w_run = kNegBig, l_run = 0.f;
+  u32x4 q[16];
+  {
+    const u32x4* src = a.q + ((size_t)pair * 4 + w) * 16 * 64 + lane;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) q[k] = src[64 * k];
+  }
+
+  // K goes four whole rows to a DMA, column c of row r to place c ^ f(r) of the row's 256 bytes, f(r) = bits 0, 1, 4 and 2 of
+  // r: lane (i, G)'s row of a tile, bits 0, 1, 3, 4 and 2 of i, has f = i % 16. V's groups of 16 dims lie as they come.
+  const unsigned ring_lds = __builtin_amdgcn_readfirstlane(npn::lds_addr(&sm.ring[0][0]));
+  const int i16 = lane & 15, G16 = lane >> 4;
+  const unsigned ksrc = (unsigned)(G16 * DH + ((i16 ^ G16) << 4)) ^ ((w & 1) << 6);
+  const unsigned k_at = ring_lds + (unsigned)((16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3)) * DH + ((G ^ i16) << 4));
+  const unsigned v_at = ring_lds + 16384u + (unsigned)((i >> 4) * 1024 + G * 256 + i16 * 16);
+
+  int cn, key0, page0;
+  bool missing;  // a page of the chunk is none
+  // A wave's eight of a step's 32 DMAs: rows 16 k + 4 w .. + 3 of K, dims 16 (w + 4 k) .. + 15 of V.
+  // Pages of a wave's part of a step: keys 16 w .. + 15 of K, and of V the lane's 16 keys of dims 64 w .. + 63.
+  int k_id, v_id;
+  auto pages_of = [&](int s) __attribute__((always_inline)) {
+    const int k0 = key0 + min(s, cn - 1) * KS;
+    k_id = sm.page[((k0 + 16 * w) >> a.sh) - page0];
+    v_id = sm.page[((k0 + 16 * G16) >> a.sh) - page0];
+  };
+  auto load_step = [&](int s) __attribute__((always_inline)) {
+    const unsigned at = ring_lds + (unsigned)((s & (NS - 1)) * 32768 + w * 4096);
+    const int kk = key0 + s * KS + 16 * w, kv = key0 + s * KS + 16 * G16;
+    const int id = __builtin_amdgcn_readfirstlane(max(k_id, 0));
+    lds_dma16x4_soff(a.cache_k + ((((size_t)id * a.Hkv + h) << a.sh) + (kk & (bs - 1))) * DH, ksrc, ksrc ^ 128u, at);
+    const uint8_t* const vp =
+        a.cache_v + ((((size_t)max(v_id, 0) * a.Hkv + h) * DH + 64 * w + i16) << a.sh) + (kv & (bs - 1));
+    lds_dma16x4(vp, (size_t)16 << a.sh, at + 16384);
+  };
+  // V bytes of keys that no row sees are cleared (0 times NaN is NaN), each wave those that it sent for. So
+  // is a NaN at a key that some rows see, and the key's node noted at its dim: the rows that see it get the NaN
+  // at the end.
+  auto clean = [&](int k0, unsigned place) __attribute__((always_inline)) {
+    const int k1 = k0 + 16 * G16;
+    const int live = sm.page[(k1 >> a.sh) - page0] >= 0 ? un.kend - k1 : 0;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const unsigned at = opaque(ring_lds + place + 16384u + (unsigned)((4 * w + n) * 1024 + lane * 16));
+      u32x4 v = lds_read(at, 0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] &= keep_bytes(live - 4 * k);
+        const uint32_t nan = nan_bytes(v[k]);
+        if (nan != 0) {
+          uint64_t nodes = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int node = k1 + 4 * k + e - un.kv;  // below 64: behind kend they have been cleared
+            if ((nan >> (8 * e)) & 1) nodes |= node < 0 ? ~0ull : 1ull << node;
+          }
+          atomicOr(reinterpret_cast<unsigned long long*>(&sm.nan_node[16 * (4 * w + n) + i16]), (unsigned long long)nodes);
+          v[k] &= ~nan;
+        }
+      }
+      lds_write(at, 0, v);
+    }
+  };
+  auto begin_chunk = [&](int c0) __attribute__((always_inline)) {
+    cn = min(kChunk, steps - c0);
+    key0 = (s_lo + c0) * KS;
+    page0 = key0 >> a.sh;
+    const int pages = ((min(key0 + cn * KS, un.kend) - 1) >> a.sh) - page0 + 1;
+    __syncthreads();  // the last chunk's pages and steps have been used
+    int none = 0;
+    for (int p = tid; p < kPages; p += 256) {
+      int id = -1;
+      if (p < pages) id = a.table[(size_t)un.b * a.P + page0 + p];
+      const bool ok = id >= 0 && id < a.N;
+      sm.page[p] = ok ? id : -1;
+      none |= p < pages && !ok;
+      sm.ks[p] = ok ? a.k_scale[(size_t)id * a.Hkv + h] : 1.0f;
+      sm.vs[p] = ok ? log2f(a.v_scale[(size_t)id * a.Hkv + h]) : 0.0f;
+    }
+    missing = __syncthreads_or(none) != 0;
+  };
+  auto first_sends = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < NS - 2; ++s)
+      if (s < cn) {
+        pages_of(s);
+        load_step(s);
+      }
+    pages_of(NS - 2);
+  };
+  for (int d = tid; d < DH; d += 256) sm.nan_node[d] = 0;
+  begin_chunk(0);
+  // What was loaded so far is waited for before the first DMAs.
+  asm volatile("" : "+v"(lim), "+v"(q_scale), "+v"(anc));
+#pragma unroll
+  for (int k = 0; k < 16; ++k) asm volatile("" : "+v"(q[k]));
+  first_sends();
+
+  // The step has landed for every wave past the barrier, and all are done with the step before, whose place the next
+  // one to be sent takes. Whether the step is masked.
+  auto begin_step = [&](int s, int k0, unsigned place) __attribute__((always_inline)) {
+    const bool tail = k0 + KS > un.kv || missing;
+    if (tail) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      clean(k0, place);
+    } else if (s + 1 < cn) {
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (s + NS - 2 < cn) load_step(s + NS - 2);
+    return tail;
+  };
+  const bool idle = __builtin_amdgcn_ballot_w64(lim >= 0) == 0;  // a wave without a row: only its part of the DMAs
+  f32x16 acc[8];
+#pragma unroll
+  for (int d = 0; d < 8; ++d) acc[d] = f32x16{};
+
+  for (int c0 = 0; idle && c0 < steps; c0 += kChunk) {
+    if (c0 > 0) {
+      begin_chunk(c0);
+      first_sends();
+    }
+    for (int s = 0; s < cn; ++s) {
+      begin_step(s, key0 + s * KS, (unsigned)(s & (NS - 1)) * 32768u);
+      pages_of(s + NS - 1);
+    }
+  }
+  u32x4 kw[3][2];
+  unsigned kat;
+  auto read_k = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) kw[c % 3][j] = lds_read(kat ^ (c << 5), 8 * j);
+  };
+  auto score = [&](f32x16 (&st)[2], int c) __attribute__((always_inline)) {  // dims 32 c .. + 31
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        st[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(to_f16x8(kw[c % 3][j][2 * b], kw[c % 3][j][2 * b + 1]),
+                                                       __builtin_bit_cast(f16x8, q[2 * c + b]), st[j], 0, 0, 0);
+  };
+  for (int c0 = 0; !idle && c0 < steps; c0 += kChunk) {
+    if (c0 > 0) {
+      begin_chunk(c0);
+      first_sends();
+    }
+    bool tail = begin_step(0, key0, 0);
+    f32x16 sn[2] = {f32x16{}, f32x16{}};
+    kat = opaque(k_at);
+    read_k(0);
+    read_k(1);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      if (c + 2 < 8) read_k(c + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      score(sn, c);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    for (int s = 0; s < cn; ++s) {
+#pragma unroll
+      for (int d = 0; d < 8; ++d) pin(acc[d]);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) asm volatile("" : "+v"(q[k]));
+      const int k0 = key0 + s * KS;
+      f32x16 st[2] = {sn[0], sn[1]};
+      asm volatile("" : "+v"(st[0]), "+v"(st[1]));
+      pages_of(s + NS - 1);
+      float ks[2], vs[2];
+      bool hidden[2] = {false, false};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int page = ((k0 + 32 * j + 16 * G) >> a.sh) - page0;
+        ks[j] = sm.ks[page];
+        vs[j] = sm.vs[page];
+        if (tail) {
+          const int kb = k0 + 32 * j + 16 * G;
+          const uint32_t bits = sm.page[page] >= 0 ? seen16(anc, kb - un.kv, lim + 1 - kb) : 0u;
+          hidden[j] = bits == 0;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) st[j][e] = if_seen(bits, e, st[j][e]);
+        }
+      }
+
+      float c[2], mx = -INFINITY, wx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        c[j] = hidden[j] ? 1.0f : not_zero(ks[j] * q_scale);
+        vs[j] = hidden[j] ? 0.0f : vs[j];
+        float x = st[j][0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) x = fmaxf(x, st[j][e]);
+        mx = fmaxf(mx, x * c[j]);
+        wx = fmaxf(wx, x * c[j] + vs[j]);
+      }
+      mx = max_over_halves(mx);
+      wx = max_over_halves(wx);
+      const bool grow = mx > m_run + kRescaleLog2, wgrow = wx > w_run + kRescaleLog2;
+      if (__builtin_amdgcn_ballot_w64(grow || wgrow) != 0) {
+        const float mnew = grow ? mx : m_run, wnew = wgrow ? wx : w_run;
+        const float corr = exp2f(w_run - wnew);
+        l_run *= exp2f(m_run - mnew);
+        m_run = mnew;
+        w_run = wnew;
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+          pin(acc[d]);  // (else it is read in every step)
+          acc[d] *= corr;
+          pin(acc[d]);
+        }
+      }
+      const unsigned place = (unsigned)(s & (NS - 1)) * 32768u, after = (unsigned)((s + 1) & (NS - 1)) * 32768u;
+      if (s + 1 < cn) tail = begin_step(s + 1, k0 + KS, after);
+      // The next step's scores between this one's weights (behind the last step they are no step's).
+      kat = opaque(k_at + after);
+      const unsigned vat = opaque(v_at + place);
+      read_k(0);
+      read_k(1);
+      float f[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) f[j] = exp2_bounded(m_run + vs[j] - w_run + kPLog2);
+      f16x8 pw[2][2];
+      u32x4 v[3][2];
+      sn[0] = sn[1] = f32x16{};
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        if (n + 2 < 8) {
+          read_k(n + 2);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) v[n - 6][j] = reinterpret_cast<lds_u32x4*>(vat)[128 * (n - 6) + 32 * j];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        score(sn, n);
+        const int j = n >> 2;
+#pragma unroll
+        for (int e = 4 * (n & 3); e < 4 * (n & 3) + 4; ++e) {
+          const float pv = __builtin_amdgcn_exp2f(fmaf(st[j][e], c[j], -m_run));
+          sum[j] += pv;
+          pw[j][e >> 3][e & 7] = (_Float16)(pv * f[j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      l_run += sum[0] + sum[1];
+#pragma unroll
+      for (int d = 0; d < 8; ++d) pin(acc[d]);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        if (d + 2 < 8) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) v[(d + 2) % 3][j] = reinterpret_cast<lds_u32x4*>(vat)[128 * (d + 2) + 32 * j];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(to_f16x8(v[d % 3][j][2 * b], v[d % 3][j][2 * b + 1]), pw[j][b],
+                                                            acc[d], 0, 0, 0);
+        pin(acc[d]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
+
+  // A wave has its rows whole: through LDS, for stores of whole rows, 16 bytes at f of dim 4 f to place
+  // f ^ i of row i.
+  const float l = sum_over_halves(l_run), scale = exp2f(w_run - m_run - kPLog2);
+  const size_t slot = (size_t)a.sstart[u] + h * parts + part;
+  __syncthreads();  // every wave is done with the ring
+  f32x4* const o = &sm.o[w][0][0];
+#pragma unroll
+  for (int d = 0; d < 8; ++d)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f32x4 x = {acc[d][4 * k], acc[d][4 * k + 1], acc[d][4 * k + 2], acc[d][4 * k + 3]};
+      o[64 * i + ((8 * d + 2 * k + G) ^ i16)] = x * scale;
+    }
+  if (G == 0) {
+    sm.inv[r] = l != 0.f ? 1.0f / l : 0.f;
+    sm.anc[r] = lim >= 0 ? anc : 0;
+    if (parts > 1) {
+      a.part_ml[(slot * R + r) * 2] = m_run;
+      a.part_ml[(slot * R + r) * 2 + 1] = l;
+    }
+  }
+  __syncthreads();
+  uint64_t nan[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) nan[e] = sm.nan_node[4 * lane + e];
+#pragma unroll 4
+  for (int k = 0; k < 32; ++k) {
+    const int rk = 32 * w + k;
     if (rk >= rows) break;
+    f32x4 x = o[64 * k + (lane ^ (k & 15))];
+    x += x * 0.0f;  // infinite: NaN
+    const uint64_t sees = sm.anc[rk];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if ((sees & nan[e]) != 0) x[e] = NAN;
     if (parts > 1)
       *reinterpret_cast<f32x4*>(a.part_o + (slot * R + rk) * DH + 4 * lane) = x;
     else
@@ -1393,23 +1769,24 @@ PagedPlan paged_plan(int B, int T, int q_heads, int kv_heads, int max_blocks, in
   // and 98, 2 of 1536 128 and 165; 16 of 96 146 and 148; but 4 of 192 59 and 54, one of 1536 over an empty
   // cache 35 and 30.
   p.R = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 48 ? 48 : kRows;
-  // Trees have groups of 48, nearly full, where those of 128 are a quarter empty or more: 16 requests of 144 rows over
-  // up to 16384 keys 207 us and 251 with groups of 128, 2 of them 49 and 59; one of 96 rows over 32768 47 and 50, of 192
-  // over 16384 47.1 and 48.4; but 16 of 96 159 and 152, and one of 60, half empty in both, 47 and 42.
-  const int64_t by48 = (rows + 47) / 48 * 48, by128 = (rows + kRows - 1) / kRows * kRows;
-  if (tree && by48 * 4 <= by128 * 3 && rows * 8 >= by48 * 7) p.R = rows <= 48 ? p.R : 48;
+  // Trees have groups of 128 too, but where there are few pairs, and groups of 48 nearly full, those: one request of 96 rows
+  // over 16384 keys of one head 30 us and 36 with groups of 128, two of 144 rows over 4 heads 49 and 54; 4 of 96 rows over
+  // up to 16384 keys 53 and 52, 16 of them 158 and 126, 8 of 192 rows over up to 8192 91 and 77.
+  const int64_t by48 = (rows + 47) / 48, by128 = (rows + kRows - 1) / kRows;
+  if (tree && rows > 48 && by48 * 48 * 4 <= by128 * kRows * 3 && rows * 8 >= by48 * 48 * 7 && B * by48 * kv_heads < 32)
+    p.R = 48;
   p.RG = (int)((rows + p.R - 1) / p.R);
   const int64_t pairs = (int64_t)B * p.RG * kv_heads;
   const int64_t keys = (int64_t)max_blocks * block_size;
   if (pairs > 65535 || pairs * ((keys + KS - 1) / KS) >= (int64_t)1 << 30) return p;
   p.pairs = (int)pairs;
   p.nw = p.R == 16 ? 8 : p.R == kRows ? 1 : 4;
-  p.ks = p.R == kRows ? 2 * KS : KS;
+  p.ks = p.R == kRows && !tree ? 2 * KS : KS;
   p.grid = max(most_workgroups(p.R, p.pairs, 1), most_workgroups(p.R, p.pairs, 2));
   const size_t slots = p.grid == 256 ? 256 : kSlots;
   const size_t units = (size_t)B * p.RG;
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  p.o_qs = up((size_t)pairs * p.R * DH * (p.R == kRows ? 3 : 2));
+  p.o_qs = up((size_t)pairs * p.R * DH * (p.R == kRows && !tree ? 3 : 2));
   p.o_po = p.o_qs + up((size_t)pairs * p.R * sizeof(float));
   p.o_ml = p.o_po + up(slots * p.R * DH * sizeof(float));
   p.o_an = p.o_ml + up(slots * p.R * 2 * sizeof(float));
@@ -1449,8 +1826,10 @@ void launch_attn(const PagedPlan& p, const PagedArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((paged_attn_kernel<2, 4, TREE>), dim3(p.grid), dim3(256), 0, s, a);
   else if (p.R == 48)
     hipLaunchKernelGGL((paged_attn_kernel<3, 4, TREE>), dim3(p.grid), dim3(256), 0, s, a);
+  else if (TREE)
+    hipLaunchKernelGGL(paged_tree_rows_kernel, dim3(p.grid), dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL(paged_rows_kernel<TREE>, dim3(p.grid), dim3(512), 0, s, a);
+    hipLaunchKernelGGL(paged_rows_kernel, dim3(p.grid), dim3(512), 0, s, a);
   if (p.pairs < 32 || p.pairs * p.R < 96 * 16)
     hipLaunchKernelGGL(paged_merge_kernel<4>, dim3(p.R, p.pairs), dim3(256), 0, s, a);
   else

@@ -335,7 +335,7 @@ def test_tree_verify_paged_of_a_chain_is_append_and_verify(ops, T):
     query, gate, key, value, qn, kn, cos, sin, *cache, table, kv, slots, n, _ = _args(d)
     ops.gqa.kv_append_paged(key, value, kn, cos, sin, kv, slots, *cache)
     want = ops.gqa.tail_verify_paged(query, gate, qn, cos, sin, *cache, table, kv, n)
-    if T == 30:  # groups of other sizes: both within the tolerance of the formula, so within twice that of each other
+    if T >= 30:  # another kernel's roundings: both within the tolerance of the formula, so within twice that of each other
         assert_rel_close(out.float().cpu().numpy(), want.float().cpu().numpy(), tol=4e-3, out_unit=2 * BF16_U)
     else:
         assert torch.equal(out, want)
