@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+from oracle import tree as ot
 from _util import BF16_U, assert_rel_close
 from test_gpu_tree import _args, _attend_inputs, cuda, trees
 
@@ -118,3 +119,40 @@ def test_on_a_stream_of_its_own(ops):
         out = ops.gqa.tree_verify_paged(*args)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(args[8:12], want_args[8:12]))
+
+
+@pytest.mark.parametrize("T", [5, 40])
+@pytest.mark.parametrize("k_exp,v_exp", [((-9, -5), (-120, 60)), ((-110, -5), (-9, -5)), ((-7, -4), (-100, -96)),
+                                         ((-9, -5), (-126, -126))])
+def test_scales_far_apart(ops, T, k_exp, v_exp):
+    """Pages whose scales are any powers of two between these: the formula's outputs, small or large as they are."""
+    d = _attend_inputs(2, T, 2, 6, 16, [300, 45], [T, T], max(1, T // 4), seed=T)
+    rng = np.random.default_rng(T)
+    for i, (lo, hi) in ((2, k_exp), (3, v_exp)):
+        used = d["table"][d["table"] >= 0]
+        far = np.exp2(rng.integers(lo, hi + 1, (len(used), 2))).astype(np.float32)
+        d["cache"][i][used] = far
+    # the tree's own values as large as its pages' scales: the last page of the committed rows holds both
+    top = 2.0 ** min(v_exp[1] + 4, 60)
+    d["value"] = (d["value"].float() * top).to(BF)
+    args = _args(d)
+    out = ops.gqa.tree_verify_paged(*args)
+    f = lambda k: d[k].double().numpy()  # noqa: E731
+    cache = [a.cpu().numpy() for a in args[8:12]]
+    cache[0], cache[1] = cache[0].view(np.uint8), cache[1].view(np.uint8)
+    with np.errstate(over="ignore", invalid="ignore"):
+        ref = ot.tree_verify(f("query"), f("gate"), f("q_norm"), d["cos"], d["sin"], cache, d["table"], d["kv"], d["n"], d["parent"])
+    assert np.isfinite(ref).all()
+    # A row against its own size, and three absolute terms. Its output is a bf16, half a step of whose subnormals is 2^-134.
+    # A weight P s (s: the value's scale) is an f16 of 2^11 to 2^15 times it over the row's largest one, so half a step of
+    # the smallest is 2^-25 2^-11 of that, at most 2^-36 smax; it meets a byte of at most 448 at each of the keys, and the
+    # sum is over l >= 2^-4 (the running maximum lags by up to 2^4). It counts where the largest scale's rows are all 0: an
+    # append's scale is 2^-100 at least, which leaves nothing of the rows of a page of 2^-126.
+    got = out.double().cpu().numpy()
+    keys = np.array([int(kv) + T for kv in d["kv"]])
+    smax = np.stack([cache[3][t[t >= 0]].max(0).astype(np.float64) for t in d["table"]])  # [B, kv head]
+    lost = np.repeat(2.0**-36 * 2**4 * 448 * keys[:, None] * smax, 6, axis=1)[:, None]
+    err = np.linalg.norm(got - ref, axis=-1)
+    assert (err <= (2e-3 + 2**-8) * np.linalg.norm(ref, axis=-1) + 16 * (2.0**-134 + lost)).all()
+    if v_exp[0] > -126:  # where no page is below an append's least scale by more than f16 reaches, the first term is enough
+        assert (err <= (2e-3 + 2**-8) * np.linalg.norm(ref, axis=-1)).all()
