@@ -34,7 +34,8 @@
 //     The bytes go from the pages by DMA to a part of LDS that is the wave's own, in groups of 8 KB
 //     in the order of their use (two K tiles, or eight V tiles of 16 dims); a wave takes a group into
 //     registers, sends its place for a later one and works on it, with one (NW = 8) to three groups
-//     in flight. Nothing else may touch memory in that loop: a reload of a spilled register waits,
+//     in flight. (A group's eight DMAs in one or two statements, which set M0 once: one by one all of these take 2 to 4 %
+//     longer, by the instructions alone.) Nothing else may touch memory in that loop: a reload of a spilled register waits,
 //     in order, for every DMA before it.
 //     The waves' (m, l, O) meet in LDS; a pair with one workgroup is written out at once. Bound by
 //     the cache's bytes: one row group over 32768 keys of 4 heads (67 MB) 18 us, 3.7 TB/s with the start
@@ -247,6 +248,73 @@ __device__ __forceinline__ void pin(f32x16& x) { asm volatile("" : "+a"(x)); }
 __device__ __forceinline__ unsigned opaque(unsigned x) {
   asm volatile("" : "+v"(x));
   return x;
+}
+
+// Four DMAs of 1 KB each: from a uniform base + o0, o1, o0 and o1, the later ones 1, 2 and 3 KB behind, as are their places.
+__device__ __forceinline__ void lds_dma16x4_soff(const void* sbase, unsigned o0, unsigned o1, unsigned lds) {
+  unsigned saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %4\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %3\n\t"
+      "global_load_lds_dwordx4 %2, %3 offset:1024\n\t"
+      "global_load_lds_dwordx4 %1, %3 offset:2048\n\t"
+      "global_load_lds_dwordx4 %2, %3 offset:3072\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(o0), "v"(o1), "s"(sbase), "s"(lds)
+      : "memory");
+}
+// The same from per-lane addresses, `step` bytes apart.
+__device__ __forceinline__ void lds_dma16x4(const uint8_t* g, size_t step, unsigned lds) {
+  unsigned saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %5\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, off\n\t"
+      "s_add_u32 m0, m0, 0x400\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %2, off\n\t"
+      "s_add_u32 m0, m0, 0x400\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %3, off\n\t"
+      "s_add_u32 m0, m0, 0x400\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %4, off\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(g), "v"(g + step), "v"(g + 2 * step), "v"(g + 3 * step), "s"(lds)
+      : "memory", "scc");
+}
+
+// Eight DMAs of 1 KB each from four uniform bases + o ^ 0, 64, 128 and 192, two 1 KB apart from each; their places follow
+// one another.
+__device__ __forceinline__ void lds_dma16x8_soff(const uint8_t* const (&base)[4], unsigned o, unsigned lds) {
+  unsigned saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_mov_b32 m0, %9\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %1, %5\n\t"
+      "global_load_lds_dwordx4 %1, %5 offset:1024\n\t"
+      "s_add_u32 m0, m0, 0x800\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %2, %6\n\t"
+      "global_load_lds_dwordx4 %2, %6 offset:1024\n\t"
+      "s_add_u32 m0, m0, 0x800\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %3, %7\n\t"
+      "global_load_lds_dwordx4 %3, %7 offset:1024\n\t"
+      "s_add_u32 m0, m0, 0x800\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dwordx4 %4, %8\n\t"
+      "global_load_lds_dwordx4 %4, %8 offset:1024\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "v"(o), "v"(o ^ 64u), "v"(o ^ 128u), "v"(o ^ 192u), "s"(base[0]), "s"(base[1]), "s"(base[2]), "s"(base[3]), "s"(lds)
+      : "memory", "scc");
 }
 
 // Four dims of a row's output: o / l * sigmoid(gate); 0 for a row without keys (inv = 0), whatever its
@@ -645,29 +713,28 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
 
   // Steps are taken kChunk at a time, [c0, c0 + cn) of this workgroup's, with their pages in LDS.
   int cn, key0, page0;
-  auto k_page = [&](int s, int k) {  // of keys 16 k .. + 15 of a step (wave-uniform)
-    const int key = key0 + s * KS + 16 * k;
-    const int id = __builtin_amdgcn_readfirstlane(max(sm.page[(key >> a.sh) - page0], 0));
-    return a.cache_k + ((((size_t)id * a.Hkv + h) << a.sh) + (key & (bs - 1))) * DH;
-  };
-  auto load_k = [&](const uint8_t* const (&pg)[4], int n, int at) {  // tiles 2 n, 2 n + 1
-    const unsigned src = opaque(ksrc);
+  // The pages of a step's keys: 16 k .. + 15 (k < 4), and the lane's 16.
+  auto pages_of = [&](int s, int (&id)[5]) {
+    const int k0 = key0 + s * KS;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        lds_dma16_soff_uniform(pg[k] + (2 * n + j) * 4 * DH, src ^ (k << 6),
-                   ring_lds + (unsigned)(at * 8192 + (k * 2 + j) * 1024));
+    for (int k = 0; k < 4; ++k) id[k] = sm.page[((k0 + 16 * k) >> a.sh) - page0];
+    id[4] = sm.page[((k0 + 16 * G) >> a.sh) - page0];
   };
-  auto v_page = [&](int s) {  // the lane's place, dim i, in the page of its 16 keys of a step
+  auto load_k = [&](int s, const int (&id)[5], int n, int at) {  // tiles 2 n, 2 n + 1
+    const uint8_t* pg[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int key = key0 + s * KS + 16 * k, page = __builtin_amdgcn_readfirstlane(max(id[k], 0));
+      pg[k] = a.cache_k + ((((size_t)page * a.Hkv + h) << a.sh) + (key & (bs - 1)) + 8 * n) * DH;
+    }
+    lds_dma16x8_soff(pg, opaque(ksrc), ring_lds + (unsigned)(at * 8192));
+  };
+  auto load_v = [&](int s, const int (&id)[5], int n, int at) {  // dims 128 n .. + 127
     const int key = key0 + s * KS + 16 * G;
-    const int id = max(sm.page[(key >> a.sh) - page0], 0);
-    return a.cache_v + ((((size_t)id * a.Hkv + h) * DH + i) << a.sh) + (key & (bs - 1));
-  };
-  auto load_v = [&](const uint8_t* pg, int n, int at) {  // dims 128 n .. + 127
-#pragma unroll
-    for (int d = 0; d < 8; ++d)
-      lds_dma16_uniform(pg + ((size_t)(8 * n + d) << (a.sh + 4)), ring_lds + (unsigned)(at * 8192 + d * 1024));
+    const uint8_t* pg = a.cache_v + ((((size_t)max(id[4], 0) * a.Hkv + h) * DH + 128 * n + i) << a.sh) + (key & (bs - 1));
+    const size_t step = (size_t)16 << a.sh;
+    lds_dma16x4(pg, step, ring_lds + (unsigned)(at * 8192));
+    lds_dma16x4(pg + 4 * step, step, ring_lds + (unsigned)(at * 8192 + 4096));
   };
   auto begin_chunk = [&](int c0) {
     cn = min(kChunk, steps - c0);
@@ -688,13 +755,13 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
   };
   auto first_sends = [&]() {
     if (w < cn) {
-      const uint8_t* const kp[4] = {k_page(w, 0), k_page(w, 1), k_page(w, 2), k_page(w, 3)};
-      load_k(kp, 0, 0);
-      load_k(kp, 1, 1);
+      int id[5];
+      pages_of(w, id);
+      load_k(w, id, 0, 0);
+      load_k(w, id, 1, 1);
       if constexpr (NR == 4) {
-        const uint8_t* const vp = v_page(w);
-        load_v(vp, 0, 2);
-        load_v(vp, 1, 3);
+        load_v(w, id, 0, 2);
+        load_v(w, id, 1, 3);
       }
     }
   };
@@ -730,8 +797,9 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
       const bool held = sm.page[page] >= 0;  // they exist
       const bool next = s + NW < cn;
       const int sn = next ? s + NW : s;
-      const uint8_t* const vp = v_page(NR == 4 ? sn : s);
-      const uint8_t* const kp[4] = {k_page(sn, 0), k_page(sn, 1), k_page(sn, 2), k_page(sn, 3)};
+      int id[5];
+      pages_of(sn, id);
+      if constexpr (NR != 4) id[4] = sm.page[page];
 
       f32x4 st[NRT][4];
 #pragma unroll
@@ -755,12 +823,12 @@ __global__ __launch_bounds__(NW * 64, NW / 4) void paged_attn_kernel(PagedArgs a
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if constexpr (NR == 4) {
           if (next) {
-            if (g < 2) load_k(kp, g, g);
-            else load_v(vp, g - 2, g);
+            if (g < 2) load_k(sn, id, g, g);
+            else load_v(sn, id, g - 2, g);
           }
         } else {
-          if (g < 2) load_v(vp, g, g);
-          else if (next) load_k(kp, g - 2, g - 2);
+          if (g < 2) load_v(s, id, g, g);
+          else if (next) load_k(sn, id, g - 2, g - 2);
         }
       };
       const unsigned kat = opaque(k_at), vat = opaque(v_at);
@@ -1300,45 +1368,6 @@ __global__ __launch_bounds__(512, 2) void paged_rows_kernel(PagedArgs a) {
 }
 
 // ---- 2c. attn of many rows of a tree -------------------------------------------------------------------
-// Four DMAs of 1 KB each: from a uniform base + o0, o1, o0 and o1, the later ones 1, 2 and 3 KB behind, as are their places.
-__device__ __forceinline__ void lds_dma16x4_soff(const void* sbase, unsigned o0, unsigned o1, unsigned lds) {
-  unsigned saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %4\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, %3\n\t"
-      "global_load_lds_dwordx4 %2, %3 offset:1024\n\t"
-      "global_load_lds_dwordx4 %1, %3 offset:2048\n\t"
-      "global_load_lds_dwordx4 %2, %3 offset:3072\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "v"(o0), "v"(o1), "s"(sbase), "s"(lds)
-      : "memory");
-}
-// The same from per-lane addresses, `step` bytes apart.
-__device__ __forceinline__ void lds_dma16x4(const uint8_t* g, size_t step, unsigned lds) {
-  unsigned saved;
-  asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_mov_b32 m0, %5\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %1, off\n\t"
-      "s_add_u32 m0, m0, 0x400\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %2, off\n\t"
-      "s_add_u32 m0, m0, 0x400\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %3, off\n\t"
-      "s_add_u32 m0, m0, 0x400\n\t"
-      "s_nop 0\n\t"
-      "global_load_lds_dwordx4 %4, off\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
-      : "v"(g), "v"(g + step), "v"(g + 2 * step), "v"(g + 3 * step), "s"(lds)
-      : "memory", "scc");
-}
-
 struct TreeRowsSmem {
   union {
     uint8_t ring[4][32768];  // four steps of 64 keys: K, 64 rows of 256 bytes, and V, 16 groups of 16 dims
