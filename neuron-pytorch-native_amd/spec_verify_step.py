@@ -170,13 +170,13 @@ class VerifySlice:
                         L[f"{name}_scale"] = torch.full(shape[:2], 2.0 ** -6, device=device)
             self.layers.append(L)
         self.kv_len = torch.as_tensor(kv_lens, dtype=torch.int32, device=device).clone()
+        self.new_len = torch.full((B,), self.T, dtype=torch.int32, device=device)
         if paged_block is not None:
             i32 = dict(dtype=torch.int32, device=device)
             P = -(-s_max // paged_block)
             self.pages = {"table": torch.full((B, P), -1, **i32), "held": torch.zeros(B, **i32),
                           "free": torch.randperm(B * P, generator=g, device=device).int(),
                           "count": torch.full((1,), B * P, **i32)}
-            self.new_len = torch.full((B,), self.T, **i32)
             self.longest = int(self.kv_len.max())  # no sequence is longer
             self._plan_pages(torch.zeros(B, **i32))  # the blocks of the rows that are there
         # RoPE table of every cache position, built once (the reference's _init_rope); each
@@ -184,7 +184,7 @@ class VerifySlice:
         self.rope_cos, self.rope_sin = rope_tables(torch.arange(s_max, device=device))
         self.prev_accepted = None
         self.timer = _untimed
-        self.nodes = self.tree = self.tree_graph = None  # how many nodes and the parents of the nodes of a step_tree; its graph
+        self.nodes = self.tree = self.tree_graph = None  # how many nodes, and their parents, of a step_tree; its graph
         self.committed, self.last_accepted = torch.zeros(2, B, dtype=torch.int32, device=device)
         self.persistent = False
         self.parity = 0

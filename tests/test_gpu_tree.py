@@ -311,7 +311,7 @@ def _check(ops, d):
     (1, 33, 1, 5, 64, [1000], [33], 33),                       # nodes that straddle groups
     (2, 64, 2, 2, 128, [255, 120], [64, 63], 1),               # chains of 64
     (9, 20, 4, 6, 16, [0, 5, 100, 300, 700, 1100, 64, 128, 33], [20, 19, 1, 20, 17, 20, 0, 20, 2], 6),
-    (1, 64, 1, 48, 32, [40], [64], 7),                         # 24 groups
+    (1, 63, 1, 48, 32, [40], [63], 7),                         # 24 groups
 ])
 def test_tree_verify_paged_matches_oracle(ops, B, T, H, grp, bs, kv, n, reach):
     _check(ops, _attend_inputs(B, T, H, grp, bs, kv, n, reach, seed=B * 7 + T))

@@ -225,3 +225,24 @@ def test_verify_slice_steps_over_trees():
     with pytest.raises(RuntimeError, match="checkpoints"):
         chain.prev_accepted = accepted
         chain.step_tree(*args)
+
+
+def test_verify_slice_of_deltanet_layers_alone():
+    """A slice without attention layers has no pages: its tree steps take every node, or as many as they are told."""
+    from spec_verify_step import HIDDEN, VerifySlice
+    B, K = 2, 4
+    one = VerifySlice(B, K, [9, 30], 64, pattern="DD", seed=2)
+    x = torch.randn(B * (K + 1), HIDDEN, device="cuda").to(BF)
+    parent = torch.tensor([[-1, 0, 0, 1, 2], [-1, 0, 1, 2, 3]], dtype=I32, device="cuda")
+    ids = torch.tensor([[0, 5, 6, 7, 8], [0, 1, 2, 3, 4]], device="cuda")
+    target = torch.tensor([[6, 1, 8, 1, 9], [1, 2, 3, 4, 5]], device="cuda")
+    before = [L["state"].clone() for L in one.layers]
+    _, accepted, path, out = one.step_tree(x, parent, ids, target)
+    assert accepted.tolist() == [2, 4] and path[0].tolist() == [0, 2, 4, -1, -1] and out[0].tolist() == [6, 8, 9, -1, -1]
+    assert one.kv_len.tolist() == [12, 35] and all(not torch.equal(L["state"], s) for L, s in zip(one.layers, before))
+    before = [L["state"].clone() for L in one.layers]
+    n = torch.tensor([0, 3], dtype=I32, device="cuda")
+    _, accepted, _, _ = one.step_tree(x, parent, ids, target, n)
+    assert accepted.tolist() == [-1, 2] and one.kv_len.tolist() == [12, 38]
+    half = before[0].shape[0] // 2
+    assert all(torch.equal(L["state"][:half], s[:half]) for L, s in zip(one.layers, before))
