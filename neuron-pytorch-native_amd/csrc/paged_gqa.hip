@@ -61,8 +61,8 @@
 //     again the next product's operand where it is, over powers of two as in 2. The next step's scores are computed
 //     between this step's weights. Of a step's 4700 cycles its products take 2200 and the bytes' conversion 1700, in
 //     the same issue slots as the softmax's 1400 and the DMAs, the page ids and the barrier's 800; start and end 13000 each: the plan,
-//     the first bytes' way, and the parts' 128 KB. 16 requests of 64 x 6 rows over up to 8192 keys 160 us, 720 TFLOP/s
-//     by the formula's operations (2b with a tree's masks 200); 8 of 32 x 6 rows 60 (groups of 48: 73).
+//     the first bytes' way, and the parts' 128 KB. 16 requests of 64 x 6 rows over up to 8192 keys 165 us, 700 TFLOP/s
+//     by the formula's operations (2b with a tree's masks 205); 8 of 32 x 6 rows 60 (groups of 48: 73).
 //     Tried: DMAs between the products, whose branches had registers spilled (283 us for 232 in all); two chains of
 //     products at once, as fast as one; the longest workgroups first, as fast.
 //  3. merge: the log-sum-exp merge of the other pairs' workgroups, times sigmoid(gate), to bf16.
@@ -283,9 +283,9 @@ __device__ __forceinline__ void lds_dma16x4_soff(const void* sbase, unsigned o0,
       "s_mov_b32 m0, %4\n\t"
       "s_nop 0\n\t"
       "global_load_lds_dwordx4 %1, %3\n\t"
-      "global_load_lds_dwordx4 %2, %3 offset:1024\n\t"
-      "global_load_lds_dwordx4 %1, %3 offset:2048\n\t"
-      "global_load_lds_dwordx4 %2, %3 offset:3072\n\t"
+      "global_load_lds_dwordx4 %2, %3 offset:0x400\n\t"
+      "global_load_lds_dwordx4 %1, %3 offset:0x800\n\t"
+      "global_load_lds_dwordx4 %2, %3 offset:0xc00\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)
       : "v"(o0), "v"(o1), "s"(sbase), "s"(lds)
@@ -323,19 +323,19 @@ __device__ __forceinline__ void lds_dma16x8_soff(const uint8_t* const (&base)[4]
       "s_mov_b32 m0, %9\n\t"
       "s_nop 0\n\t"
       "global_load_lds_dwordx4 %1, %5\n\t"
-      "global_load_lds_dwordx4 %1, %5 offset:1024\n\t"
+      "global_load_lds_dwordx4 %1, %5 offset:0x400\n\t"
       "s_add_u32 m0, m0, 0x800\n\t"
       "s_nop 0\n\t"
       "global_load_lds_dwordx4 %2, %6\n\t"
-      "global_load_lds_dwordx4 %2, %6 offset:1024\n\t"
+      "global_load_lds_dwordx4 %2, %6 offset:0x400\n\t"
       "s_add_u32 m0, m0, 0x800\n\t"
       "s_nop 0\n\t"
       "global_load_lds_dwordx4 %3, %7\n\t"
-      "global_load_lds_dwordx4 %3, %7 offset:1024\n\t"
+      "global_load_lds_dwordx4 %3, %7 offset:0x400\n\t"
       "s_add_u32 m0, m0, 0x800\n\t"
       "s_nop 0\n\t"
       "global_load_lds_dwordx4 %4, %8\n\t"
-      "global_load_lds_dwordx4 %4, %8 offset:1024\n\t"
+      "global_load_lds_dwordx4 %4, %8 offset:0x400\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)
       : "v"(o), "v"(o ^ 64u), "v"(o ^ 128u), "v"(o ^ 192u), "s"(base[0]), "s"(base[1]), "s"(base[2]), "s"(base[3]), "s"(lds)
