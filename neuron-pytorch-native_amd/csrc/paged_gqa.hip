@@ -1838,6 +1838,10 @@ PagedPlan paged_plan(int B, int T, int q_heads, int kv_heads, int max_blocks, in
   const int64_t by48 = (rows + 47) / 48, by128 = (rows + kRows - 1) / kRows;
   if (tree && rows > 48 && by48 * 48 * 4 <= by128 * kRows * 3 && rows * 8 >= by48 * 48 * 7 && B * by48 * kv_heads < 32)
     p.R = 48;
+  // And up to 64 rows two groups of 32, as of 128 half would be empty: one request of 60 rows over 32768 keys 39 us and 45
+  // with a group of 128, 32 of them over up to 16384 186 and 193, 8 of 54 rows over up to 8192 49 and 51.5, 4 over up to
+  // 2000 25 and 31. (72 rows as 48 and 24: 8 requests 59 us and 53 with a group of 128, 32 of them 220 and 197.)
+  if (tree && rows > 48 && rows <= 64) p.R = 32;
   p.RG = (int)((rows + p.R - 1) / p.R);
   const int64_t pairs = (int64_t)B * p.RG * kv_heads;
   const int64_t keys = (int64_t)max_blocks * block_size;

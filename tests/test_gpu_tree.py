@@ -306,6 +306,8 @@ def _check(ops, d):
     (2, 8, 4, 6, 64, [37, 600], [8, 8], 4),                    # 48 rows
     (4, 8, 2, 6, 128, [127, 0, 1500, 11], [8, 0, 3, 8], 8),    # padded and idle requests
     (2, 3, 2, 16, 16, [100, 33], [3, 3], 2),                   # 48 rows of 16 a node
+    (3, 9, 2, 6, 32, [250, 0, 63], [9, 4, 9], 3),              # 54 rows: two groups
+    (2, 16, 1, 4, 64, [1000, 60], [16, 11], 5),                # 64 rows
     (3, 16, 2, 6, 16, [500, 0, 61], [16, 16, 9], 5),           # 96 rows
     (2, 64, 1, 6, 16, [70, 0], [64, 20], 16),                  # groups without a live node; five pages
     (1, 33, 1, 5, 64, [1000], [33], 33),                       # nodes that straddle groups
