@@ -72,7 +72,7 @@ __device__ __forceinline__ uint32_t to_e4m3(const float* x, float inv, bool all_
   return (uint32_t)p | nan;
 }
 
-// e4m3 bytes times a power of two <= 1.
+// e4m3 bytes times a power of two, finite, with which none passes 448; NaN stays.
 __device__ __forceinline__ uint32_t rescale_e4m3(uint32_t w, float by) {
   const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
   const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);

@@ -96,6 +96,12 @@ __device__ __forceinline__ float need_of(int big, float scale) {
   const auto v = __builtin_amdgcn_cvt_pk_f32_fp8(big, false);
   return v[0] > 0.f ? append::scale_of(v[0] * scale) : 0.f;
 }
+// The factor from a row's scale to its new page's: infinite only for a row without a finite number but 0, as any
+// other has made its page's scale grow. Such a row's bytes stay, as do those of a row whose scale is its new page's.
+__device__ __forceinline__ float factor_of(float from, float to) {
+  const float by = from / to;
+  return from == to || (by == INFINITY && from < INFINITY) ? 1.0f : by;
+}
 // The new scale of each row's page, from what its rows need.
 __device__ __forceinline__ float grown_scale(const Path& p, float need) {
   float now = p.d_old;
@@ -181,7 +187,7 @@ __device__ __forceinline__ void compact_k(const CompactArgs& a, uint8_t* cache, 
       if (lane == 0) scale[page * a.Hkv + h] = to_scale;
     });
   }
-  const float by = p.s_old / now;
+  const float by = factor_of(p.s_old, now);
   uint64_t left = p.moving;
   while (left != 0) {
     int d[kBatch];
@@ -260,7 +266,7 @@ __device__ __forceinline__ void compact_v(const CompactArgs& a, uint8_t* cache, 
     });
   }
 
-  const float by = p.s_old / now;
+  const float by = factor_of(p.s_old, now);
   uint64_t left = p.moving;
   while (left != 0) {
     int d[kBatch];
