@@ -121,7 +121,7 @@ class VerifySlice:
                  fuse_splitk=True, fuse_swiglu=True, fuse_launches=True, paged_block=None):
         """paged_block: None for dense bf16 KV caches, or the block size of a paged e4m3 cache
         with one block table for all GQA layers, planned on the device at every step. A step with
-        pages raises where a sequence has fewer than K + 1 rows left of its s_max."""
+        pages raises where a sequence has fewer than K + 1 rows left of its s_max, or than its nodes in step_tree."""
         self.B, self.K, self.T = B, K, K + 1
         self.paged_block, self.s_max = paged_block, s_max
         self.fuse_splitk = fuse_splitk
@@ -196,17 +196,22 @@ class VerifySlice:
         return torch.ops.paged.update_blocks_(self.kv_len, new_len, p["table"], p["held"], p["free"],
                                               p["count"], self.paged_block, self.T)
 
-    def _take_rows(self):
-        """Before a step with pages: every sequence has room for its T rows. The step cannot go on
-        without: a sequence that is refused its blocks would be committed all the same. The host
-        counts T rows a step for all and looks at the lengths (a wait) only where that is too many."""
+    def _take_rows(self, n_nodes=None):
+        """Before a step with pages: every sequence has room for its T rows, or for those of its n_nodes nodes.
+        A chain's step cannot go on without: a sequence that is refused its blocks would be committed
+        all the same. The host counts T rows a step for all and looks at the lengths (a wait) only where
+        that is too many."""
         if self.paged_block is None or "G" not in self.pattern or torch.cuda.is_current_stream_capturing():
             return
         if self.longest + self.T > self.s_max:
             self.longest = int(self.kv_len.max())
             if self.longest + self.T > self.s_max:
-                raise RuntimeError(f"a sequence of {self.longest} rows has no room for {self.T} more: "
-                                   f"s_max is {self.s_max}")
+                new = self.new_len if n_nodes is None else n_nodes.clamp(0, self.T)
+                after = torch.where(new > 0, self.kv_len + new, 0)
+                if int(after.max()) > self.s_max:
+                    b = int(after.argmax())
+                    raise RuntimeError(f"a sequence of {int(self.kv_len[b])} rows has no room for {int(new[b])} more: "
+                                       f"s_max is {self.s_max}")
         self.longest += self.T
 
     # ---- layers: each takes the normed input and returns the residual delta -------------
@@ -320,7 +325,7 @@ class VerifySlice:
         if self.paged_block is not None and "G" in self.pattern:
             if cos is not None:
                 raise ValueError("the paged cache takes its RoPE rows from the tables")
-            self._take_rows()
+            self._take_rows(self.nodes)
             self.plan = self.timer("paged.update_blocks", self._plan_pages,
                                    self.new_len if self.nodes is None else self.nodes)
         elif cos is None and not self.fuse_launches and "G" in self.pattern:
@@ -449,9 +454,9 @@ class VerifySlice:
     def step_tree(self, x, parent, draft_ids, target_ids, n_nodes=None, trace=None):
         """One verify + accept + commit step over trees of T = K + 1 nodes: x [B*T, 5120], parent [B, T] int32,
         draft_ids and target_ids [B, T] int64 (the target's token of each node), n_nodes [B] int32 where
-        some have fewer than T (nodes [0, n_nodes[b]) count; 0: the sequence sits out). All state is
-        updated in place. Returns (hidden, accepted, path, out_ids). Steps over chains (step) leave
-        their DeltaNet states as checkpoints, so a slice takes steps of the one kind only."""
+        some have fewer than T (nodes [0, n_nodes[b]) count; 0: the sequence sits out, as one without room for
+        more rows has to). All state is updated in place. Returns (hidden, accepted, path, out_ids). Steps
+        over chains (step) leave their DeltaNet states as checkpoints, so a slice takes steps of the one kind only."""
         if self.paged_block is None and "G" in self.pattern:
             raise ValueError("a tree needs the paged cache")
         if self.prev_accepted is not None:
@@ -479,12 +484,13 @@ class VerifySlice:
     def capture_tree(self, x, parent, draft_ids, target_ids, n_nodes=None):
         """Capture step_tree over these tensors, which keep their addresses, as a HIP graph. Run one
         eager step_tree before. replay_tree() runs it and returns the same four tensors every time."""
-        self.tree_graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.tree_graph):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
             self.tree_outputs = self.step_tree(x, parent, draft_ids, target_ids, n_nodes)
+        self.tree_graph, self.tree_nodes = graph, n_nodes
 
     def replay_tree(self):
-        self._take_rows()
+        self._take_rows(self.tree_nodes)
         self.tree_graph.replay()
         return self.tree_outputs
 
