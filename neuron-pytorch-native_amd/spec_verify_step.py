@@ -459,8 +459,7 @@ class VerifySlice:
         over chains (step) leave their DeltaNet states as checkpoints, so a slice takes steps of the one kind only."""
         if self.paged_block is None and "G" in self.pattern:
             raise ValueError("a tree needs the paged cache")
-        if self.prev_accepted is not None:
-            raise RuntimeError("step_tree after step: the states are in the chain's checkpoints")
+        self._refuse_after_chain("step_tree")
         self.tree, self.nodes = parent, n_nodes
         try:
             hidden = self.forward(x, trace=trace)
@@ -481,6 +480,11 @@ class VerifySlice:
         self.timer("spec.commit", torch.ops.spec.commit_, accepted, self.last_accepted, self.kv_len, self.committed)
         return hidden, accepted, path, out_ids
 
+    def _refuse_after_chain(self, name):
+        """A chain's step leaves the DeltaNet states in checkpoints and the lengths in another tensor."""
+        if self.prev_accepted is not None:
+            raise RuntimeError(f"{name} after step: the states are in the chain's checkpoints")
+
     def capture_tree(self, x, parent, draft_ids, target_ids, n_nodes=None):
         """Capture step_tree over these tensors, which keep their addresses, as a HIP graph. Run one
         eager step_tree before. replay_tree() runs it and returns the same four tensors every time."""
@@ -490,6 +494,9 @@ class VerifySlice:
         self.tree_graph, self.tree_nodes = graph, n_nodes
 
     def replay_tree(self):
+        if self.tree_graph is None:
+            raise RuntimeError("replay_tree before capture_tree")
+        self._refuse_after_chain("replay_tree")
         self._take_rows(self.tree_nodes)
         self.tree_graph.replay()
         return self.tree_outputs

@@ -50,3 +50,21 @@ def test_slice_at_the_end_of_its_pages(kv, n, ok):
     for v in (eager, replayed):
         assert v.kv_len.tolist() == [k + int(m) for k, m in zip(kv, nodes)]
     assert accepted.tolist() == got[1].tolist() == [int(m) - 1 for m in nodes]
+
+
+def test_replay_tree_after_a_chain_s_step():
+    """The captured step reads states and lengths that a chain's step has left behind: refused, as step_tree is."""
+    B, T = 2, 4
+    v, args = _slice([5, 10]), _step_args(B, T, [4, 4])
+    with pytest.raises(RuntimeError, match="capture_tree"):
+        v.replay_tree()
+    v.step_tree(*args)
+    v.capture_tree(*args)
+    v.replay_tree()
+    v.forward(args[0])
+    v.accept_and_rollback(torch.tensor([1, 2], dtype=I32, device="cuda"))
+    kv = v.kv_len.tolist()
+    for call in (v.replay_tree, lambda: v.step_tree(*args)):
+        with pytest.raises(RuntimeError, match="checkpoints"):
+            call()
+    assert v.kv_len.tolist() == kv
