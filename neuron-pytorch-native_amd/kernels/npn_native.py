@@ -225,20 +225,20 @@ class Addresses:
 
 
 _DTYPE = operator.attrgetter("dtype")
+_SHAPE = operator.attrgetter("shape")
 
 
 def check_lists(dev, *specs):
     """specs: (list of tensors, name, dtype, shape, or a number of elements in any shape), one tensor a layer:
-    `check_all` for each, the shape by the first and the others' number of elements. Returns their `Addresses`."""
+    `check_all` for each, all of a list's at once where they are as they have to be. Returns their `Addresses`."""
     out = []
     for ts, name, dtype, shape in specs:
         if ts:
-            check_all(dev, (ts[0], name, dtype, shape))
-            if len(ts) > 1 and not (
-                    set(map(torch.Tensor.numel, ts)) == {ts[0].numel()} and set(map(_DTYPE, ts)) == {dtype}
+            sizes = set(map(torch.Tensor.numel if type(shape) is int else _SHAPE, ts))
+            if not (sizes == {shape} and set(map(_DTYPE, ts)) == {dtype}
                     and set(map(torch.Tensor.get_device, ts)) == {dev.index}
                     and all(map(torch.Tensor.is_contiguous, ts))):
-                check_all(dev, *[(t, f"{name}[{i}]", dtype, ts[0].numel()) for i, t in enumerate(ts)])
+                check_all(dev, *[(t, f"{name}[{i}]", dtype, shape) for i, t in enumerate(ts)])
         out.append(Addresses(ts))
     return out
 
