@@ -164,8 +164,16 @@ def register(qualname, schema, fake):
         written = [i for i, a in enumerate(specs) if a.alias_info is not None and a.alias_info.is_write]
 
         def flat(args):
-            """The arguments with the lists' tensors in the lists' places."""
-            return [t for a in args for t in (a if isinstance(a, list) else (a,))]
+            """The arguments with the lists' tensors in the lists' places (as they are, of an op without lists)."""
+            if not lists:
+                return args
+            out = []
+            for a in args:
+                if isinstance(a, list):
+                    out += a
+                else:
+                    out.append(a)
+            return out
 
         def count_as_written(args):
             tensors = flat([args[i] for i in written])
@@ -182,7 +190,7 @@ def register(qualname, schema, fake):
             if torch._C._any_requires_grad(*args) or forward_ad._current_level >= 0:
                 _refuse_gradients(qualname, [(arg, args[i]) for i, arg in names] +
                                   [(arg, t) for i, arg in lists for t in args[i]])
-            plain = (args[first].is_cuda and _PLAIN.issuperset(map(type, flat(args) if lists else args))
+            plain = (args[first].is_cuda and _PLAIN.issuperset(map(type, flat(args)))
                      and torch._C._len_torch_dispatch_stack() == 0
                      and torch._C._functorch.peek_interpreter_stack() is None)
             if plain:
