@@ -657,9 +657,10 @@ int npn_deltanet_commit_tree(float* const* state, uint16_t* const* conv_state,
  * front of the tree's: row path[b, d]'s, at slots[b, path[b, d]], to slots[b, d], where the row behind
  * the last committed one is slots[b, 0]. One launch for up to 32 layers.
  *   cache_k, cache_v, k_scale, v_scale: host arrays of `layers` device pointers;
- *   slots [B, T] int64 as npn_paged_update_blocks made them (a path ends where one of its two slots
- *   is out of [0, n_blocks * block_size) or, counted from slots[b, 0], out of place in its 16 rows);
- *   a block may belong to one request only.
+ *   slots [B, T] int64 as npn_paged_update_blocks made them: each one behind the last one, or at the
+ *   beginning of a block where that one is the end of one. A path ends at its first row whose place,
+ *   now or then, is out of [0, n_blocks * block_size), or that is not before the first slot that breaks
+ *   this order. A block may belong to one request only, once.
  * A row that comes from a block of another scale is rounded to its new block's, nearest even, which
  * first grows to the least power of two s with amax <= 448 s over the finite values of the rows
  * that move there, if that is more; the block's rows up to the path's last one are moved to it.

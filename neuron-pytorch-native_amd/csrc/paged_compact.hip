@@ -54,14 +54,16 @@ __device__ __forceinline__ Path path_of(const CompactArgs& a, const float* scale
   p.node = lane < a.T ? a.path[at] : -1;
   p.dst = lane < a.T ? a.slots[at] : -1;
   p.src = (int64_t)npn::shfl64((uint64_t)p.dst, min(max(p.node, 0), a.T - 1));
-  // A row's place counted from the beginning of the first one's piece of 16 positions tells where its own piece begins.
+  // Rows lie one behind the other, in a block to its end and from the next one's begin: then a row's place counted from
+  // the beginning of the first one's piece of 16 positions tells where its own piece begins, and a block's rows among the
+  // path's are a run of them. The first row that does not ends what can move.
   p.off = (int)(npn::tree_bits((uint64_t)p.dst, 0) & 15);
-  const int first = max(16 * ((p.off + lane) >> 4) - p.off, 0);
-  const bool run = p.dst == (int64_t)npn::shfl64((uint64_t)p.dst, first) + lane - first &&
-                   (int)(p.dst & 15) == ((p.off + lane) & 15);
-  const bool both = run && __shfl((int)run, min(max(p.node, 0), a.T - 1), 64);
+  const int64_t mask = (1 << a.sh) - 1, next = (int64_t)npn::shfl64((uint64_t)p.dst, max(lane - 1, 0)) + 1;
+  const bool behind = lane == 0 || ((p.dst & mask) == 0 ? (next & mask) == 0 : p.dst == next);
+  const uint64_t breaks = __builtin_amdgcn_ballot_w64(!behind);
+  const int rows = breaks ? __builtin_ctzll(breaks) : npn::kMaxNodes;
   const bool in = p.dst >= 0 && p.dst < end && p.src >= 0 && p.src < end;
-  const int n = npn::path_length(p.node, a.T, lane, in && both);
+  const int n = npn::path_length(p.node, a.T, lane, in && p.node < rows);
   p.dst_page = p.dst >> a.sh;
   p.row = lane < n;
   p.moves = p.row && p.src != p.dst;

@@ -133,15 +133,25 @@ def accept(target, draft, parent, q_len):
     return accepted, path, ids
 
 
+def rows_in_place(slots, bs):
+    """How many of a request's rows, from the first on, lie one behind the other, in a block to its end and from the
+    next one's begin; slots [T]."""
+    for t in range(1, len(slots)):
+        last, at = int(slots[t - 1]), int(slots[t])
+        if (last + 1) % bs != 0 if at % bs == 0 else at != last + 1:
+            return t
+    return len(slots)
+
+
 def compact(path, slots, cache):
     """In place on one layer's (cache_k, cache_v, k_scale, v_scale)."""
     N, H, bs, _ = cache[0].shape
     B, T = path.shape
     inside = lambda s: 0 <= s < N * bs  # noqa: E731
     for b in range(B):
-        n = path_length(path[b], T)
+        n, rows_held = path_length(path[b], T), rows_in_place(slots[b], bs)
         for d in range(n):
-            if not (inside(slots[b, d]) and inside(slots[b, path[b, d]])):
+            if path[b, d] >= rows_held or not (inside(slots[b, d]) and inside(slots[b, path[b, d]])):
                 n = d
                 break
         src, dst = [int(slots[b, p]) for p in path[b, :n]], [int(s) for s in slots[b, :n]]

@@ -49,3 +49,39 @@ def test_compact_paged_scales_of_zero(ops):
     got = _compact(ops, cache, path, slots)
     ot.compact(path, slots, cache[0])
     _same_pages(got[0], cache[0])
+
+
+@pytest.mark.parametrize("bs,kind", [(64, "pieces"), (128, "pieces"), (64, "rows"), (16, "blocks"), (128, "jump"), (32, "none")])
+def test_compact_paged_slots_out_of_order(ops, bs, kind):
+    """Slots that no block table makes: rows move up to the first that is not behind the last one, and no other page
+    or row changes. (none: a block that is none in the middle, which a table may have; the path goes past it.)"""
+    T, H, B = 64, 2, 3
+    rng = np.random.default_rng(bs)
+    N = B * 5 + 2
+    cache, ids = _pages(1, N, H, bs, rng, 9), rng.permutation(N)[:B * 5].reshape(B, 5)
+    at = np.array([0, 5, bs - 3])[:, None] + np.arange(T)
+    slots = np.take_along_axis(ids, at // bs, 1) * bs + at % bs
+    for b in range(B):
+        if kind == "pieces":    # two of a block's pieces of 16 have changed places
+            x, y = slots[b, :16].copy(), slots[b, 16:32].copy()
+            slots[b, :16], slots[b, 16:32] = y, x
+        elif kind == "rows":
+            slots[b, 20], slots[b, 21] = slots[b, 21], slots[b, 20]
+        elif kind == "blocks":  # begins a block where the last one has not ended
+            slots[b, 30:] += 3
+        elif kind == "jump" and b == 0:  # in order in each 16, far behind in the block
+            slots[b, 16:32] = slots[b, 0] + 112 + np.arange(16)
+        elif kind == "none":
+            hole = (at[b] // bs) == at[b, 0] // bs + 1
+            slots[b, hole] = -bs + at[b, hole] % bs
+    path = np.full((B, T), -1, np.int32)
+    for b in range(B):
+        nodes = np.sort(rng.choice(np.arange(1, T), 12, replace=False))
+        path[b, :13] = np.concatenate([[0], nodes])
+    if kind == "none":
+        path[:, :6] = [0, 2, 8, 50, 60, 63]
+        path[:, 6:] = -1
+    want = cache[0]
+    got = _compact(ops, cache, path, slots.astype(np.int64))
+    ot.compact(path, slots, want)
+    _same_pages(got[0], want)
