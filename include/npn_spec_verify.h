@@ -586,8 +586,12 @@ int npn_deltanet_rollback_commit(const uint16_t* const* mixed_qkv, uint16_t* con
  *   parent [B, T] int32, 1 <= T <= 64: node t of request b hangs on node parent[b, t] where
  *   that lies in [0, t), else on the committed tokens alone. Node 0 is the last committed
  *   token. A node sees the committed tokens, its ancestors and itself, and lies at position
- *   kv_len[b] + its number of ancestors. What a node gets depends on nothing of other nodes,
- *   NaN included. A chain (parent[t] = t - 1) is what the verify calls above take.
+ *   kv_len[b] + its number of ancestors. What a node gets depends on nothing of the other
+ *   nodes, NaN included, but for the scales of K/V pages: all T rows are appended first, and the
+ *   largest finite value A that was ever in a block sets the scale of its rows. Each number there is
+ *   off by up to 2^-4 of itself and 2^-16 A, the committed rows' too, and the rows of rejected
+ *   nodes count (as a rejected chain's do). A chain (parent[t] = t - 1) is what the verify
+ *   calls above take.
  * A step: npn_paged_update_blocks for T rows; per layer npn_deltanet_verify_tree or
  * npn_gqa_tree_verify_paged; the target's token of every node (npn_sample: lossless, or
  * npn_argmax_parts); npn_accept_tree; npn_deltanet_commit_tree, npn_gqa_compact_paged and
