@@ -608,9 +608,10 @@ size_t npn_gqa_tree_verify_paged_workspace_size(int B, int T, int q_heads, int k
  * [B, T, Hkv, 256] bf16 to slots [B, T]) with the positions of the tree, and
  * npn_gqa_tail_verify_paged's attention over the pages, node t < q_len[b] seeing the keys
  * [0, kv_len[b]) and of those behind its ancestors and itself (node s's row is the one at
- * kv_len[b] + s of the block table). Rows t >= q_len[b] are 0. Other arguments, roundings and
- * limits as in those two; T <= 64. (Of a chain's outputs these are the same bits for up to 48
- * rows of a kv head, T * q_heads / kv_heads.) */
+ * kv_len[b] + s of the block table). Rows t >= q_len[b] are 0. Other arguments and limits as in
+ * those two; T <= 64. Roundings too for up to 48 rows of a kv head, T * q_heads / kv_heads, where
+ * a chain's outputs are the same bits; above, the normed query and the softmax weights are
+ * rounded to 11 bits as they are below, where npn_gqa_tail_verify_paged has 12 and 13. */
 int npn_gqa_tree_verify_paged(const uint16_t* query, const uint16_t* gate, const uint16_t* key,
                               const uint16_t* value, const float* q_norm, const float* k_norm,
                               const float* cos_table, const float* sin_table, int positions,
@@ -623,6 +624,9 @@ int npn_gqa_tree_verify_paged(const uint16_t* query, const uint16_t* gate, const
 
 /* torch.ops.deltanet.verify_tree -- npn_deltanet_verify's token step of every node from the state and
  * conv window behind its parent, without forming a state per node (64 KB each for every head).
+ * The products of normed keys and queries with each other and with the state take 22 bits of each
+ * factor, with steps of 2^-36 of a row's norm or of the largest in the state's column for the
+ * smallest; sums are in fp32 and those of g in 64 bits.
  *   state [B, Hv, 128, 128] f32 and conv_state [B, QKV, 3] bf16: the committed ones;
  *   the other inputs as npn_deltanet_verify's, T <= 64; Hv <= 4096, B <= 65536, B * Hv <= 2^22.
  * Outputs: out [B, T, Hv, 128] bf16; records, B * T * ((Hk + Hv) * 128 + Hv) f32, what

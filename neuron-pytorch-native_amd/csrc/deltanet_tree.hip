@@ -64,7 +64,8 @@ typedef float f32x4 __attribute__((__vector_size__(4 * sizeof(float))));
 //
 // Bound by the state and the rows' bytes where heads are many and trees small: 1536 heads of 16 nodes 37.5 us (141 MB, 27.4
 // at a copy's rate); by the length of the steps above, one behind the other with a barrier between, where a CU has a head
-// or two: 48 heads of 16 nodes 9.2 us, of 64 nodes 21.7, 384 heads of 64 nodes 37.5 (65 MB, 13 us; its products take 5).
+// or two: 48 heads of 16 nodes 9.2 us, of 64 nodes 21.7, 384 heads of 64 nodes 37.5 (65 MB, 13 us; its products take 5);
+// calls one behind the other, traced alone 9.8 and 40 for the first and the last.
 template <int NT, int NW, bool APART>
 struct TreeSmem {
   static constexpr int TM = 16 * NT, kTiles = NT * (NT + 1) / 2;

@@ -7,8 +7,9 @@
 //   K and V the e4m3 bytes times their (block, head) scale. Rows t >= q_len[b] are 0.
 //
 // The rows of a kv head (token-major, grp heads per token) are cut into groups of R = 16, 32 or 48 rows,
-// as they need, or of 128 where they are more; a (request, row group) is a unit, a (unit, kv head) a
-// pair of its rows and its keys, taken in steps of 64 keys (128 with R = 128). Three launches:
+// as they need, or of 128 where they are more (of a tree also two of 32, or several of 48: paged_plan has
+// the rule); a (request, row group) is a unit, a (unit, kv head) a pair of its rows and its keys, taken in
+// steps of 64 keys (128 with R = 128 but for trees). Three launches:
 //  1. prep: q' of every pair as MFMA B operands, and, in its first block, the plan: the host does not
 //     know the lengths. A pair of n steps gets ceil(n / Q) workgroups, Q the least number of steps
 //     (a multiple of what the waves take at a time) with which all pairs' workgroups are at most `most`.
@@ -59,14 +60,17 @@
 //  2c. the same of a tree: four waves of 32 rows, one to a SIMD, share steps of 64 keys in f16, K's and V's bytes made f16 for
 //     32 rows at a time in 32x32x16 products. A lane (i, G) has 16 keys of row i in a tile of 32, in order, so that P is
 //     again the next product's operand where it is, over powers of two as in 2. The next step's scores are computed
-//     between this step's weights. Of a step's 4700 cycles its products take 2200 and the bytes' conversion 1700, in
-//     the same issue slots as the softmax's 1400 and the DMAs, the page ids and the barrier's 800; start and end 13000 each: the plan,
-//     the first bytes' way, and the parts' 128 KB. 16 requests of 64 x 6 rows over up to 8192 keys 165 us, 700 TFLOP/s
-//     by the formula's operations (2b with a tree's masks 205); 8 of 32 x 6 rows 60 (groups of 48: 73).
+//     between this step's weights. Of a step's 4700 cycles the matrix unit is busy for 2050 and the vector unit for 2900, the
+//     bytes' conversion and the softmax, in the same issue slots as the products; start and end 13000 each: the plan,
+//     the first bytes' way, and the parts' 128 KB. 16 requests of 64 x 6 rows over up to 8192 keys 187 us, 620 TFLOP/s
+//     by the formula's operations (2b with a tree's masks 224); 8 of 32 x 6 rows 60 (groups of 48: 73).
+//     In f16, q' over its row's power of two and the weights over a running one have 11 bits, where 2b's parts have 12
+//     and 13: outputs are off by 0.00168 of their norm, their own rounding to bf16 alone and 2b by 0.00166.
 //     Tried: DMAs between the products, whose branches had registers spilled (283 us for 232 in all); two chains of
 //     products at once, as fast as one; the longest workgroups first, as fast.
 //  3. merge: the log-sum-exp merge of the other pairs' workgroups, times sigmoid(gate), to bf16.
-// prep takes 4 to 9 us and merge 5 to 10 for these.
+// prep takes 4 to 9 us and merge 5 to 10 for 2's and 2b's cases; for trees prep, with their append, 6 (96 rows) to 18
+// (24576), and merge 5 to 21.
 #include "npn_common.h"
 #include "paged_append.h"
 #include "tree.h"

@@ -5,7 +5,7 @@
 //
 // One wave a request, lane t its node t: a step is one ballot over "my parent is this node and my token
 // is its target's", so the walk takes as many steps as it accepts drafts and no memory in between. Bound
-// by a launch and one chain of loads: 2.9 us, of one request or of 256 with 64 nodes.
+// by a launch and one chain of loads: 1.9 us for one request of 16 nodes, 2.9 for 256 of 64.
 #include "tree.h"
 
 namespace {
