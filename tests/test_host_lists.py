@@ -1,4 +1,4 @@
-"""npn_native.check_lists and the version counts of ops without lists, without a GPU."""
+"""npn_native.check_lists without a GPU."""
 import types
 
 import pytest
